@@ -15,6 +15,9 @@ stubs __init__.pyi:99-107,208-236):
 - ``qgemm`` / ``qgemm_perchannel``: W8A8 GEMM with exact int32 accumulation;
 - ``rmsnorm`` (+ residual), ``rope`` (interleaved / NeoX, ``pos_offset``),
   ``swiglu``;
+- a paged KV cache held in 8 bits (build additions): ``block_table_extend``
+  (block tables and slots on the GPU), ``kv_append_paged_int8`` and
+  ``attention_decode_paged_int8``;
 - the post-logits step: ``argmax`` / ``argmax_batched`` (greedy),
   ``sample_topp`` / ``sample_topp_batched`` and ``decode_step`` /
   ``decode_step_batched`` (repetition penalty -> temperature -> nucleus
@@ -68,6 +71,7 @@ from ._contract import Arr as _Arr
 from ._contract import Contract as _Contract
 from ._contract import Idx as _Idx
 from ._contract import Rule as _Rule
+from ._contract import current_device as _current_device
 from ._contract import current_stream as _stream
 from . import _sampling_args as _sargs
 
@@ -91,6 +95,9 @@ __all__ = [
     "attention_prefill",
     "kv_append",
     "kv_append_paged",
+    "block_table_extend",
+    "kv_append_paged_int8",
+    "attention_decode_paged_int8",
     "rmsnorm_quant",
     "rmsnorm_qgemm",
     "swiglu_quant",
@@ -516,6 +523,183 @@ def kv_append(k_cache, v_cache, k_new, v_new, lens, *, cuda=False):
         c.ptr("k_new"), c.ptr("v_new"), c.ptr("lens"), c.ptr("k_cache"), c.ptr("v_cache"),
         c.B, c.Hkv, c.D, c.T, _stream())
     return None
+
+
+# ---------------------------------------------------------------------------
+# a paged KV cache held in 8 bits (build additions; GPU tensors only): int8
+# pools [Nb, Hkv, P, D] with one float32 scale per block and kv head
+# ---------------------------------------------------------------------------
+
+_I32 = (torch.int32,)
+_F32 = (torch.float32,)
+_POOL8_MISMATCH = "k_pool and v_pool must be int8 [Nb, Hkv, P, D] of one shape"
+_SCALE8_MISMATCH = "k_scales and v_scales must be float32 [Nb, Hkv]"
+_PAGE8 = _Rule(lambda c: 1 <= c.P <= 1024, "page must be in [1, 1024]")
+_DIM8 = _Rule(lambda c: c.D % 4 == 0 and 4 <= c.D <= 512,
+              "dim must be a multiple of 4 and at most 512")
+_NUM_SLOTS8 = _Rule(lambda c: c.Nb * c.P < 2 ** 31 and c.Nb * c.P * c.Hkv < 2 ** 32,
+                    "the cache has too many rows (slots must fit 31 bits, rows 32)")
+
+
+def _pools8(inplace):
+    return (_Arr("k_pool", "Nb Hkv P D", _INT8, inplace=inplace, mismatch=_POOL8_MISMATCH),
+            _Arr("v_pool", "=k_pool", _INT8, inplace=inplace, mismatch=_POOL8_MISMATCH),
+            _Arr("k_scales", "Nb Hkv", _F32, inplace=inplace, mismatch=_SCALE8_MISMATCH),
+            _Arr("v_scales", "Nb Hkv", _F32, inplace=inplace, mismatch=_SCALE8_MISMATCH))
+
+
+def _one_device(c):
+    """Every operand on the primary one's device; True when that is also the
+    current one (else the op runs again under it, on its current stream)."""
+    dev = c.device
+    for name, v in c._values.items():
+        if isinstance(v, torch.Tensor) and v.is_cuda and v.device != dev:
+            raise ValueError(f"{name} is on {v.device}, another operand on {dev}")
+    return dev.index == _current_device()
+
+
+_EXTEND = _Contract(
+    _Arr("block_table", "B S", _I32, inplace=True, rank_msg="block_table must be [B, S]"),
+    _Arr("lens", "B", _I32, mismatch=_LENS_WHAT, rank_msg=_LENS_WHAT),
+    _Arr("counts", "B", _I32, mismatch="counts must be 1-D with batch entries",
+         rank_msg="counts must be 1-D with batch entries"),
+    _Arr("free_blocks", "F", _I32, rank_msg="free_blocks must be 1-D"),
+    _Arr("n_free", "one", _I32, rank_msg="n_free must hold one value"),
+    rules=(_Rule(lambda c: c.one == 1, "n_free must hold one value"),
+           _Rule(lambda c: c.B <= 4096, "block_table_extend takes at most 4096 sequences"),
+           _Rule(lambda c: 1 <= c.page <= 1024, "page must be in [1, 1024]"),
+           _Rule(lambda c: 0 <= c.tokens < 2 ** 30, "tokens must be in [0, 2**30)")),
+    host=False)
+
+
+def block_table_extend(block_table, lens, counts, free_blocks, n_free, page, tokens):
+    """Block tables and slots of a paged cache's next tokens, on the GPU.
+
+    Sequence b holds ``lens[b]`` tokens and gets ``counts[b]`` more. The
+    blocks they need are taken from the end of ``free_blocks[:n_free]``, in the
+    order of the sequences, and written into ``block_table`` [B, S] in place
+    (-1 once the list is spent; entries in use are left alone). n_free is a
+    1-element tensor. Returns int32 tensors ``(slots, positions, offsets,
+    new_lens, new_free)``:
+
+    - slots [tokens]: ``block * page + row`` of each fresh token, the
+      sequences' tokens one after another; -1 behind the last and for a token
+      without a block or behind the table's end;
+    - positions [tokens]: its position in its sequence (0 behind the last), as
+      :func:`rope` takes them;
+    - offsets [B + 1]: sequence b's tokens are rows offsets[b] to
+      offsets[b + 1];
+    - new_lens [B]: ``min(lens + counts, S * page)``;
+    - new_free [1]: ``n_free`` minus the blocks needed; negative when that
+      many were missing.
+
+    A fresh batch has lens 0 and counts the request lengths; a decode step has
+    counts 1 (0 for an idle row). ``tokens`` is the outputs' size, known on
+    the host; fresh tokens beyond it get a block and no slot. int32 GPU tensors
+    only, values trusted (negative lens and counts count as 0); at most 4096
+    sequences. Build addition."""
+    c = _EXTEND.bind(block_table=block_table, lens=lens, counts=counts, free_blocks=free_blocks,
+                     n_free=n_free, page=int(page), tokens=int(tokens))
+    if not _one_device(c):
+        with torch.cuda.device(c.device):
+            return block_table_extend(block_table, lens, counts, free_blocks, n_free, page,
+                                      tokens)
+    B, T = c.B, c._values["tokens"]
+    out = torch.empty(2 * T + 2 * B + 2, dtype=torch.int32, device=c.device)
+    slots, positions, offsets, new_lens, new_free = out.split((T, T, B + 1, B, 1))
+    at = out.data_ptr()
+    _fusedtok.block_table_extend_launch(
+        c.ptr("block_table"), c.ptr("lens"), c.ptr("counts"), c.ptr("free_blocks"), c.F,
+        c.ptr("n_free"), at, at + 4 * T, at + 8 * T, at + 8 * T + 4 * (B + 1),
+        at + 8 * T + 4 * (2 * B + 1), B, c._values["page"], c.S, T, _stream())
+    return slots, positions, offsets, new_lens, new_free
+
+
+_APPEND8 = _Contract(
+    *_pools8(True),
+    _Arr("k_new", "T Hkv D", mismatch=_NEW_KV_MISMATCH,
+         rank_msg="k_new/v_new must be [T, Hkv, D]"),
+    _Arr("v_new", "=k_new", same_dtype="k_new", mismatch=_NEW_KV_MISMATCH),
+    _Arr("slots", "T", _I32, mismatch="slots must be 1-D with one entry per fresh row",
+         rank_msg="slots must be 1-D with one entry per fresh row"),
+    rank_msg="pools must be [Nb, Hkv, P, D], scales [Nb, Hkv]",
+    rules=(_PAGE8, _DIM8, _NUM_SLOTS8), host=False)
+
+
+def kv_append_paged_int8(k_pool, v_pool, k_scales, v_scales, k_new, v_new, slots):
+    """Write fresh K / V rows into a paged cache held in 8 bits, in place.
+
+    k_pool / v_pool: int8 [Nb, Hkv, P, D]; k_scales / v_scales: float32 [Nb,
+    Hkv], a value being ``code * scale`` of its block and head; k_new / v_new:
+    [T, Hkv, D] (f32 / bf16 / fp16), row i going to slot ``slots[i]`` = block *
+    P + row (int32; a slot outside the pools, such as -1, is skipped), as
+    :func:`block_table_extend` gives them: one row a sequence in a decode step,
+    whole prompts, or both mixed.
+
+    For each touched block and head, with ``a`` the largest magnitude among
+    the finite fresh values that go there: the scale becomes ``max(scale, a /
+    127, 2**-120)``, without the old scale when row 0 is among the fresh rows
+    (the block starts over); a code is ``rint(x * (1 / scale))`` clamped to
+    +-127 (infinities too; NaN gives 0). Where a scale grew, the other codes
+    of the block become ``rint(code * (old / new))``. Codes therefore depend
+    on how the rows were spread over calls, by up to half a step for each
+    growth. The rows of one block must be next to each other in ``slots``, and
+    no block may be written for two sequences in one call. Of two rows with
+    one slot the later counts. Returns None. Build addition."""
+    c = _APPEND8.bind(k_pool=k_pool, v_pool=v_pool, k_scales=k_scales, v_scales=v_scales,
+                      k_new=k_new, v_new=v_new, slots=slots)
+    if not _one_device(c):
+        with torch.cuda.device(c.device):
+            return kv_append_paged_int8(k_pool, v_pool, k_scales, v_scales, k_new, v_new, slots)
+    if c.T and c.Nb:
+        if c.ptr("k_pool") == c.ptr("v_pool") or c.ptr("k_scales") == c.ptr("v_scales"):
+            raise ValueError("k and v must have pools and scales of their own")
+        _fusedtok.kv_append_paged_int8_launch(
+            c.ptr("k_new"), c.ptr("v_new"), _CODE[c.k_new.dtype], c.ptr("slots"),
+            c.ptr("k_pool"), c.ptr("v_pool"), c.ptr("k_scales"), c.ptr("v_scales"), c.T, c.Hkv,
+            c.D, c.Nb, c.P, _stream())
+    return None
+
+
+_DECODE8 = _Contract(
+    _Arr("q", "B Hq D"),
+    *_pools8(False),
+    _table(),
+    _Idx("lens", "B", lambda c: c.S * c.P, optional=True, what=_LENS_WHAT),
+    rank_msg="q must be [B, Hq, D]; pools [Nb, Hkv, P, D], scales [Nb, Hkv]",
+    rules=(_HEADS, _GQA, _PAGE8, _DIM8, _NUM_SLOTS8), host=False)
+
+
+def attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales, block_table, lens=None):
+    """Single-token GQA attention over a paged cache held in 8 bits
+    (:func:`kv_append_paged_int8`):
+
+    ``out[b, h] = softmax(q[b, h] . K[b, kv(h)]^T / sqrt(D)) . V[b, kv(h)]``
+
+    q: [B, Hq, D] (f32 / bf16 / fp16, also the output's type; products of q
+    with the codes exact, softmax and sums float32); k_pool / v_pool: int8
+    [Nb, Hkv, P, D]; k_scales / v_scales: float32 [Nb, Hkv]; block_table: [B,
+    S], token t of sequence b at row ``t % P`` of block ``block_table[b, t //
+    P]``; lens: [B] (None = S * P rows each). Any group size Hq / Hkv, D a
+    multiple of 4 up to 512. Tokens of a table entry outside [0, Nb) (such as
+    -1) weigh nothing; a sequence without a token gives zero rows. Each call
+    has a workspace of its own from torch's allocator, so calls on several
+    streams are independent. Build addition."""
+    c = _DECODE8.bind(q=q, k_pool=k_pool, v_pool=v_pool, k_scales=k_scales, v_scales=v_scales,
+                      block_table=block_table, lens=lens)
+    if not _one_device(c):
+        with torch.cuda.device(c.device):
+            return attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales,
+                                               block_table, lens)
+    out = torch.empty((c.B, c.Hq, c.D), dtype=c.q.dtype, device=c.device)
+    if c.B:
+        nbytes = _fusedtok.attention_decode_paged_int8_workspace(c.B, c.Hq, c.Hkv, c.P, c.S, c.D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=c.device)
+        _fusedtok.attention_decode_paged_int8_launch(
+            c.ptr("q"), _CODE[c.q.dtype], c.ptr("k_pool"), c.ptr("v_pool"), c.ptr("k_scales"),
+            c.ptr("v_scales"), c.ptr("block_table"), c.ptr("lens"), out.data_ptr(),
+            ws.data_ptr(), nbytes, c.B, c.Hq, c.Hkv, c.Nb, c.P, c.S, c.D, _stream())
+    return out
 
 
 # ---------------------------------------------------------------------------

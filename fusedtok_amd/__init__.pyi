@@ -84,6 +84,19 @@ def kv_append_paged(k_pool: Array, v_pool: Array, block_table: IntArray,
                     k_new: Array, v_new: Array, lens: IntArray, *,
                     cuda: bool = ...) -> None: ...
 
+# -- a paged KV cache in 8 bits (GPU tensors only) ------------------------------
+def block_table_extend(block_table: torch.Tensor, lens: torch.Tensor, counts: torch.Tensor,
+                       free_blocks: torch.Tensor, n_free: torch.Tensor, page: int, tokens: int
+                       ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                                  torch.Tensor]: ...
+def kv_append_paged_int8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scales: torch.Tensor,
+                         v_scales: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+                         slots: torch.Tensor) -> None: ...
+def attention_decode_paged_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                                k_scales: torch.Tensor, v_scales: torch.Tensor,
+                                block_table: IntArray, lens: Optional[IntArray] = ...
+                                ) -> torch.Tensor: ...
+
 # -- int8 ------------------------------------------------------------------------
 @overload
 def quantize_int8(x: Array) -> Tuple[Array, float]: ...

@@ -41,6 +41,7 @@ HIP_SOURCES = [
     "layer.hip",
     "prefill.hip",
     "sampling.hip",
+    "cache8.hip",
 ]
 
 HIP_FLAGS = [

@@ -157,6 +157,11 @@ def current_stream():
     return _raw_stream(_raw_device())
 
 
+def current_device():
+    """The current device's index (as torch.cuda.current_device)."""
+    return torch.cuda.current_device() if _raw_device is None else _raw_device()
+
+
 def _parse(shape):
     if shape == "*" or shape.startswith("="):
         return shape

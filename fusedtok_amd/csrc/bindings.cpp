@@ -150,6 +150,61 @@ PYBIND11_MODULE(_fusedtok, m) {
           py::arg("dtype"), py::arg("batch"), py::arg("q_heads"), py::arg("kv_heads"),
           py::arg("page"), py::arg("tbl_width"), py::arg("dim"), py::arg("stream") = 0);
 
+    // ---- paged KV cache in 8 bits -------------------------------------------
+    m.def("block_table_extend_launch",
+          [](uintptr_t table, uintptr_t lens, uintptr_t counts, uintptr_t free_blocks,
+             int free_len, uintptr_t n_free, uintptr_t slots, uintptr_t positions,
+             uintptr_t offsets, uintptr_t lens_out, uintptr_t n_free_out, int batch, int page,
+             int tbl_width, int tokens, uintptr_t stream) {
+              check(ft_block_table_extend_launch(
+                  P<int>(table), P<const int>(lens), P<const int>(counts),
+                  P<const int>(free_blocks), free_len, P<const int>(n_free), P<int>(slots),
+                  P<int>(positions), P<int>(offsets), P<int>(lens_out), P<int>(n_free_out), batch,
+                  page, tbl_width, tokens, stream));
+          },
+          py::arg("table"), py::arg("lens"), py::arg("counts"), py::arg("free_blocks"),
+          py::arg("free_len"), py::arg("n_free"), py::arg("slots"), py::arg("positions"),
+          py::arg("offsets"), py::arg("lens_out"), py::arg("n_free_out"), py::arg("batch"),
+          py::arg("page"), py::arg("tbl_width"), py::arg("tokens"), py::arg("stream") = 0);
+    m.def("kv_append_paged_int8_launch",
+          [](uintptr_t kn, uintptr_t vn, int dtype, uintptr_t slots, uintptr_t kp, uintptr_t vp,
+             uintptr_t ks, uintptr_t vs, int tokens, int hkv, int dim, int blocks, int page,
+             uintptr_t stream) {
+              check(ft_kv_append_paged_int8_launch(
+                  P<const void>(kn), P<const void>(vn), dtype, P<const int>(slots),
+                  P<signed char>(kp), P<signed char>(vp), P<float>(ks), P<float>(vs), tokens, hkv,
+                  dim, blocks, page, stream));
+          },
+          py::arg("k_new"), py::arg("v_new"), py::arg("dtype"), py::arg("slots"),
+          py::arg("k_pool"), py::arg("v_pool"), py::arg("k_scales"), py::arg("v_scales"),
+          py::arg("tokens"), py::arg("kv_heads"), py::arg("dim"), py::arg("blocks"),
+          py::arg("page"), py::arg("stream") = 0);
+    m.def("attention_decode_paged_int8_workspace",
+          [](int batch, int hq, int hkv, int page, int tbl_width, int dim) {
+              long long bytes = 0;
+              check(ft_attention_decode_paged_int8_workspace(batch, hq, hkv, page, tbl_width, dim,
+                                                             &bytes));
+              return bytes;
+          },
+          py::arg("batch"), py::arg("q_heads"), py::arg("kv_heads"), py::arg("page"),
+          py::arg("tbl_width"), py::arg("dim"));
+    m.def("attention_decode_paged_int8_launch",
+          [](uintptr_t q, int dtype, uintptr_t kp, uintptr_t vp, uintptr_t ks, uintptr_t vs,
+             uintptr_t table, py::object lens, uintptr_t out, uintptr_t ws, long long ws_bytes,
+             int batch, int hq, int hkv, int blocks, int page, int tbl_width, int dim,
+             uintptr_t stream) {
+              check(ft_attention_decode_paged_int8_launch(
+                  P<const void>(q), dtype, P<const signed char>(kp), P<const signed char>(vp),
+                  P<const float>(ks), P<const float>(vs), P<const int>(table),
+                  P<const int>(opt_ptr(lens)), P<void>(out), P<void>(ws), ws_bytes, batch, hq, hkv,
+                  blocks, page, tbl_width, dim, stream));
+          },
+          py::arg("q"), py::arg("dtype"), py::arg("k_pool"), py::arg("v_pool"),
+          py::arg("k_scales"), py::arg("v_scales"), py::arg("table"), py::arg("lens"),
+          py::arg("out"), py::arg("workspace"), py::arg("workspace_bytes"), py::arg("batch"),
+          py::arg("q_heads"), py::arg("kv_heads"), py::arg("blocks"), py::arg("page"),
+          py::arg("tbl_width"), py::arg("dim"), py::arg("stream") = 0);
+
     // ---- kv append --------------------------------------------------------
 #define FT_KVP(NAME, FN, T)                                                    \
     m.def(NAME,                                                                \

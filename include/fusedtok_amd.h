@@ -230,6 +230,61 @@ int ft_attention_prefill_launch_fp16(const void* q, const void* k, const void* v
                                      int seq, int dim, int causal, uintptr_t stream);
 
 /* ------------------------------------------------------------------ */
+/* A paged KV cache held in 8 bits (build addition, no reference        */
+/* counterpart). k_pool / v_pool int8 [blocks, kv_heads, page, dim],    */
+/* k_scales / v_scales float32 [blocks, kv_heads]: a value is code *    */
+/* scale of its block and head. A slot is block * page + row. page is   */
+/* in [1, 1024], dim a multiple of 4 up to 512. None of these uses the  */
+/* library's scratch: calls on several streams are independent.         */
+/* ------------------------------------------------------------------ */
+/* Block tables and slot maps from lengths. Sequence b holds lens[b]
+ * tokens and gets counts[b] more; the fresh blocks it needs are taken from
+ * the end of free_blocks[0, *n_free) in the order of the sequences and
+ * written to table [batch, tbl_width] (-1 when the list is spent; entries
+ * that hold tokens already are not touched). For the fresh tokens, those of
+ * sequence 0 first: slots[i] and positions[i], -1 and 0 behind the last,
+ * -1 for a token without a block or behind the table's end. offsets
+ * [batch + 1]: sequence b's rows are [offsets[b], offsets[b + 1]). lens_out =
+ * min(lens + counts, tbl_width * page); *n_free_out = *n_free minus the
+ * blocks needed (negative: that many are missing). slots and positions hold
+ * `tokens` entries (more fresh tokens than that have none). batch <= 4096;
+ * the outputs overlap no input. */
+int ft_block_table_extend_launch(int* table, const int* lens, const int* counts,
+                                 const int* free_blocks, int free_len, const int* n_free,
+                                 int* slots, int* positions, int* offsets, int* lens_out,
+                                 int* n_free_out, int batch, int page, int tbl_width, int tokens,
+                                 uintptr_t stream);
+/* Fresh rows k_new / v_new [tokens, kv_heads, dim] (dtype FT_DT_*) into
+ * their slots; a slot outside the pools is skipped. Per head, with a = max
+ * |x| over the finite values of the rows that go to a block: scale' =
+ * max(scale, a / 127, 2^-120), without the old scale when row 0 is among
+ * them (the block starts over); codes rint(x * (1 / scale')) clamped to
+ * +-127 (infinities too; NaN gives 0); where the scale grew, the block's
+ * other rows become rint(code * (scale / scale')). The rows of one block
+ * must be next to each other in slots (runs of one block at two places race
+ * with each other); of two rows with one slot the later counts. */
+int ft_kv_append_paged_int8_launch(const void* k_new, const void* v_new, int dtype,
+                                   const int* slots, signed char* k_pool, signed char* v_pool,
+                                   float* k_scales, float* v_scales, int tokens, int kv_heads,
+                                   int dim, int blocks, int page, uintptr_t stream);
+/* Decode attention over the cache: out [batch, q_heads, dim] (dtype FT_DT_*,
+ * q's) = softmax(q . k / sqrt(dim)) . v over the first lens[b] tokens (lens
+ * NULL: tbl_width * page) of sequence b, token t at row t % page of block
+ * table[b, t / page]. Any group size. Tokens of a table entry outside
+ * [0, blocks) weigh nothing; a row without a token gives zeros. The
+ * workspace (device memory, 16-byte aligned) is the caller's: it is written
+ * by the call and free again when the stream has passed it. */
+int ft_attention_decode_paged_int8_workspace(int batch, int q_heads, int kv_heads, int page,
+                                             int tbl_width, int dim, long long* bytes);
+int ft_attention_decode_paged_int8_launch(const void* q, int dtype, const signed char* k_pool,
+                                          const signed char* v_pool, const float* k_scales,
+                                          const float* v_scales, const int* table,
+                                          const int* lens, void* out, void* workspace,
+                                          long long workspace_bytes, int batch, int q_heads,
+                                          int kv_heads, int blocks, int page, int tbl_width,
+                                          int dim, uintptr_t stream);
+
+/* ------------------------------------------------------------------ */
 /* INT8 per-tensor symmetric quantize                                  */
 /* scale = max|x|/127 (1.0 for all-zero input); inv = 1.0f/scale;      */
 /* q = clamp(rint(x*inv), -127, 127). scale_out is a DEVICE float.     */

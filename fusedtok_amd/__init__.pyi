@@ -33,6 +33,9 @@ __all__ = [
     "attention_prefill",
     "kv_append",
     "kv_append_paged",
+    "block_table_extend",
+    "kv_append_paged_int8",
+    "attention_decode_paged_int8",
     "rmsnorm_quant",
     "rmsnorm_qgemm",
     "swiglu_quant",

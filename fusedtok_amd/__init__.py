@@ -693,7 +693,8 @@ def attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales, block_tab
                                                block_table, lens)
     out = torch.empty((c.B, c.Hq, c.D), dtype=c.q.dtype, device=c.device)
     if c.B:
-        nbytes = _fusedtok.attention_decode_paged_int8_workspace(c.B, c.Hq, c.Hkv, c.P, c.S, c.D)
+        nbytes = _fusedtok.attention_decode_paged_int8_workspace(
+            _CODE[c.q.dtype], c.B, c.Hq, c.Hkv, c.P, c.S, c.D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=c.device)
         _fusedtok.attention_decode_paged_int8_launch(
             c.ptr("q"), _CODE[c.q.dtype], c.ptr("k_pool"), c.ptr("v_pool"), c.ptr("k_scales"),

@@ -180,13 +180,13 @@ PYBIND11_MODULE(_fusedtok, m) {
           py::arg("tokens"), py::arg("kv_heads"), py::arg("dim"), py::arg("blocks"),
           py::arg("page"), py::arg("stream") = 0);
     m.def("attention_decode_paged_int8_workspace",
-          [](int batch, int hq, int hkv, int page, int tbl_width, int dim) {
+          [](int dtype, int batch, int hq, int hkv, int page, int tbl_width, int dim) {
               long long bytes = 0;
-              check(ft_attention_decode_paged_int8_workspace(batch, hq, hkv, page, tbl_width, dim,
-                                                             &bytes));
+              check(ft_attention_decode_paged_int8_workspace(dtype, batch, hq, hkv, page,
+                                                             tbl_width, dim, &bytes));
               return bytes;
           },
-          py::arg("batch"), py::arg("q_heads"), py::arg("kv_heads"), py::arg("page"),
+          py::arg("dtype"), py::arg("batch"), py::arg("q_heads"), py::arg("kv_heads"), py::arg("page"),
           py::arg("tbl_width"), py::arg("dim"));
     m.def("attention_decode_paged_int8_launch",
           [](uintptr_t q, int dtype, uintptr_t kp, uintptr_t vp, uintptr_t ks, uintptr_t vs,

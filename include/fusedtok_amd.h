@@ -262,7 +262,8 @@ int ft_block_table_extend_launch(int* table, const int* lens, const int* counts,
  * +-127 (infinities too; NaN gives 0); where the scale grew, the block's
  * other rows become rint(code * (scale / scale')). The rows of one block
  * must be next to each other in slots (runs of one block at two places race
- * with each other); of two rows with one slot the later counts. */
+ * with each other); of two rows with one slot the later counts. k_new and
+ * v_new are aligned to 4 elements, the pools to 4 bytes. */
 int ft_kv_append_paged_int8_launch(const void* k_new, const void* v_new, int dtype,
                                    const int* slots, signed char* k_pool, signed char* v_pool,
                                    float* k_scales, float* v_scales, int tokens, int kv_heads,
@@ -271,11 +272,12 @@ int ft_kv_append_paged_int8_launch(const void* k_new, const void* v_new, int dty
  * q's) = softmax(q . k / sqrt(dim)) . v over the first lens[b] tokens (lens
  * NULL: tbl_width * page) of sequence b, token t at row t % page of block
  * table[b, t / page]. Any group size. Tokens of a table entry outside
- * [0, blocks) weigh nothing; a row without a token gives zeros. The
+ * [0, blocks) weigh nothing; a row without a token gives zeros. q and out
+ * are aligned to 4 elements, the pools to 16 bytes (4 where dim % 16). The
  * workspace (device memory, 16-byte aligned) is the caller's: it is written
  * by the call and free again when the stream has passed it. */
-int ft_attention_decode_paged_int8_workspace(int batch, int q_heads, int kv_heads, int page,
-                                             int tbl_width, int dim, long long* bytes);
+int ft_attention_decode_paged_int8_workspace(int dtype, int batch, int q_heads, int kv_heads,
+                                             int page, int tbl_width, int dim, long long* bytes);
 int ft_attention_decode_paged_int8_launch(const void* q, int dtype, const signed char* k_pool,
                                           const signed char* v_pool, const float* k_scales,
                                           const float* v_scales, const int* table,

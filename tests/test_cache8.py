@@ -23,7 +23,7 @@ def lib():
     lib.ft_last_error.restype = ctypes.c_char_p
     lib.ft_block_table_extend_launch.argtypes = [P, P, P, P, I] + [P] * 6 + [I] * 4 + [U]
     lib.ft_kv_append_paged_int8_launch.argtypes = [P, P, I] + [P] * 5 + [I] * 5 + [U]
-    lib.ft_attention_decode_paged_int8_workspace.argtypes = [I] * 6 + [P]
+    lib.ft_attention_decode_paged_int8_workspace.argtypes = [I] * 7 + [P]
     lib.ft_attention_decode_paged_int8_launch.argtypes = [P, I] + [P] * 8 + [L] + [I] * 7 + [U]
     return lib
 
@@ -73,7 +73,7 @@ def test_attention_refusals(lib, change, word):
     a = dict(batch=2, hq=8, hkv=2, page=16, width=4, dim=64)
     a.update(change)
     got = ctypes.c_longlong(-1)
-    st = lib.ft_attention_decode_paged_int8_workspace(a["batch"], a["hq"], a["hkv"], a["page"],
+    st = lib.ft_attention_decode_paged_int8_workspace(1, a["batch"], a["hq"], a["hkv"], a["page"],
                                                       a["width"], a["dim"], ctypes.byref(got))
     assert st == FT_EINVAL and word in lib.ft_last_error() and got.value == -1
     st = lib.ft_attention_decode_paged_int8_launch(X, 1, X, X, X, X, X, X, X, X, 1 << 40,

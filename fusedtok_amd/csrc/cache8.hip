@@ -37,6 +37,26 @@ void check_aligned(const void* p, size_t bytes, const char* what) {
 }
 inline size_t size_of(int dtype) { return dtype == FT_DT_F32 ? 4 : 2; }
 
+// Division by a size known at launch, n / d for 0 <= n < 2^31: with l =
+// ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1, n / d = (mulhi(m, n) + n)
+// >> l (Granlund and Montgomery 1994). Three instructions for the ~25 of a
+// 32-bit division.
+struct FastDiv {
+    unsigned d, m, l;
+    FastDiv() = default;
+    explicit FastDiv(int by) : d((unsigned)by), m(0), l(0) {
+        while ((1ull << l) < d) ++l;
+        m = (unsigned)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int div(int n) const {
+        return (int)((__umulhi(m, (unsigned)n) + (unsigned)n) >> l);
+    }
+    __device__ __forceinline__ int up(int n) const {  // ceil(n / d), n <= 2^30
+        return div(n + (int)d - 1);
+    }
+    __device__ __forceinline__ int mod(int n) const { return n - div(n) * (int)d; }
+};
+
 // ---------------------------------------------------------------------------
 // Block tables and slot maps.
 //
@@ -54,69 +74,83 @@ inline size_t size_of(int dtype) { return dtype == FT_DT_F32 ? 4 : 2; }
 // from the table entry that another workgroup may be writing. What bounds it:
 // launch and the dependent chain length -> scan -> bisection -> table.
 // ---------------------------------------------------------------------------
+constexpr int kExtendTokens = 512;  // tokens of a workgroup
+
 __global__ __launch_bounds__(256) void block_table_extend_kernel(
     int* __restrict__ table, const int* __restrict__ lens, const int* __restrict__ counts,
     const int* __restrict__ free_blocks, int free_len, const int* __restrict__ n_free,
     int* __restrict__ slots, int* __restrict__ positions, int* __restrict__ offsets,
-    int* __restrict__ lens_out, int* __restrict__ n_free_out, int batch, int page, int width,
+    int* __restrict__ lens_out, int* __restrict__ n_free_out, int batch, FastDiv page, int width,
     int tokens) {
+    constexpr int PER = kExtendSeqs / 256;
     __shared__ int s_off[kExtendSeqs + 1];   // fresh tokens before sequence b (saturated)
     __shared__ int s_need[kExtendSeqs + 1];  // fresh blocks before sequence b
-    __shared__ long long s_wave[2][4];
+    __shared__ long long s_toks[4];
+    __shared__ int s_blocks[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const long long span = (long long)width * page;
+    const int span = width * (int)page.d;  // <= 2^30
+    const int have = *n_free;
 
-    const int per = (batch + 255) / 256;
-    const int b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
-    auto len_of = [&](int b) { return min((long long)max(lens[b], 0), span); };
-    auto need_of = [&](long long len, long long add) {
-        const long long end = min(len + add, span);
-        return (end + page - 1) / page - (len + page - 1) / page;
-    };
-    long long toks = 0, need = 0;
-    for (int b = b0; b < b1; ++b) {
-        const long long add = max(counts[b], 0);
-        toks += add;
-        need += need_of(len_of(b), add);
+    // each thread's run of sequences, all loaded before any is used
+    const int per = (batch + 255) / 256, b0 = tid * per;
+    int len[PER], add[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const bool in = i < per && b0 + i < batch;
+        len[i] = in ? lens[b0 + i] : 0;
+        add[i] = in ? counts[b0 + i] : 0;
     }
-    long long it = toks, in = need;  // inclusive over the wave, then the workgroup
+    long long toks = 0;
+    int need = 0;  // all sequences': at most the table's entries, which fit
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        len[i] = min(max(len[i], 0), span);
+        add[i] = max(add[i], 0);
+        toks += add[i];
+        need += page.up(len[i] + min(add[i], span - len[i])) - page.up(len[i]);
+    }
+    long long it = toks;  // inclusive over the wave, then the workgroup
+    int in = need;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const long long yt = __shfl_up(it, o, 64), yn = __shfl_up(in, o, 64);
+        const long long yt = __shfl_up(it, o, 64);
+        const int yn = __shfl_up(in, o, 64);
         if (lane >= o) {
             it += yt;
             in += yn;
         }
     }
     if (lane == 63) {
-        s_wave[0][wave] = it;
-        s_wave[1][wave] = in;
+        s_toks[wave] = it;
+        s_blocks[wave] = in;
     }
     __syncthreads();
-    long long rt = it - toks, rn = in - need;
-    long long all_t = 0, all_n = 0;
+    long long rt = it - toks, all = 0;
+    int rn = in - need, fresh = 0;
+#pragma unroll
     for (int w = 0; w < 4; ++w) {
         if (w < wave) {
-            rt += s_wave[0][w];
-            rn += s_wave[1][w];
+            rt += s_toks[w];
+            rn += s_blocks[w];
         }
-        all_t += s_wave[0][w];
-        all_n += s_wave[1][w];
+        all += s_toks[w];
+        fresh += s_blocks[w];
     }
-    const int total = (int)min(all_t, (long long)INT_MAX);
-    const int fresh = (int)all_n;  // <= batch * width, which fits (the table's entries)
-    for (int b = b0; b < b1; ++b) {
-        s_off[b] = (int)min(rt, (long long)INT_MAX);
-        s_need[b] = (int)rn;
-        const long long add = max(counts[b], 0), len = len_of(b);
-        if (blockIdx.x == 0) {
-            offsets[b] = (int)min(rt, (long long)INT_MAX);
-            lens_out[b] = (int)min(len + add, span);
+    const int total = (int)min(all, (long long)INT_MAX);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (i < per && b0 + i < batch) {
+            const int b = b0 + i, off = (int)min(rt, (long long)INT_MAX);
+            const int end = len[i] + min(add[i], span - len[i]);
+            s_off[b] = off;
+            s_need[b] = rn;
+            if (blockIdx.x == 0) {
+                offsets[b] = off;
+                lens_out[b] = end;
+            }
+            rt += add[i];
+            rn += page.up(end) - page.up(len[i]);
         }
-        rt += add;
-        rn += need_of(len, add);
-    }
-    const int have = *n_free;
     if (tid == 0) {
         s_off[batch] = total;
         s_need[batch] = fresh;
@@ -140,20 +174,20 @@ __global__ __launch_bounds__(256) void block_table_extend_kernel(
         const long long at = (long long)have - 1 - k;
         return at >= 0 && at < free_len ? free_blocks[at] : -1;
     };
+    auto len_of = [&](int b) { return min(max(lens[b], 0), span); };
 
-    const int stride = gridDim.x * 256;
+    const long long stride = gridDim.x * 256;
     for (long long t = blockIdx.x * 256 + tid; t < tokens; t += stride) {
         int slot = -1, pos = 0;
         if (t < total) {
-            const int b = find(s_off, (int)t);
-            const int len = (int)len_of(b);
-            const long long p = (long long)len + (t - s_off[b]);
+            const int b = find(s_off, (int)t), n = len_of(b);
+            const long long p = (long long)n + (t - s_off[b]);
             pos = (int)min(p, (long long)INT_MAX);
             if (p < span) {
-                const int col = (int)(p / page), first = (int)(((long long)len + page - 1) / page);
+                const int col = page.div(pos), first = page.up(n);
                 const int block = col < first ? table[(size_t)b * width + col]
                                               : taken(s_need[b] + col - first);
-                const long long s = (long long)block * page + p % page;
+                const long long s = (long long)block * (int)page.d + (pos - col * (int)page.d);
                 if (block >= 0 && s <= INT_MAX) slot = (int)s;
             }
         }
@@ -162,8 +196,7 @@ __global__ __launch_bounds__(256) void block_table_extend_kernel(
     }
     for (long long k = blockIdx.x * 256 + tid; k < fresh; k += stride) {
         const int b = find(s_need, (int)k);
-        const int first = (int)((len_of(b) + page - 1) / page);
-        table[(size_t)b * width + first + (k - s_need[b])] = taken((int)k);
+        table[(size_t)b * width + page.up(len_of(b)) + ((int)k - s_need[b])] = taken((int)k);
     }
 }
 
@@ -186,66 +219,207 @@ __device__ __forceinline__ signed char code8(float x, float inv) {
     return v == v ? (signed char)fmaxf(-127.0f, fminf(127.0f, v)) : (signed char)0;
 }
 
-// One wave per (token, kv head, K or V): the wave whose token starts a run
-// does the whole run.
-template <typename T>
-__global__ __launch_bounds__(64) void kv_append8_kernel(
+// V values of x widened to float32, 16 bytes a load where they fill them.
+template <int V, typename T>
+__device__ __forceinline__ void load_f(const T* p, float (&x)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    const vec u = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = (float)u[i];
+}
+
+template <int V>
+struct Codes {
+    signed char c[V];
+} __attribute__((aligned(V)));
+
+// A unit is (window of `window` consecutive fresh rows, kv head, K or V): the
+// runs that start in the window, one after another (a run may reach past it).
+// UT threads a unit, 256 a workgroup. Windows are as long as a block where
+// that leaves enough units (about one run each: a prompt), else one row (a
+// decode step). A lane has V values of a row; the first kKeep passes of a run
+// stay in registers between the maximum and the codes, so a run is read once.
+// Rows in order, as a sequence's are, need no map; others (gaps, a slot twice)
+// go by a map in LDS from the block's row to the last fresh row for it.
+//
+// What bounds it: memory latency in a decode step; for prompts, HBM.
+template <typename T, int V, int UT>
+__global__ __launch_bounds__(256) void kv_append8_kernel(
     const T* __restrict__ k_new, const T* __restrict__ v_new, const int* __restrict__ slots,
     signed char* __restrict__ k_pool, signed char* __restrict__ v_pool,
-    float* __restrict__ k_scales, float* __restrict__ v_scales, int tokens, int hkv, int dim,
-    int nslots, int page) {
-    __shared__ int s_src[kMaxPage8];  // row of the block -> its fresh row, or -1
-    const int lane = threadIdx.x, i = blockIdx.x, h = blockIdx.y;
-    auto block_of = [&](int t) {
-        const int s = slots[t];
-        return s >= 0 && s < nslots ? s / page : -1;
+    float* __restrict__ k_scales, float* __restrict__ v_scales, int tokens, FastDiv heads, int dim,
+    int nslots, FastDiv page, FastDiv lanes, int window, long long units) {
+    constexpr int kKeep = 4, kUnits = 256 / UT;
+    __shared__ int s_map[kUnits][kMaxPage8];
+    __shared__ float s_red[4];
+    const int lane = threadIdx.x & 63;
+    const int ut = UT == 64 ? lane : (int)threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long unit = (long long)blockIdx.x * kUnits + (UT == 64 ? wave : 0);
+    if (unit >= units) return;
+    int* const map = s_map[UT == 64 ? wave : 0];
+    // (units / 2 <= tokens * heads < 2^31: checked by the host)
+    const bool is_v = unit >= units / 2;
+    const int wh = (int)(is_v ? unit - units / 2 : unit);
+    const int h = heads.mod(wh), hkv = (int)heads.d, first = heads.div(wh) * window;
+    const T* const x = (is_v ? v_new : k_new) + (size_t)h * dim;
+    signed char* const pool = is_v ? v_pool : k_pool;
+    float* const scales = is_v ? v_scales : k_scales;
+    const size_t row_stride = (size_t)hkv * dim;
+    auto sync = [&] {
+        if (UT == 64) wave_lds_order();
+        else __syncthreads();
     };
-    const int block = block_of(i);
-    if (block < 0 || (i > 0 && block_of(i - 1) == block)) return;
-    const T* x = blockIdx.z ? v_new : k_new;
-    signed char* codes = (blockIdx.z ? v_pool : k_pool) + ((size_t)block * hkv + h) * page * dim;
-    float* scale = (blockIdx.z ? v_scales : k_scales) + (size_t)block * hkv + h;
+    auto slot_of = [&](int t) { return t >= 0 && t < tokens ? slots[t] : -1; };
+    auto block_of = [&](int s) { return s >= 0 && s < nslots ? page.div(s) : -1; };
 
-    for (int r = lane; r < page; r += 64) s_src[r] = -1;
-    __syncthreads();
-    for (long long t = i;; t += 64) {
-        const bool in = t + lane < tokens && block_of((int)t + lane) == block;
-        const unsigned long long out = __ballot(!in);
-        const int n = out ? __builtin_ctzll(out) : 64;
-        if (lane < n) atomicMax(&s_src[slots[t + lane] % page], (int)t + lane);
-        if (n < 64) break;
-    }
-    __syncthreads();
-    const int dc = dim / 4;
-    float most = 0.0f;
-    for (int j = lane; j < page * dc; j += 64) {
-        const int r = j / dc, src = s_src[r];
-        if (src < 0) continue;
-        const float4 v = St<T>::ld4(x + ((size_t)src * hkv + h) * dim + 4 * (j - r * dc));
-        const float e[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
-        for (int c = 0; c < 4; ++c)
-            if (e[c] < INFINITY) most = fmaxf(most, e[c]);
-    }
-    most = wave_max(most);
-    const bool over = s_src[0] >= 0;
-    const float held = over ? 0.0f : *scale;
-    const float now = fmaxf(fmaxf(held, most / 127.0f), kLeastScale);
-    const float inv = 1.0f / now, ratio = held / now;
-    const bool grown = !over && now > held;
-    for (int j = lane; j < page * dc; j += 64) {
-        const int r = j / dc, src = s_src[r];
-        char4* p = reinterpret_cast<char4*>(codes + (size_t)r * dim + 4 * (j - r * dc));
-        if (src >= 0) {
-            const float4 v = St<T>::ld4(x + ((size_t)src * hkv + h) * dim + 4 * (j - r * dc));
-            *p = make_char4(code8(v.x, inv), code8(v.y, inv), code8(v.z, inv), code8(v.w, inv));
-        } else if (grown) {
-            const char4 c = *p;
-            *p = make_char4(code8(c.x, ratio), code8(c.y, ratio), code8(c.z, ratio),
-                            code8(c.w, ratio));
+    for (int w0 = 0; w0 < window; w0 += 64) {
+        const int t = first + w0 + lane;
+        const int mine = w0 + lane < window ? block_of(slot_of(t)) : -1;
+        unsigned long long starts = __ballot(mine >= 0 && block_of(slot_of(t - 1)) != mine);
+        while (starts) {
+            const int at = __builtin_ctzll(starts);
+            starts &= starts - 1;
+            const int i = first + w0 + at;             // the run's first fresh row
+            const int block = __shfl(mine, at, 64);
+            const int slot0 = slots[i], row0 = page.mod(slot0);
+            // its length, and whether its rows are in order
+            int n = 0;
+            bool ordered = true;
+            for (;; n += 64) {
+                const int s = slot_of(i + n + lane);
+                const unsigned long long out = __ballot(block_of(s) != block);
+                const int got = out ? __builtin_ctzll(out) : 64;
+                ordered = ordered && !__any(lane < got && s != slot0 + n + lane);
+                if (got < 64) {
+                    n += got;
+                    break;
+                }
+            }
+            n = __builtin_amdgcn_readfirstlane(n);
+            bool over = row0 == 0;
+            if (!ordered) {
+                sync();
+                for (int r = ut; r < (int)page.d; r += UT) map[r] = -1;
+                sync();
+                for (int k = ut; k < n; k += UT) atomicMax(&map[page.mod(slots[i + k])], i + k);
+                sync();
+                over = map[0] >= 0;
+            }
+            const int base = ordered ? row0 : 0;                 // the rows gone over
+            const int nvec = (ordered ? n : (int)page.d) * (int)lanes.d;
+            // the fresh row for the j-th vector of them, -1 where there is none
+            auto source = [&](int r) { return ordered ? i + r : map[r]; };
+            float keep[kKeep][V];
+            float most = 0.0f;
+            auto fold = [&](const float (&v)[V]) {
+#pragma unroll
+                for (int c = 0; c < V; ++c) {
+                    const float a = fabsf(v[c]);
+                    most = fmaxf(most, a < INFINITY ? a : 0.0f);
+                }
+            };
+            auto load = [&](int j, float (&v)[V]) {
+                const int r = lanes.div(j), src = source(r);
+#pragma unroll
+                for (int c = 0; c < V; ++c) v[c] = 0.0f;
+                if (src >= 0) load_f<V>(x + src * row_stride + V * (j - r * (int)lanes.d), v);
+            };
+#pragma unroll
+            for (int p = 0; p < kKeep; ++p) {
+                const int j = p * UT + ut;
+                if (j < nvec) load(j, keep[p]);
+            }
+#pragma unroll
+            for (int p = 0; p < kKeep; ++p)
+                if (p * UT + ut < nvec) fold(keep[p]);
+            for (int j = kKeep * UT + ut; j < nvec; j += UT) {
+                float v[V];
+                load(j, v);
+                fold(v);
+            }
+            const size_t bh = (size_t)block * hkv + h;
+            const float held = over ? 0.0f : scales[bh];
+            most = UT == 64 ? wave_max(most) : block_max<256>(most, s_red);
+            const float now = fmaxf(fmaxf(held, most / 127.0f), kLeastScale);
+            const float inv = 1.0f / now;
+            signed char* const codes = pool + bh * page.d * dim;
+            auto store = [&](int j, const float (&v)[V]) {
+                const int r = lanes.div(j);
+                if (source(r) < 0) return;
+                Codes<V> o;
+#pragma unroll
+                for (int c = 0; c < V; ++c) o.c[c] = code8(v[c], inv);
+                *reinterpret_cast<Codes<V>*>(codes + (size_t)(base + r) * dim +
+                                             V * (j - r * (int)lanes.d)) = o;
+            };
+#pragma unroll
+            for (int p = 0; p < kKeep; ++p) {
+                const int j = p * UT + ut;
+                if (j < nvec) store(j, keep[p]);
+            }
+            for (int j = kKeep * UT + ut; j < nvec; j += UT) {
+                float v[V];
+                load(j, v);
+                store(j, v);
+            }
+            if (!over && now > held) {  // the block's other rows
+                const float ratio = held / now;
+                for (int j = ut; j < (int)(page.d * lanes.d); j += UT) {
+                    const int r = lanes.div(j);
+                    if (ordered ? (unsigned)(r - row0) < (unsigned)n : map[r] >= 0) continue;
+                    Codes<V>* p = reinterpret_cast<Codes<V>*>(codes + (size_t)V * j);
+                    Codes<V> o = *p;
+#pragma unroll
+                    for (int c = 0; c < V; ++c) o.c[c] = code8((float)o.c[c], ratio);
+                    *p = o;
+                }
+            }
+            if (ut == 0) scales[bh] = now;
         }
     }
-    __syncthreads();
-    if (lane == 0) *scale = now;
+}
+
+// Fresh rows from which windows are as long as a block: so many (row, head)
+// pairs fill the GPU with units a block long.
+constexpr long long kAppendLong = 1 << 15;
+
+template <typename T, int V, int UT>
+void append8_run(const T* k_new, const T* v_new, const int* slots, signed char* k_pool,
+                 signed char* v_pool, float* k_scales, float* v_scales, int tokens, int hkv,
+                 int dim, int blocks, int page, hipStream_t s) {
+    const int window = (long long)tokens * hkv >= kAppendLong ? page : 1;
+    const long long units = 2LL * ((tokens + window - 1) / window) * hkv;
+    const long long wgs = (units * UT + 255) / 256;
+    if (wgs >= 1LL << 24) inval("kv_append_paged_int8: too many rows for one call");
+    kv_append8_kernel<T, V, UT><<<(unsigned)wgs, 256, 0, s>>>(
+        k_new, v_new, slots, k_pool, v_pool, k_scales, v_scales, tokens, FastDiv(hkv), dim,
+        blocks * page, FastDiv(page), FastDiv(dim / V), window, units);
+    launch_check("int8 kv append kernel launch");
+}
+
+template <typename T>
+void append8(const T* k_new, const T* v_new, const int* slots, signed char* k_pool,
+             signed char* v_pool, float* k_scales, float* v_scales, int tokens, int hkv, int dim,
+             int blocks, int page, hipStream_t s) {
+    auto go = [&](auto v, auto ut) {
+        append8_run<T, decltype(v)::value, decltype(ut)::value>(
+            k_new, v_new, slots, k_pool, v_pool, k_scales, v_scales, tokens, hkv, dim, blocks,
+            page, s);
+    };
+    using I4 = std::integral_constant<int, 4>;
+    using I8 = std::integral_constant<int, 8>;
+    using Wave = std::integral_constant<int, 64>;
+    using Group = std::integral_constant<int, 256>;
+    auto aligned = [](const void* p, size_t by) { return (uintptr_t)p % by == 0; };
+    const bool eight = dim % 8 == 0 && aligned(k_new, 16) && aligned(v_new, 16) &&
+                       aligned(k_pool, 8) && aligned(v_pool, 8);
+    // a wave a unit where a block stays in its registers
+    const bool wave = page * (dim / (eight ? 8 : 4)) <= 4 * 64;
+    if (eight && wave) go(I8{}, Wave{});
+    else if (eight) go(I8{}, Group{});
+    else if (wave) go(I4{}, Wave{});
+    else go(I4{}, Group{});
 }
 
 // ---------------------------------------------------------------------------
@@ -260,8 +434,15 @@ __global__ __launch_bounds__(64) void kv_append8_kernel(
 // its tokens weigh nothing, and nothing is read for them.
 // ---------------------------------------------------------------------------
 
+// a / b for 0 <= a < 2^52, b > 0, by way of a float64 quotient (off by less
+// than one): a fifth of the instructions of a 64-bit division.
+__host__ __device__ __forceinline__ long long div64(long long a, long long b) {
+    const long long q = (long long)((double)a / (double)b), r = a - q * b;
+    return r < 0 ? q - 1 : r >= b ? q + 1 : q;
+}
+
 // Where the pieces of row (b, head) lie in the workspace: piece i at slot
-// at(i), `rows` q heads a slot. count 0: no token; -1: the row is stored
+// at(i), `tile` q heads a slot. count 0: no token; -1: the row is stored
 // already.
 struct Chunked8 {  // attn8_general: a slot per (row, chunk)
     int cmax, chunk;
@@ -270,7 +451,9 @@ struct Chunked8 {  // attn8_general: a slot per (row, chunk)
         int count;
         __device__ __forceinline__ size_t at(int i) const { return first + i; }
     };
-    __device__ __forceinline__ Row row(int b, int vrow, int vrows, int len) const {
+    __device__ __forceinline__ Row row(const int* lens, int span, int b, int vrow,
+                                       int vrows) const {
+        const int len = clamp_len(lens, b, span);
         return Row{((size_t)b * vrows + vrow) * cmax, (len + chunk - 1) / chunk};
     }
 };
@@ -286,58 +469,151 @@ struct Streamed8 {  // attn8_stream: two slots a segment (kernel comment)
             return (size_t)(2 * s + (end >= (s + 1) * seg ? 1 : 0));
         }
     };
-    __device__ __forceinline__ Row row(int b, int vrow, int vrows, int len) const {
-        const long long seg = pref[batch + 1], start = pref[b] * vrows + (long long)vrow * len;
+    __device__ __forceinline__ Row row(const int*, int, int b, int vrow, int vrows) const {
+        const long long seg = pref[batch + 1], p0 = pref[b], len = pref[b + 1] - p0;
+        const long long start = p0 * vrows + vrow * len;
         if (len == 0) return Row{0, 0, seg, 0};
-        const long long lo = start / seg, hi = (start + len - 1) / seg;
+        const long long lo = div64(start, seg), hi = div64(start + len - 1, seg);
         return Row{lo, start + len, seg, lo == hi ? -1 : (int)(hi - lo + 1)};
     }
 };
 
-// One workgroup per (sequence, q head).
+constexpr int kMaxPieces8 = 4096;  // of a row (their weights are kept in LDS)
+constexpr int kWavePieces8 = 32;   // folded by one wave, at most
+
+// `per` (1 or 4) q heads a workgroup, a wave each; a head of many pieces is
+// folded by the whole workgroup, afterwards. Bound by latency: the row's
+// place, its pieces' (m, l), their sums.
 template <typename T, typename Pieces>
 __global__ __launch_bounds__(256) void attn8_combine(
     const float* __restrict__ ws_ml, const float* __restrict__ ws_acc,
-    const int* __restrict__ lens, T* __restrict__ out, Pieces pieces, int hq, int hkv, int dim,
-    int span, int tile, int tiles) {
-    __shared__ float s_red[4];
+    const int* __restrict__ lens, T* __restrict__ out, Pieces pieces, int heads, int hq, int hkv,
+    int dim, int span, int tile, int tiles, int per) {
+    __shared__ float s_w[kMaxPieces8];
     __shared__ float4 s_acc[256];
-    const int tid = threadIdx.x, b = blockIdx.x / hq, hh = blockIdx.x - b * hq;
-    const int group = hq / hkv, kv = hh / group, gi = hh - kv * group, dc = dim / 4;
-    T* o = out + (size_t)blockIdx.x * dim;
-    const auto row = pieces.row(b, kv * tiles + gi / tile, hkv * tiles, clamp_len(lens, b, span));
-    const int np = row.count;
-    if (np < 0) return;
-    auto slot = [&](int i) { return row.at(i) * tile + gi % tile; };
-    float mx = -INFINITY;
-    for (int i = tid; i < np; i += 256) mx = fmaxf(mx, ws_ml[slot(i) * 2]);
-    mx = block_max<256>(mx, s_red);
-    auto weight = [&](int i) {
-        return ws_ml[slot(i) * 2 + 1] == 0.0f ? 0.0f : exp2f(ws_ml[slot(i) * 2] - mx);
+    __shared__ float s_max[4], s_sum[4];
+    __shared__ int s_many[4];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int group = hq / hkv, dc = dim / 4;
+    auto row_of = [&](int head) {
+        const int b = head / hq, hh = head - b * hq, kv = hh / group, gi = hh - kv * group;
+        return pieces.row(lens, span, b, kv * tiles + gi / tile, hkv * tiles);
     };
-    float l = 0.0f;
-    for (int i = tid; i < np; i += 256) l += weight(i) * ws_ml[slot(i) * 2 + 1];
-    l = block_sum<256>(l, s_red);
-    const int ng = 256 / dc, tg = tid / dc, d4 = tid - tg * dc;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (tg < ng) {
-#pragma unroll 4
-        for (int i = tg; i < np; i += ng) {
-            const float w = weight(i);
-            const float4 x = *reinterpret_cast<const float4*>(ws_acc + slot(i) * dim + 4 * d4);
-            a.x += w * x.x; a.y += w * x.y; a.z += w * x.z; a.w += w * x.w;
+    auto in_tile = [&](int head) { return head % hq % group % tile; };
+    const float2* const ml = reinterpret_cast<const float2*>(ws_ml);
+    // (a piece of no weight has l = 0)
+    auto weight = [&](float2 p, float mx) { return p.y == 0.0f ? 0.0f : exp2f(p.x - mx); };
+    auto store = [&](int head, int d4, float4 a, float l) {
+        if (l == 0.0f) a = make_float4(0.f, 0.f, 0.f, 0.f);
+        else a = make_float4(a.x / l, a.y / l, a.z / l, a.w / l);
+        St<T>::st4(out + (size_t)head * dim + 4 * d4, a);
+    };
+
+    {
+        const int head = blockIdx.x * per + wave;
+        bool many = false;
+        if (wave < per && head < heads) {
+            const auto row = row_of(head);
+            const int np = row.count, gi = in_tile(head);
+            many = np > kWavePieces8 || (np >= 0 && 64 % dc != 0);
+            if (!many && np >= 0) {
+                const size_t slot = row.at(min(lane, np)) * tile + gi;
+                const float2 p = lane < np ? ml[slot] : make_float2(-INFINITY, 0.0f);
+                const int grp = lane / dc, d4 = lane - grp * dc, ng = 64 / dc;
+                float4 x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {  // (under way before the weights are known)
+                    const int i = grp + k * ng;
+                    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (i < np)
+                        x[k] = *reinterpret_cast<const float4*>(
+                            ws_acc + (row.at(i) * tile + gi) * dim + 4 * d4);
+                }
+                const float mx = wave_max(p.x), w = weight(p, mx), l = wave_sum(w * p.y);
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                auto add = [&](int i, float4 v) {
+                    const float wi = __shfl(w, i & 63, 64);
+                    if (i < np) {
+                        a.x += wi * v.x; a.y += wi * v.y; a.z += wi * v.z; a.w += wi * v.w;
+                    }
+                };
+#pragma unroll
+                for (int k = 0; k < 4; ++k) add(grp + k * ng, x[k]);
+                for (int i0 = 4 * ng; i0 < np; i0 += ng) {
+                    const int i = i0 + grp;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (i < np)
+                        v = *reinterpret_cast<const float4*>(
+                            ws_acc + (row.at(i) * tile + gi) * dim + 4 * d4);
+                    add(i, v);
+                }
+                for (int o = dc; o < 64; o <<= 1) {
+                    a.x += __shfl_xor(a.x, o, 64);
+                    a.y += __shfl_xor(a.y, o, 64);
+                    a.z += __shfl_xor(a.z, o, 64);
+                    a.w += __shfl_xor(a.w, o, 64);
+                }
+                if (grp == 0) store(head, d4, a, l);
+            }
         }
+        if (lane == 0) s_many[wave] = many;
     }
-    s_acc[tid] = a;
     __syncthreads();
-    if (tg != 0) return;
-    for (int j = 1; j < ng; ++j) {
-        const float4 x = s_acc[j * dc + d4];
-        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+    for (int k = 0; k < per; ++k) {
+        if (!s_many[k]) continue;
+        const int head = blockIdx.x * per + k, gi = in_tile(head);
+        const auto row = row_of(head);
+        const int np = row.count, ng = 256 / dc, tg = tid / dc, d4 = tid - tg * dc;
+        auto at = [&](int i) { return row.at(i) * tile + gi; };
+        float mx = -INFINITY;
+        for (int i = tid; i < np; i += 256) mx = fmaxf(mx, ml[at(i)].x);
+        mx = wave_max(mx);
+        if (lane == 0) s_max[wave] = mx;
+        __syncthreads();
+        mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+        float l = 0.0f;
+        for (int i = tid; i < np; i += 256) {
+            const float2 p = ml[at(i)];
+            const float w = weight(p, mx);
+            s_w[i] = w;
+            l += w * p.y;
+        }
+        l = wave_sum(l);
+        if (lane == 0) s_sum[wave] = l;
+        __syncthreads();
+        l = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (tg < ng) {
+#pragma unroll 8
+            for (int i = tg; i < np; i += ng) {
+                const float w = s_w[i];
+                const float4 v = *reinterpret_cast<const float4*>(ws_acc + at(i) * dim + 4 * d4);
+                a.x += w * v.x; a.y += w * v.y; a.z += w * v.z; a.w += w * v.w;
+            }
+        }
+        s_acc[tid] = a;
+        __syncthreads();
+        if (tg == 0) {
+            for (int j = 1; j < ng; ++j) {
+                const float4 v = s_acc[j * dc + d4];
+                a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+            }
+            store(head, d4, a, l);
+        }
+        __syncthreads();  // LDS is the next head's
     }
-    if (l == 0.0f) a = make_float4(0.f, 0.f, 0.f, 0.f);
-    else a = make_float4(a.x / l, a.y / l, a.z / l, a.w / l);
-    St<T>::st4(o + 4 * d4, a);
+}
+
+template <typename T, typename Pieces>
+void combine8(const float* ml, const float* acc, const int* lens, T* out, const Pieces& pieces,
+              int batch, int hq, int hkv, int dim, int span, int tile, int tiles, hipStream_t s) {
+    const int heads = batch * hq;
+    // few heads have many pieces each: a workgroup a head
+    const int per = heads >= 4 * dev_info().cu_count && 256 % dim == 0 ? 4 : 1;
+    attn8_combine<T, Pieces><<<(unsigned)((heads + per - 1) / per), 256, 0, s>>>(
+        ml, acc, lens, out, pieces, heads, hq, hkv, dim, span, tile, tiles, per);
+    launch_check("int8 decode attention combine launch");
 }
 
 // ---------------------------------------------------------------------------
@@ -565,6 +841,30 @@ __device__ __forceinline__ f32x4_8 mma8(b16x8 a, b16x8 b, f32x4_8 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// The row that holds flat position pos (in units of 1 / vrows of the prefix):
+// the sequences' ends are counted 64 at a time, by the lanes.
+__device__ __forceinline__ StreamPiece piece8(const long long* s_pref, int batch, int vrows,
+                                              long long pos, long long seg_hi, int lane) {
+    int b = 0;
+    for (int step = (batch + 63) >> 6;; step = 1) {
+        const int at = b + (lane + 1) * step;
+        b += step * __popcll(__ballot(at <= batch && s_pref[min(at, batch)] * vrows <= pos));
+        if (step == 1) break;
+        // (the coarse count's last stretch may hold fewer than 64 sequences)
+    }
+    StreamPiece p;
+    p.b = b;
+    const long long pb = uniform64(s_pref[b]), base = pb * vrows;
+    const int len = (int)(uniform64(s_pref[b + 1]) - pb);
+    p.kv = (int)div64(pos - base, len);
+    p.t0 = (int)(pos - base - (long long)p.kv * len);
+    p.next = min(seg_hi, base + (long long)(p.kv + 1) * len);
+    p.n = (int)(p.next - pos);
+    p.whole = p.t0 == 0 && p.n == len;
+    p.row = b * vrows + p.kv;
+    return p;
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(Stream8<T, D>::kOcc, Stream8<T, D>::kOcc)))
@@ -589,8 +889,8 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
     __syncthreads();
     const int vrows = hkv * tiles;
     const long long total = uniform64(s_pref[batch]) * vrows;
-    long long S = max((total + nseg - 1) / nseg, (long long)min_seg);
-    S = (S + TOK - 1) / TOK * TOK;
+    long long S = max(div64(total + nseg - 1, nseg), (long long)min_seg);
+    S = (S + TOK - 1) & ~(long long)(TOK - 1);
     if (blockIdx.x == 0) {  // the combine's copy of the prefix, and S
         for (int i = tid; i <= batch; i += 256) pref_out[i] = s_pref[i];
         if (tid == 0) pref_out[batch + 1] = S;
@@ -617,7 +917,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
 
     long long pos = seg_lo;
     while (pos < seg_hi) {
-        const StreamPiece pc = stream_piece(s_pref, batch, vrows, pos, seg_hi);
+        const StreamPiece pc = piece8(s_pref, batch, vrows, pos, seg_hi, lane);
         const int b = pc.b, kv = pc.kv / tiles, t0 = pc.t0, n = pc.n;
         const int h0 = kv * (hq / hkv) + (pc.kv - kv * tiles) * tile;     // first q head
         const int heads = min(tile, (kv + 1) * (hq / hkv) - h0);
@@ -865,12 +1165,13 @@ Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int widt
         s.min_seg = kMinSeg8;
         const long long rows = (long long)std::min(batch, kStreamScanRows) * hkv * s.tiles;
         const long long most = rows * ((span + s.min_seg - 1) / s.min_seg);
-        s.nseg = (int)std::min((long long)4 * cus * occ, most);
+        s.nseg = (int)std::min(std::min((long long)4 * cus * occ, most), (long long)kMaxPieces8);
         s.slots = (size_t)2 * s.nseg * s.tile;
     } else {
         if (hkv > 65535 || batch > 65535) inval("attention: batch and kv heads must be <= 65535");
         // about 16 workgroups a CU, at least 256 tokens each
-        const long long units = std::max(1LL, 16LL * cus / ((long long)batch * hkv));
+        const long long units =
+            std::min((long long)kMaxPieces8, std::max(1LL, 16LL * cus / ((long long)batch * hkv)));
         s.chunk = (int)std::max(1LL, (span + units - 1) / units);
         s.chunk = (s.chunk + kGen8Step - 1) / kGen8Step * kGen8Step;
         s.cmax = (int)((span + s.chunk - 1) / s.chunk);
@@ -910,9 +1211,8 @@ void attn8_stream_run(const Attn8Shape& sh, const Attn8Args& a, float* ml, float
             nb, sh.hq, sh.hkv, sh.tile, sh.tiles, a.blocks, sh.page, shift, sh.width, sh.span,
             sh.nseg, sh.min_seg, scale);
         launch_check("int8 decode attention kernel launch");
-        attn8_combine<T, Streamed8><<<(unsigned)(nb * sh.hq), 256, 0, s>>>(
-            ml, acc, lens, out, Streamed8{pref, nb}, sh.hq, sh.hkv, D, sh.span, sh.tile, sh.tiles);
-        launch_check("int8 decode attention combine launch");
+        combine8(ml, acc, lens, out, Streamed8{pref, nb}, nb, sh.hq, sh.hkv, D, sh.span, sh.tile,
+                 sh.tiles, s);
     }
 }
 
@@ -935,10 +1235,8 @@ void attn8_run(const Attn8Shape& sh, const Attn8Args& a, hipStream_t s) {
             (1.0f / sqrtf((float)sh.dim)) * kLog2e);
         launch_check("int8 decode attention kernel launch");
     }
-    attn8_combine<T, Chunked8><<<(unsigned)(sh.batch * sh.hq), 256, 0, s>>>(
-        ml, acc, any ? a.lens : nullptr, (T*)a.out, Chunked8{sh.cmax, std::max(sh.chunk, 1)}, sh.hq,
-        sh.hkv, sh.dim, any ? sh.span : 0, sh.tile, sh.tiles);
-    launch_check("int8 decode attention combine launch");
+    combine8(ml, acc, any ? a.lens : nullptr, (T*)a.out, Chunked8{sh.cmax, std::max(sh.chunk, 1)},
+             sh.batch, sh.hq, sh.hkv, sh.dim, any ? sh.span : 0, sh.tile, sh.tiles, s);
 }
 
 }  // namespace
@@ -964,10 +1262,10 @@ int ft_block_table_extend_launch(int* table, const int* lens, const int* counts,
             (batch && (!lens || !counts || !lens_out || (tbl_width && !table))) ||
             (free_len && !free_blocks))
             inval("block_table_extend: null operand");
-        const unsigned grid = std::min(256u, grid_1d(tokens, 2048));
+        const unsigned grid = grid_1d(tokens, kExtendTokens, 4 * dev_info().cu_count);
         block_table_extend_kernel<<<grid, 256, 0, as_stream(stream)>>>(
             table, lens, counts, free_blocks, free_len, n_free, slots, positions, offsets,
-            lens_out, n_free_out, batch, page, tbl_width, tokens);
+            lens_out, n_free_out, batch, FastDiv(page), tbl_width, tokens);
         launch_check("block table kernel launch");
     });
 }
@@ -978,7 +1276,7 @@ int ft_kv_append_paged_int8_launch(const void* k_new, const void* v_new, int dty
                                    int dim, int blocks, int page, uintptr_t stream) {
     return guarded([&] {
         check_pools(blocks, kv_heads, page, dim);
-        if (tokens < 0 || kv_heads > 65535) inval("kv_append_paged_int8: tokens >= 0, heads <= 65535");
+        if (tokens < 0) inval("kv_append_paged_int8: tokens must be >= 0");
         if (dtype != FT_DT_F32 && dtype != FT_DT_BF16 && dtype != FT_DT_F16)
             inval("kv_append_paged_int8: unknown element type");
         if (tokens == 0 || blocks == 0) return;
@@ -988,17 +1286,17 @@ int ft_kv_append_paged_int8_launch(const void* k_new, const void* v_new, int dty
         check_aligned(v_new, 4 * size_of(dtype), "v_new");
         check_aligned(k_pool, 4, "k_pool");
         check_aligned(v_pool, 4, "v_pool");
+        if ((long long)tokens * kv_heads > (1LL << 30))
+            inval("kv_append_paged_int8: too many rows for one call");
         const hipStream_t s = as_stream(stream);
         auto go = [&](auto zero) {
             using T = decltype(zero);
-            kv_append8_kernel<T><<<dim3(tokens, kv_heads, 2), 64, 0, s>>>(
-                (const T*)k_new, (const T*)v_new, slots, k_pool, v_pool, k_scales, v_scales,
-                tokens, kv_heads, dim, blocks * page, page);
+            append8((const T*)k_new, (const T*)v_new, slots, k_pool, v_pool, k_scales, v_scales,
+                    tokens, kv_heads, dim, blocks, page, s);
         };
         if (dtype == FT_DT_F32) go(0.0f);
         else if (dtype == FT_DT_BF16) go((bf16)0.0f);
         else go((f16)0.0f);
-        launch_check("int8 kv append kernel launch");
     });
 }
 

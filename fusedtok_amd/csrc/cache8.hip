@@ -510,6 +510,63 @@ __global__ __launch_bounds__(256) void attn8_combine(
         St<T>::st4(out + (size_t)head * dim + 4 * d4, a);
     };
 
+    // one head by the whole workgroup
+    auto fold = [&](int head, const typename Pieces::Row& row) {
+        constexpr int kAhead = 8;
+        const int np = row.count, ng = 256 / dc, tg = tid / dc, d4 = tid - tg * dc;
+        const int gi = in_tile(head);
+        auto at = [&](int i) { return row.at(i) * tile + gi; };
+        auto piece = [&](int i) {
+            return tg < ng && i < np
+                       ? *reinterpret_cast<const float4*>(ws_acc + at(i) * dim + 4 * d4)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        const float2 p0 = tid < np ? ml[at(tid)] : make_float2(-INFINITY, 0.0f);
+        float4 x[kAhead];  // under way before the weights are known
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) x[k] = piece(tg + k * ng);
+        float mx = p0.x;
+        for (int i = tid + 256; i < np; i += 256) mx = fmaxf(mx, ml[at(i)].x);
+        mx = wave_max(mx);
+        if (lane == 0) s_max[wave] = mx;
+        __syncthreads();
+        mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+        float l = 0.0f;
+        for (int i = tid; i < np; i += 256) {
+            const float2 p = i == tid ? p0 : ml[at(i)];
+            const float w = weight(p, mx);
+            s_w[i] = w;
+            l += w * p.y;
+        }
+        l = wave_sum(l);
+        if (lane == 0) s_sum[wave] = l;
+        __syncthreads();
+        l = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](int i, float4 v) {
+            const float w = tg < ng && i < np ? s_w[i] : 0.0f;
+            a.x += w * v.x; a.y += w * v.y; a.z += w * v.z; a.w += w * v.w;
+        };
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) add(tg + k * ng, x[k]);
+#pragma unroll 4
+        for (int i = tg + kAhead * ng; i < np; i += ng) add(i, piece(i));
+        s_acc[tid] = a;
+        __syncthreads();
+        if (tg == 0) {
+            for (int j = 1; j < ng; ++j) {
+                const float4 v = s_acc[j * dc + d4];
+                a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+            }
+            store(head, d4, a, l);
+        }
+        __syncthreads();  // LDS is the next head's
+    };
+
+    if (per == 1) {
+        const auto row = row_of(blockIdx.x);
+        if (row.count > kWavePieces8) return fold(blockIdx.x, row);
+    }
     {
         const int head = blockIdx.x * per + wave;
         bool many = false;
@@ -560,49 +617,8 @@ __global__ __launch_bounds__(256) void attn8_combine(
         if (lane == 0) s_many[wave] = many;
     }
     __syncthreads();
-    for (int k = 0; k < per; ++k) {
-        if (!s_many[k]) continue;
-        const int head = blockIdx.x * per + k, gi = in_tile(head);
-        const auto row = row_of(head);
-        const int np = row.count, ng = 256 / dc, tg = tid / dc, d4 = tid - tg * dc;
-        auto at = [&](int i) { return row.at(i) * tile + gi; };
-        float mx = -INFINITY;
-        for (int i = tid; i < np; i += 256) mx = fmaxf(mx, ml[at(i)].x);
-        mx = wave_max(mx);
-        if (lane == 0) s_max[wave] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-        float l = 0.0f;
-        for (int i = tid; i < np; i += 256) {
-            const float2 p = ml[at(i)];
-            const float w = weight(p, mx);
-            s_w[i] = w;
-            l += w * p.y;
-        }
-        l = wave_sum(l);
-        if (lane == 0) s_sum[wave] = l;
-        __syncthreads();
-        l = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (tg < ng) {
-#pragma unroll 8
-            for (int i = tg; i < np; i += ng) {
-                const float w = s_w[i];
-                const float4 v = *reinterpret_cast<const float4*>(ws_acc + at(i) * dim + 4 * d4);
-                a.x += w * v.x; a.y += w * v.y; a.z += w * v.z; a.w += w * v.w;
-            }
-        }
-        s_acc[tid] = a;
-        __syncthreads();
-        if (tg == 0) {
-            for (int j = 1; j < ng; ++j) {
-                const float4 v = s_acc[j * dc + d4];
-                a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
-            }
-            store(head, d4, a, l);
-        }
-        __syncthreads();  // LDS is the next head's
-    }
+    for (int k = 0; k < per; ++k)
+        if (s_many[k]) fold(blockIdx.x * per + k, row_of(blockIdx.x * per + k));
 }
 
 template <typename T, typename Pieces>
@@ -874,8 +890,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                   const int* __restrict__ lens, float* __restrict__ ws_ml,
                   float* __restrict__ ws_acc, long long* __restrict__ pref_out,
                   T* __restrict__ out, int batch, int hq, int hkv, int tile, int tiles,
-                  int blocks, int page, int page_shift, int width, int span, int nseg, int min_seg,
-                  float scale_log2) {
+                  int blocks, FastDiv page, int width, int span, int nseg, int min_seg, float scale_log2) {
     using C = Stream8<T, D>;
     constexpr int TOK = C::kTok, NL = C::kLoads, SUB = TOK / 32, KE = D / 64;
     __shared__ __align__(16) char s_stage[4][C::kLds];
@@ -927,7 +942,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
         auto token = [&](int st) { return t0 + min(st * TOK + my, n - 1); };
         auto entry = [&](int st) {
             const int t = token(st);
-            return trow[page_shift >= 0 ? t >> page_shift : t / page];
+            return trow[page.div(t)];
         };
         u32x4 kt[NL], vt[NL];
         float ksn, vsn;
@@ -936,7 +951,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
             const int t = token(st);
             const bool held = (unsigned)ent < (unsigned)blocks;
             const unsigned bh = (unsigned)(held ? ent : 0) * hkv + kv;
-            const unsigned row = bh * page + (page_shift >= 0 ? t & (page - 1) : t % page);
+            const unsigned row = bh * page.d + page.mod(t);
             const bool ok = held && st * TOK + my < n;
             seen = __ballot(ok);
             const float ks = k_scales[bh], vs = v_scales[bh];
@@ -1197,9 +1212,6 @@ template <typename T, int D>
 void attn8_stream_run(const Attn8Shape& sh, const Attn8Args& a, float* ml, float* acc,
                       hipStream_t s) {
     long long* pref = (long long*)(acc + sh.slots * D);
-    int shift = -1;
-    if ((sh.page & (sh.page - 1)) == 0)
-        for (shift = 0; (1 << shift) < sh.page;) ++shift;
     const float scale = (1.0f / sqrtf((float)D)) * kLog2e;
     for (int b0 = 0; b0 < sh.batch; b0 += kStreamScanRows) {
         const int nb = std::min(kStreamScanRows, sh.batch - b0);
@@ -1208,7 +1220,7 @@ void attn8_stream_run(const Attn8Shape& sh, const Attn8Args& a, float* ml, float
         const int* lens = a.lens ? a.lens + b0 : nullptr;
         attn8_stream<T, D><<<(sh.nseg + 3) / 4, 256, 0, s>>>(
             q, a.kp, a.vp, a.ks, a.vs, a.table + (size_t)b0 * sh.width, lens, ml, acc, pref, out,
-            nb, sh.hq, sh.hkv, sh.tile, sh.tiles, a.blocks, sh.page, shift, sh.width, sh.span,
+            nb, sh.hq, sh.hkv, sh.tile, sh.tiles, a.blocks, FastDiv(sh.page), sh.width, sh.span,
             sh.nseg, sh.min_seg, scale);
         launch_check("int8 decode attention kernel launch");
         combine8(ml, acc, lens, out, Streamed8{pref, nb}, nb, sh.hq, sh.hkv, D, sh.span, sh.tile,

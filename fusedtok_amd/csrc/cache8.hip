@@ -772,10 +772,10 @@ __global__ __launch_bounds__(256) void attn8_general(
 // one of each. Waves share nothing but the length prefix, so after it there
 // is no barrier and no merge in the kernel.
 //
-// A step is TOK tokens (32; 64 for D = 64), K and V of the next one in flight
-// in registers while this one is computed from the wave's own LDS staging.
-// With r = lane % 16, g = lane / 16 (v_mfma_f32_16x16x32_bf16: A[r][8g+i],
-// B[8g+i][r], C[4g+i][r]):
+// A step is TOK tokens (32; 64 for D = 64), K and V of the next one - of the
+// next piece at a piece's end - in flight in registers while this one is
+// computed from the wave's own LDS staging. With r = lane % 16, g = lane / 16
+// (v_mfma_f32_16x16x32_bf16: A[r][8g+i], B[8g+i][r], C[4g+i][r]):
 //
 //  loads    whole 128-byte lines per instruction, non-temporal, of rows whose
 //           places the lanes have worked out from the table (a lane a token)
@@ -783,17 +783,22 @@ __global__ __launch_bounds__(256) void attn8_general(
 //  scores   S^T[tok][head] = K . Q^T. Codes become bf16 (exact: 8 bits); q
 //           goes in as 1, 2 or 3 bf16 parts (bf16, fp16, float32: all its
 //           bits), so every product is exact and sums are float32. Any order
-//           of dims serves if q has the same: the lane reads 16-byte chunks;
+//           of dims serves if q has the same: the lane reads 16-byte chunks.
+//           (Integer products with q in base-256 digits take 56 vector
+//           instructions a step less, but the loop waits on memory either way
+//           and the digits cost every piece 3-7 us at its start);
 //  softmax  lane (r, g) holds head r's scores of tokens 4g+i (+ 16 a tile);
 //           scaled by the block's K scale, running maximum over the 4 lanes
 //           of a head; the weight takes the block's V scale, then goes into 2
 //           bf16 parts (3 for float32 outputs), which hold any float's
-//           magnitude: small weights count as they weigh;
-//  PV       O^T[dim][head] = V^T . W^T. The weights are where B wants them; for
-//           A, lane (r, g) reads dims (D/16) r .. of its 8 tokens from the
-//           staging and pairs the tokens up while it widens them, so the
-//           transpose costs nothing. Lane (r, g) ends with D/4 consecutive
-//           dims of head r.
+//           magnitude: small weights count as they weigh. (Groups of up to 4
+//           heads could fill the 16 columns with copies that share the tokens
+//           out: a quarter of the exponentials, and 1-2% of the time.);
+//  PV       O^T[dim][head] = V^T . W^T, codes widened to bf16 (exact). The
+//           weights are where B wants them; for A, lane (r, g) reads dims
+//           (D/16) r .. of its 8 tokens from the staging and pairs the tokens
+//           up while it widens them, so the transpose costs nothing. Lane
+//           (r, g) ends with D/4 consecutive dims of head r.
 //
 // Masked tokens (behind the piece, holes) weigh 0 exactly: score -inf, V scale
 // 0, the row read in its place a real one (its own last, or block 0's).
@@ -801,7 +806,6 @@ __global__ __launch_bounds__(256) void attn8_general(
 typedef float f32x4_8 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 template <typename T, int D>
 struct Stream8 {
@@ -809,10 +813,10 @@ struct Stream8 {
     static constexpr int kLoads = kTok * D / 1024;   // 16-byte loads a lane and pool
     static constexpr int kRowsPer = 1024 / D;        // rows a load instruction covers
     static constexpr int kChunks = D / 16;           // 16-byte chunks of a row
-    static constexpr int kQ = std::is_same<T, float>::value ? 3 : std::is_same<T, f16>::value ? 2 : 1;
     static constexpr int kW = std::is_same<T, float>::value ? 3 : 2;  // weight parts
-    static constexpr int kOcc = D == 256 ? 1 : std::is_same<T, float>::value ? 2 : 3;  // waves a SIMD
+    static constexpr int kOcc = D == 256 ? 1 : 2;    // waves a SIMD
     static constexpr int kLds = 2 * kTok * D + 8 * kTok;  // bytes a wave
+    static constexpr int kQ = std::is_same<T, float>::value ? 3 : std::is_same<T, f16>::value ? 2 : 1;  // q parts
 };
 
 // upper halves of two float32 (as two bf16, truncated)
@@ -831,36 +835,22 @@ __device__ __forceinline__ b16x8 widen8(unsigned a, unsigned b) {
     o[3] = pack_hi(byte_f(b, 2), byte_f(b, 3));
     return __builtin_bit_cast(b16x8, o);
 }
-// x[8] as N bf16 parts, each truncated, the first the largest (an infinity
-// leaves NaN behind it: only a scale that is not finite makes one).
-template <int N>
-__device__ __forceinline__ void split8(const float (&x)[8], b16x8 (&part)[N]) {
-    float rest[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) rest[i] = x[i];
-#pragma unroll
-    for (int p = 0; p < N; ++p) {
-        u32x4 o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = pack_hi(rest[2 * i], rest[2 * i + 1]);
-        part[p] = __builtin_bit_cast(b16x8, o);
-        if (p + 1 < N) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float hi = __uint_as_float(__float_as_uint(rest[i]) & 0xffff0000u);
-                rest[i] -= hi;
-            }
-        }
-    }
-}
-__device__ __forceinline__ f32x4_8 mma8(b16x8 a, b16x8 b, f32x4_8 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
+// A stretch of one row (b, virtual head kv): tokens [t0, t0 + n), up to flat
+// position next. (No padding: the compiler keeps a copied struct's padding in
+// LDS, and to place it reads the workgroup's size from the dispatch packet in
+// host memory, 3-7 us at the kernel's start.)
+struct Piece8 {
+    long long next;
+    int b, kv, t0, n;
+    int whole;  // the row's every token
+    int heads;  // q heads of the row
+};
 
 // The row that holds flat position pos (in units of 1 / vrows of the prefix):
 // the sequences' ends are counted 64 at a time, by the lanes.
-__device__ __forceinline__ StreamPiece piece8(const long long* s_pref, int batch, int vrows,
-                                              long long pos, long long seg_hi, int lane) {
+__device__ __forceinline__ Piece8 piece8(const long long* s_pref, int batch, int vrows,
+                                         long long pos, long long seg_hi, int lane, int group,
+                                         int tile, int tiles) {
     int b = 0;
     for (int step = (batch + 63) >> 6;; step = 1) {
         const int at = b + (lane + 1) * step;
@@ -868,7 +858,7 @@ __device__ __forceinline__ StreamPiece piece8(const long long* s_pref, int batch
         if (step == 1) break;
         // (the coarse count's last stretch may hold fewer than 64 sequences)
     }
-    StreamPiece p;
+    Piece8 p;
     p.b = b;
     const long long pb = uniform64(s_pref[b]), base = pb * vrows;
     const int len = (int)(uniform64(s_pref[b + 1]) - pb);
@@ -877,7 +867,7 @@ __device__ __forceinline__ StreamPiece piece8(const long long* s_pref, int batch
     p.next = min(seg_hi, base + (long long)(p.kv + 1) * len);
     p.n = (int)(p.next - pos);
     p.whole = p.t0 == 0 && p.n == len;
-    p.row = b * vrows + p.kv;
+    p.heads = min(tile, group - p.kv % tiles * tile);
     return p;
 }
 
@@ -890,7 +880,8 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                   const int* __restrict__ lens, float* __restrict__ ws_ml,
                   float* __restrict__ ws_acc, long long* __restrict__ pref_out,
                   T* __restrict__ out, int batch, int hq, int hkv, int tile, int tiles,
-                  int blocks, FastDiv page, int width, int span, int nseg, int min_seg, float scale_log2) {
+                  int blocks, FastDiv page, int width, int span, int nseg, int min_seg,
+                  float scale_log2) {
     using C = Stream8<T, D>;
     constexpr int TOK = C::kTok, NL = C::kLoads, SUB = TOK / 32, KE = D / 64;
     __shared__ __align__(16) char s_stage[4][C::kLds];
@@ -902,7 +893,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
     const int r = lane & 15, g = lane >> 4;
     if (wave == 0) scan_lengths(lens, batch, span, lane, s_pref, s_mm);
     __syncthreads();
-    const int vrows = hkv * tiles;
+    const int vrows = hkv * tiles, group = hq / hkv;
     const long long total = uniform64(s_pref[batch]) * vrows;
     long long S = max(div64(total + nseg - 1, nseg), (long long)min_seg);
     S = (S + TOK - 1) & ~(long long)(TOK - 1);
@@ -929,64 +920,87 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
     auto v_at = [&](int w) { return ((w & ~15) | ((w & 3) << 2) | ((w >> 2) & 3)) * D; };
     const int my = lane & (TOK - 1);                 // the lane's token of a step
     const int lc = lane % C::kChunks, lr = lane / C::kChunks;  // its place in a load
+    // the lane's i-th score of 32 tokens is that of token at(i)
+    auto at = [&](int i) { return 16 * (i >> 2) + 4 * g + (i & 3); };
 
-    long long pos = seg_lo;
-    while (pos < seg_hi) {
-        const StreamPiece pc = piece8(s_pref, batch, vrows, pos, seg_hi, lane);
-        const int b = pc.b, kv = pc.kv / tiles, t0 = pc.t0, n = pc.n;
-        const int h0 = kv * (hq / hkv) + (pc.kv - kv * tiles) * tile;     // first q head
-        const int heads = min(tile, (kv + 1) * (hq / hkv) - h0);
-        const int* trow = table + (size_t)b * width;
-        const int nsteps = (n + TOK - 1) / TOK;
-
-        auto token = [&](int st) { return t0 + min(st * TOK + my, n - 1); };
-        auto entry = [&](int st) {
-            const int t = token(st);
-            return trow[page.div(t)];
-        };
-        u32x4 kt[NL], vt[NL];
-        float ksn, vsn;
-        unsigned long long seen;  // lanes whose token of the loaded step counts
-        auto issue = [&](int st, int ent) {
-            const int t = token(st);
-            const bool held = (unsigned)ent < (unsigned)blocks;
-            const unsigned bh = (unsigned)(held ? ent : 0) * hkv + kv;
-            const unsigned row = bh * page.d + page.mod(t);
-            const bool ok = held && st * TOK + my < n;
-            seen = __ballot(ok);
-            const float ks = k_scales[bh], vs = v_scales[bh];
-            ksn = ok ? ks * scale_log2 : 0.0f;
-            vsn = ok ? vs : 0.0f;
+    // ---- a step's loads ------------------------------------------------------
+    auto steps = [&](const Piece8& p) { return (p.n + TOK - 1) / TOK; };
+    auto token = [&](const Piece8& p, int st) { return p.t0 + min(st * TOK + my, p.n - 1); };
+    auto entry = [&](const Piece8& p, int st) {
+        return table[(size_t)p.b * width + page.div(token(p, min(st, steps(p) - 1)))];
+    };
+    u32x4 kt[NL], vt[NL];
+    float ksn, vsn;
+    unsigned long long seen;  // lanes whose token of the loaded step counts
+    auto issue = [&](const Piece8& p, int st, int ent) {
+        const int t = token(p, st);
+        const bool held = (unsigned)ent < (unsigned)blocks;
+        const unsigned bh = (unsigned)(held ? ent : 0) * hkv + p.kv / tiles;
+        const unsigned row = bh * page.d + page.mod(t);
+        const bool ok = held && st * TOK + my < p.n;
+        seen = __ballot(ok);
+        ksn = k_scales[bh];  // (not touched before the step is staged: a use here
+        vsn = v_scales[bh];  // would wait for loads behind them, at a join)
 #pragma unroll
-            for (int p = 0; p < NL; ++p) {
-                const unsigned rw = __shfl(row, C::kRowsPer * p + lr, 64);
-                const size_t off = (size_t)rw * D + 16 * lc;
-                kt[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k_pool + off));
-                vt[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v_pool + off));
-            }
-        };
+        for (int i = 0; i < NL; ++i) {
+            const unsigned rw = __shfl(row, C::kRowsPer * i + lr, 64);
+            const size_t off = (size_t)rw * D + 16 * lc;
+            kt[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k_pool + off));
+            vt[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v_pool + off));
+        }
+    };
+    // ---- a row's q: column r's dims 64 e + 16 g .. + 15 ----------------------
+    auto first_head = [&](const Piece8& p) {
+        const int kv = p.kv / tiles;
+        return kv * group + (p.kv - kv * tiles) * tile;
+    };
+    typedef T tx8 __attribute__((ext_vector_type(8)));
+    tx8 qx[KE][2];
+    auto load_q = [&](const Piece8& p) {
+        const T* row = q + ((size_t)p.b * hq + first_head(p) + (r < p.heads ? r : 0)) * D;
+#pragma unroll
+        for (int e = 0; e < KE; ++e)
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+                qx[e][f] = *reinterpret_cast<const tx8*>(row + 64 * e + 16 * g + 8 * f);
+    };
 
-        int ent = entry(0);
-        // B operand of the score products: Q[head r], parts
+    Piece8 pc = piece8(s_pref, batch, vrows, seg_lo, seg_hi, lane, group, tile, tiles);
+    int ent = entry(pc, 0);
+    load_q(pc);
+    issue(pc, 0, ent);
+    ent = entry(pc, 1);
+
+    for (;;) {
+        const int nsteps = steps(pc);
+        const bool more = pc.next < seg_hi;
+        Piece8 nx = pc;
+        // B operand of the score products: q in parts, each truncated
         b16x8 qf[KE][2][C::kQ];
-        {
-            const T* qrow = q + ((size_t)b * hq + h0 + (r < heads ? r : 0)) * D;
 #pragma unroll
-            for (int e = 0; e < KE; ++e)
+        for (int e = 0; e < KE; ++e)
 #pragma unroll
-                for (int f = 0; f < 2; ++f) {
+            for (int f = 0; f < 2; ++f) {
+                if constexpr (C::kQ == 1) {
+                    qf[e][f][0] = qx[e][f];
+                } else {
                     float x[8];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float4 y = St<T>::ld4(qrow + 64 * e + 16 * g + 8 * f + 4 * i);
-                        x[4 * i] = y.x; x[4 * i + 1] = y.y; x[4 * i + 2] = y.z; x[4 * i + 3] = y.w;
+                    for (int i = 0; i < 8; ++i) x[i] = (float)qx[e][f][i];
+#pragma unroll
+                    for (int p = 0; p < C::kQ; ++p) {
+                        u32x4 o;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[i] = pack_hi(x[2 * i], x[2 * i + 1]);
+                        qf[e][f][p] = __builtin_bit_cast(b16x8, o);
+                        if (p + 1 < C::kQ) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                x[i] -= __uint_as_float(__float_as_uint(x[i]) & 0xffff0000u);
+                        }
                     }
-                    split8<C::kQ>(x, qf[e][f]);
                 }
-        }
-        issue(0, ent);
-        ent = entry(min(1, nsteps - 1));
-
+            }
         f32x4_8 acc[C::kChunks];
 #pragma unroll
         for (int i = 0; i < C::kChunks; ++i) acc[i] = f32x4_8{0.f, 0.f, 0.f, 0.f};
@@ -996,51 +1010,63 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
             // ---- this step into the staging, the next one on its way -------
             wave_lds_order();  // (the step before has read it)
 #pragma unroll
-            for (int p = 0; p < NL; ++p) {
-                const int w = C::kRowsPer * p + lr;
-                *reinterpret_cast<u32x4*>(sk + k_at(w, lc)) = kt[p];
-                *reinterpret_cast<u32x4*>(sv + v_at(w) + 16 * lc) = vt[p];
+            for (int i = 0; i < NL; ++i) {
+                const int w = C::kRowsPer * i + lr;
+                *reinterpret_cast<u32x4*>(sk + k_at(w, lc)) = kt[i];
+                *reinterpret_cast<u32x4*>(sv + v_at(w) + 16 * lc) = vt[i];
             }
-            if (TOK == 64 || lane < 32) ss[my] = make_float2(ksn, vsn);
             const unsigned long long now = seen;
+            if (TOK == 64 || lane < 32) {
+                const bool ok = now >> lane & 1;
+                ss[my] = make_float2(ok ? ksn * scale_log2 : 0.0f, ok ? vsn : 0.0f);
+            }
             wave_lds_order();
             if (st + 1 < nsteps) {
                 const int e = ent;
-                ent = entry(min(st + 2, nsteps - 1));
-                issue(st + 1, e);
+                ent = entry(pc, st + 2);
+                issue(pc, st + 1, e);
+            } else if (more) {
+                nx = piece8(s_pref, batch, vrows, pc.next, seg_hi, lane, group, tile, tiles);
+                const int e = entry(nx, 0);
+                ent = entry(nx, 1);
+                issue(nx, 0, e);
             }
             __builtin_amdgcn_sched_barrier(0);
 
             // ---- scores ------------------------------------------------------
             float x[8 * SUB], vsc[8 * SUB];
 #pragma unroll
-            for (int h = 0; h < 2 * SUB; ++h) {
-                f32x4_8 s = {0.f, 0.f, 0.f, 0.f};
+            for (int u = 0; u < SUB; ++u) {
 #pragma unroll
-                for (int e = 0; e < KE; ++e) {
-                    const u32x4 kc = *reinterpret_cast<const u32x4*>(sk + k_at(16 * h + r, 4 * e + g));
+                for (int h = 0; h < 2; ++h) {
+                    f32x4_8 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int f = 0; f < 2; ++f) {
-                        const b16x8 a = widen8(kc[2 * f], kc[2 * f + 1]);
+                    for (int e = 0; e < KE; ++e) {
+                        const u32x4 kc = *reinterpret_cast<const u32x4*>(
+                            sk + k_at(32 * u + 16 * h + r, 4 * e + g));
 #pragma unroll
-                        for (int p = C::kQ - 1; p >= 0; --p) s = mma8(a, qf[e][f][p], s);
+                        for (int f = 0; f < 2; ++f) {
+                            const b16x8 a = widen8(kc[2 * f], kc[2 * f + 1]);
+#pragma unroll
+                            for (int p = C::kQ - 1; p >= 0; --p)
+                                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[e][f][p], c, 0,
+                                                                            0, 0);
+                        }
                     }
-                }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 sc = ss[16 * h + 4 * g + i];
-                    x[4 * h + i] = s[i] * sc.x;
-                    vsc[4 * h + i] = sc.y;
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 sc = ss[32 * u + at(4 * h + i)];
+                        x[8 * u + 4 * h + i] = c[i] * sc.x;
+                        vsc[8 * u + 4 * h + i] = sc.y;
+                    }
                 }
             }
             if (now != ~0ull) {
 #pragma unroll
-                for (int h = 0; h < 2 * SUB; ++h) {
-                    const unsigned bits = (unsigned)(now >> (16 * h + 4 * g));
+                for (int u = 0; u < SUB; ++u)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!(bits >> i & 1)) x[4 * h + i] = -INFINITY;
-                }
+                    for (int i = 0; i < 8; ++i)
+                        if (!(now >> (32 * u + at(i)) & 1)) x[8 * u + i] = -INFINITY;
             }
             // ---- running softmax ---------------------------------------------
             float top = x[0];
@@ -1065,8 +1091,22 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                     l_run += p;
                     w[i] = p * vsc[8 * u + i];
                 }
+                // bf16 parts, each truncated, the first the largest (an
+                // infinity, which only a scale that is not finite makes,
+                // leaves NaN behind it)
                 b16x8 wp[C::kW];
-                split8<C::kW>(w, wp);
+#pragma unroll
+                for (int p = 0; p < C::kW; ++p) {
+                    u32x4 o;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = pack_hi(w[2 * i], w[2 * i + 1]);
+                    wp[p] = __builtin_bit_cast(b16x8, o);
+                    if (p + 1 < C::kW) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            w[i] -= __uint_as_float(__float_as_uint(w[i]) & 0xffff0000u);
+                    }
+                }
                 const char* vr[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -1086,19 +1126,19 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                         const b16x8 a = __builtin_bit_cast(b16x8, o);
 #pragma unroll
                         for (int p = C::kW - 1; p >= 0; --p)
-                            acc[4 * j + d] = mma8(a, wp[p], acc[4 * j + d]);
+                            acc[4 * j + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                a, wp[p], acc[4 * j + d], 0, 0, 0);
                     }
                 }
             }
         }
-
         // ---- the row, or its partial -----------------------------------------
         l_run += __shfl_xor(l_run, 16, 64);
         l_run += __shfl_xor(l_run, 32, 64);
-        if (r < heads) {
+        if (r < pc.heads) {
             // dims (D/4) g + (D/16) i + d of head r: acc[d][i]
             if (pc.whole) {
-                T* o = out + ((size_t)b * hq + h0 + r) * D + (D / 4) * g;
+                T* o = out + ((size_t)pc.b * hq + first_head(pc) + r) * D + (D / 4) * g;
                 const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -1115,9 +1155,9 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                         St<T>::st4(o + (D / 16) * i + d, make_float4(y[0], y[1], y[2], y[3]));
                     }
             } else {
-                const long long end = uniform64(s_pref[b]) * vrows +
-                                      (long long)(pc.kv + 1) * (uniform64(s_pref[b + 1]) -
-                                                                uniform64(s_pref[b]));
+                const long long pb = uniform64(s_pref[pc.b]);
+                const long long end =
+                    pb * vrows + (pc.kv + 1) * (uniform64(s_pref[pc.b + 1]) - pb);
                 const size_t slot =
                     (2 * (size_t)seg + (end >= seg_lo + S ? 1 : 0)) * tile + r;
                 float* o = ws_acc + slot * D + (D / 4) * g;
@@ -1133,7 +1173,9 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                 }
             }
         }
-        pos = pc.next;
+        if (!more) break;
+        load_q(nx);
+        pc = nx;
     }
 }
 
@@ -1152,8 +1194,7 @@ constexpr int kMinSeg8 = 64;  // tokens of a segment, at least
 
 template <int D>
 int stream_occ(int dtype) {
-    return dtype == FT_DT_F32 ? Stream8<float, D>::kOcc
-                              : dtype == FT_DT_F16 ? Stream8<f16, D>::kOcc : Stream8<bf16, D>::kOcc;
+    return dtype == FT_DT_F32 ? Stream8<float, D>::kOcc : Stream8<bf16, D>::kOcc;
 }
 
 Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int width, int dim) {
@@ -1333,8 +1374,8 @@ int ft_attention_decode_paged_int8_launch(const void* q, int dtype, const signed
         const size_t by = dim % 16 == 0 ? 16 : 4;
         check_aligned(k_pool, by, "k_pool");
         check_aligned(v_pool, by, "v_pool");
-        check_aligned(q, 4 * size_of(dtype), "q");
-        check_aligned(out, 4 * size_of(dtype), "out");
+        check_aligned(q, std::max(by, 4 * size_of(dtype)), "q");
+        check_aligned(out, std::max(by, 4 * size_of(dtype)), "out");
         check_aligned(workspace, 16, "the workspace");
         const Attn8Shape sh =
             attn8_shape(dtype, batch, q_heads, kv_heads, page, tbl_width, dim);

@@ -765,8 +765,10 @@ __global__ __launch_bounds__(256) void attn8_general(
 //
 // Work split. The rows are (sequence b, kv head, tile of up to 16 q heads),
 // b-major, len_b tokens each, laid end to end; every WAVE takes one equal
-// contiguous segment of that range, whatever the length mix. A segment is one
-// or more pieces, one per row it touches. A piece that is a whole row is
+// contiguous segment of that range, whatever the length mix; where kMinSeg8
+// tokens a segment leave waves over, each row is rounded up to whole segments,
+// so that none has two rows. A segment is one or more pieces, one per row it
+// touches. A piece that is a whole row is
 // normalised and stored; another leaves its partial in the segment's slot 1
 // if its row reaches the segment's end, else in slot 0: a segment has at most
 // one of each. Waves share nothing but the length prefix, so after it there
@@ -835,6 +837,31 @@ __device__ __forceinline__ b16x8 widen8(unsigned a, unsigned b) {
     o[3] = pack_hi(byte_f(b, 2), byte_f(b, 3));
     return __builtin_bit_cast(b16x8, o);
 }
+// Exclusive prefix of the clamped lengths, each rounded up to a multiple of
+// `to` (a power of two), by one wave.
+__device__ __forceinline__ void scan8(const int* __restrict__ lens, int batch, int span, int lane,
+                                      int to, long long* pref) {
+    const int per = (batch + 63) >> 6, b0 = lane * per;
+    auto len = [&](int i) {
+        return b0 + i < batch ? (clamp_len(lens, b0 + i, span) + to - 1) & -to : 0;
+    };
+    long long sum = 0;
+    for (int i = 0; i < per; ++i) sum += len(i);
+    long long incl = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long long y = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += y;
+    }
+    long long at = incl - sum;
+    for (int i = 0; i < per; ++i) {
+        const int n = len(i);
+        if (b0 + i < batch) pref[b0 + i] = at;
+        at += n;
+    }
+    if (lane == 63) pref[batch] = incl;
+}
+
 // A stretch of one row (b, virtual head kv): tokens [t0, t0 + n), up to flat
 // position next. (No padding: the compiler keeps a copied struct's padding in
 // LDS, and to place it reads the workgroup's size from the dispatch packet in
@@ -850,7 +877,7 @@ struct Piece8 {
 // the sequences' ends are counted 64 at a time, by the lanes.
 __device__ __forceinline__ Piece8 piece8(const long long* s_pref, int batch, int vrows,
                                          long long pos, long long seg_hi, int lane, int group,
-                                         int tile, int tiles) {
+                                         int tile, int tiles, const int* lens, int span) {
     int b = 0;
     for (int step = (batch + 63) >> 6;; step = 1) {
         const int at = b + (lane + 1) * step;
@@ -865,8 +892,10 @@ __device__ __forceinline__ Piece8 piece8(const long long* s_pref, int batch, int
     p.kv = (int)div64(pos - base, len);
     p.t0 = (int)(pos - base - (long long)p.kv * len);
     p.next = min(seg_hi, base + (long long)(p.kv + 1) * len);
-    p.n = (int)(p.next - pos);
-    p.whole = p.t0 == 0 && p.n == len;
+    // (the prefix may be of padded lengths)
+    const int end = __builtin_amdgcn_readfirstlane(clamp_len(lens, b, span));
+    p.n = min((int)(p.next - pos), end - p.t0);
+    p.whole = p.t0 == 0 && p.n == end;
     p.heads = min(tile, group - p.kv % tiles * tile);
     return p;
 }
@@ -885,18 +914,25 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
     using C = Stream8<T, D>;
     constexpr int TOK = C::kTok, NL = C::kLoads, SUB = TOK / 32, KE = D / 64;
     __shared__ __align__(16) char s_stage[4][C::kLds];
-    __shared__ long long s_pref[kStreamScanRows + 1];
-    __shared__ int s_mm[2];
+    __shared__ long long s_prefix[2][kStreamScanRows + 1];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
-    if (wave == 0) scan_lengths(lens, batch, span, lane, s_pref, s_mm);
+    if (wave < 2) scan8(lens, batch, span, lane, wave ? min_seg : 1, s_prefix[wave]);
     __syncthreads();
     const int vrows = hkv * tiles, group = hq / hkv;
-    const long long total = uniform64(s_pref[batch]) * vrows;
-    long long S = max(div64(total + nseg - 1, nseg), (long long)min_seg);
-    S = (S + TOK - 1) & ~(long long)(TOK - 1);
+    long long total = uniform64(s_prefix[0][batch]) * vrows, S = min_seg;
+    const long long padded = uniform64(s_prefix[1][batch]) * vrows;
+    // few tokens: a segment a stretch of min_seg tokens of one row
+    const bool few = padded <= (long long)nseg * min_seg;
+    const long long* const s_pref = s_prefix[few];
+    if (few) {
+        total = padded;
+    } else {
+        S = max(div64(total + nseg - 1, nseg), (long long)min_seg);
+        S = (S + TOK - 1) & ~(long long)(TOK - 1);
+    }
     if (blockIdx.x == 0) {  // the combine's copy of the prefix, and S
         for (int i = tid; i <= batch; i += 256) pref_out[i] = s_pref[i];
         if (tid == 0) pref_out[batch + 1] = S;
@@ -965,7 +1001,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                 qx[e][f] = *reinterpret_cast<const tx8*>(row + 64 * e + 16 * g + 8 * f);
     };
 
-    Piece8 pc = piece8(s_pref, batch, vrows, seg_lo, seg_hi, lane, group, tile, tiles);
+    Piece8 pc = piece8(s_pref, batch, vrows, seg_lo, seg_hi, lane, group, tile, tiles, lens, span);
     int ent = entry(pc, 0);
     load_q(pc);
     issue(pc, 0, ent);
@@ -1026,7 +1062,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                 ent = entry(pc, st + 2);
                 issue(pc, st + 1, e);
             } else if (more) {
-                nx = piece8(s_pref, batch, vrows, pc.next, seg_hi, lane, group, tile, tiles);
+                nx = piece8(s_pref, batch, vrows, pc.next, seg_hi, lane, group, tile, tiles, lens, span);
                 const int e = entry(nx, 0);
                 ent = entry(nx, 1);
                 issue(nx, 0, e);
@@ -1190,7 +1226,10 @@ struct Attn8Shape {
     size_t slots, bytes;             // slots: (partial, q head) pairs
 };
 
-constexpr int kMinSeg8 = 64;  // tokens of a segment, at least
+// Tokens of a segment, at least (a power of two, whole steps): 7 ragged rows of
+// up to 9001 tokens, float32, 12.4 us of kernel time at 64 or 128, 18.9 at 32
+// (which leaves no wave over); 4 short rows, D = 64, 5.8 at 64, 7.1 at 128.
+constexpr int kMinSeg8 = 64;
 
 template <int D>
 int stream_occ(int dtype) {

@@ -47,6 +47,8 @@ decode-chain steps ``rmsnorm_quant``, ``rmsnorm_qgemm``, ``swiglu_quant``
 and ``rope_kv_append_paged`` (GPU tensors only).
 """
 
+import functools
+
 import numpy as np
 
 # torch first: its bundled HIP runtime (libamdhip64.so, soname
@@ -534,13 +536,6 @@ _I32 = (torch.int32,)
 _F32 = (torch.float32,)
 _POOL8_MISMATCH = "k_pool and v_pool must be int8 [Nb, Hkv, P, D] of one shape"
 _SCALE8_MISMATCH = "k_scales and v_scales must be float32 [Nb, Hkv]"
-_PAGE8 = _Rule(lambda c: 1 <= c.P <= 1024, "page must be in [1, 1024]")
-_DIM8 = _Rule(lambda c: c.D % 4 == 0 and 4 <= c.D <= 512,
-              "dim must be a multiple of 4 and at most 512")
-_NUM_SLOTS8 = _Rule(lambda c: c.Nb * c.P < 2 ** 31 and c.Nb * c.P * c.Hkv < 2 ** 32,
-                    "the cache has too many rows (slots must fit 31 bits, rows 32)")
-
-
 def _pools8(inplace):
     return (_Arr("k_pool", "Nb Hkv P D", _INT8, inplace=inplace, mismatch=_POOL8_MISMATCH),
             _Arr("v_pool", "=k_pool", _INT8, inplace=inplace, mismatch=_POOL8_MISMATCH),
@@ -548,14 +543,14 @@ def _pools8(inplace):
             _Arr("v_scales", "Nb Hkv", _F32, inplace=inplace, mismatch=_SCALE8_MISMATCH))
 
 
-def _one_device(c):
-    """Every operand on the primary one's device; True when that is also the
-    current one (else the op runs again under it, on its current stream)."""
-    dev = c.device
-    for name, v in c._values.items():
-        if isinstance(v, torch.Tensor) and v.is_cuda and v.device != dev:
-            raise ValueError(f"{name} is on {v.device}, another operand on {dev}")
-    return dev.index == _current_device()
+def _one_device(names, tensors):
+    """Every operand on one device; True when that is also the current one
+    (else the op runs again under it, on its current stream)."""
+    at = [t.get_device() for t in tensors]
+    if at.count(at[0]) != len(at):
+        raise ValueError("operands are on different devices: " +
+                         ", ".join(f"{n} on {d}" for n, d in zip(names, at)))
+    return at[0] == _current_device()
 
 
 _EXTEND = _Contract(
@@ -565,11 +560,7 @@ _EXTEND = _Contract(
          rank_msg="counts must be 1-D with batch entries"),
     _Arr("free_blocks", "F", _I32, rank_msg="free_blocks must be 1-D"),
     _Arr("n_free", "one", _I32, rank_msg="n_free must hold one value"),
-    rules=(_Rule(lambda c: c.one == 1, "n_free must hold one value"),
-           _Rule(lambda c: c.B <= 4096, "block_table_extend takes at most 4096 sequences"),
-           _Rule(lambda c: 1 <= c.page <= 1024, "page must be in [1, 1024]"),
-           _Rule(lambda c: 0 <= c.tokens < 2 ** 30, "tokens must be in [0, 2**30)")),
-    host=False)
+    rules=(_Rule(lambda c: c.one == 1, "n_free must hold one value"),), host=False)
 
 
 def block_table_extend(block_table, lens, counts, free_blocks, n_free, page, tokens):
@@ -599,19 +590,23 @@ def block_table_extend(block_table, lens, counts, free_blocks, n_free, page, tok
     only, values trusted (negative lens and counts count as 0); at most 4096
     sequences. Build addition."""
     c = _EXTEND.bind(block_table=block_table, lens=lens, counts=counts, free_blocks=free_blocks,
-                     n_free=n_free, page=int(page), tokens=int(tokens))
-    if not _one_device(c):
+                     n_free=n_free)
+    if not _one_device(("block_table", "lens", "counts", "free_blocks", "n_free"),
+                       (block_table, lens, counts, free_blocks, n_free)):
         with torch.cuda.device(c.device):
             return block_table_extend(block_table, lens, counts, free_blocks, n_free, page,
                                       tokens)
-    B, T = c.B, c._values["tokens"]
+    B, T = c.B, int(tokens)
+    if not 0 <= T < 2 ** 30:
+        raise ValueError("tokens must be in [0, 2**30)")
     out = torch.empty(2 * T + 2 * B + 2, dtype=torch.int32, device=c.device)
-    slots, positions, offsets, new_lens, new_free = out.split((T, T, B + 1, B, 1))
+    slots, positions, offsets, new_lens, new_free = torch.split_with_sizes(
+        out, (T, T, B + 1, B, 1))
     at = out.data_ptr()
     _fusedtok.block_table_extend_launch(
-        c.ptr("block_table"), c.ptr("lens"), c.ptr("counts"), c.ptr("free_blocks"), c.F,
-        c.ptr("n_free"), at, at + 4 * T, at + 8 * T, at + 8 * T + 4 * (B + 1),
-        at + 8 * T + 4 * (2 * B + 1), B, c._values["page"], c.S, T, _stream())
+        block_table.data_ptr(), lens.data_ptr(), counts.data_ptr(), free_blocks.data_ptr(), c.F,
+        n_free.data_ptr(), at, at + 4 * T, at + 8 * T, at + 8 * T + 4 * (B + 1),
+        at + 8 * T + 4 * (2 * B + 1), B, int(page), c.S, T, _stream())
     return slots, positions, offsets, new_lens, new_free
 
 
@@ -622,8 +617,7 @@ _APPEND8 = _Contract(
     _Arr("v_new", "=k_new", same_dtype="k_new", mismatch=_NEW_KV_MISMATCH),
     _Arr("slots", "T", _I32, mismatch="slots must be 1-D with one entry per fresh row",
          rank_msg="slots must be 1-D with one entry per fresh row"),
-    rank_msg="pools must be [Nb, Hkv, P, D], scales [Nb, Hkv]",
-    rules=(_PAGE8, _DIM8, _NUM_SLOTS8), host=False)
+    rank_msg="pools must be [Nb, Hkv, P, D], scales [Nb, Hkv]", host=False)
 
 
 def kv_append_paged_int8(k_pool, v_pool, k_scales, v_scales, k_new, v_new, slots):
@@ -648,16 +642,15 @@ def kv_append_paged_int8(k_pool, v_pool, k_scales, v_scales, k_new, v_new, slots
     one slot the later counts. Returns None. Build addition."""
     c = _APPEND8.bind(k_pool=k_pool, v_pool=v_pool, k_scales=k_scales, v_scales=v_scales,
                       k_new=k_new, v_new=v_new, slots=slots)
-    if not _one_device(c):
+    at = [x.data_ptr() for x in (k_new, v_new, slots, k_pool, v_pool, k_scales, v_scales)]
+    if not _one_device(("k_new", "v_new", "slots", "k_pool", "v_pool", "k_scales", "v_scales"),
+                       (k_new, v_new, slots, k_pool, v_pool, k_scales, v_scales)):
         with torch.cuda.device(c.device):
             return kv_append_paged_int8(k_pool, v_pool, k_scales, v_scales, k_new, v_new, slots)
-    if c.T and c.Nb:
-        if c.ptr("k_pool") == c.ptr("v_pool") or c.ptr("k_scales") == c.ptr("v_scales"):
-            raise ValueError("k and v must have pools and scales of their own")
-        _fusedtok.kv_append_paged_int8_launch(
-            c.ptr("k_new"), c.ptr("v_new"), _CODE[c.k_new.dtype], c.ptr("slots"),
-            c.ptr("k_pool"), c.ptr("v_pool"), c.ptr("k_scales"), c.ptr("v_scales"), c.T, c.Hkv,
-            c.D, c.Nb, c.P, _stream())
+    if c.T and c.Nb and (at[3] == at[4] or at[5] == at[6]):
+        raise ValueError("k and v must have pools and scales of their own")
+    _fusedtok.kv_append_paged_int8_launch(at[0], at[1], _CODE[k_new.dtype], *at[2:], c.T, c.Hkv,
+                                          c.D, c.Nb, c.P, _stream())
     return None
 
 
@@ -666,8 +659,14 @@ _DECODE8 = _Contract(
     *_pools8(False),
     _table(),
     _Idx("lens", "B", lambda c: c.S * c.P, optional=True, what=_LENS_WHAT),
-    rank_msg="q must be [B, Hq, D]; pools [Nb, Hkv, P, D], scales [Nb, Hkv]",
-    rules=(_HEADS, _GQA, _PAGE8, _DIM8, _NUM_SLOTS8), host=False)
+    rank_msg="q must be [B, Hq, D]; pools [Nb, Hkv, P, D], scales [Nb, Hkv]", host=False)
+
+
+@functools.lru_cache(maxsize=1024)
+def _decode8_workspace(device, *sizes):
+    """Workspace bytes of an attention_decode_paged_int8 call of these sizes
+    on the (current) device; the checks of the sizes are made here."""
+    return _fusedtok.attention_decode_paged_int8_workspace(*sizes)
 
 
 def attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales, block_table, lens=None):
@@ -687,19 +686,20 @@ def attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales, block_tab
     streams are independent. Build addition."""
     c = _DECODE8.bind(q=q, k_pool=k_pool, v_pool=v_pool, k_scales=k_scales, v_scales=v_scales,
                       block_table=block_table, lens=lens)
-    if not _one_device(c):
+    table, lens = c.block_table, c.lens
+    if not _one_device(("q", "k_pool", "v_pool", "k_scales", "v_scales", "block_table", "lens"),
+                       (q, k_pool, v_pool, k_scales, v_scales, table) +
+                       (() if lens is None else (lens,))):
         with torch.cuda.device(c.device):
-            return attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales,
-                                               block_table, lens)
-    out = torch.empty((c.B, c.Hq, c.D), dtype=c.q.dtype, device=c.device)
-    if c.B:
-        nbytes = _fusedtok.attention_decode_paged_int8_workspace(
-            _CODE[c.q.dtype], c.B, c.Hq, c.Hkv, c.P, c.S, c.D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=c.device)
-        _fusedtok.attention_decode_paged_int8_launch(
-            c.ptr("q"), _CODE[c.q.dtype], c.ptr("k_pool"), c.ptr("v_pool"), c.ptr("k_scales"),
-            c.ptr("v_scales"), c.ptr("block_table"), c.ptr("lens"), out.data_ptr(),
-            ws.data_ptr(), nbytes, c.B, c.Hq, c.Hkv, c.Nb, c.P, c.S, c.D, _stream())
+            return attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales, table, lens)
+    code = _CODE[q.dtype]
+    nbytes = _decode8_workspace(c.device.index, code, c.B, c.Hq, c.Hkv, c.P, c.S, c.D)
+    out = torch.empty_like(q)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=c.device)
+    _fusedtok.attention_decode_paged_int8_launch(
+        q.data_ptr(), code, k_pool.data_ptr(), v_pool.data_ptr(), k_scales.data_ptr(),
+        v_scales.data_ptr(), table.data_ptr(), None if lens is None else lens.data_ptr(),
+        out.data_ptr(), ws.data_ptr(), nbytes, c.B, c.Hq, c.Hkv, c.Nb, c.P, c.S, c.D, _stream())
     return out
 
 

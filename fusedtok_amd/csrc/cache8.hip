@@ -219,18 +219,62 @@ __device__ __forceinline__ signed char code8(float x, float inv) {
     return v == v ? (signed char)fmaxf(-127.0f, fminf(127.0f, v)) : (signed char)0;
 }
 
-// V values of x widened to float32, 16 bytes a load where they fill them.
-template <int V, typename T>
-__device__ __forceinline__ void load_f(const T* p, float (&x)[V]) {
-    typedef T vec __attribute__((ext_vector_type(V)));
-    const vec u = *reinterpret_cast<const vec*>(p);
+// V values of a row as they are stored, in 32-bit words.
+template <typename T, int V>
+struct Raw {
+    static constexpr int kWords = V * (int)sizeof(T) / 4;
+    // the bits of the type's infinity: magnitudes from there are not finite
+    static constexpr unsigned kInf = sizeof(T) == 4 ? 0x7f800000u
+                                     : std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
+    typedef unsigned vec __attribute__((ext_vector_type(kWords)));
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    vec w;
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = (float)u[i];
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const T* p) {
+        w = *reinterpret_cast<const vec*>(p);
+    }
+    // max of m and the magnitudes' bits (both halves of m for a 16-bit type):
+    // magnitudes order as their bits do
+    __device__ __forceinline__ unsigned most(unsigned m) const {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4)
+                m = max(m, w[i] & 0x7fffffffu);
+            else
+                m = __builtin_bit_cast(
+                    unsigned,
+                    __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                              __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu)));
+        }
+        return m;
+    }
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else return value_of(w[i / 2] >> (i % 2 * 16));
+    }
+    static __device__ __forceinline__ float value_of(unsigned bits) {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(bits);
+        else return (float)__builtin_bit_cast(T, (unsigned short)bits);
+    }
+};
+
+// Low bytes of rint(x inv) of four values, |x inv| < 127.5: added to 1.5 * 2^23
+// the product rounds to a whole number, half to even, whose low byte is the
+// sum's. The product is rounded by itself first.
+__device__ __forceinline__ unsigned codes4(float a, float b, float c, float d, float inv) {
+#pragma clang fp contract(off)
+    constexpr float kWhole = 12582912.0f;
+    const unsigned x = __float_as_uint(a * inv + kWhole), y = __float_as_uint(b * inv + kWhole);
+    const unsigned z = __float_as_uint(c * inv + kWhole), w = __float_as_uint(d * inv + kWhole);
+    return __builtin_amdgcn_perm(y, x, 0x0c0c0400u) | __builtin_amdgcn_perm(w, z, 0x04000c0cu);
 }
 
 template <int V>
 struct Codes {
-    signed char c[V];
+    unsigned w[V / 4];
 } __attribute__((aligned(V)));
 
 // A unit is (window of `window` consecutive fresh rows, kv head, K or V): the
@@ -240,9 +284,13 @@ struct Codes {
 // decode step). A lane has V values of a row; the first kKeep passes of a run
 // stay in registers between the maximum and the codes, so a run is read once.
 // Rows in order, as a sequence's are, need no map; others (gaps, a slot twice)
-// go by a map in LDS from the block's row to the last fresh row for it.
+// go by a map in LDS from the block's row to the last fresh row for it. Values
+// stay as they are stored: the maximum is one of their bits (two instructions
+// for two 16-bit values), and only a run with an infinity or NaN in it, which
+// the maximum shows, goes through the code that looks at each value.
 //
-// What bounds it: memory latency in a decode step; for prompts, HBM.
+// What bounds it: memory latency in a decode step; for prompts, HBM and the
+// ~5 vector instructions a value.
 template <typename T, int V, int UT>
 __global__ __launch_bounds__(256) void kv_append8_kernel(
     const T* __restrict__ k_new, const T* __restrict__ v_new, const int* __restrict__ slots,
@@ -251,7 +299,7 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
     int nslots, FastDiv page, FastDiv lanes, int window, long long units) {
     constexpr int kKeep = 4, kUnits = 256 / UT;
     __shared__ int s_map[kUnits][kMaxPage8];
-    __shared__ float s_red[4];
+    __shared__ unsigned s_red[4];
     const int lane = threadIdx.x & 63;
     const int ut = UT == 64 ? lane : (int)threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -269,6 +317,16 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
     auto sync = [&] {
         if (UT == 64) wave_lds_order();
         else __syncthreads();
+    };
+    auto unit_max = [&](unsigned v) {  // over the unit's threads
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+        if (UT == 64) return v;
+        if (lane == 0) s_red[wave] = v;
+        __syncthreads();
+        v = max(max(s_red[0], s_red[1]), max(s_red[2], s_red[3]));
+        __syncthreads();
+        return v;
     };
     auto slot_of = [&](int t) { return t >= 0 && t < tokens ? slots[t] : -1; };
     auto block_of = [&](int s) { return s >= 0 && s < nslots ? page.div(s) : -1; };
@@ -310,21 +368,14 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
             const int nvec = (ordered ? n : (int)page.d) * (int)lanes.d;
             // the fresh row for the j-th vector of them, -1 where there is none
             auto source = [&](int r) { return ordered ? i + r : map[r]; };
-            float keep[kKeep][V];
-            float most = 0.0f;
-            auto fold = [&](const float (&v)[V]) {
-#pragma unroll
-                for (int c = 0; c < V; ++c) {
-                    const float a = fabsf(v[c]);
-                    most = fmaxf(most, a < INFINITY ? a : 0.0f);
-                }
-            };
-            auto load = [&](int j, float (&v)[V]) {
+            using R = Raw<T, V>;
+            R keep[kKeep];
+            auto load = [&](int j, R& v) {
                 const int r = lanes.div(j), src = source(r);
-#pragma unroll
-                for (int c = 0; c < V; ++c) v[c] = 0.0f;
-                if (src >= 0) load_f<V>(x + src * row_stride + V * (j - r * (int)lanes.d), v);
+                if (src >= 0) v.load(x + src * row_stride + V * (j - r * (int)lanes.d));
+                else v.zero();
             };
+            unsigned bits = 0;
 #pragma unroll
             for (int p = 0; p < kKeep; ++p) {
                 const int j = p * UT + ut;
@@ -332,24 +383,52 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
             }
 #pragma unroll
             for (int p = 0; p < kKeep; ++p)
-                if (p * UT + ut < nvec) fold(keep[p]);
+                if (p * UT + ut < nvec) bits = keep[p].most(bits);
             for (int j = kKeep * UT + ut; j < nvec; j += UT) {
-                float v[V];
+                R v;
                 load(j, v);
-                fold(v);
+                bits = v.most(bits);
             }
             const size_t bh = (size_t)block * hkv + h;
             const float held = over ? 0.0f : scales[bh];
-            most = UT == 64 ? wave_max(most) : block_max<256>(most, s_red);
+            if constexpr (sizeof(T) == 2) bits = max(bits & 0xffffu, bits >> 16);
+            bits = unit_max(bits);
+            float most = R::value_of(bits);
+            const bool finite = bits < R::kInf;
+            if (!finite) {  // of the finite values alone
+                float m = 0.0f;
+                for (int j = ut; j < nvec; j += UT) {
+                    R v;
+                    load(j, v);
+#pragma unroll
+                    for (int c = 0; c < V; ++c) {
+                        const float a = fabsf(v.value(c));
+                        m = fmaxf(m, a < INFINITY ? a : 0.0f);
+                    }
+                }
+                most = __uint_as_float(unit_max(__float_as_uint(m)));
+            }
             const float now = fmaxf(fmaxf(held, most / 127.0f), kLeastScale);
             const float inv = 1.0f / now;
             signed char* const codes = pool + bh * page.d * dim;
-            auto store = [&](int j, const float (&v)[V]) {
+            auto store = [&](int j, const R& v) {
                 const int r = lanes.div(j);
                 if (source(r) < 0) return;
                 Codes<V> o;
 #pragma unroll
-                for (int c = 0; c < V; ++c) o.c[c] = code8(v[c], inv);
+                for (int c = 0; c < V; c += 4)
+                    o.w[c / 4] = codes4(v.value(c), v.value(c + 1), v.value(c + 2),
+                                        v.value(c + 3), inv);
+                if (!finite) {
+#pragma unroll
+                    for (int c = 0; c < V; c += 4) {
+                        o.w[c / 4] = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            o.w[c / 4] |= (unsigned)(unsigned char)code8(v.value(c + i), inv)
+                                          << (8 * i);
+                    }
+                }
                 *reinterpret_cast<Codes<V>*>(codes + (size_t)(base + r) * dim +
                                              V * (j - r * (int)lanes.d)) = o;
             };
@@ -359,7 +438,7 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
                 if (j < nvec) store(j, keep[p]);
             }
             for (int j = kKeep * UT + ut; j < nvec; j += UT) {
-                float v[V];
+                R v;
                 load(j, v);
                 store(j, v);
             }
@@ -371,7 +450,12 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
                     Codes<V>* p = reinterpret_cast<Codes<V>*>(codes + (size_t)V * j);
                     Codes<V> o = *p;
 #pragma unroll
-                    for (int c = 0; c < V; ++c) o.c[c] = code8((float)o.c[c], ratio);
+                    for (int c = 0; c < V / 4; ++c) {
+                        const unsigned u = o.w[c];
+                        o.w[c] = codes4((float)(signed char)u, (float)(signed char)(u >> 8),
+                                        (float)(signed char)(u >> 16), (float)((int)u >> 24),
+                                        ratio);
+                    }
                     *p = o;
                 }
             }
@@ -1346,8 +1430,8 @@ int ft_block_table_extend_launch(int* table, const int* lens, const int* counts,
     return guarded([&] {
         if (batch < 0 || batch > kExtendSeqs)
             inval("block_table_extend: batch must be in [0, 4096]");
-        if (page < 1 || tbl_width < 0 || tokens < 0 || free_len < 0)
-            inval("block_table_extend: page >= 1, width >= 0, tokens >= 0");
+        if (page < 1 || page > kMaxPage8 || tbl_width < 0 || tokens < 0 || free_len < 0)
+            inval("block_table_extend: page in [1, 1024], width >= 0, tokens >= 0");
         if ((long long)tbl_width * page > (1LL << 30)) inval("table capacity too large");
         if ((long long)tbl_width * batch > INT_MAX) inval("block_table_extend: table too large");
         if (!n_free || !n_free_out || !offsets || (tokens && (!slots || !positions)) ||

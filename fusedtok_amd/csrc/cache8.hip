@@ -74,8 +74,6 @@ struct FastDiv {
 // from the table entry that another workgroup may be writing. What bounds it:
 // launch and the dependent chain length -> scan -> bisection -> table.
 // ---------------------------------------------------------------------------
-constexpr int kExtendTokens = 512;  // tokens of a workgroup
-
 __global__ __launch_bounds__(256) void block_table_extend_kernel(
     int* __restrict__ table, const int* __restrict__ lens, const int* __restrict__ counts,
     const int* __restrict__ free_blocks, int free_len, const int* __restrict__ n_free,
@@ -85,6 +83,7 @@ __global__ __launch_bounds__(256) void block_table_extend_kernel(
     constexpr int PER = kExtendSeqs / 256;
     __shared__ int s_off[kExtendSeqs + 1];   // fresh tokens before sequence b (saturated)
     __shared__ int s_need[kExtendSeqs + 1];  // fresh blocks before sequence b
+    __shared__ int s_len[kExtendSeqs];
     __shared__ long long s_toks[4];
     __shared__ int s_blocks[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -144,6 +143,7 @@ __global__ __launch_bounds__(256) void block_table_extend_kernel(
             const int end = len[i] + min(add[i], span - len[i]);
             s_off[b] = off;
             s_need[b] = rn;
+            s_len[b] = len[i];
             if (blockIdx.x == 0) {
                 offsets[b] = off;
                 lens_out[b] = end;
@@ -174,13 +174,18 @@ __global__ __launch_bounds__(256) void block_table_extend_kernel(
         const long long at = (long long)have - 1 - k;
         return at >= 0 && at < free_len ? free_blocks[at] : -1;
     };
-    auto len_of = [&](int b) { return min(max(lens[b], 0), span); };
 
-    const long long stride = gridDim.x * 256;
-    for (long long t = blockIdx.x * 256 + tid; t < tokens; t += stride) {
+    // the tokens, then the fresh blocks
+    const long long items = (long long)tokens + fresh, stride = gridDim.x * 256;
+    for (long long t = blockIdx.x * 256 + tid; t < items; t += stride) {
+        if (t >= tokens) {
+            const int k = (int)(t - tokens), b = find(s_need, k);
+            table[(size_t)b * width + page.up(s_len[b]) + (k - s_need[b])] = taken(k);
+            continue;
+        }
         int slot = -1, pos = 0;
         if (t < total) {
-            const int b = find(s_off, (int)t), n = len_of(b);
+            const int b = find(s_off, (int)t), n = s_len[b];
             const long long p = (long long)n + (t - s_off[b]);
             pos = (int)min(p, (long long)INT_MAX);
             if (p < span) {
@@ -193,10 +198,6 @@ __global__ __launch_bounds__(256) void block_table_extend_kernel(
         }
         slots[t] = slot;
         positions[t] = pos;
-    }
-    for (long long k = blockIdx.x * 256 + tid; k < fresh; k += stride) {
-        const int b = find(s_need, (int)k);
-        table[(size_t)b * width + page.up(len_of(b)) + ((int)k - s_need[b])] = taken((int)k);
     }
 }
 
@@ -1438,7 +1439,10 @@ int ft_block_table_extend_launch(int* table, const int* lens, const int* counts,
             (batch && (!lens || !counts || !lens_out || (tbl_width && !table))) ||
             (free_len && !free_blocks))
             inval("block_table_extend: null operand");
-        const unsigned grid = grid_1d(tokens, kExtendTokens, 4 * dev_info().cu_count);
+        // a thread a token or fresh block, of which there is about one a sequence
+        // and one a page of tokens
+        const unsigned grid = grid_1d((long long)tokens + tokens / page + batch, 256,
+                                      4 * dev_info().cu_count);
         block_table_extend_kernel<<<grid, 256, 0, as_stream(stream)>>>(
             table, lens, counts, free_blocks, free_len, n_free, slots, positions, offsets,
             lens_out, n_free_out, batch, FastDiv(page), tbl_width, tokens);

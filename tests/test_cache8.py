@@ -94,6 +94,24 @@ def test_host_tensors_are_refused():
         ft.block_table_extend(i.view(1, 1), i, i, i, i, 16, 1)
 
 
+class On:
+    """A stand-in for a tensor on a device."""
+
+    def __init__(self, device):
+        self.device = device
+
+    def get_device(self):
+        return self.device
+
+
+def test_operands_of_two_devices(monkeypatch):
+    monkeypatch.setattr(ft, "_current_device", lambda: 1)
+    assert ft._one_device("ab", (On(1), On(1)))
+    assert not ft._one_device("ab", (On(0), On(0)))   # another than the current one
+    with pytest.raises(ValueError, match="a on 0, b on 1"):
+        ft._one_device("ab", (On(0), On(1)))
+
+
 # ---- the plain forms --------------------------------------------------------
 
 

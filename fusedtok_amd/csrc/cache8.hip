@@ -718,7 +718,7 @@ void combine8(const float* ml, const float* acc, const int* lens, T* out, const 
 }
 
 // ---------------------------------------------------------------------------
-// Any head dim (attn8_general): one workgroup per (sequence, kv head, chunk of
+// The other head dims (attn8_general): one workgroup per (sequence, kv head, chunk of
 // tokens), 8 q heads at a time, dot products on the vector ALU, 256 tokens at
 // a time with a running maximum.
 // ---------------------------------------------------------------------------
@@ -846,7 +846,9 @@ __global__ __launch_bounds__(256) void attn8_general(
 }
 
 // ---------------------------------------------------------------------------
-// D = 64, 128, 256 (attn8_stream): matrix cores, each K / V byte read once.
+// dim a multiple of 16 up to 256 (attn8_stream): matrix cores, each K / V byte
+// read once. The kernel is built for D = 64, 128 and 256; another dim runs in
+// the next larger (FULL false), its rows' missing chunks never read and zero.
 //
 // Work split. The rows are (sequence b, kv head, tile of up to 16 q heads),
 // b-major, len_b tokens each, laid end to end; every WAVE takes one equal
@@ -985,7 +987,7 @@ __device__ __forceinline__ Piece8 piece8(const long long* s_pref, int batch, int
     return p;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool FULL>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(Stream8<T, D>::kOcc, Stream8<T, D>::kOcc)))
 void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_pool,
@@ -995,7 +997,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                   float* __restrict__ ws_acc, long long* __restrict__ pref_out,
                   T* __restrict__ out, int batch, int hq, int hkv, int tile, int tiles,
                   int blocks, FastDiv page, int width, int span, int nseg, int min_seg,
-                  float scale_log2) {
+                  float scale_log2, int dim_) {
     using C = Stream8<T, D>;
     constexpr int TOK = C::kTok, NL = C::kLoads, SUB = TOK / 32, KE = D / 64;
     __shared__ __align__(16) char s_stage[4][C::kLds];
@@ -1004,6 +1006,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
+    const int dim = FULL ? D : dim_;
     if (wave < 2) scan8(lens, batch, span, lane, wave ? min_seg : 1, s_prefix[wave]);
     __syncthreads();
     const int vrows = hkv * tiles, group = hq / hkv;
@@ -1051,6 +1054,11 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
         return table[(size_t)p.b * width + page.div(token(p, min(st, steps(p) - 1)))];
     };
     u32x4 kt[NL], vt[NL];
+    const bool has = FULL || 16 * lc < dim;  // the row has the lane's chunk
+    if (!FULL) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) kt[i] = vt[i] = u32x4{0, 0, 0, 0};
+    }
     float ksn, vsn;
     unsigned long long seen;  // lanes whose token of the loaded step counts
     auto issue = [&](const Piece8& p, int st, int ent) {
@@ -1065,9 +1073,11 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const unsigned rw = __shfl(row, C::kRowsPer * i + lr, 64);
-            const size_t off = (size_t)rw * D + 16 * lc;
-            kt[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k_pool + off));
-            vt[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v_pool + off));
+            const size_t off = (size_t)rw * dim + 16 * lc;
+            if (has) {
+                kt[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k_pool + off));
+                vt[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v_pool + off));
+            }
         }
     };
     // ---- a row's q: column r's dims 64 e + 16 g .. + 15 ----------------------
@@ -1078,12 +1088,15 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
     typedef T tx8 __attribute__((ext_vector_type(8)));
     tx8 qx[KE][2];
     auto load_q = [&](const Piece8& p) {
-        const T* row = q + ((size_t)p.b * hq + first_head(p) + (r < p.heads ? r : 0)) * D;
+        const T* row = q + ((size_t)p.b * hq + first_head(p) + (r < p.heads ? r : 0)) * dim;
 #pragma unroll
         for (int e = 0; e < KE; ++e)
 #pragma unroll
-            for (int f = 0; f < 2; ++f)
-                qx[e][f] = *reinterpret_cast<const tx8*>(row + 64 * e + 16 * g + 8 * f);
+            for (int f = 0; f < 2; ++f) {
+                if (!FULL) qx[e][f] = tx8{};
+                if (FULL || 64 * e + 16 * g < dim)
+                    qx[e][f] = *reinterpret_cast<const tx8*>(row + 64 * e + 16 * g + 8 * f);
+            }
     };
 
     Piece8 pc = piece8(s_pref, batch, vrows, seg_lo, seg_hi, lane, group, tile, tiles, lens, span);
@@ -1259,12 +1272,13 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
         if (r < pc.heads) {
             // dims (D/4) g + (D/16) i + d of head r: acc[d][i]
             if (pc.whole) {
-                T* o = out + ((size_t)pc.b * hq + first_head(pc) + r) * D + (D / 4) * g;
+                T* o = out + ((size_t)pc.b * hq + first_head(pc) + r) * dim + (D / 4) * g;
                 const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int d = 0; d < C::kChunks; d += 4) {
+                        if (!FULL && (D / 4) * g + (D / 16) * i + d >= dim) continue;
                         float y[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -1281,13 +1295,15 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                     pb * vrows + (pc.kv + 1) * (uniform64(s_pref[pc.b + 1]) - pb);
                 const size_t slot =
                     (2 * (size_t)seg + (end >= seg_lo + S ? 1 : 0)) * tile + r;
-                float* o = ws_acc + slot * D + (D / 4) * g;
+                float* o = ws_acc + slot * dim + (D / 4) * g;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int d = 0; d < C::kChunks; d += 4)
+                    for (int d = 0; d < C::kChunks; d += 4) {
+                        if (!FULL && (D / 4) * g + (D / 16) * i + d >= dim) continue;
                         *reinterpret_cast<float4*>(o + (D / 16) * i + d) = make_float4(
                             acc[d][i], acc[d + 1][i], acc[d + 2][i], acc[d + 3][i]);
+                    }
                 if (g == 0) {
                     ws_ml[slot * 2] = m_run;
                     ws_ml[slot * 2 + 1] = l_run;
@@ -1335,13 +1351,13 @@ Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int widt
     s.span = (int)span;
     if (batch == 0) return s;
     const int cus = dev_info().cu_count, group = hq / hkv;
-    s.stream = span > 0 && (dim == 64 || dim == 128 || dim == 256);
+    s.stream = span > 0 && dim % 16 == 0 && dim <= 256;
     if (s.stream) {
         s.tiles = (group + 15) / 16;
         s.tile = (group + s.tiles - 1) / s.tiles;
         s.tiles = (group + s.tile - 1) / s.tile;
-        const int occ = dim == 64 ? stream_occ<64>(dtype)
-                                  : dim == 128 ? stream_occ<128>(dtype) : stream_occ<256>(dtype);
+        const int occ = dim <= 64 ? stream_occ<64>(dtype)
+                                  : dim <= 128 ? stream_occ<128>(dtype) : stream_occ<256>(dtype);
         s.min_seg = kMinSeg8;
         const long long rows = (long long)std::min(batch, kStreamScanRows) * hkv * s.tiles;
         const long long most = rows * ((span + s.min_seg - 1) / s.min_seg);
@@ -1376,19 +1392,21 @@ struct Attn8Args {
 template <typename T, int D>
 void attn8_stream_run(const Attn8Shape& sh, const Attn8Args& a, float* ml, float* acc,
                       hipStream_t s) {
-    long long* pref = (long long*)(acc + sh.slots * D);
-    const float scale = (1.0f / sqrtf((float)D)) * kLog2e;
+    const int dim = sh.dim;
+    long long* pref = (long long*)(acc + sh.slots * dim);
+    const float scale = (1.0f / sqrtf((float)dim)) * kLog2e;
+    const auto kernel = dim == D ? attn8_stream<T, D, true> : attn8_stream<T, D, false>;
     for (int b0 = 0; b0 < sh.batch; b0 += kStreamScanRows) {
         const int nb = std::min(kStreamScanRows, sh.batch - b0);
-        const T* q = (const T*)a.q + (size_t)b0 * sh.hq * D;
-        T* out = (T*)a.out + (size_t)b0 * sh.hq * D;
+        const T* q = (const T*)a.q + (size_t)b0 * sh.hq * dim;
+        T* out = (T*)a.out + (size_t)b0 * sh.hq * dim;
         const int* lens = a.lens ? a.lens + b0 : nullptr;
-        attn8_stream<T, D><<<(sh.nseg + 3) / 4, 256, 0, s>>>(
+        kernel<<<(sh.nseg + 3) / 4, 256, 0, s>>>(
             q, a.kp, a.vp, a.ks, a.vs, a.table + (size_t)b0 * sh.width, lens, ml, acc, pref, out,
             nb, sh.hq, sh.hkv, sh.tile, sh.tiles, a.blocks, FastDiv(sh.page), sh.width, sh.span,
-            sh.nseg, sh.min_seg, scale);
+            sh.nseg, sh.min_seg, scale, dim);
         launch_check("int8 decode attention kernel launch");
-        combine8(ml, acc, lens, out, Streamed8{pref, nb}, nb, sh.hq, sh.hkv, D, sh.span, sh.tile,
+        combine8(ml, acc, lens, out, Streamed8{pref, nb}, nb, sh.hq, sh.hkv, dim, sh.span, sh.tile,
                  sh.tiles, s);
     }
 }
@@ -1398,8 +1416,8 @@ void attn8_run(const Attn8Shape& sh, const Attn8Args& a, hipStream_t s) {
     float* ml = (float*)a.ws;
     float* acc = ml + ((sh.slots * 2 + 63) & ~(size_t)63);
     if (sh.stream && a.blocks > 0) {
-        if (sh.dim == 64) attn8_stream_run<T, 64>(sh, a, ml, acc, s);
-        else if (sh.dim == 128) attn8_stream_run<T, 128>(sh, a, ml, acc, s);
+        if (sh.dim <= 64) attn8_stream_run<T, 64>(sh, a, ml, acc, s);
+        else if (sh.dim <= 128) attn8_stream_run<T, 128>(sh, a, ml, acc, s);
         else attn8_stream_run<T, 256>(sh, a, ml, acc, s);
         return;
     }

@@ -330,7 +330,9 @@ LENS = {"short": [1, 0, 2, 17], "mixed": [33, 1, 0, 300, 64, 129], "long": [2500
 @pytest.mark.parametrize("hkv,group,page,d", [
     (2, 4, 16, 128), (2, 4, 16, 64), (1, 16, 64, 128), (3, 1, 24, 64), (2, 5, 5, 128),
     (1, 20, 16, 128), (1, 33, 16, 64), (2, 3, 1, 64), (2, 4, 16, 256), (1, 8, 128, 128),
-    (2, 2, 7, 36), (1, 4, 16, 512), (1, 1, 1024, 4), (2, 4, 16, 96)])
+    (2, 2, 7, 36), (1, 4, 16, 512), (1, 1, 1024, 4), (2, 4, 16, 96), (2, 3, 16, 16),
+    (1, 4, 5, 48), (2, 8, 16, 80), (1, 17, 24, 112), (2, 4, 16, 144), (1, 2, 32, 192),
+    (1, 9, 16, 240), (2, 4, 16, 260), (1, 6, 3, 100)])
 def test_attend(hkv, group, page, d, lens, dtype):
     lens = LENS[lens]
     rng = np.random.default_rng(hkv + 7 * group + 11 * page + d + len(lens))
@@ -339,7 +341,7 @@ def test_attend(hkv, group, page, d, lens, dtype):
     check_attend(q, cache, table, lens, dtype)
 
 
-@pytest.mark.parametrize("d", [64, 128, 32])
+@pytest.mark.parametrize("d", [64, 128, 32, 20])
 def test_attend_whole_table(d):
     """lens None: every row; lens beyond the capacity and negative ones are
     clamped."""
@@ -356,7 +358,7 @@ def test_attend_whole_table(d):
 
 
 @pytest.mark.parametrize("page", [16, 5, 64])
-@pytest.mark.parametrize("d", [64, 128, 96])
+@pytest.mark.parametrize("d", [64, 128, 96, 36])
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_attend_holes(d, page, dtype):
     """Table entries outside the pools: their tokens weigh nothing; a row of
@@ -372,7 +374,7 @@ def test_attend_holes(d, page, dtype):
     assert not out[1].any() and not out[2].any()
 
 
-@pytest.mark.parametrize("d", [64, 128, 96])
+@pytest.mark.parametrize("d", [64, 128, 96, 36])
 def test_attend_unused_values(d):
     """Blocks and scales behind a row's last token - NaN, infinity, anything -
     reach no output."""
@@ -390,7 +392,7 @@ def test_attend_unused_values(d):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("d", [64, 128, 96])
+@pytest.mark.parametrize("d", [64, 128, 96, 36])
 def test_attend_small_weights(d, dtype):
     """Thousands of keys 25 nats below four dominant ones whose values are 0:
     what they add is small, and has to come out right."""
@@ -409,7 +411,7 @@ def test_attend_small_weights(d, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("d", [64, 128, 96])
+@pytest.mark.parametrize("d", [64, 128, 96, 36])
 def test_attend_scales_of_all_sizes(d, dtype):
     """Blocks' scales from 1e-30 to 1e4, zero scales, large and small q."""
     rng = np.random.default_rng(2)
@@ -431,7 +433,7 @@ def test_attend_many_rows(b, hkv, lens):
     check_attend(q, cache, table, lens, torch.float32)
 
 
-@pytest.mark.parametrize("d", [128, 96])
+@pytest.mark.parametrize("d", [128, 96, 100])
 def test_cache_beyond_32_bits(d):
     """A pool of more than 2^32 bytes: append to its last blocks, attend
     them."""

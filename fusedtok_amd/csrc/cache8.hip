@@ -964,7 +964,7 @@ struct Piece8 {
 // the sequences' ends are counted 64 at a time, by the lanes.
 __device__ __forceinline__ Piece8 piece8(const long long* s_pref, int batch, int vrows,
                                          long long pos, long long seg_hi, int lane, int group,
-                                         int tile, int tiles, const int* lens, int span) {
+                                         int tile, int tiles, const long long* s_tokens) {
     int b = 0;
     for (int step = (batch + 63) >> 6;; step = 1) {
         const int at = b + (lane + 1) * step;
@@ -979,8 +979,8 @@ __device__ __forceinline__ Piece8 piece8(const long long* s_pref, int batch, int
     p.kv = (int)div64(pos - base, len);
     p.t0 = (int)(pos - base - (long long)p.kv * len);
     p.next = min(seg_hi, base + (long long)(p.kv + 1) * len);
-    // (the prefix may be of padded lengths)
-    const int end = __builtin_amdgcn_readfirstlane(clamp_len(lens, b, span));
+    // (s_pref may be of padded lengths, s_tokens is of the true ones)
+    const int end = (int)(uniform64(s_tokens[b + 1]) - uniform64(s_tokens[b]));
     p.n = min((int)(p.next - pos), end - p.t0);
     p.whole = p.t0 == 0 && p.n == end;
     p.heads = min(tile, group - p.kv % tiles * tile);
@@ -1099,7 +1099,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
             }
     };
 
-    Piece8 pc = piece8(s_pref, batch, vrows, seg_lo, seg_hi, lane, group, tile, tiles, lens, span);
+    Piece8 pc = piece8(s_pref, batch, vrows, seg_lo, seg_hi, lane, group, tile, tiles, s_prefix[0]);
     int ent = entry(pc, 0);
     load_q(pc);
     issue(pc, 0, ent);
@@ -1160,7 +1160,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                 ent = entry(pc, st + 2);
                 issue(pc, st + 1, e);
             } else if (more) {
-                nx = piece8(s_pref, batch, vrows, pc.next, seg_hi, lane, group, tile, tiles, lens, span);
+                nx = piece8(s_pref, batch, vrows, pc.next, seg_hi, lane, group, tile, tiles, s_prefix[0]);
                 const int e = entry(nx, 0);
                 ent = entry(nx, 1);
                 issue(nx, 0, e);
@@ -1345,7 +1345,8 @@ Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int widt
     if (hq % hkv != 0) inval("q heads must be a multiple of kv heads (contiguous GQA groups)");
     const long long span = (long long)width * page;
     if (span > (1LL << 30)) inval("table capacity too large");
-    if ((long long)batch * hq > INT_MAX) inval("attention: too many rows");
+    if ((long long)std::min(batch, kStreamScanRows) * hq >= 1 << 24)
+        inval("attention problem too large for one launch");
     Attn8Shape s{};
     s.batch = batch; s.hq = hq; s.hkv = hkv; s.page = page; s.width = width; s.dim = dim;
     s.span = (int)span;
@@ -1373,6 +1374,8 @@ Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int widt
         s.cmax = (int)((span + s.chunk - 1) / s.chunk);
         s.tile = group;
         s.tiles = 1;
+        if ((long long)batch * hq >= 1 << 24 || (long long)batch * hkv * s.cmax >= 1 << 24)
+            inval("attention problem too large for one launch");
         s.slots = (size_t)batch * hq * s.cmax;
     }
     s.bytes = (((s.slots * 2 + 63) & ~(size_t)63) + s.slots * dim) * sizeof(float) +

@@ -200,6 +200,28 @@ def test_append_prompts(t, hkv, page, d, dtype):
     check_append(cache, k, v, slots, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,hkv,page,d", [(9, 2, 16, 128), (70, 8, 16, 128), (200, 16, 64, 64),
+                                             (300, 8, 24, 96)])
+def test_append_padded_batch(rows, hkv, page, d, dtype):
+    """[sequences, rows] padded to one length: -1 behind each sequence's own,
+    some sequences with none; few rows and enough for windows of a block."""
+    rng = np.random.default_rng(rows)
+    b = 14
+    lens = rng.integers(0, 3 * page, b)
+    fresh = rng.integers(0, rows + 1, b)
+    fresh[[0, 5, b - 1]] = 0, rows, 0
+    nb = int(sum(-(-(n + a) // page) for n, a in zip(lens, fresh))) + 2
+    cache = pools(rng, nb, hkv, page, d)
+    flat, at = seq_slots(rng, nb, page, lens, fresh), 0
+    slots = np.full((b, rows), -1)
+    for i, a in enumerate(fresh):
+        slots[i, :a] = flat[at:at + a]
+        at += a
+    k, v = (rng.standard_normal((b * rows, hkv, d)) * 2 for _ in range(2))
+    check_append(cache, k, v, slots.reshape(-1), dtype)
+
+
 @pytest.mark.parametrize("page,d", [(16, 128), (5, 64), (64, 128)])
 def test_append_odd_slots(page, d):
     """Slots outside the pools, gaps between a block's rows, rows out of
@@ -217,14 +239,39 @@ def test_append_odd_slots(page, d):
     check_append(cache, k, v, slots, torch.float32)
 
 
-def test_append_longer_run_than_a_block():
-    """The same rows again and again: a run of more rows than the block has."""
+@pytest.mark.parametrize("rows,hkv,page,d", [(150, 1, 16, 64), (700, 64, 16, 64),
+                                             (900, 40, 64, 128)])
+def test_append_longer_run_than_a_block(rows, hkv, page, d):
+    """The same rows again and again: a run of more rows than the block has,
+    and one that reaches over several windows."""
     rng = np.random.default_rng(3)
-    page, d = 16, 64
-    cache = pools(rng, 4, 1, page, d)
-    slots = [page + (7 * i) % 11 + 2 for i in range(150)]
-    k, v = (rng.standard_normal((150, 1, d)) for _ in range(2))
+    cache = pools(rng, 4, hkv, page, d)
+    slots = [page + (7 * i) % 11 + 2 for i in range(rows)]
+    k, v = (rng.standard_normal((rows, hkv, d)) for _ in range(2))
     check_append(cache, k, v, slots, torch.bfloat16)
+
+
+def test_append_off_alignment():
+    """Rows at 8 elements' alignment and at 4: the same codes."""
+    rng = np.random.default_rng(14)
+    cache = pools(rng, 3, 2, 16, 64)
+    k, v = (rng.standard_normal((20, 2, 64)).astype(np.float32) for _ in range(2))
+    slots = i32(np.arange(20))
+    got = []
+    for off in (0, 4, 12):
+        at = [dev(x) for x in cache]
+        kv = []
+        for x in (k, v):
+            buf = torch.zeros(x.size + 16, dtype=torch.float16, device=DEV)
+            kv.append(buf[off:off + x.size].view(x.shape))
+            kv[-1].copy_(dev(x))
+        ft.kv_append_paged_int8(*at, *kv, slots)
+        got.append(at)
+    for other in got[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(got[0], other))
+    with pytest.raises(ValueError):
+        bad = torch.zeros(20 * 2 * 64 + 2, dtype=torch.float16, device=DEV)[2:].view(20, 2, 64)
+        ft.kv_append_paged_int8(*got[0], bad, kv[1], slots)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)

@@ -567,7 +567,8 @@ constexpr int kMaxPieces8 = 4096;  // of a row (their weights are kept in LDS)
 constexpr int kWavePieces8 = 32;   // folded by one wave, at most
 
 // `per` (1 or 4) q heads a workgroup, a wave each; a head of many pieces is
-// folded by the whole workgroup, afterwards. Bound by latency: the row's
+// folded by the whole workgroup, afterwards. Where heads are few, gridDim.y
+// workgroups share the dims of one of many pieces. Bound by latency: the row's
 // place, its pieces' (m, l), their sums.
 template <typename T, typename Pieces>
 __global__ __launch_bounds__(256) void attn8_combine(
@@ -595,10 +596,10 @@ __global__ __launch_bounds__(256) void attn8_combine(
         St<T>::st4(out + (size_t)head * dim + 4 * d4, a);
     };
 
-    // one head by the whole workgroup
-    auto fold = [&](int head, const typename Pieces::Row& row) {
+    // dims [4 v0, 4 v0 + 4 nv) of one head by the whole workgroup
+    auto fold = [&](int head, const typename Pieces::Row& row, int v0, int nv) {
         constexpr int kAhead = 8;
-        const int np = row.count, ng = 256 / dc, tg = tid / dc, d4 = tid - tg * dc;
+        const int np = row.count, ng = 256 / nv, tg = tid / nv, d4 = v0 + tid - tg * nv;
         const int gi = in_tile(head);
         auto at = [&](int i) { return row.at(i) * tile + gi; };
         auto piece = [&](int i) {
@@ -634,23 +635,34 @@ __global__ __launch_bounds__(256) void attn8_combine(
         };
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) add(tg + k * ng, x[k]);
-#pragma unroll 4
-        for (int i = tg + kAhead * ng; i < np; i += ng) add(i, piece(i));
+        for (int i = tg + kAhead * ng; i < np; i += kAhead * ng) {
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) x[k] = piece(i + k * ng);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) add(i + k * ng, x[k]);
+        }
         s_acc[tid] = a;
         __syncthreads();
-        if (tg == 0) {
-            for (int j = 1; j < ng; ++j) {
-                const float4 v = s_acc[j * dc + d4];
+        // the groups' sums, halved until one is left
+        for (int n = ng; n > 1;) {
+            const int half = (n + 1) >> 1;
+            if (tg + half < n) {
+                const float4 v = s_acc[tid + half * nv];
                 a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+                s_acc[tid] = a;
             }
-            store(head, d4, a, l);
+            n = half;
+            __syncthreads();
         }
+        if (tg == 0) store(head, d4, a, l);
         __syncthreads();  // LDS is the next head's
     };
 
     if (per == 1) {
         const auto row = row_of(blockIdx.x);
-        if (row.count > kWavePieces8) return fold(blockIdx.x, row);
+        const int nv = dc / gridDim.y;
+        if (row.count > kWavePieces8) return fold(blockIdx.x, row, blockIdx.y * nv, nv);
+        if (blockIdx.y) return;
     }
     {
         const int head = blockIdx.x * per + wave;
@@ -703,16 +715,19 @@ __global__ __launch_bounds__(256) void attn8_combine(
     }
     __syncthreads();
     for (int k = 0; k < per; ++k)
-        if (s_many[k]) fold(blockIdx.x * per + k, row_of(blockIdx.x * per + k));
+        if (s_many[k]) fold(blockIdx.x * per + k, row_of(blockIdx.x * per + k), 0, dc);
 }
 
 template <typename T, typename Pieces>
 void combine8(const float* ml, const float* acc, const int* lens, T* out, const Pieces& pieces,
               int batch, int hq, int hkv, int dim, int span, int tile, int tiles, hipStream_t s) {
     const int heads = batch * hq;
-    // few heads have many pieces each: a workgroup a head
+    // few heads have many pieces each: a workgroup a head, or one for 32 of its
+    // dims (one row of 131072 tokens, 8 heads, attention
+    // and combine: 54 -> 27 us)
     const int per = heads >= 4 * dev_info().cu_count && 256 % dim == 0 ? 4 : 1;
-    attn8_combine<T, Pieces><<<(unsigned)((heads + per - 1) / per), 256, 0, s>>>(
+    const int parts = per == 1 && heads < dev_info().cu_count && dim % 32 == 0 ? dim / 32 : 1;
+    attn8_combine<T, Pieces><<<dim3((heads + per - 1) / per, parts), 256, 0, s>>>(
         ml, acc, lens, out, pieces, heads, hq, hkv, dim, span, tile, tiles, per);
     launch_check("int8 decode attention combine launch");
 }
@@ -844,6 +859,16 @@ __global__ __launch_bounds__(256) void attn8_general(
         __syncthreads();
     }
 }
+
+// ---------------------------------------------------------------------------
+// Tokens of a segment, at least (a power of two, whole steps). Calls of few
+// tokens take segments of one row each: of 64 tokens while those are at most
+// four a CU (eight at D = 64), else of 128 while those do not outnumber the
+// waves. Attention and combine together, graph replays: 4 rows of 500-1000
+// tokens, 8 kv heads, D = 128, 13.6 us at 64, 14.5 at 128; 8 rows of 1000-2000
+// 18.7 and 16.6; 32 rows of 500-1000 19.8 at 128, 23.1 as equal segments.
+constexpr int kMinSeg8 = 64;
+constexpr int kScanRows8 = 1024;  // sequences of a launch (their prefixes are in LDS)
 
 // ---------------------------------------------------------------------------
 // dim a multiple of 16 up to 256 (attn8_stream): matrix cores, each K / V byte
@@ -996,29 +1021,31 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                   const int* __restrict__ lens, float* __restrict__ ws_ml,
                   float* __restrict__ ws_acc, long long* __restrict__ pref_out,
                   T* __restrict__ out, int batch, int hq, int hkv, int tile, int tiles,
-                  int blocks, FastDiv page, int width, int span, int nseg, int min_seg,
+                  int blocks, FastDiv page, int width, int span, int nseg, int short_segs,
                   float scale_log2, int dim_) {
     using C = Stream8<T, D>;
     constexpr int TOK = C::kTok, NL = C::kLoads, SUB = TOK / 32, KE = D / 64;
     __shared__ __align__(16) char s_stage[4][C::kLds];
-    __shared__ long long s_prefix[2][kStreamScanRows + 1];
+    __shared__ long long s_prefix[3][kScanRows8 + 1];  // of lens, rounded up to 1, 64, 128
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
     const int dim = FULL ? D : dim_;
-    if (wave < 2) scan8(lens, batch, span, lane, wave ? min_seg : 1, s_prefix[wave]);
+    if (wave < 3) scan8(lens, batch, span, lane, wave ? kMinSeg8 * wave : 1, s_prefix[wave]);
     __syncthreads();
     const int vrows = hkv * tiles, group = hq / hkv;
-    long long total = uniform64(s_prefix[0][batch]) * vrows, S = min_seg;
-    const long long padded = uniform64(s_prefix[1][batch]) * vrows;
-    // few tokens: a segment a stretch of min_seg tokens of one row
-    const bool few = padded <= (long long)nseg * min_seg;
+    // few tokens: a segment a stretch of S tokens of one row
+    const long long pad1 = uniform64(s_prefix[1][batch]) * vrows;
+    const long long pad2 = uniform64(s_prefix[2][batch]) * vrows;
+    const int few = pad1 <= (long long)short_segs * kMinSeg8     ? 1
+                    : pad2 <= (long long)nseg * (2 * kMinSeg8) ? 2
+                                                               : 0;
     const long long* const s_pref = s_prefix[few];
-    if (few) {
-        total = padded;
-    } else {
-        S = max(div64(total + nseg - 1, nseg), (long long)min_seg);
+    const long long total = uniform64(s_pref[batch]) * vrows;
+    long long S = kMinSeg8 * few;
+    if (!few) {
+        S = max(div64(total + nseg - 1, nseg), (long long)kMinSeg8);
         S = (S + TOK - 1) & ~(long long)(TOK - 1);
     }
     if (blockIdx.x == 0) {  // the combine's copy of the prefix, and S
@@ -1322,15 +1349,10 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
 struct Attn8Shape {
     int batch, hq, hkv, page, width, dim, span;
     bool stream;
-    int tile, tiles, nseg, min_seg;  // stream
-    int cmax, chunk;                 // general
-    size_t slots, bytes;             // slots: (partial, q head) pairs
+    int tile, tiles, nseg, short_segs;  // stream
+    int cmax, chunk;                    // general
+    size_t slots, bytes;                // slots: (partial, q head) pairs
 };
-
-// Tokens of a segment, at least (a power of two, whole steps): 7 ragged rows of
-// up to 9001 tokens, float32, 12.4 us of kernel time at 64 or 128, 18.9 at 32
-// (which leaves no wave over); 4 short rows, D = 64, 5.8 at 64, 7.1 at 128.
-constexpr int kMinSeg8 = 64;
 
 template <int D>
 int stream_occ(int dtype) {
@@ -1345,7 +1367,7 @@ Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int widt
     if (hq % hkv != 0) inval("q heads must be a multiple of kv heads (contiguous GQA groups)");
     const long long span = (long long)width * page;
     if (span > (1LL << 30)) inval("table capacity too large");
-    if ((long long)std::min(batch, kStreamScanRows) * hq >= 1 << 24)
+    if ((long long)std::min(batch, kScanRows8) * hq >= 1 << 24)
         inval("attention problem too large for one launch");
     Attn8Shape s{};
     s.batch = batch; s.hq = hq; s.hkv = hkv; s.page = page; s.width = width; s.dim = dim;
@@ -1359,10 +1381,10 @@ Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int widt
         s.tiles = (group + s.tile - 1) / s.tile;
         const int occ = dim <= 64 ? stream_occ<64>(dtype)
                                   : dim <= 128 ? stream_occ<128>(dtype) : stream_occ<256>(dtype);
-        s.min_seg = kMinSeg8;
-        const long long rows = (long long)std::min(batch, kStreamScanRows) * hkv * s.tiles;
-        const long long most = rows * ((span + s.min_seg - 1) / s.min_seg);
+        const long long rows = (long long)std::min(batch, kScanRows8) * hkv * s.tiles;
+        const long long most = rows * ((span + kMinSeg8 - 1) / kMinSeg8);
         s.nseg = (int)std::min(std::min((long long)4 * cus * occ, most), (long long)kMaxPieces8);
+        s.short_segs = std::min(s.nseg, (dim <= 64 ? 8 : 4) * cus);
         s.slots = (size_t)2 * s.nseg * s.tile;
     } else {
         if (hkv > 65535 || batch > 65535) inval("attention: batch and kv heads must be <= 65535");
@@ -1379,7 +1401,7 @@ Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int widt
         s.slots = (size_t)batch * hq * s.cmax;
     }
     s.bytes = (((s.slots * 2 + 63) & ~(size_t)63) + s.slots * dim) * sizeof(float) +
-              (s.stream ? (std::min(batch, kStreamScanRows) + 2) * sizeof(long long) : 0);
+              (s.stream ? (std::min(batch, kScanRows8) + 2) * sizeof(long long) : 0);
     return s;
 }
 
@@ -1399,15 +1421,15 @@ void attn8_stream_run(const Attn8Shape& sh, const Attn8Args& a, float* ml, float
     long long* pref = (long long*)(acc + sh.slots * dim);
     const float scale = (1.0f / sqrtf((float)dim)) * kLog2e;
     const auto kernel = dim == D ? attn8_stream<T, D, true> : attn8_stream<T, D, false>;
-    for (int b0 = 0; b0 < sh.batch; b0 += kStreamScanRows) {
-        const int nb = std::min(kStreamScanRows, sh.batch - b0);
+    for (int b0 = 0; b0 < sh.batch; b0 += kScanRows8) {
+        const int nb = std::min(kScanRows8, sh.batch - b0);
         const T* q = (const T*)a.q + (size_t)b0 * sh.hq * dim;
         T* out = (T*)a.out + (size_t)b0 * sh.hq * dim;
         const int* lens = a.lens ? a.lens + b0 : nullptr;
         kernel<<<(sh.nseg + 3) / 4, 256, 0, s>>>(
             q, a.kp, a.vp, a.ks, a.vs, a.table + (size_t)b0 * sh.width, lens, ml, acc, pref, out,
             nb, sh.hq, sh.hkv, sh.tile, sh.tiles, a.blocks, FastDiv(sh.page), sh.width, sh.span,
-            sh.nseg, sh.min_seg, scale, dim);
+            sh.nseg, sh.short_segs, scale, dim);
         launch_check("int8 decode attention kernel launch");
         combine8(ml, acc, lens, out, Streamed8{pref, nb}, nb, sh.hq, sh.hkv, dim, sh.span, sh.tile,
                  sh.tiles, s);

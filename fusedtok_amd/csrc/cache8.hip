@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kMaxDim8 = 512;
 constexpr int kMaxPage8 = 1024;      // rows of a block (the append's row map in LDS)
-constexpr int kExtendSeqs = 4096;    // sequences of one table call (two prefixes in LDS)
+constexpr int kExtendSeqs = 4096;    // sequences of one table call (their prefixes in LDS)
 
 void check_pools(int blocks, int hkv, int page, int dim) {
     if (blocks < 0 || hkv < 1 || dim < 1) inval("int8 cache: blocks >= 0, kv heads >= 1, dim >= 1");
@@ -72,7 +72,8 @@ struct FastDiv {
 // token's sequence in the prefix by bisection: one launch without a hand-over
 // between workgroups. A token's slot is worked out from the free list, not
 // from the table entry that another workgroup may be writing. What bounds it:
-// launch and the dependent chain length -> scan -> bisection -> table.
+// launch and the dependent chain length -> scan -> bisection -> table: 3.9 us
+// for 64 sequences, 7.3 for 2000, 5.4 for 125k tokens of 32 prompts.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void block_table_extend_kernel(
     int* __restrict__ table, const int* __restrict__ lens, const int* __restrict__ counts,
@@ -278,11 +279,18 @@ struct Codes {
     unsigned w[V / 4];
 } __attribute__((aligned(V)));
 
-// A unit is (window of `window` consecutive fresh rows, kv head, K or V): the
-// runs that start in the window, one after another (a run may reach past it).
-// UT threads a unit, 256 a workgroup. Windows are as long as a block where
-// that leaves enough units (about one run each: a prompt), else one row (a
-// decode step). A lane has V values of a row; the first kKeep passes of a run
+// UT threads (a wave or a workgroup) have a run, kv head and pool at a time.
+// How runs are found is chosen by the number of fresh rows, since how many
+// there are a run the host does not know:
+//   few rows        (a decode step) a unit a row; those that start no run end;
+//   up to 1024      every workgroup lists the starts of all runs in LDS, and
+//                   the units share them out;
+//   more            a unit a window of as many rows as a block has: the runs
+//                   that start in it, one after another (about one, in prompts).
+// (8 heads, D = 128, blocks of 16, graph replays, us, the three in turn: a step
+// of 64 sequences 5.1, 6.2, 23.8, of 512 8.4, 8.7, 23.2, of 1024 12.6, 13.2, 23.4;
+// a prompt of 512 tokens 9.7, 6.3, 5.8, of 2048 28.7, 10.3, 6.2.)
+// A lane has V values of a row; the first kKeep passes of a run
 // stay in registers between the maximum and the codes, so a run is read once.
 // Rows in order, as a sequence's are, need no map; others (gaps, a slot twice)
 // go by a map in LDS from the block's row to the last fresh row for it. Values
@@ -290,9 +298,15 @@ struct Codes {
 // for two 16-bit values), and only a run with an infinity or NaN in it, which
 // the maximum shows, goes through the code that looks at each value.
 //
-// What bounds it: memory latency in a decode step; for prompts, HBM and the
-// ~5 vector instructions a value.
-template <typename T, int V, int UT>
+// What bounds it: memory latency in a decode step (4.1 us for 64 rows); for
+// prompts, HBM: 30k rows, 8 heads, D = 128, bf16, 41 us, 4.4 TB/s read and written,
+// where a large copy has 4.8. (Values widened and compared one by one: 61 us,
+// bound by the vector ALU.)
+constexpr long long kRowEach = 16;  // units a CU, at most, where each row has its own
+constexpr int kListTokens = 1024;   // rows whose runs are listed, at most
+constexpr int kListWgs = 4;         // workgroups a CU of a listed call, at most
+
+template <typename T, int V, int UT, bool LISTED>
 __global__ __launch_bounds__(256) void kv_append8_kernel(
     const T* __restrict__ k_new, const T* __restrict__ v_new, const int* __restrict__ slots,
     signed char* __restrict__ k_pool, signed char* __restrict__ v_pool,
@@ -300,20 +314,15 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
     int nslots, FastDiv page, FastDiv lanes, int window, long long units) {
     constexpr int kKeep = 4, kUnits = 256 / UT;
     __shared__ int s_map[kUnits][kMaxPage8];
+    __shared__ int s_runs[LISTED ? kListTokens : 1];
     __shared__ unsigned s_red[4];
     const int lane = threadIdx.x & 63;
     const int ut = UT == 64 ? lane : (int)threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long unit = (long long)blockIdx.x * kUnits + (UT == 64 ? wave : 0);
-    if (unit >= units) return;
+    if (!LISTED && unit >= units) return;
     int* const map = s_map[UT == 64 ? wave : 0];
-    // (units / 2 <= tokens * heads < 2^31: checked by the host)
-    const bool is_v = unit >= units / 2;
-    const int wh = (int)(is_v ? unit - units / 2 : unit);
-    const int h = heads.mod(wh), hkv = (int)heads.d, first = heads.div(wh) * window;
-    const T* const x = (is_v ? v_new : k_new) + (size_t)h * dim;
-    signed char* const pool = is_v ? v_pool : k_pool;
-    float* const scales = is_v ? v_scales : k_scales;
+    const int hkv = (int)heads.d;
     const size_t row_stride = (size_t)hkv * dim;
     auto sync = [&] {
         if (UT == 64) wave_lds_order();
@@ -332,152 +341,204 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
     auto slot_of = [&](int t) { return t >= 0 && t < tokens ? slots[t] : -1; };
     auto block_of = [&](int s) { return s >= 0 && s < nslots ? page.div(s) : -1; };
 
-    for (int w0 = 0; w0 < window; w0 += 64) {
-        const int t = first + w0 + lane;
-        const int mine = w0 + lane < window ? block_of(slot_of(t)) : -1;
-        unsigned long long starts = __ballot(mine >= 0 && block_of(slot_of(t - 1)) != mine);
-        while (starts) {
-            const int at = __builtin_ctzll(starts);
-            starts &= starts - 1;
-            const int i = first + w0 + at;             // the run's first fresh row
-            const int block = __shfl(mine, at, 64);
-            const int slot0 = slots[i], row0 = page.mod(slot0);
-            // its length, and whether its rows are in order
-            int n = 0;
-            bool ordered = true;
-            for (;; n += 64) {
-                const int s = slot_of(i + n + lane);
-                const unsigned long long out = __ballot(block_of(s) != block);
-                const int got = out ? __builtin_ctzll(out) : 64;
-                ordered = ordered && !__any(lane < got && s != slot0 + n + lane);
-                if (got < 64) {
-                    n += got;
-                    break;
-                }
+    // the run of K or V (is_v), head h, whose first fresh row is i, in `block`
+    auto run = [&](int i, int block, bool is_v, int h) {
+        const T* const x = (is_v ? v_new : k_new) + (size_t)h * dim;
+        signed char* const pool = is_v ? v_pool : k_pool;
+        float* const scales = is_v ? v_scales : k_scales;
+        const int slot0 = slots[i], row0 = page.mod(slot0);
+        // its length, and whether its rows are in order
+        int n = 0;
+        bool ordered = true;
+        for (;; n += 64) {
+            const int s = slot_of(i + n + lane);
+            const unsigned long long out = __ballot(block_of(s) != block);
+            const int got = out ? __builtin_ctzll(out) : 64;
+            ordered = ordered && !__any(lane < got && s != slot0 + n + lane);
+            if (got < 64) {
+                n += got;
+                break;
             }
-            n = __builtin_amdgcn_readfirstlane(n);
-            bool over = row0 == 0;
-            if (!ordered) {
-                sync();
-                for (int r = ut; r < (int)page.d; r += UT) map[r] = -1;
-                sync();
-                for (int k = ut; k < n; k += UT) atomicMax(&map[page.mod(slots[i + k])], i + k);
-                sync();
-                over = map[0] >= 0;
-            }
-            const int base = ordered ? row0 : 0;                 // the rows gone over
-            const int nvec = (ordered ? n : (int)page.d) * (int)lanes.d;
-            // the fresh row for the j-th vector of them, -1 where there is none
-            auto source = [&](int r) { return ordered ? i + r : map[r]; };
-            using R = Raw<T, V>;
-            R keep[kKeep];
-            auto load = [&](int j, R& v) {
-                const int r = lanes.div(j), src = source(r);
-                if (src >= 0) v.load(x + src * row_stride + V * (j - r * (int)lanes.d));
-                else v.zero();
-            };
-            unsigned bits = 0;
+        }
+        n = __builtin_amdgcn_readfirstlane(n);
+        bool over = row0 == 0;
+        if (!ordered) {
+            sync();
+            for (int r = ut; r < (int)page.d; r += UT) map[r] = -1;
+            sync();
+            for (int k = ut; k < n; k += UT) atomicMax(&map[page.mod(slots[i + k])], i + k);
+            sync();
+            over = map[0] >= 0;
+        }
+        const int base = ordered ? row0 : 0;                 // the rows gone over
+        const int nvec = (ordered ? n : (int)page.d) * (int)lanes.d;
+        // the fresh row for the j-th vector of them, -1 where there is none
+        auto source = [&](int r) { return ordered ? i + r : map[r]; };
+        using R = Raw<T, V>;
+        R keep[kKeep];
+        auto load = [&](int j, R& v) {
+            const int r = lanes.div(j), src = source(r);
+            if (src >= 0) v.load(x + src * row_stride + V * (j - r * (int)lanes.d));
+            else v.zero();
+        };
+        unsigned bits = 0;
 #pragma unroll
-            for (int p = 0; p < kKeep; ++p) {
-                const int j = p * UT + ut;
-                if (j < nvec) load(j, keep[p]);
-            }
+        for (int p = 0; p < kKeep; ++p) {
+            const int j = p * UT + ut;
+            if (j < nvec) load(j, keep[p]);
+        }
 #pragma unroll
-            for (int p = 0; p < kKeep; ++p)
-                if (p * UT + ut < nvec) bits = keep[p].most(bits);
-            for (int j = kKeep * UT + ut; j < nvec; j += UT) {
+        for (int p = 0; p < kKeep; ++p)
+            if (p * UT + ut < nvec) bits = keep[p].most(bits);
+        for (int j = kKeep * UT + ut; j < nvec; j += UT) {
+            R v;
+            load(j, v);
+            bits = v.most(bits);
+        }
+        const size_t bh = (size_t)block * hkv + h;
+        const float held = over ? 0.0f : scales[bh];
+        if constexpr (sizeof(T) == 2) bits = max(bits & 0xffffu, bits >> 16);
+        bits = unit_max(bits);
+        float most = R::value_of(bits);
+        const bool finite = bits < R::kInf;
+        if (!finite) {  // of the finite values alone
+            float m = 0.0f;
+            for (int j = ut; j < nvec; j += UT) {
                 R v;
                 load(j, v);
-                bits = v.most(bits);
-            }
-            const size_t bh = (size_t)block * hkv + h;
-            const float held = over ? 0.0f : scales[bh];
-            if constexpr (sizeof(T) == 2) bits = max(bits & 0xffffu, bits >> 16);
-            bits = unit_max(bits);
-            float most = R::value_of(bits);
-            const bool finite = bits < R::kInf;
-            if (!finite) {  // of the finite values alone
-                float m = 0.0f;
-                for (int j = ut; j < nvec; j += UT) {
-                    R v;
-                    load(j, v);
 #pragma unroll
-                    for (int c = 0; c < V; ++c) {
-                        const float a = fabsf(v.value(c));
-                        m = fmaxf(m, a < INFINITY ? a : 0.0f);
-                    }
+                for (int c = 0; c < V; ++c) {
+                    const float a = fabsf(v.value(c));
+                    m = fmaxf(m, a < INFINITY ? a : 0.0f);
                 }
-                most = __uint_as_float(unit_max(__float_as_uint(m)));
             }
-            const float now = fmaxf(fmaxf(held, most / 127.0f), kLeastScale);
-            const float inv = 1.0f / now;
-            signed char* const codes = pool + bh * page.d * dim;
-            auto store = [&](int j, const R& v) {
+            most = __uint_as_float(unit_max(__float_as_uint(m)));
+        }
+        const float now = fmaxf(fmaxf(held, most / 127.0f), kLeastScale);
+        const float inv = 1.0f / now;
+        signed char* const codes = pool + bh * page.d * dim;
+        auto store = [&](int j, const R& v) {
+            const int r = lanes.div(j);
+            if (source(r) < 0) return;
+            Codes<V> o;
+#pragma unroll
+            for (int c = 0; c < V; c += 4)
+                o.w[c / 4] = codes4(v.value(c), v.value(c + 1), v.value(c + 2),
+                                    v.value(c + 3), inv);
+            if (!finite) {
+#pragma unroll
+                for (int c = 0; c < V; c += 4) {
+                    o.w[c / 4] = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o.w[c / 4] |= (unsigned)(unsigned char)code8(v.value(c + i), inv)
+                                      << (8 * i);
+                }
+            }
+            *reinterpret_cast<Codes<V>*>(codes + (size_t)(base + r) * dim +
+                                         V * (j - r * (int)lanes.d)) = o;
+        };
+#pragma unroll
+        for (int p = 0; p < kKeep; ++p) {
+            const int j = p * UT + ut;
+            if (j < nvec) store(j, keep[p]);
+        }
+        for (int j = kKeep * UT + ut; j < nvec; j += UT) {
+            R v;
+            load(j, v);
+            store(j, v);
+        }
+        if (!over && now > held) {  // the block's other rows
+            const float ratio = held / now;
+            for (int j = ut; j < (int)(page.d * lanes.d); j += UT) {
                 const int r = lanes.div(j);
-                if (source(r) < 0) return;
-                Codes<V> o;
+                if (ordered ? (unsigned)(r - row0) < (unsigned)n : map[r] >= 0) continue;
+                Codes<V>* p = reinterpret_cast<Codes<V>*>(codes + (size_t)V * j);
+                Codes<V> o = *p;
 #pragma unroll
-                for (int c = 0; c < V; c += 4)
-                    o.w[c / 4] = codes4(v.value(c), v.value(c + 1), v.value(c + 2),
-                                        v.value(c + 3), inv);
-                if (!finite) {
-#pragma unroll
-                    for (int c = 0; c < V; c += 4) {
-                        o.w[c / 4] = 0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            o.w[c / 4] |= (unsigned)(unsigned char)code8(v.value(c + i), inv)
-                                          << (8 * i);
-                    }
+                for (int c = 0; c < V / 4; ++c) {
+                    const unsigned u = o.w[c];
+                    o.w[c] = codes4((float)(signed char)u, (float)(signed char)(u >> 8),
+                                    (float)(signed char)(u >> 16), (float)((int)u >> 24),
+                                    ratio);
                 }
-                *reinterpret_cast<Codes<V>*>(codes + (size_t)(base + r) * dim +
-                                             V * (j - r * (int)lanes.d)) = o;
-            };
+                *p = o;
+            }
+        }
+        if (ut == 0) scales[bh] = now;
+    };
+
+    if constexpr (LISTED) {
+        // the starts of all runs: a thread looks at consecutive fresh rows
+        constexpr int PER = kListTokens / 256;
+        const int per = (tokens + 255) / 256, t0 = (int)threadIdx.x * per;
+        int s[PER];
 #pragma unroll
-            for (int p = 0; p < kKeep; ++p) {
-                const int j = p * UT + ut;
-                if (j < nvec) store(j, keep[p]);
-            }
-            for (int j = kKeep * UT + ut; j < nvec; j += UT) {
-                R v;
-                load(j, v);
-                store(j, v);
-            }
-            if (!over && now > held) {  // the block's other rows
-                const float ratio = held / now;
-                for (int j = ut; j < (int)(page.d * lanes.d); j += UT) {
-                    const int r = lanes.div(j);
-                    if (ordered ? (unsigned)(r - row0) < (unsigned)n : map[r] >= 0) continue;
-                    Codes<V>* p = reinterpret_cast<Codes<V>*>(codes + (size_t)V * j);
-                    Codes<V> o = *p;
+        for (int k = 0; k < PER; ++k) s[k] = k < per ? slot_of(t0 + k) : -1;
+        int before = block_of(slot_of(t0 - 1));
+        unsigned starts = 0;
 #pragma unroll
-                    for (int c = 0; c < V / 4; ++c) {
-                        const unsigned u = o.w[c];
-                        o.w[c] = codes4((float)(signed char)u, (float)(signed char)(u >> 8),
-                                        (float)(signed char)(u >> 16), (float)((int)u >> 24),
-                                        ratio);
-                    }
-                    *p = o;
-                }
+        for (int k = 0; k < PER; ++k) {
+            const int block = block_of(s[k]);
+            if (block >= 0 && block != before) starts |= 1u << k;
+            before = block;
+        }
+        const int mine = __popc(starts);
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(incl, o, 64);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 63) s_red[wave] = incl;
+        __syncthreads();
+        int at = incl - mine, runs = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) at += s_red[w];
+            runs += s_red[w];
+        }
+        for (; starts; starts &= starts - 1) s_runs[at++] = t0 + __builtin_ctz(starts);
+        __syncthreads();  // (s_red is free again too)
+        const int all = runs * 2 * hkv;  // <= 2 tokens * heads
+        const int step = (int)gridDim.x * kUnits;
+        for (int u = (int)unit; u < all; u += step) {
+            const int rk = heads.div(u);  // (run, K or V)
+            const int i = __builtin_amdgcn_readfirstlane(s_runs[rk >> 1]);
+            run(i, block_of(slots[i]), rk & 1, u - rk * hkv);
+        }
+    } else {
+        // (units / 2 <= tokens * heads < 2^31: checked by the host)
+        const bool is_v = unit >= units / 2;
+        const int wh = (int)(is_v ? unit - units / 2 : unit);
+        const int h = heads.mod(wh), first = heads.div(wh) * window;
+        for (int w0 = 0; w0 < window; w0 += 64) {
+            const int t = first + w0 + lane;
+            const int mine = w0 + lane < window ? block_of(slot_of(t)) : -1;
+            unsigned long long starts = __ballot(mine >= 0 && block_of(slot_of(t - 1)) != mine);
+            for (; starts; starts &= starts - 1) {
+                const int at = __builtin_ctzll(starts);
+                run(first + w0 + at, __shfl(mine, at, 64), is_v, h);
             }
-            if (ut == 0) scales[bh] = now;
         }
     }
 }
-
-// Fresh rows from which windows are as long as a block: so many (row, head)
-// pairs fill the GPU with units a block long.
-constexpr long long kAppendLong = 1 << 15;
 
 template <typename T, int V, int UT>
 void append8_run(const T* k_new, const T* v_new, const int* slots, signed char* k_pool,
                  signed char* v_pool, float* k_scales, float* v_scales, int tokens, int hkv,
                  int dim, int blocks, int page, hipStream_t s) {
-    const int window = (long long)tokens * hkv >= kAppendLong ? page : 1;
+    const int cus = dev_info().cu_count;
+    const long long pairs = 2LL * tokens * hkv;  // one a row, head and pool
+    const bool row_each = pairs <= kRowEach * cus;
+    const bool listed = !row_each && tokens <= kListTokens;
+    const int window = row_each ? 1 : page;
     const long long units = 2LL * ((tokens + window - 1) / window) * hkv;
-    const long long wgs = (units * UT + 255) / 256;
+    const long long wgs = listed ? std::min((pairs * UT + 255) / 256, (long long)kListWgs * cus)
+                                 : (units * UT + 255) / 256;
     if (wgs >= 1LL << 24) inval("kv_append_paged_int8: too many rows for one call");
-    kv_append8_kernel<T, V, UT><<<(unsigned)wgs, 256, 0, s>>>(
+    const auto kernel = listed ? kv_append8_kernel<T, V, UT, true> : kv_append8_kernel<T, V, UT, false>;
+    kernel<<<(unsigned)wgs, 256, 0, s>>>(
         k_new, v_new, slots, k_pool, v_pool, k_scales, v_scales, tokens, FastDiv(hkv), dim,
         blocks * page, FastDiv(page), FastDiv(dim / V), window, units);
     launch_check("int8 kv append kernel launch");
@@ -499,7 +560,9 @@ void append8(const T* k_new, const T* v_new, const int* slots, signed char* k_po
     auto aligned = [](const void* p, size_t by) { return (uintptr_t)p % by == 0; };
     const bool eight = dim % 8 == 0 && aligned(k_new, 16) && aligned(v_new, 16) &&
                        aligned(k_pool, 8) && aligned(v_pool, 8);
-    // a wave a unit where a block stays in its registers
+    // a wave has a run where a block stays in its registers, else a workgroup
+    // (16384 prompt tokens, 8 heads, D = 128: blocks of 16 22.3 us by waves, 43.0
+    // by workgroups; blocks of 64 28.2 and 22.8)
     const bool wave = page * (dim / (eight ? 8 : 4)) <= 4 * 64;
     if (eight && wave) go(I8{}, Wave{});
     else if (eight) go(I8{}, Group{});
@@ -569,7 +632,7 @@ constexpr int kWavePieces8 = 32;   // folded by one wave, at most
 // `per` (1 or 4) q heads a workgroup, a wave each; a head of many pieces is
 // folded by the whole workgroup, afterwards. Where heads are few, gridDim.y
 // workgroups share the dims of one of many pieces. Bound by latency: the row's
-// place, its pieces' (m, l), their sums.
+// place, its pieces' (m, l) and sums, the launch; 4-7 us.
 template <typename T, typename Pieces>
 __global__ __launch_bounds__(256) void attn8_combine(
     const float* __restrict__ ws_ml, const float* __restrict__ ws_acc,
@@ -723,8 +786,8 @@ void combine8(const float* ml, const float* acc, const int* lens, T* out, const 
               int batch, int hq, int hkv, int dim, int span, int tile, int tiles, hipStream_t s) {
     const int heads = batch * hq;
     // few heads have many pieces each: a workgroup a head, or one for 32 of its
-    // dims (one row of 131072 tokens, 8 heads, attention
-    // and combine: 54 -> 27 us)
+    // dims (one row of 131072 tokens, 8 heads, attention and combine: 54 -> 27 us);
+    // many have few: four a workgroup (4096 heads: 19 -> 6.9 us)
     const int per = heads >= 4 * dev_info().cu_count && 256 % dim == 0 ? 4 : 1;
     const int parts = per == 1 && heads < dev_info().cu_count && dim % 32 == 0 ? dim / 32 : 1;
     attn8_combine<T, Pieces><<<dim3((heads + per - 1) / per, parts), 256, 0, s>>>(
@@ -877,14 +940,15 @@ constexpr int kScanRows8 = 1024;  // sequences of a launch (their prefixes are i
 //
 // Work split. The rows are (sequence b, kv head, tile of up to 16 q heads),
 // b-major, len_b tokens each, laid end to end; every WAVE takes one equal
-// contiguous segment of that range, whatever the length mix; where kMinSeg8
-// tokens a segment leave waves over, each row is rounded up to whole segments,
-// so that none has two rows. A segment is one or more pieces, one per row it
-// touches. A piece that is a whole row is
-// normalised and stored; another leaves its partial in the segment's slot 1
-// if its row reaches the segment's end, else in slot 0: a segment has at most
-// one of each. Waves share nothing but the length prefix, so after it there
-// is no barrier and no merge in the kernel.
+// contiguous segment of that range, whatever the length mix; for few tokens
+// (kMinSeg8) each row is rounded up to whole segments, so that none has two
+// rows. A segment is one or more pieces, one per row it touches. A piece that
+// is a whole row is normalised and stored; another leaves its partial in the
+// segment's slot 1 if its row reaches the segment's end, else in slot 0: a
+// segment has at most one of each. Waves share nothing but the length prefix,
+// so after it there is no barrier and no merge in the kernel. (More segments
+// than waves, or smaller ones behind the large, cost more at their starts than
+// the even end saves: 32 ragged rows 215 against 201 us with twice as many.)
 //
 // A step is TOK tokens (32; 64 for D = 64), K and V of the next one - of the
 // next piece at a piece's end - in flight in registers while this one is
@@ -899,8 +963,8 @@ constexpr int kScanRows8 = 1024;  // sequences of a launch (their prefixes are i
 //           bits), so every product is exact and sums are float32. Any order
 //           of dims serves if q has the same: the lane reads 16-byte chunks.
 //           (Integer products with q in base-256 digits take 56 vector
-//           instructions a step less, but the loop waits on memory either way
-//           and the digits cost every piece 3-7 us at its start);
+//           instructions a step less, but the loop waits on memory either way:
+//           32 ragged rows 197 us both, 4 short ones 8.7 against 8.1);
 //  softmax  lane (r, g) holds head r's scores of tokens 4g+i (+ 16 a tile);
 //           scaled by the block's K scale, running maximum over the 4 lanes
 //           of a head; the weight takes the block's V scale, then goes into 2
@@ -916,6 +980,15 @@ constexpr int kScanRows8 = 1024;  // sequences of a launch (their prefixes are i
 //
 // Masked tokens (behind the piece, holes) weigh 0 exactly: score -inf, V scale
 // 0, the row read in its place a real one (its own last, or block 0's).
+//
+// What bounds it: HBM. Behind the first 6 us (lengths, piece, table, first
+// rows) 32 rows of 512-32768 tokens, 32 / 8 heads, D = 128, bf16, read at 6.6
+// TB/s (197 us in all; bare reads of such pages reach 6.7-6.8); 64 rows of 4097,
+// 64 / 8 heads, fp16, take 95 us, 2 rows of 131071, D = 64, 49. The vector ALU is
+// busy 55-60% of the cycles, the matrix cores 14-18%. Two waves a SIMD: at three
+// the registers spill (226 against 210 us for the first of these, all else
+// equal). For short rows, latency: 5.8 us for 4 rows of 128-1024 tokens, D = 64,
+// and 4.2 for the combine.
 // ---------------------------------------------------------------------------
 typedef float f32x4_8 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));

@@ -1111,7 +1111,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
     // few tokens: a segment a stretch of S tokens of one row
     const long long pad1 = uniform64(s_prefix[1][batch]) * vrows;
     const long long pad2 = uniform64(s_prefix[2][batch]) * vrows;
-    const int few = pad1 <= (long long)short_segs * kMinSeg8     ? 1
+    const int few = pad1 <= (long long)short_segs * kMinSeg8   ? 1
                     : pad2 <= (long long)nseg * (2 * kMinSeg8) ? 2
                                                                : 0;
     const long long* const s_pref = s_prefix[few];

@@ -222,6 +222,22 @@ def test_append_padded_batch(rows, hkv, page, d, dtype):
     check_append(cache, k, v, slots.reshape(-1), dtype)
 
 
+@pytest.mark.parametrize("b", [1, 100, 1024, 1025, 3000])
+@pytest.mark.parametrize("page,d", [(16, 64), (5, 32), (64, 128)])
+def test_append_step(b, page, d):
+    """One token for each of b sequences, in the middle of a block, at its
+    start and at its end."""
+    rng = np.random.default_rng(b)
+    nb = b + 2
+    cache = pools(rng, nb, 2, page, d)
+    rows = rng.integers(0, page, b)
+    rows[::5], rows[1::5] = 0, page - 1
+    slots = rng.permutation(nb)[:b] * page + rows
+    slots[3::11] = -1
+    k, v = (rng.standard_normal((b, 2, d)) * rng.choice([0.1, 5], (b, 1, 1)) for _ in range(2))
+    check_append(cache, k, v, slots, torch.bfloat16)
+
+
 @pytest.mark.parametrize("page,d", [(16, 128), (5, 64), (64, 128)])
 def test_append_odd_slots(page, d):
     """Slots outside the pools, gaps between a block's rows, rows out of
@@ -240,7 +256,7 @@ def test_append_odd_slots(page, d):
 
 
 @pytest.mark.parametrize("rows,hkv,page,d", [(150, 1, 16, 64), (700, 64, 16, 64),
-                                             (900, 40, 64, 128)])
+                                             (900, 40, 64, 128), (2000, 8, 16, 64)])
 def test_append_longer_run_than_a_block(rows, hkv, page, d):
     """The same rows again and again: a run of more rows than the block has,
     and one that reaches over several windows."""
@@ -611,6 +627,28 @@ def test_captured_step_replays():
         for x, y in zip(graphed["cache"] + [graphed["table"], graphed["lens"], graphed["n_free"]],
                         eager["cache"] + [eager["table"], eager["lens"], eager["n_free"]]):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("d", [128, 36])
+def test_values_that_are_not_finite(d):
+    """A query or a scale that is not finite reaches the rows that attend it
+    and no other."""
+    rng = np.random.default_rng(13)
+    lens = [40, 70, 100]
+    (kp, vp, ks, vs), table = paged(rng, 3, 2, 16, d, lens)
+    q = rng.standard_normal((3, 8, d)).astype(np.float32)
+    args = [dev(x) for x in (q, kp, vp, ks, vs)]
+    clean = ft.attention_decode_paged_int8(*args, i32(table), i32(lens))
+    bad_q, bad_v = args[0].clone(), args[4].clone()
+    bad_q[0, 3, 1] = float("nan")
+    bad_q[1, 0, 2] = float("inf")
+    bad_v[int(table[2, 1]), 1] = float("nan")
+    out = ft.attention_decode_paged_int8(bad_q, *args[1:4], bad_v, i32(table), i32(lens))
+    hit = torch.zeros(3, 8, dtype=torch.bool, device=DEV)
+    hit[0, 3] = hit[1, 0] = True
+    hit[2, 4:] = True
+    assert torch.equal(out[~hit], clean[~hit])
+    assert out[hit].isnan().any(-1).all()
 
 
 def test_calls_on_two_streams():

@@ -560,11 +560,14 @@ def _one_device(names, tensors):
 # small call of attention, append and tables).
 
 
+_T8, _TI, _TF = torch.int8, torch.int32, torch.float32
+
+
 def _pools_ready(k_pool, v_pool, k_scales, v_scales):
     """The usual case of the four cache operands."""
     shape = k_pool.shape
-    return (k_pool.dtype is torch.int8 and v_pool.dtype is torch.int8 and v_pool.shape == shape and
-            k_scales.dtype is torch.float32 and v_scales.dtype is torch.float32 and
+    return (k_pool.dtype is _T8 and v_pool.dtype is _T8 and v_pool.shape == shape and
+            k_scales.dtype is _TF and v_scales.dtype is _TF and
             k_scales.shape == shape[:2] and v_scales.shape == shape[:2] and
             k_pool.is_contiguous() and v_pool.is_contiguous() and k_scales.is_contiguous() and
             v_scales.is_contiguous() and
@@ -576,7 +579,7 @@ def _pools_ready(k_pool, v_pool, k_scales, v_scales):
 def _i32_ready(device, *tensors):
     """int32, contiguous and on that device."""
     for t in tensors:
-        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != device:
+        if t.dtype is not _TI or not t.is_contiguous() or t.get_device() != device:
             return False
     return True
 

@@ -1047,22 +1047,33 @@ __device__ __forceinline__ void scan8(const int* __restrict__ lens, int batch, i
     if (lane == 63) pref[batch] = incl;
 }
 
-// A stretch of one row (b, virtual head kv): tokens [t0, t0 + n), up to flat
-// position next. (No padding: the compiler keeps a copied struct's padding in
-// LDS, and to place it reads the workgroup's size from the dispatch packet in
-// host memory, 3-7 us at the kernel's start.)
+// floor(a / b) for 0 <= a, b > 0 and a quotient below 2^20, by way of a float32
+// one, which is then off by at most one: an address's worth of latency where
+// a 64-bit division, or a float64 one, takes a microsecond off every start.
+__device__ __forceinline__ int small_div(long long a, int b) {
+    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+    const long long r = a - (long long)q * b;
+    return r < 0 ? q - 1 : r >= b ? q + 1 : q;
+}
+
+// A stretch of one row: tokens [t0, t0 + n) of sequence b for q heads [h0, h0 +
+// heads), up to flat position next. (No padding: the compiler keeps a copied
+// struct's padding in LDS, and to place it reads the workgroup's size from the
+// dispatch packet in host memory, 3-7 us at the kernel's start.)
 struct Piece8 {
     long long next;
     int b, kv, t0, n;
+    int h0, heads;
     int whole;  // the row's every token
-    int heads;  // q heads of the row
+    int ends;   // the row reaches the segment's end
 };
 
-// The row that holds flat position pos (in units of 1 / vrows of the prefix):
-// the sequences' ends are counted 64 at a time, by the lanes.
+// The row that holds flat position pos (in units of 1 / vrows of the prefix),
+// cut at seg_end: the sequences' ends are counted 64 at a time, by the lanes.
 __device__ __forceinline__ Piece8 piece8(const long long* s_pref, int batch, int vrows,
-                                         long long pos, long long seg_hi, int lane, int group,
-                                         int tile, int tiles, const long long* s_tokens) {
+                                         long long pos, long long seg_end, int lane, int group,
+                                         int tile, const FastDiv& tiles,
+                                         const long long* s_tokens) {
     int b = 0;
     for (int step = (batch + 63) >> 6;; step = 1) {
         const int at = b + (lane + 1) * step;
@@ -1074,14 +1085,19 @@ __device__ __forceinline__ Piece8 piece8(const long long* s_pref, int batch, int
     p.b = b;
     const long long pb = uniform64(s_pref[b]), base = pb * vrows;
     const int len = (int)(uniform64(s_pref[b + 1]) - pb);
-    p.kv = (int)div64(pos - base, len);
-    p.t0 = (int)(pos - base - (long long)p.kv * len);
-    p.next = min(seg_hi, base + (long long)(p.kv + 1) * len);
     // (s_pref may be of padded lengths, s_tokens is of the true ones)
     const int end = (int)(uniform64(s_tokens[b + 1]) - uniform64(s_tokens[b]));
+    const int v = __builtin_amdgcn_readfirstlane(small_div(pos - base, len));
+    const long long row_end = base + (long long)(v + 1) * len;
+    p.t0 = (int)(pos - base - (long long)v * len);
+    p.next = min(seg_end, row_end);
     p.n = min((int)(p.next - pos), end - p.t0);
     p.whole = p.t0 == 0 && p.n == end;
-    p.heads = min(tile, group - p.kv % tiles * tile);
+    p.ends = row_end >= seg_end;
+    p.kv = tiles.div(v);
+    const int first = (v - p.kv * (int)tiles.d) * tile;
+    p.h0 = p.kv * group + first;
+    p.heads = min(tile, group - first);
     return p;
 }
 
@@ -1093,9 +1109,9 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                   const float* __restrict__ v_scales, const int* __restrict__ table,
                   const int* __restrict__ lens, float* __restrict__ ws_ml,
                   float* __restrict__ ws_acc, long long* __restrict__ pref_out,
-                  T* __restrict__ out, int batch, int hq, int hkv, int tile, int tiles,
+                  T* __restrict__ out, int batch, int hq, int hkv, int tile, FastDiv tiles,
                   int blocks, FastDiv page, int width, int span, int nseg, int short_segs,
-                  float scale_log2, int dim_) {
+                  float scale_log2, float inv_nseg, int dim_) {
     using C = Stream8<T, D>;
     constexpr int TOK = C::kTok, NL = C::kLoads, SUB = TOK / 32, KE = D / 64;
     __shared__ __align__(16) char s_stage[4][C::kLds];
@@ -1107,7 +1123,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
     const int dim = FULL ? D : dim_;
     if (wave < 3) scan8(lens, batch, span, lane, wave ? kMinSeg8 * wave : 1, s_prefix[wave]);
     __syncthreads();
-    const int vrows = hkv * tiles, group = hq / hkv;
+    const int vrows = hkv * (int)tiles.d, group = hq / hkv;
     // few tokens: a segment a stretch of S tokens of one row
     const long long pad1 = uniform64(s_prefix[1][batch]) * vrows;
     const long long pad2 = uniform64(s_prefix[2][batch]) * vrows;
@@ -1118,7 +1134,8 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
     const long long total = uniform64(s_pref[batch]) * vrows;
     long long S = kMinSeg8 * few;
     if (!few) {
-        S = max(div64(total + nseg - 1, nseg), (long long)kMinSeg8);
+        // at least total / nseg, whole steps (float32, off by 2^-22: rounded up)
+        S = max((long long)((float)total * inv_nseg) + 1, (long long)kMinSeg8);
         S = (S + TOK - 1) & ~(long long)(TOK - 1);
     }
     if (blockIdx.x == 0) {  // the combine's copy of the prefix, and S
@@ -1164,7 +1181,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
     auto issue = [&](const Piece8& p, int st, int ent) {
         const int t = token(p, st);
         const bool held = (unsigned)ent < (unsigned)blocks;
-        const unsigned bh = (unsigned)(held ? ent : 0) * hkv + p.kv / tiles;
+        const unsigned bh = (unsigned)(held ? ent : 0) * hkv + p.kv;
         const unsigned row = bh * page.d + page.mod(t);
         const bool ok = held && st * TOK + my < p.n;
         seen = __ballot(ok);
@@ -1181,14 +1198,10 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
         }
     };
     // ---- a row's q: column r's dims 64 e + 16 g .. + 15 ----------------------
-    auto first_head = [&](const Piece8& p) {
-        const int kv = p.kv / tiles;
-        return kv * group + (p.kv - kv * tiles) * tile;
-    };
     typedef T tx8 __attribute__((ext_vector_type(8)));
     tx8 qx[KE][2];
     auto load_q = [&](const Piece8& p) {
-        const T* row = q + ((size_t)p.b * hq + first_head(p) + (r < p.heads ? r : 0)) * dim;
+        const T* row = q + ((size_t)p.b * hq + p.h0 + (r < p.heads ? r : 0)) * dim;
 #pragma unroll
         for (int e = 0; e < KE; ++e)
 #pragma unroll
@@ -1199,7 +1212,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
             }
     };
 
-    Piece8 pc = piece8(s_pref, batch, vrows, seg_lo, seg_hi, lane, group, tile, tiles, s_prefix[0]);
+    Piece8 pc = piece8(s_pref, batch, vrows, seg_lo, seg_lo + S, lane, group, tile, tiles, s_prefix[0]);
     int ent = entry(pc, 0);
     load_q(pc);
     issue(pc, 0, ent);
@@ -1260,7 +1273,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                 ent = entry(pc, st + 2);
                 issue(pc, st + 1, e);
             } else if (more) {
-                nx = piece8(s_pref, batch, vrows, pc.next, seg_hi, lane, group, tile, tiles, s_prefix[0]);
+                nx = piece8(s_pref, batch, vrows, pc.next, seg_lo + S, lane, group, tile, tiles, s_prefix[0]);
                 const int e = entry(nx, 0);
                 ent = entry(nx, 1);
                 issue(nx, 0, e);
@@ -1372,7 +1385,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
         if (r < pc.heads) {
             // dims (D/4) g + (D/16) i + d of head r: acc[d][i]
             if (pc.whole) {
-                T* o = out + ((size_t)pc.b * hq + first_head(pc) + r) * dim + (D / 4) * g;
+                T* o = out + ((size_t)pc.b * hq + pc.h0 + r) * dim + (D / 4) * g;
                 const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -1390,11 +1403,7 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                         St<T>::st4(o + (D / 16) * i + d, make_float4(y[0], y[1], y[2], y[3]));
                     }
             } else {
-                const long long pb = uniform64(s_pref[pc.b]);
-                const long long end =
-                    pb * vrows + (pc.kv + 1) * (uniform64(s_pref[pc.b + 1]) - pb);
-                const size_t slot =
-                    (2 * (size_t)seg + (end >= seg_lo + S ? 1 : 0)) * tile + r;
+                const size_t slot = (2 * (size_t)seg + (size_t)pc.ends) * tile + r;
                 float* o = ws_acc + slot * dim + (D / 4) * g;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -1442,6 +1451,7 @@ Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int widt
     if (span > (1LL << 30)) inval("table capacity too large");
     if ((long long)std::min(batch, kScanRows8) * hq >= 1 << 24)
         inval("attention problem too large for one launch");
+    if (hq >= 1 << 20) inval("attention: too many q heads");
     Attn8Shape s{};
     s.batch = batch; s.hq = hq; s.hkv = hkv; s.page = page; s.width = width; s.dim = dim;
     s.span = (int)span;
@@ -1493,6 +1503,7 @@ void attn8_stream_run(const Attn8Shape& sh, const Attn8Args& a, float* ml, float
     const int dim = sh.dim;
     long long* pref = (long long*)(acc + sh.slots * dim);
     const float scale = (1.0f / sqrtf((float)dim)) * kLog2e;
+    const float inv_nseg = (1.0f + 0x1p-21f) / (float)sh.nseg;
     const auto kernel = dim == D ? attn8_stream<T, D, true> : attn8_stream<T, D, false>;
     for (int b0 = 0; b0 < sh.batch; b0 += kScanRows8) {
         const int nb = std::min(kScanRows8, sh.batch - b0);
@@ -1501,8 +1512,8 @@ void attn8_stream_run(const Attn8Shape& sh, const Attn8Args& a, float* ml, float
         const int* lens = a.lens ? a.lens + b0 : nullptr;
         kernel<<<(sh.nseg + 3) / 4, 256, 0, s>>>(
             q, a.kp, a.vp, a.ks, a.vs, a.table + (size_t)b0 * sh.width, lens, ml, acc, pref, out,
-            nb, sh.hq, sh.hkv, sh.tile, sh.tiles, a.blocks, FastDiv(sh.page), sh.width, sh.span,
-            sh.nseg, sh.short_segs, scale, dim);
+            nb, sh.hq, sh.hkv, sh.tile, FastDiv(sh.tiles), a.blocks, FastDiv(sh.page), sh.width,
+            sh.span, sh.nseg, sh.short_segs, scale, inv_nseg, dim);
         launch_check("int8 decode attention kernel launch");
         combine8(ml, acc, lens, out, Streamed8{pref, nb}, nb, sh.hq, sh.hkv, dim, sh.span, sh.tile,
                  sh.tiles, s);

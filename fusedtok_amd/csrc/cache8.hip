@@ -582,10 +582,12 @@ void append8(const T* k_new, const T* v_new, const int* slots, signed char* k_po
 // its tokens weigh nothing, and nothing is read for them.
 // ---------------------------------------------------------------------------
 
-// a / b for 0 <= a < 2^52, b > 0, by way of a float64 quotient (off by less
-// than one): a fifth of the instructions of a 64-bit division.
-__host__ __device__ __forceinline__ long long div64(long long a, long long b) {
-    const long long q = (long long)((double)a / (double)b), r = a - q * b;
+// floor(a / b) for 0 <= a, b > 0 and a quotient below 2^20, by way of a float32
+// one, which is then off by at most one (a 64-bit division, or a float64 one,
+// costs a kernel's start 0.2-0.3 us).
+__device__ __forceinline__ int small_div(long long a, long long b) {
+    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+    const long long r = a - q * b;
     return r < 0 ? q - 1 : r >= b ? q + 1 : q;
 }
 
@@ -610,10 +612,11 @@ struct Streamed8 {  // attn8_stream: two slots a segment (kernel comment)
     const long long* pref;  // prefix of the lengths [batch + 1], then the segment length
     int batch;
     struct Row {
-        long long s_lo, end, seg;
+        int s_lo;
+        long long end, seg;
         int count;
         __device__ __forceinline__ size_t at(int i) const {
-            const long long s = s_lo + i;
+            const int s = s_lo + i;
             return (size_t)(2 * s + (end >= (s + 1) * seg ? 1 : 0));
         }
     };
@@ -621,8 +624,8 @@ struct Streamed8 {  // attn8_stream: two slots a segment (kernel comment)
         const long long seg = pref[batch + 1], p0 = pref[b], len = pref[b + 1] - p0;
         const long long start = p0 * vrows + vrow * len;
         if (len == 0) return Row{0, 0, seg, 0};
-        const long long lo = div64(start, seg), hi = div64(start + len - 1, seg);
-        return Row{lo, start + len, seg, lo == hi ? -1 : (int)(hi - lo + 1)};
+        const int lo = small_div(start, seg), hi = small_div(start + len - 1, seg);
+        return Row{lo, start + len, seg, lo == hi ? -1 : hi - lo + 1};
     }
 };
 
@@ -1045,15 +1048,6 @@ __device__ __forceinline__ void scan8(const int* __restrict__ lens, int batch, i
         at += n;
     }
     if (lane == 63) pref[batch] = incl;
-}
-
-// floor(a / b) for 0 <= a, b > 0 and a quotient below 2^20, by way of a float32
-// one, which is then off by at most one: an address's worth of latency where
-// a 64-bit division, or a float64 one, takes a microsecond off every start.
-__device__ __forceinline__ int small_div(long long a, int b) {
-    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
-    const long long r = a - (long long)q * b;
-    return r < 0 ? q - 1 : r >= b ? q + 1 : q;
 }
 
 // A stretch of one row: tokens [t0, t0 + n) of sequence b for q heads [h0, h0 +

@@ -617,9 +617,10 @@ def block_table_extend(block_table, lens, counts, free_blocks, n_free, page, tok
 
     A fresh batch has lens 0 and counts the request lengths; a decode step has
     counts 1 (0 for an idle row). ``tokens`` is the outputs' size, known on
-    the host; fresh tokens beyond it get a block and no slot. int32 GPU tensors
-    only, values trusted (negative lens and counts count as 0); at most 4096
-    sequences. Build addition."""
+    the host; fresh tokens beyond it get a block and no slot. Blocks are given
+    back by writing their ids to ``free_blocks[n_free:]`` and raising n_free.
+    int32 GPU tensors only; any values are safe, negative lens and counts
+    count as 0; at most 4096 sequences, page up to 1024. Build addition."""
     try:
         (B, S), (F,) = block_table.shape, free_blocks.shape
         ready = (lens.shape == (B,) and counts.shape == (B,) and n_free.shape == (1,) and
@@ -735,8 +736,9 @@ def attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales, block_tab
     with the codes exact, softmax and sums float32); k_pool / v_pool: int8
     [Nb, Hkv, P, D]; k_scales / v_scales: float32 [Nb, Hkv]; block_table: [B,
     S], token t of sequence b at row ``t % P`` of block ``block_table[b, t //
-    P]``; lens: [B] (None = S * P rows each). Any group size Hq / Hkv, D a
-    multiple of 4 up to 512. Tokens of a table entry outside [0, Nb) (such as
+    P]``; lens: [B] (None = S * P rows each); host-origin ones are range-checked.
+    Any group size Hq / Hkv, D a multiple of 4 up to 512, tensors aligned to
+    16 bytes (where D % 16: to 4 elements). Tokens of a table entry outside [0, Nb) (such as
     -1) weigh nothing; a sequence without a token gives zero rows. Each call
     has a workspace of its own from torch's allocator, so calls on several
     streams are independent. Build addition."""

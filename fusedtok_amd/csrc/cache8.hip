@@ -285,8 +285,9 @@ struct Codes {
 //   few rows        (a decode step) a unit a row; those that start no run end;
 //   up to 1024      every workgroup lists the starts of all runs in LDS, and
 //                   the units share them out;
-//   more            a unit a window of as many rows as a block has: the runs
-//                   that start in it, one after another (about one, in prompts).
+//   more            a unit a window of as many rows as a block has (64 at most):
+//                   the runs that start in it, one after another (about one, in
+//                   prompts).
 // (8 heads, D = 128, blocks of 16, graph replays, us, the three in turn: a step
 // of 64 sequences 5.1, 6.2, 23.8, of 512 8.4, 8.7, 23.2, of 1024 12.6, 13.2, 23.4;
 // a prompt of 512 tokens 9.7, 6.3, 5.8, of 2048 28.7, 10.3, 6.2.)
@@ -512,14 +513,12 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
         const bool is_v = unit >= units / 2;
         const int wh = (int)(is_v ? unit - units / 2 : unit);
         const int h = heads.mod(wh), first = heads.div(wh) * window;
-        for (int w0 = 0; w0 < window; w0 += 64) {
-            const int t = first + w0 + lane;
-            const int mine = w0 + lane < window ? block_of(slot_of(t)) : -1;
-            unsigned long long starts = __ballot(mine >= 0 && block_of(slot_of(t - 1)) != mine);
-            for (; starts; starts &= starts - 1) {
-                const int at = __builtin_ctzll(starts);
-                run(first + w0 + at, __shfl(mine, at, 64), is_v, h);
-            }
+        const int mine = lane < window ? block_of(slot_of(first + lane)) : -1;
+        unsigned long long starts =
+            __ballot(mine >= 0 && block_of(slot_of(first + lane - 1)) != mine);
+        for (; starts; starts &= starts - 1) {
+            const int at = __builtin_ctzll(starts);
+            run(first + at, __shfl(mine, at, 64), is_v, h);
         }
     }
 }
@@ -532,7 +531,7 @@ void append8_run(const T* k_new, const T* v_new, const int* slots, signed char* 
     const long long pairs = 2LL * tokens * hkv;  // one a row, head and pool
     const bool row_each = pairs <= kRowEach * cus;
     const bool listed = !row_each && tokens <= kListTokens;
-    const int window = row_each ? 1 : page;
+    const int window = row_each ? 1 : std::min(page, 64);  // (a lane a row)
     const long long units = 2LL * ((tokens + window - 1) / window) * hkv;
     const long long wgs = listed ? std::min((pairs * UT + 255) / 256, (long long)kListWgs * cus)
                                  : (units * UT + 255) / 256;
@@ -990,7 +989,7 @@ constexpr int kScanRows8 = 1024;  // sequences of a launch (their prefixes are i
 // 64 / 8 heads, fp16, take 95 us, 2 rows of 131071, D = 64, 49. The vector ALU is
 // busy 55-60% of the cycles, the matrix cores 14-18%. Two waves a SIMD: at three
 // the registers spill (226 against 210 us for the first of these, all else
-// equal). For short rows, latency: 5.8 us for 4 rows of 128-1024 tokens, D = 64,
+// equal). For short rows, latency: 5.4 us for 4 rows of 128-1024 tokens, D = 64,
 // and 4.2 for the combine.
 // ---------------------------------------------------------------------------
 typedef float f32x4_8 __attribute__((ext_vector_type(4)));

@@ -1586,7 +1586,8 @@ int ft_kv_append_paged_int8_launch(const void* k_new, const void* v_new, int dty
         check_aligned(v_new, 4 * size_of(dtype), "v_new");
         check_aligned(k_pool, 4, "k_pool");
         check_aligned(v_pool, 4, "v_pool");
-        if ((long long)tokens * kv_heads > (1LL << 30))
+        // (twice as many, a grid's step on top, are counted in 31 bits)
+        if ((long long)tokens * kv_heads > (1LL << 29))
             inval("kv_append_paged_int8: too many rows for one call");
         const hipStream_t s = as_stream(stream);
         auto go = [&](auto zero) {

@@ -60,6 +60,13 @@ def test_append_refusals(lib, change, word):
     assert st == FT_EINVAL and word in lib.ft_last_error()
 
 
+def test_append_of_more_rows_than_are_counted(lib):
+    """Rows and heads whose (run, head, pool) triples pass 31 bits."""
+    f = lib.ft_kv_append_paged_int8_launch
+    assert f(X, X, 1, X, X, X, X, X, 1024, 2 ** 20, 4, 1024, 1, 0) == FT_EINVAL
+    assert b"too many rows" in lib.ft_last_error()
+
+
 def test_append_of_nothing(lib):
     f = lib.ft_kv_append_paged_int8_launch
     assert f(None, None, 1, None, None, None, None, None, 0, 2, 64, 4, 16, 0) == FT_OK

@@ -1618,6 +1618,9 @@ int ft_attention_decode_paged_int8_launch(const void* q, int dtype, const signed
                                           int dim, uintptr_t stream) {
     return guarded([&] {
         check_pools(blocks, kv_heads, page, dim);
+        // (without a block, one launch writes every head's zeros)
+        if (blocks == 0 && (long long)batch * q_heads >= 1 << 24)
+            inval("attention problem too large for one launch");
         // whole 16-byte chunks of a row on the matrix-core path
         const size_t by = dim % 16 == 0 ? 16 : 4;
         check_aligned(k_pool, by, "k_pool");

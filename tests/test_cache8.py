@@ -89,6 +89,12 @@ def test_attention_refusals(lib, change, word):
     assert st == FT_EINVAL and word in lib.ft_last_error()
 
 
+def test_attention_of_too_many_heads_without_a_block(lib):
+    st = lib.ft_attention_decode_paged_int8_launch(X, 1, 0, 0, 0, 0, X, X, X, X, 1 << 40, 2 ** 21,
+                                                   1024, 8, 0, 16, 4, 64, 0)
+    assert st == FT_EINVAL and b"too large" in lib.ft_last_error()
+
+
 def test_host_tensors_are_refused():
     x = torch.zeros(1, 2, 64)
     pool, scale = torch.zeros(1, 2, 16, 64, dtype=torch.int8), torch.zeros(1, 2)

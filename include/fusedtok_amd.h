@@ -263,7 +263,8 @@ int ft_block_table_extend_launch(int* table, const int* lens, const int* counts,
  * other rows become rint(code * (scale / scale')). The rows of one block
  * must be next to each other in slots (runs of one block at two places race
  * with each other); of two rows with one slot the later counts. k_new and
- * v_new are aligned to 4 elements, the pools to 4 bytes. */
+ * v_new are aligned to 4 elements, the pools to 4 bytes; tokens * kv_heads <=
+ * 2^29. */
 int ft_kv_append_paged_int8_launch(const void* k_new, const void* v_new, int dtype,
                                    const int* slots, signed char* k_pool, signed char* v_pool,
                                    float* k_scales, float* v_scales, int tokens, int kv_heads,

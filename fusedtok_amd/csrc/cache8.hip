@@ -969,11 +969,13 @@ constexpr int kScanRows8 = 1024;  // sequences of a launch (their prefixes are i
 //           32 ragged rows 197 us both, 4 short ones 8.7 against 8.1);
 //  softmax  lane (r, g) holds head r's scores of tokens 4g+i (+ 16 a tile);
 //           scaled by the block's K scale, running maximum over the 4 lanes
-//           of a head; the weight takes the block's V scale, then goes into 2
-//           bf16 parts (3 for float32 outputs), which hold any float's
-//           magnitude: small weights count as they weigh. (Groups of up to 4
-//           heads could fill the 16 columns with copies that share the tokens
-//           out: a quarter of the exponentials, and 1-2% of the time.);
+//           of a head; the weight takes the block's V scale, then goes into 3
+//           bf16 parts: all its bits, small ones too, so that products are
+//           exact here as well. (Two parts leave out up to 2^-15, always
+//           downwards, and a result in a hundred is another fp16 number.)
+//           (Groups of up to 4 heads could fill the 16 columns with copies that
+//           share the tokens out: a quarter of the exponentials, and 1-2% of
+//           the time.);
 //  PV       O^T[dim][head] = V^T . W^T, codes widened to bf16 (exact). The
 //           weights are where B wants them; for A, lane (r, g) reads dims
 //           (D/16) r .. of its 8 tokens from the staging and pairs the tokens
@@ -1002,7 +1004,7 @@ struct Stream8 {
     static constexpr int kLoads = kTok * D / 1024;   // 16-byte loads a lane and pool
     static constexpr int kRowsPer = 1024 / D;        // rows a load instruction covers
     static constexpr int kChunks = D / 16;           // 16-byte chunks of a row
-    static constexpr int kW = std::is_same<T, float>::value ? 3 : 2;  // weight parts
+    static constexpr int kW = 3;                     // weight parts: all 24 bits
     static constexpr int kOcc = D == 256 ? 1 : 2;    // waves a SIMD
     static constexpr int kLds = 2 * kTok * D + 8 * kTok;  // bytes a wave
     static constexpr int kQ = std::is_same<T, float>::value ? 3 : std::is_same<T, f16>::value ? 2 : 1;  // q parts
@@ -1331,9 +1333,10 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                     l_run += p;
                     w[i] = p * vsc[8 * u + i];
                 }
-                // bf16 parts, each truncated, the first the largest (an
-                // infinity, which only a scale that is not finite makes,
-                // leaves NaN behind it)
+                // bf16 parts, each truncated, the first the largest: all bits of
+                // a weight from 2^-102 up, whose last part is a normal number
+                // still (an infinity, which only a scale that is not finite
+                // makes, leaves NaN behind it)
                 b16x8 wp[C::kW];
 #pragma unroll
                 for (int p = 0; p < C::kW; ++p) {

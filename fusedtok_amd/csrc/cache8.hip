@@ -312,7 +312,7 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
     const T* __restrict__ k_new, const T* __restrict__ v_new, const int* __restrict__ slots,
     signed char* __restrict__ k_pool, signed char* __restrict__ v_pool,
     float* __restrict__ k_scales, float* __restrict__ v_scales, int tokens, FastDiv heads, int dim,
-    int nslots, FastDiv page, FastDiv lanes, int window, long long units) {
+    int nslots, FastDiv page, FastDiv lanes, int window, long long first_wg, long long units) {
     constexpr int kKeep = 4, kUnits = 256 / UT;
     __shared__ int s_map[kUnits][kMaxPage8];
     __shared__ int s_runs[LISTED ? kListTokens : 1];
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(
     const int lane = threadIdx.x & 63;
     const int ut = UT == 64 ? lane : (int)threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long unit = (long long)blockIdx.x * kUnits + (UT == 64 ? wave : 0);
+    const long long unit = (first_wg + blockIdx.x) * kUnits + (UT == 64 ? wave : 0);
     if (!LISTED && unit >= units) return;
     int* const map = s_map[UT == 64 ? wave : 0];
     const int hkv = (int)heads.d;
@@ -535,12 +535,15 @@ void append8_run(const T* k_new, const T* v_new, const int* slots, signed char* 
     const long long units = 2LL * ((tokens + window - 1) / window) * hkv;
     const long long wgs = listed ? std::min((pairs * UT + 255) / 256, (long long)kListWgs * cus)
                                  : (units * UT + 255) / 256;
-    if (wgs >= 1LL << 24) inval("kv_append_paged_int8: too many rows for one call");
     const auto kernel = listed ? kv_append8_kernel<T, V, UT, true> : kv_append8_kernel<T, V, UT, false>;
-    kernel<<<(unsigned)wgs, 256, 0, s>>>(
-        k_new, v_new, slots, k_pool, v_pool, k_scales, v_scales, tokens, FastDiv(hkv), dim,
-        blocks * page, FastDiv(page), FastDiv(dim / V), window, units);
-    launch_check("int8 kv append kernel launch");
+    // (a grid's threads fit 32 bits; units share nothing, so a call may take several)
+    constexpr long long kGrid = (1LL << 24) - 1;
+    for (long long at = 0; at < wgs; at += kGrid) {
+        kernel<<<(unsigned)std::min(kGrid, wgs - at), 256, 0, s>>>(
+            k_new, v_new, slots, k_pool, v_pool, k_scales, v_scales, tokens, FastDiv(hkv), dim,
+            blocks * page, FastDiv(page), FastDiv(dim / V), window, at, units);
+        launch_check("int8 kv append kernel launch");
+    }
 }
 
 template <typename T>

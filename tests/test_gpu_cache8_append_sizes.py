@@ -64,3 +64,24 @@ def test_append_4_values_a_lane(page, d, who, dtype, rows, how, off):
         np.testing.assert_array_equal(got[2 + i].cpu().numpy(), scales)
         np.testing.assert_array_equal(got[i].cpu().numpy(), codes)
         assert (scales > cache[2 + i]).any()
+
+
+def test_append_of_more_rows_than_a_grid():
+    """Blocks of one row: a wave for each of 2^25 rows of K and of V, 2^24
+    workgroups, the last of which a second launch has. Every block starts over,
+    so its scale is max |x| / 127 and its codes rint(x * (1 / scale)), in
+    float32 with divisions rounded once (by way of 64 bits)."""
+    rows, d = 2 ** 25, 4
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    k, v = (torch.randn(rows, 1, d, generator=gen, device=DEV, dtype=torch.float16)
+            for _ in range(2))
+    kp, vp = (torch.full((rows, 1, 1, d), 99, dtype=torch.int8, device=DEV) for _ in range(2))
+    ks, vs = (torch.full((rows, 1), 7.0, device=DEV) for _ in range(2))
+    slots = torch.randperm(rows, generator=gen, device=DEV).int()
+    ft.kv_append_paged_int8(kp, vp, ks, vs, k, v, slots)
+    for pool, scales, new in ((kp, ks, k), (vp, vs, v)):
+        x = new[:, 0].float()
+        want = (x.abs().amax(1).double() / 127).float().clamp(min=2.0 ** -120)
+        codes = torch.round(x * (1 / want.double()).float()[:, None]).clamp(-127, 127)
+        assert torch.equal(scales[slots.long(), 0], want)
+        assert torch.equal(pool[slots.long(), 0, 0], codes.to(torch.int8))

@@ -28,7 +28,7 @@
 //     + attn_combine   dot products, chunk scores staged in LDS; the grid
 //                      covers the cache capacity in fixed chunks.
 #include <climits>
-#include "attn_stream.hpp"
+#include "attn_common.hpp"
 #include "ft_common.hpp"
 
 #include <algorithm>
@@ -306,6 +306,7 @@ template <> struct Mfma<f16> {
 
 constexpr int kMfmaDim = 128;
 constexpr int kMfmaAccPitch = kMfmaDim + 4;  // LDS row pitch (bank spread)
+constexpr int kStreamScanRows = 2048;        // sequences per launch (LDS prefix)
 // Default minimum tokens per segment. Large decode batches are unaffected
 // (C3's segments hold ~8.9k tokens); for a small one the floor trades
 // per-segment set-up and combine work against idle CUs: 1 x 32 rows x 4096
@@ -333,6 +334,47 @@ constexpr int kStreamUniformLong = 4096;
 // Row addressing modes of attn_decode_stream.
 enum RowMode { kRowsContig = 0, kRowsPagedPow2 = 1, kRowsPagedDiv = 2 };
 
+// Exclusive prefix of the clamped lengths into s_pref[0..batch] (wave 0;
+// each lane takes a contiguous run of rows, then a wave scan of the runs),
+// and their minimum and maximum into s_mm[0], s_mm[1].
+__device__ __forceinline__ void scan_lengths(const int* __restrict__ lens,
+                                             int batch, int span, int lane,
+                                             long long* s_pref, int* s_mm) {
+    const int per = (batch + 63) / 64;
+    const int r0 = lane * per;
+    long long local = 0;
+    int lmin = INT_MAX, lmax = 0;
+    for (int i = 0; i < per; ++i)
+        if (r0 + i < batch) {
+            const int l = clamp_len(lens, r0 + i, span);
+            local += l;
+            lmin = min(lmin, l);
+            lmax = max(lmax, l);
+        }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        lmin = min(lmin, __shfl_xor(lmin, o, 64));
+        lmax = max(lmax, __shfl_xor(lmax, o, 64));
+    }
+    if (lane == 0) {
+        s_mm[0] = lmin;
+        s_mm[1] = lmax;
+    }
+    long long incl = local;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long long y = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += y;
+    }
+    long long run = incl - local;
+    for (int i = 0; i < per; ++i)
+        if (r0 + i < batch) {
+            s_pref[r0 + i] = run;
+            run += clamp_len(lens, r0 + i, span);
+        }
+    if (lane == 63) s_pref[batch] = incl;
+}
+
 // Tokens per segment: `total` over nseg segments, at least min_seg of them -
 // or, when that would leave CUs without a segment (cus > 0: their count), as
 // many as give each CU one, down to low_seg (half of it where even those
@@ -355,6 +397,35 @@ __device__ __forceinline__ int stream_segments(const int* s_mm, int cus) {
     int nseg = (int)gridDim.x;
     if (cus > 0 && nseg > cus && s_mm[0] == s_mm[1] && s_mm[0] >= kStreamUniformLong) nseg = (nseg + 1) >> 1;
     return __builtin_amdgcn_readfirstlane(nseg);
+}
+
+// A flat position's place: row (b, kv) and the tokens [t0, t0 + n) of it
+// that lie before seg_hi. Everything is wave-uniform.
+struct StreamPiece {
+    int b, kv, row, t0, n;
+    bool whole;       // the row's every token
+    long long next;   // the flat position behind the piece
+};
+
+__device__ __forceinline__ StreamPiece stream_piece(const long long* s_pref, int batch, int hkv,
+                                                    long long pos, long long seg_hi) {
+    int lo = 0, hi = batch - 1;  // last sequence starting at or before pos
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (uniform64(s_pref[mid]) * hkv <= pos) lo = mid; else hi = mid - 1;
+    }
+    StreamPiece p;
+    p.b = lo;
+    const long long pb = uniform64(s_pref[lo]);
+    const long long base = pb * hkv;
+    const int len = (int)(uniform64(s_pref[lo + 1]) - pb);
+    p.kv = (int)((pos - base) / len);
+    p.t0 = (int)(pos - base - (long long)p.kv * len);
+    p.next = min(seg_hi, base + (long long)(p.kv + 1) * len);
+    p.n = (int)(p.next - pos);
+    p.whole = p.t0 == 0 && p.n == len;
+    p.row = lo * hkv + p.kv;
+    return p;
 }
 
 // acc / l. Half storage rounds the quotient anyway: one reciprocal.

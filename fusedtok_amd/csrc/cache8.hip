@@ -4,7 +4,7 @@
 // The cache. k_pool / v_pool are int8 [blocks, kv heads, page, dim], k_scales /
 // v_scales float32 [blocks, kv heads]; the value at row r of block n, head h is
 // code * scale[n, h]. A slot is block * page + row.
-#include "attn_stream.hpp"
+#include "attn_common.hpp"
 #include "ft_common.hpp"
 
 #include <algorithm>

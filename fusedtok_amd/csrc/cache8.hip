@@ -210,9 +210,9 @@ __global__ __launch_bounds__(256) void block_table_extend_kernel(
 //   scale' = max(held, f32(a / 127), 2^-120),
 //   code   = clamp(rint(f32(x * f32(1 / scale'))), -127, 127), NaN -> 0,
 // held being the block's scale, or 0 where row 0 is in the run (the block
-// starts over). Where scale' > held > 0 the block's other rows become
-// rint(f32(code * f32(held / scale'))). All float32, IEEE divisions: codes
-// are the same on every path.
+// starts over). Where scale' > held and row 0 is not in the run, the block's
+// other rows become rint(f32(code * f32(held / scale'))): zeros where held was
+// 0. All float32, IEEE divisions: codes are the same on every path.
 // ---------------------------------------------------------------------------
 constexpr float kLeastScale = 0x1p-120f;
 
@@ -1001,6 +1001,8 @@ typedef float f32x4_8 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
+constexpr int stream_occ(int dim) { return dim > 128 ? 1 : 2; }
+
 template <typename T, int D>
 struct Stream8 {
     static constexpr int kTok = D == 64 ? 64 : 32;   // tokens a step
@@ -1008,7 +1010,7 @@ struct Stream8 {
     static constexpr int kRowsPer = 1024 / D;        // rows a load instruction covers
     static constexpr int kChunks = D / 16;           // 16-byte chunks of a row
     static constexpr int kW = 3;                     // weight parts: all 24 bits
-    static constexpr int kOcc = D == 256 ? 1 : 2;    // waves a SIMD
+    static constexpr int kOcc = stream_occ(D);       // waves a SIMD
     static constexpr int kLds = 2 * kTok * D + 8 * kTok;  // bytes a wave
     static constexpr int kQ = std::is_same<T, float>::value ? 3 : std::is_same<T, f16>::value ? 2 : 1;  // q parts
 };
@@ -1435,11 +1437,6 @@ struct Attn8Shape {
     size_t slots, bytes;                // slots: (partial, q head) pairs
 };
 
-template <int D>
-int stream_occ(int dtype) {
-    return dtype == FT_DT_F32 ? Stream8<float, D>::kOcc : Stream8<bf16, D>::kOcc;
-}
-
 Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int width, int dim) {
     check_pools(0, hkv, page, dim);
     if (dtype != FT_DT_F32 && dtype != FT_DT_BF16 && dtype != FT_DT_F16)
@@ -1461,8 +1458,7 @@ Attn8Shape attn8_shape(int dtype, int batch, int hq, int hkv, int page, int widt
         s.tiles = (group + 15) / 16;
         s.tile = (group + s.tiles - 1) / s.tiles;
         s.tiles = (group + s.tile - 1) / s.tile;
-        const int occ = dim <= 64 ? stream_occ<64>(dtype)
-                                  : dim <= 128 ? stream_occ<128>(dtype) : stream_occ<256>(dtype);
+        const int occ = stream_occ(dim);
         const long long rows = (long long)std::min(batch, kScanRows8) * hkv * s.tiles;
         const long long most = rows * ((span + kMinSeg8 - 1) / kMinSeg8);
         s.nseg = (int)std::min(std::min((long long)4 * cus * occ, most), (long long)kMaxPieces8);

@@ -617,10 +617,19 @@ def block_table_extend(block_table, lens, counts, free_blocks, n_free, page, tok
 
     A fresh batch has lens 0 and counts the request lengths; a decode step has
     counts 1 (0 for an idle row). ``tokens`` is the outputs' size, known on
-    the host; fresh tokens beyond it get a block and no slot. Blocks are given
-    back by writing their ids to ``free_blocks[n_free:]`` and raising n_free.
-    int32 GPU tensors only; any values are safe, negative lens and counts
-    count as 0; at most 4096 sequences, page up to 1024. Build addition."""
+    the host; fresh tokens beyond it get a block and no slot. int32 GPU tensors
+    only; any values are safe, negative lens and counts count as 0; at most 4096
+    sequences, page up to 1024.
+
+    Blocks are given back by writing their ids from ``free_blocks[max(n_free,
+    0)]`` on and setting n_free to that place plus their number. Not to be
+    given back: the -1 entries of a sequence that went short (an id of -1 in the
+    list would be handed out as no block). A negative n_free only says how many
+    were missing: it is no debt to be paid off first. The sequences that went
+    short keep their -1 entries and their new_lens, later calls do not fill
+    them: give back the blocks that such a sequence got in the call, put its
+    lens back to what it was and call again when there are blocks, or give back
+    all of its blocks and start it over with lens 0. Build addition."""
     try:
         (B, S), (F,) = block_table.shape, free_blocks.shape
         ready = (lens.shape == (B,) and counts.shape == (B,) and n_free.shape == (1,) and

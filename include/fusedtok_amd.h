@@ -246,7 +246,8 @@ int ft_attention_prefill_launch_fp16(const void* q, const void* k, const void* v
  * -1 for a token without a block or behind the table's end. offsets
  * [batch + 1]: sequence b's rows are [offsets[b], offsets[b + 1]). lens_out =
  * min(lens + counts, tbl_width * page); *n_free_out = *n_free minus the
- * blocks needed (negative: that many are missing). slots and positions hold
+ * blocks needed (negative: that many are missing; blocks are given back from
+ * free_blocks[max(*n_free, 0)] on, and never a -1). slots and positions hold
  * `tokens` entries (more fresh tokens than that have none). batch <= 4096;
  * the outputs overlap no input. */
 int ft_block_table_extend_launch(int* table, const int* lens, const int* counts,

@@ -741,16 +741,20 @@ def attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales, block_tab
 
     ``out[b, h] = softmax(q[b, h] . K[b, kv(h)]^T / sqrt(D)) . V[b, kv(h)]``
 
-    q: [B, Hq, D] (f32 / bf16 / fp16, also the output's type; products of q
-    with the codes exact, softmax and sums float32); k_pool / v_pool: int8
+    q: [B, Hq, D] (f32 / bf16 / fp16, also the output's type; softmax, weights
+    and sums float32, rounded once at the end); k_pool / v_pool: int8
     [Nb, Hkv, P, D]; k_scales / v_scales: float32 [Nb, Hkv]; block_table: [B,
     S], token t of sequence b at row ``t % P`` of block ``block_table[b, t //
     P]``; lens: [B] (None = S * P rows each); host-origin ones are range-checked.
     Any group size Hq / Hkv, D a multiple of 4 up to 512, tensors aligned to
     16 bytes (where D % 16: to 4 elements). Tokens of a table entry outside [0, Nb) (such as
-    -1) weigh nothing; a sequence without a token gives zero rows. Each call
-    has a workspace of its own from torch's allocator, so calls on several
-    streams are independent. Build addition."""
+    -1) weigh nothing; a sequence without a token gives zero rows. How a
+    sequence's tokens are cut into pieces depends on the lengths of the whole
+    batch: the same call gives the same bits, but a sequence's last bits may
+    change with its neighbours. min(B, 1024) * Hq is below 2**24 (for D % 16 or
+    D > 256: B * Hq is, B and Hkv at most 65535). Each call has a workspace of
+    its own from torch's allocator, so calls on several streams are independent.
+    Build addition."""
     try:
         (B, Hq, D), (Nb, Hkv, P, dim), (rows, S) = q.shape, k_pool.shape, block_table.shape
         dev = q.get_device()

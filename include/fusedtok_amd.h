@@ -274,8 +274,12 @@ int ft_kv_append_paged_int8_launch(const void* k_new, const void* v_new, int dty
  * q's) = softmax(q . k / sqrt(dim)) . v over the first lens[b] tokens (lens
  * NULL: tbl_width * page) of sequence b, token t at row t % page of block
  * table[b, t / page]. Any group size. Tokens of a table entry outside
- * [0, blocks) weigh nothing; a row without a token gives zeros. q, out
- * and the pools are aligned to 16 bytes (where dim % 16: 4 elements). The
+ * [0, blocks) weigh nothing; a row without a token gives zeros. How a row is
+ * cut depends on the lengths of the whole batch, and so may its last bits (not
+ * from one run of a call to the next). min(batch, 1024) * q_heads < 2^24; for
+ * dim % 16, dim > 256 or no block or table column, batch * q_heads < 2^24 and
+ * batch, kv_heads <= 65535. q, out and the pools are aligned to 16 bytes (where
+ * dim % 16: 4 elements). The
  * workspace (device memory, 16-byte aligned) is the caller's: it is written
  * by the call and free again when the stream has passed it. */
 int ft_attention_decode_paged_int8_workspace(int dtype, int batch, int q_heads, int kv_heads,

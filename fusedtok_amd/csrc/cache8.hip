@@ -299,10 +299,12 @@ struct Codes {
 // for two 16-bit values), and only a run with an infinity or NaN in it, which
 // the maximum shows, goes through the code that looks at each value.
 //
-// What bounds it: memory latency in a decode step (4.1 us for 64 rows); for
-// prompts, HBM: 30k rows, 8 heads, D = 128, bf16, 41 us, 4.4 TB/s read and written,
-// where a large copy has 4.8. (Values widened and compared one by one: 61 us,
-// bound by the vector ALU.)
+// What bounds it: memory latency in a decode step (4 us for 64 rows); a step
+// whose scales grow reads and writes its blocks' other rows too (graph replays,
+// 64 rows 4.4 us for 4.3, of blocks of 64 6.8 for 5.2, 512 rows 12.0 for 8.1). For
+// prompts, HBM: 30k rows, 8 heads, D = 128, bf16, 38.7 us, 4.7 TB/s read and
+// written, where a large copy has 4.8. (Values widened and compared one by one:
+// 61 us, bound by the vector ALU.)
 constexpr long long kRowEach = 16;  // units a CU, at most, where each row has its own
 constexpr int kListTokens = 1024;   // rows whose runs are listed, at most
 constexpr int kListWgs = 4;         // workgroups a CU of a listed call, at most
@@ -637,7 +639,7 @@ constexpr int kWavePieces8 = 32;   // folded by one wave, at most
 // `per` (1 or 4) q heads a workgroup, a wave each; a head of many pieces is
 // folded by the whole workgroup, afterwards. Where heads are few, gridDim.y
 // workgroups share the dims of one of many pieces. Bound by latency: the row's
-// place, its pieces' (m, l) and sums, the launch; 4-7 us.
+// place, its pieces' (m, l) and sums, the launch; 4-7 us of kernel.
 template <typename T, typename Pieces>
 __global__ __launch_bounds__(256) void attn8_combine(
     const float* __restrict__ ws_ml, const float* __restrict__ ws_acc,
@@ -791,8 +793,9 @@ void combine8(const float* ml, const float* acc, const int* lens, T* out, const 
               int batch, int hq, int hkv, int dim, int span, int tile, int tiles, hipStream_t s) {
     const int heads = batch * hq;
     // few heads have many pieces each: a workgroup a head, or one for 32 of its
-    // dims (one row of 131072 tokens, 8 heads, attention and combine: 54 -> 27 us);
-    // many have few: four a workgroup (4096 heads: 19 -> 6.9 us)
+    // dims (one row of 131072 tokens, 8 heads, attention and combine, graph
+    // replays: 32.7 us without, 22.8 with); many have few: four a workgroup (4096
+    // heads, 128 rows of 500 tokens, both: 49.3 and 37.5)
     const int per = heads >= 4 * dev_info().cu_count && 256 % dim == 0 ? 4 : 1;
     const int parts = per == 1 && heads < dev_info().cu_count && dim % 32 == 0 ? dim / 32 : 1;
     attn8_combine<T, Pieces><<<dim3((heads + per - 1) / per, parts), 256, 0, s>>>(
@@ -933,8 +936,9 @@ __global__ __launch_bounds__(256) void attn8_general(
 // tokens take segments of one row each: of 64 tokens while those are at most
 // four a CU (eight at D = 64), else of 128 while those do not outnumber the
 // waves. Attention and combine together, graph replays: 4 rows of 500-1000
-// tokens, 8 kv heads, D = 128, 13.6 us at 64, 14.5 at 128; 8 rows of 1000-2000
-// 18.7 and 16.6; 32 rows of 500-1000 19.8 at 128, 23.1 as equal segments.
+// tokens, 8 kv heads, D = 128, 13.6 us at 64, 14.7 at 128, 15.8 as equal
+// segments; 8 rows of 1000-2000 16.8 at 128 (18.7 at 64, measured with a weight of
+// two parts), 21.4 equal; 32 rows of 500-1000 20.5 at 128, 22.9 equal.
 constexpr int kMinSeg8 = 64;
 constexpr int kScanRows8 = 1024;  // sequences of a launch (their prefixes are in LDS)
 
@@ -953,7 +957,8 @@ constexpr int kScanRows8 = 1024;  // sequences of a launch (their prefixes are i
 // segment has at most one of each. Waves share nothing but the length prefix,
 // so after it there is no barrier and no merge in the kernel. (More segments
 // than waves, or smaller ones behind the large, cost more at their starts than
-// the even end saves: 32 ragged rows 215 against 201 us with twice as many.)
+// the even end saves: 32 ragged rows, with the combine, 224 against 214 us with
+// twice as many.)
 //
 // A step is TOK tokens (32; 64 for D = 64), K and V of the next one - of the
 // next piece at a piece's end - in flight in registers while this one is
@@ -968,8 +973,9 @@ constexpr int kScanRows8 = 1024;  // sequences of a launch (their prefixes are i
 //           bits), so every product is exact and sums are float32. Any order
 //           of dims serves if q has the same: the lane reads 16-byte chunks.
 //           (Integer products with q in base-256 digits take 56 vector
-//           instructions a step less, but the loop waits on memory either way:
-//           32 ragged rows 197 us both, 4 short ones 8.7 against 8.1);
+//           instructions a step less, but the loop waited on memory either way,
+//           with a weight of two parts: 32 ragged rows 197 us both, 4 short ones
+//           8.7 against 8.1);
 //  softmax  lane (r, g) holds head r's scores of tokens 4g+i (+ 16 a tile);
 //           scaled by the block's K scale, running maximum over the 4 lanes
 //           of a head; the weight takes the block's V scale, then goes into 3
@@ -988,14 +994,15 @@ constexpr int kScanRows8 = 1024;  // sequences of a launch (their prefixes are i
 // Masked tokens (behind the piece, holes) weigh 0 exactly: score -inf, V scale
 // 0, the row read in its place a real one (its own last, or block 0's).
 //
-// What bounds it: HBM. Behind the first 6 us (lengths, piece, table, first
-// rows) 32 rows of 512-32768 tokens, 32 / 8 heads, D = 128, bf16, read at 6.6
-// TB/s (197 us in all; bare reads of such pages reach 6.7-6.8); 64 rows of 4097,
-// 64 / 8 heads, fp16, take 95 us, 2 rows of 131071, D = 64, 49. The vector ALU is
-// busy 55-60% of the cycles, the matrix cores 14-18%. Two waves a SIMD: at three
-// the registers spill (226 against 210 us for the first of these, all else
-// equal). For short rows, latency: 5.4 us for 4 rows of 128-1024 tokens, D = 64,
-// and 4.2 for the combine.
+// What bounds it: HBM, and the vector ALU behind it. After the first 6 us
+// (lengths, piece, table, first rows) 32 rows of 512-32768 tokens, 32 / 8 heads,
+// D = 128, bf16, read at 6.4 TB/s (202 us in all; bare reads of such pages reach
+// 6.7-6.8); 64 rows of 4097, 64 / 8 heads, fp16, take 94.5 us, 2 rows of 131071,
+// D = 64, 51.4. The vector ALU is busy 63-70% of the cycles, the matrix cores
+// 20-23%. (A weight of two parts, which is not exact: 197, 94.1 and 48.8 us.) Two
+// waves a SIMD: at three the registers spill (226 against 210 us for the first of
+// these, all else equal, in an earlier form). For short rows, latency: 5.6 us for
+// 4 rows of 128-1024 tokens, D = 64, and 4.2 for the combine.
 // ---------------------------------------------------------------------------
 typedef float f32x4_8 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));

@@ -83,11 +83,10 @@ def attend(q, k_pool, v_pool, k_scales, v_scales, table, lens):
     product with q is exact or rounded once), scaled twice: off by at most
     (D + 4) u sum|q k| sd, and its exponential's argument by another 2 u |s| in
     log2 units and back - (D + 8) u sum|q k| sd together, e. Each weight is
-    then off by a factor of 1 +- (e + 4 u) (the exponential itself), and the
-    weights' representation by 2^-16 for half outputs (two bf16 parts) - taken
-    for every type here, float32 by `parts` below. T terms are summed in
-    chains of at most T. Numerator and denominator both: twice. The result is
-    relative to the weighted sum of |v|."""
+    then off by a factor of 1 +- (e + 4 u) (the exponential itself). T terms are
+    summed in chains of at most T. Numerator and denominator both: twice. The
+    result is relative to the weighted sum of |v|. What the weights' parts may
+    leave out (PARTS below) is not in it: the caller adds that."""
     b, hq, d = q.shape
     nb, hkv, page, _ = k_pool.shape
     out = np.zeros((b, hq, d))
@@ -121,6 +120,7 @@ def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
-#: what the weights' parts leave out: two bf16 parts for half outputs, three
-#: for float32 (each part 8 bits, truncated)
+#: what the weights' parts may leave out, relative to the weighted sum of |v|
+#: (three parts of 8 bits, truncated, leave out 2^-23 at most: the half types'
+#: 2^-15, of two parts, is wider than they need)
 PARTS = {"torch.bfloat16": 2.0 ** -15, "torch.float16": 2.0 ** -15, "torch.float32": 2.0 ** -22}

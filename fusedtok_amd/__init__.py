@@ -742,7 +742,8 @@ def attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales, block_tab
     ``out[b, h] = softmax(q[b, h] . K[b, kv(h)]^T / sqrt(D)) . V[b, kv(h)]``
 
     q: [B, Hq, D] (f32 / bf16 / fp16, also the output's type; softmax, weights
-    and sums float32, rounded once at the end); k_pool / v_pool: int8
+    and sums float32, rounded once at the end; V scales below 2**-110 keep
+    fewer bits, 13 at 2**-120, but for D % 16 or D > 256); k_pool / v_pool: int8
     [Nb, Hkv, P, D]; k_scales / v_scales: float32 [Nb, Hkv]; block_table: [B,
     S], token t of sequence b at row ``t % P`` of block ``block_table[b, t //
     P]``; lens: [B] (None = S * P rows each); host-origin ones are range-checked.

@@ -1346,9 +1346,10 @@ void attn8_stream(const T* __restrict__ q, const signed char* __restrict__ k_poo
                     w[i] = p * vsc[8 * u + i];
                 }
                 // bf16 parts, each truncated, the first the largest: all bits of
-                // a weight from 2^-102 up, whose last part is a normal number
-                // still (an infinity, which only a scale that is not finite
-                // makes, leaves NaN behind it)
+                // a weight from 2^-110 up (the products keep subnormal parts,
+                // whose last bit is 2^-133; 2^-13 of the least scale) (an
+                // infinity, which only a scale that is not finite makes, leaves
+                // NaN behind it)
                 b16x8 wp[C::kW];
 #pragma unroll
                 for (int p = 0; p < C::kW; ++p) {

@@ -18,6 +18,8 @@ stubs __init__.pyi:99-107,208-236):
 - a paged KV cache held in 8 bits (build additions): ``block_table_extend``
   (block tables and slots on the GPU), ``kv_append_paged_int8`` and
   ``attention_decode_paged_int8``;
+- norms of query and key heads with the rotation (build additions):
+  ``qk_norm_rope`` and, into a paged cache, ``qk_norm_rope_kv_append_paged``;
 - the post-logits step: ``argmax`` / ``argmax_batched`` (greedy),
   ``sample_topp`` / ``sample_topp_batched`` and ``decode_step`` /
   ``decode_step_batched`` (repetition penalty -> temperature -> nucleus
@@ -100,6 +102,8 @@ __all__ = [
     "block_table_extend",
     "kv_append_paged_int8",
     "attention_decode_paged_int8",
+    "qk_norm_rope",
+    "qk_norm_rope_kv_append_paged",
     "rmsnorm_quant",
     "rmsnorm_qgemm",
     "swiglu_quant",
@@ -787,6 +791,151 @@ def attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales, block_tab
         v_scales.data_ptr(), block_table.data_ptr(), None if lens is None else lens.data_ptr(),
         out.data_ptr(), ws.data_ptr(), nbytes, B, Hq, Hkv, Nb, P, S, D, _stream())
     return out
+
+
+# ---------------------------------------------------------------------------
+# norms of query and key heads with the rotation (build additions; GPU tensors
+# only): a projection's rows in one pass, dense or into a paged cache's slots
+# ---------------------------------------------------------------------------
+
+_QK_POOLS = "pools must be [Nb, kv_heads, P, D] of qkv's dtype and head size, contiguous"
+
+
+def _qk_weight(w, name, D, device):
+    """A head's norm weights as a float32 vector on the device (or None)."""
+    if w is None:
+        return None
+    if not (torch.is_tensor(w) and w.is_cuda):
+        raise TypeError(f"{name} must be a GPU tensor")
+    if w.shape != (D,):
+        raise ValueError(f"{name} must be 1-D with D entries")
+    if w.dtype is not _TF:
+        if w.dtype not in _FLOATS:
+            raise TypeError(f"{name} must be float32, bfloat16 or float16")
+        w = w.to(_TF)
+    return w.contiguous()
+
+
+def _i32_operand(t, name, shape, what):
+    """Checks an int32 GPU tensor of that shape."""
+    if not (torch.is_tensor(t) and t.is_cuda):
+        raise TypeError(f"{name} must be a GPU tensor")
+    if t.dtype is not _TI:
+        raise TypeError(f"{name} must be int32")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(what)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, pools, slots, sections,
+                  theta, rotary_dim, eps, neox):
+    q_heads, kv_heads = int(q_heads), int(kv_heads)
+    if q_heads < 1 or kv_heads < 1:
+        raise ValueError("q_heads and kv_heads must be >= 1")
+    if not (torch.is_tensor(qkv) and qkv.is_cuda):
+        raise TypeError("qkv must be a GPU tensor (fused ops have no host path)")
+    if qkv.dtype not in _CODE:
+        raise TypeError("qkv must be float32, bfloat16 or float16")
+    heads = q_heads + 2 * kv_heads
+    if qkv.ndim != 2 or qkv.shape[1] % heads or not qkv.shape[1]:
+        raise ValueError("qkv must be [T, (q_heads + 2 * kv_heads) * D]")
+    T, width = qkv.shape
+    D = width // heads
+    if qkv.stride(1) != 1:
+        raise ValueError("qkv rows must be contiguous")
+    ld = qkv.stride(0) if T > 1 else width
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight are given together or not at all")
+    qw = _qk_weight(q_weight, "q_weight", D, qkv.device)
+    kw = _qk_weight(k_weight, "k_weight", D, qkv.device)
+    if torch.is_tensor(positions) and positions.ndim == 2:
+        axes = positions.shape[0]
+        if sections is None or len(sections) != axes:
+            raise ValueError("positions [axes, T] need sections with an entry for each axis")
+        _i32_operand(positions, "positions", (axes, T), "positions must be [T] or [axes, T]")
+    else:
+        axes = 1
+        _i32_operand(positions, "positions", (T,), "positions must be [T] or [axes, T]")
+        if sections is not None and len(sections) != 1:
+            raise ValueError("sections need positions [axes, T] with a row for each")
+    names, operands = ["qkv", "positions"], [qkv, positions]
+    if qw is not None:
+        names += ["q_weight", "k_weight"]
+        operands += [qw, kw]
+    Nb = P = 0
+    if pools is not None:
+        for name, t in zip(("k_pool", "v_pool"), pools):
+            if not (torch.is_tensor(t) and t.is_cuda):
+                raise TypeError(f"{name} must be a GPU tensor")
+            if t.dtype is not qkv.dtype:
+                raise TypeError(f"{name} must have the qkv dtype")
+        if (pools[0].ndim != 4 or pools[0].shape != pools[1].shape or
+                pools[0].shape[1] != kv_heads or pools[0].shape[3] != D or
+                not pools[0].is_contiguous() or not pools[1].is_contiguous()):
+            raise ValueError(_QK_POOLS)
+        Nb, _, P, _ = pools[0].shape
+        _i32_operand(slots, "slots", (T,), "slots must be 1-D with one entry per row")
+        names += ["k_pool", "v_pool", "slots"]
+        operands += [pools[0], pools[1], slots]
+    if not _one_device(names, operands):
+        with torch.cuda.device(qkv.device):
+            return _qk_norm_rope(qkv, q_heads, kv_heads, qw, kw, positions, pools, slots,
+                                 sections, theta, rotary_dim, eps, neox)
+    q = torch.empty((T, q_heads, D), dtype=qkv.dtype, device=qkv.device)
+    args = (qkv.data_ptr(), _CODE[qkv.dtype], ld, None if qw is None else qw.data_ptr(),
+            None if kw is None else kw.data_ptr(), positions.data_ptr(),
+            [D // 2 if rotary_dim is None else int(rotary_dim) // 2] if axes == 1
+            else [int(n) for n in sections],
+            D if rotary_dim is None else int(rotary_dim), float(theta), float(eps), bool(neox),
+            q.data_ptr())
+    if pools is not None:
+        k, v = pools
+        if T and Nb and k.data_ptr() == v.data_ptr():
+            raise ValueError("k and v must have pools of their own")
+        _fusedtok.qk_norm_rope_kv_append_paged_launch(
+            *args, k.data_ptr(), v.data_ptr(), slots.data_ptr(), T, q_heads, kv_heads, D, Nb, P,
+            _stream())
+        return q
+    k, v = torch.empty((2, T, kv_heads, D), dtype=qkv.dtype, device=qkv.device).unbind(0)
+    _fusedtok.qk_norm_rope_launch(*args, k.data_ptr(), v.data_ptr(), T, q_heads, kv_heads, D,
+                                  _stream())
+    return q, k, v
+
+
+def qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, *, sections=None,
+                 theta=10000.0, rotary_dim=None, eps=1e-6, neox=False):
+    """The RMS norm of each query and key head, RoPE, and the split of a
+    projection's rows, in one pass.
+
+    qkv: [T, (q_heads + 2 * kv_heads) * D] (f32 / bf16 / fp16; rows may be
+    strided), each row a token's q heads, k heads and v heads; D even, up to 512.
+    q_weight / k_weight: [D] norm weights (float32; others are upcast), ``n = x
+    * rsqrt(mean(x^2) + eps) * weight`` over a head's D values, or None both: no
+    norm. positions: int32 [T] (any values), or [axes, T] for positions of up
+    to 4 axes (time, height, width), with ``sections`` the number of pairs
+    that turn by each axis, in order. The first ``rotary_dim`` values of a head
+    (None: D) turn as :func:`rope` does, pair j by ``position *
+    theta^(-2j/rotary_dim)``; ``neox=True`` pairs (j, j + rotary_dim/2), else (2j,
+    2j+1). Returns ``(q [T, q_heads, D], k [T, kv_heads, D], v [T, kv_heads,
+    D])``, contiguous, as the appends and the attention take them; v is a copy.
+    All in float32 (angles in float64), rounded once. Build addition."""
+    return _qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, None, None,
+                         sections, theta, rotary_dim, eps, neox)
+
+
+def qk_norm_rope_kv_append_paged(qkv, q_heads, kv_heads, q_weight, k_weight, positions, k_pool,
+                                 v_pool, slots, *, sections=None, theta=10000.0, rotary_dim=None,
+                                 eps=1e-6, neox=False):
+    """:func:`qk_norm_rope` with the keys and values written into a paged
+    cache in the same launch: row i's go to slot ``slots[i]`` = block * P + row
+    of k_pool / v_pool [Nb, kv_heads, P, D] (of qkv's dtype, in place; int32; a
+    slot outside the pools, such as -1, is skipped), as
+    :func:`block_table_extend` gives them. Steps, prompts and both mixed are
+    one call. Returns q [T, q_heads, D]. Slots of one call differ: of two rows
+    with one slot either may land, head by head. Build addition."""
+    return _qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions,
+                         (k_pool, v_pool), slots, sections, theta, rotary_dim, eps, neox)
 
 
 # ---------------------------------------------------------------------------

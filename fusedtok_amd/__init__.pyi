@@ -36,6 +36,8 @@ __all__ = [
     "block_table_extend",
     "kv_append_paged_int8",
     "attention_decode_paged_int8",
+    "qk_norm_rope",
+    "qk_norm_rope_kv_append_paged",
     "rmsnorm_quant",
     "rmsnorm_qgemm",
     "swiglu_quant",
@@ -99,6 +101,20 @@ def attention_decode_paged_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: t
                                 k_scales: torch.Tensor, v_scales: torch.Tensor,
                                 block_table: IntArray, lens: Optional[IntArray] = ...
                                 ) -> torch.Tensor: ...
+
+# -- head norms with the rotation (GPU tensors only) -------------------------------
+def qk_norm_rope(qkv: torch.Tensor, q_heads: int, kv_heads: int,
+                 q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                 positions: torch.Tensor, *, sections: Optional[Sequence[int]] = ...,
+                 theta: float = ..., rotary_dim: Optional[int] = ..., eps: float = ...,
+                 neox: bool = ...) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]: ...
+def qk_norm_rope_kv_append_paged(qkv: torch.Tensor, q_heads: int, kv_heads: int,
+                                 q_weight: Optional[torch.Tensor],
+                                 k_weight: Optional[torch.Tensor], positions: torch.Tensor,
+                                 k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Tensor,
+                                 *, sections: Optional[Sequence[int]] = ..., theta: float = ...,
+                                 rotary_dim: Optional[int] = ..., eps: float = ...,
+                                 neox: bool = ...) -> torch.Tensor: ...
 
 # -- int8 ------------------------------------------------------------------------
 @overload

@@ -42,6 +42,7 @@ HIP_SOURCES = [
     "prefill.hip",
     "sampling.hip",
     "cache8.hip",
+    "qknorm.hip",
 ]
 
 HIP_FLAGS = [

@@ -205,6 +205,41 @@ PYBIND11_MODULE(_fusedtok, m) {
           py::arg("q_heads"), py::arg("kv_heads"), py::arg("blocks"), py::arg("page"),
           py::arg("tbl_width"), py::arg("dim"), py::arg("stream") = 0);
 
+    // ---- head norms with the rotation --------------------------------------
+    m.def("qk_norm_rope_launch",
+          [](uintptr_t qkv, int dtype, long long ld, py::object qw, py::object kw, uintptr_t pos,
+             const std::vector<int>& sections, int rot, double theta, float eps, bool neox,
+             uintptr_t q, uintptr_t k, uintptr_t v, int tokens, int hq, int hkv, int dim,
+             uintptr_t stream) {
+              check(ft_qk_norm_rope_launch(
+                  P<const void>(qkv), dtype, ld, P<const float>(opt_ptr(qw)),
+                  P<const float>(opt_ptr(kw)), P<const int>(pos), (int)sections.size(),
+                  sections.data(), rot, theta, eps, neox, P<void>(q), P<void>(k), P<void>(v),
+                  tokens, hq, hkv, dim, stream));
+          },
+          py::arg("qkv"), py::arg("dtype"), py::arg("ld"), py::arg("q_weight"),
+          py::arg("k_weight"), py::arg("positions"), py::arg("sections"), py::arg("rotary_dim"),
+          py::arg("theta"), py::arg("eps"), py::arg("neox"), py::arg("q_out"), py::arg("k_out"),
+          py::arg("v_out"), py::arg("tokens"), py::arg("q_heads"), py::arg("kv_heads"),
+          py::arg("dim"), py::arg("stream") = 0);
+    m.def("qk_norm_rope_kv_append_paged_launch",
+          [](uintptr_t qkv, int dtype, long long ld, py::object qw, py::object kw, uintptr_t pos,
+             const std::vector<int>& sections, int rot, double theta, float eps, bool neox,
+             uintptr_t q, uintptr_t kp, uintptr_t vp, uintptr_t slots, int tokens, int hq, int hkv,
+             int dim, int blocks, int page, uintptr_t stream) {
+              check(ft_qk_norm_rope_kv_append_paged_launch(
+                  P<const void>(qkv), dtype, ld, P<const float>(opt_ptr(qw)),
+                  P<const float>(opt_ptr(kw)), P<const int>(pos), (int)sections.size(),
+                  sections.data(), rot, theta, eps, neox, P<void>(q), P<void>(kp), P<void>(vp),
+                  P<const int>(slots), tokens, hq, hkv, dim, blocks, page, stream));
+          },
+          py::arg("qkv"), py::arg("dtype"), py::arg("ld"), py::arg("q_weight"),
+          py::arg("k_weight"), py::arg("positions"), py::arg("sections"), py::arg("rotary_dim"),
+          py::arg("theta"), py::arg("eps"), py::arg("neox"), py::arg("q_out"), py::arg("k_pool"),
+          py::arg("v_pool"), py::arg("slots"), py::arg("tokens"), py::arg("q_heads"),
+          py::arg("kv_heads"), py::arg("dim"), py::arg("blocks"), py::arg("page"),
+          py::arg("stream") = 0);
+
     // ---- kv append --------------------------------------------------------
 #define FT_KVP(NAME, FN, T)                                                    \
     m.def(NAME,                                                                \

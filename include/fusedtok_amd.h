@@ -293,6 +293,32 @@ int ft_attention_decode_paged_int8_launch(const void* q, int dtype, const signed
                                           int dim, uintptr_t stream);
 
 /* ------------------------------------------------------------------ */
+/* Norms of query and key heads with the rotation (build addition).     */
+/* ------------------------------------------------------------------ */
+/* qkv rows [tokens, (q_heads + 2 kv_heads) * dim] (dtype FT_DT_*, row stride
+ * ld elements): per q and k head n = x / sqrt(mean(x^2) + eps) * weight (both
+ * weights NULL: n = x), then pair j of the first rotary_dim values - (j, j +
+ * rotary_dim / 2) with neox, else (2j, 2j + 1) - turned by positions[axis][t] *
+ * theta^(-2j / rotary_dim); v heads are copied. positions [axes, tokens],
+ * axes 1..4; sections (host memory, axes entries that sum to rotary_dim / 2;
+ * ignored for one axis): the pairs of each axis in order. q_out [tokens,
+ * q_heads, dim], k_out / v_out [tokens, kv_heads, dim]. dim even, up to 512. The
+ * outputs overlap no input. */
+int ft_qk_norm_rope_launch(const void* qkv, int dtype, long long ld, const float* q_weight,
+                           const float* k_weight, const int* positions, int axes,
+                           const int* sections, int rotary_dim, double theta, float eps, int neox,
+                           void* q_out, void* k_out, void* v_out, int tokens, int q_heads,
+                           int kv_heads, int dim, uintptr_t stream);
+/* The same with k and v in paged pools [blocks, kv_heads, page, dim]: token t's
+ * at row slots[t] % page of block slots[t] / page; a slot outside the pools is
+ * skipped. Slots of one call differ. */
+int ft_qk_norm_rope_kv_append_paged_launch(
+    const void* qkv, int dtype, long long ld, const float* q_weight, const float* k_weight,
+    const int* positions, int axes, const int* sections, int rotary_dim, double theta, float eps,
+    int neox, void* q_out, void* k_pool, void* v_pool, const int* slots, int tokens, int q_heads,
+    int kv_heads, int dim, int blocks, int page, uintptr_t stream);
+
+/* ------------------------------------------------------------------ */
 /* INT8 per-tensor symmetric quantize                                  */
 /* scale = max|x|/127 (1.0 for all-zero input); inv = 1.0f/scale;      */
 /* q = clamp(rint(x*inv), -127, 127). scale_out is a DEVICE float.     */

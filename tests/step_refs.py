@@ -1,0 +1,33 @@
+"""Plain forms in 64 bits of the head norms with rotation, the shared-prefix
+attention and the filtered sampling, written from their definitions."""
+
+import numpy as np
+
+
+def turn(x, pos, rot, theta, neox, sections=None):
+    """x [T, heads, D] with its first rot values turned; pos [axes, T]."""
+    half = rot // 2
+    sections = sections or [half]
+    axis = np.repeat(np.arange(len(sections)), sections)
+    freq = np.power(np.longdouble(theta), np.arange(half, dtype=np.longdouble) * -2 / rot)
+    angle = pos[axis].T.astype(np.longdouble) * freq
+    c, s = np.cos(angle)[:, None], np.sin(angle)[:, None]
+    out = x.astype(np.longdouble).copy()
+    lo = np.arange(half) if neox else 2 * np.arange(half)
+    hi = lo + (half if neox else 1)
+    a, b = x[..., lo], x[..., hi]
+    out[..., lo], out[..., hi] = a * c - b * s, b * c + a * s
+    return out.astype(np.float64)
+
+
+def qk_norm_rope(qkv, hq, hkv, qw, kw, pos, rot, theta, eps, neox, sections=None):
+    """q, k, v and, for each, the largest magnitude that a head's value may
+    take (the norm's output), which roundings are relative to."""
+    t = qkv.shape[0]
+    x = qkv.astype(np.float64).reshape(t, hq + 2 * hkv, -1)
+    parts = []
+    for part, w in ((x[:, :hq], qw), (x[:, hq:hq + hkv], kw)):
+        if w is not None:
+            part = part / np.sqrt((part ** 2).mean(-1, keepdims=True) + eps) * w
+        parts.append(turn(part, pos, rot, theta, neox, sections))
+    return parts[0], parts[1], x[:, hq + hkv:]

@@ -18,6 +18,8 @@ stubs __init__.pyi:99-107,208-236):
 - a paged KV cache held in 8 bits (build additions): ``block_table_extend``
   (block tables and slots on the GPU), ``kv_append_paged_int8`` and
   ``attention_decode_paged_int8``;
+- decode attention of sequences that share prefixes (build addition):
+  ``attention_decode_paged_prefix``;
 - norms of query and key heads with the rotation (build additions):
   ``qk_norm_rope`` and, into a paged cache, ``qk_norm_rope_kv_append_paged``;
 - the post-logits step: ``argmax`` / ``argmax_batched`` (greedy),
@@ -102,6 +104,7 @@ __all__ = [
     "block_table_extend",
     "kv_append_paged_int8",
     "attention_decode_paged_int8",
+    "attention_decode_paged_prefix",
     "qk_norm_rope",
     "qk_norm_rope_kv_append_paged",
     "rmsnorm_quant",
@@ -790,6 +793,119 @@ def attention_decode_paged_int8(q, k_pool, v_pool, k_scales, v_scales, block_tab
         q.data_ptr(), code, k_pool.data_ptr(), v_pool.data_ptr(), k_scales.data_ptr(),
         v_scales.data_ptr(), block_table.data_ptr(), None if lens is None else lens.data_ptr(),
         out.data_ptr(), ws.data_ptr(), nbytes, B, Hq, Hkv, Nb, P, S, D, _stream())
+    return out
+
+
+# ---------------------------------------------------------------------------
+# decode attention of sequences that share prefixes (build addition; GPU
+# tensors only)
+# ---------------------------------------------------------------------------
+
+_DECODE_PREFIX = _Contract(
+    _Arr("q", "B Hq D"),
+    _Arr("k_pool", "Nb Hkv P D", same_dtype="q",
+         mismatch="pools must match q's dim and each other"),
+    _Arr("v_pool", "=k_pool", same_dtype="q",
+         mismatch="pools must match q's dim and each other"),
+    _Idx("prefix_table", "G W", lambda c: c.Nb, open_bound=True,
+         what="prefix_table must be [G, W]"),
+    _Idx("prefix_lens", "G", lambda c: c.W * c.P, optional=True,
+         what="prefix_lens must be 1-D with an entry for each group"),
+    _table(),
+    _Idx("lens", "B", lambda c: c.S * c.P, optional=True, what=_LENS_WHAT),
+    _Idx("group_offsets", "O", lambda c: c.B, optional=True,
+         what="group_offsets must be 1-D"),
+    rank_msg="q must be [B, Hq, D]; pools [Nb, Hkv, P, D]", rules=(_HEADS, _GQA), host=False)
+
+
+@functools.lru_cache(maxsize=1024)
+def _prefix_workspace(device, *sizes):
+    """Workspace bytes of an attention_decode_paged_prefix call of these sizes
+    on the (current) device; the checks of the sizes are made here."""
+    return _fusedtok.attention_decode_paged_prefix_workspace(*sizes)
+
+
+def attention_decode_paged_prefix(q, k_pool, v_pool, prefix_table, prefix_lens, block_table,
+                                  lens=None, group_offsets=None):
+    """Single-token GQA attention over a paged cache for sequences that share
+    prefixes, such as the system prompt of a batch of conversations:
+
+    ``out[b, h] = softmax(q[b, h] . K[kv(h)]^T / sqrt(D)) . V[kv(h)]`` over the
+    tokens of the prefix of b's group, then b's own.
+
+    q: [B, Hq, D]; k_pool / v_pool: [Nb, Hkv, P, D] (f32 / bf16 / fp16, one type,
+    also the output's). Group g is the sequences ``group_offsets[g]`` to
+    ``group_offsets[g + 1] - 1`` ([G + 1], not falling; None: one group of all)
+    and shares the first ``prefix_lens[g]`` tokens (None: all) of row g of
+    ``prefix_table`` [G, W]; token t lies at row ``t % P`` of block
+    ``prefix_table[g, t // P]``. ``lens[b]`` own tokens (None: all) follow, in row
+    b of ``block_table`` [B, S] as :func:`attention_decode_paged` has it,
+    counted from 0: a sequence's own tokens start in a block of their own. A
+    sequence in no group has no prefix. A prefix' keys and values are read once
+    for all heads of its group that share them, up to 128 rows at a time, so
+    this pays from two sequences on.
+
+    Any group size Hq / Hkv, D a multiple of 4 up to 512 (on the matrix cores: bf16
+    and fp16 with D % 8 == 0 up to 128, tensors aligned to 16 bytes), at most
+    4096 sequences and groups together, B * Hq below 2**24. Softmax and sums are
+    float32; bf16 / fp16 weights go into the product with V as two parts of the
+    type, off by at most 2**-17 of a weight, and fp16 weights below 2**-32 of a
+    row's largest count as 0. K and V of the tokens that count are finite;
+    whatever lies in the blocks behind them does not matter. Host-origin tables
+    and lengths are range-checked; of GPU-resident ones any values are safe:
+    lengths are clamped to the tables, tokens of a table entry outside [0, Nb)
+    (such as -1) weigh nothing, offsets are clamped to [0, B] and to those before them.
+    A sequence without a token gives zero rows. How the tokens are cut into
+    pieces depends on the whole batch: the same call gives the same bits, but a
+    sequence's last bits may change with its neighbours. Each call has a
+    workspace of its own from torch's allocator, so calls on several streams
+    are independent. Build addition."""
+    try:
+        (B, Hq, D), (Nb, Hkv, P, dim), (rows, S) = q.shape, k_pool.shape, block_table.shape
+        G, W = prefix_table.shape
+        dev = q.get_device()
+        ready = (D == dim and B == rows and q.dtype in _CODE and k_pool.dtype is q.dtype and
+                 v_pool.dtype is q.dtype and v_pool.shape == k_pool.shape and
+                 q.is_contiguous() and k_pool.is_contiguous() and v_pool.is_contiguous() and
+                 Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and q.is_cuda and
+                 dev == k_pool.get_device() == v_pool.get_device() == _current_device() and
+                 _i32_ready(dev, block_table, prefix_table) and
+                 (lens is None or lens.shape == (B,) and _i32_ready(dev, lens)) and
+                 (prefix_lens is None or prefix_lens.shape == (G,) and
+                  _i32_ready(dev, prefix_lens)) and
+                 (group_offsets is None or _i32_ready(dev, group_offsets) and
+                  group_offsets.ndim == 1))
+    except (AttributeError, TypeError, ValueError):
+        ready = False
+    if not ready:
+        c = _DECODE_PREFIX.bind(q=q, k_pool=k_pool, v_pool=v_pool, prefix_table=prefix_table,
+                                prefix_lens=prefix_lens, block_table=block_table, lens=lens,
+                                group_offsets=group_offsets)
+        given = [(n, getattr(c, n)) for n in ("q", "k_pool", "v_pool", "prefix_table",
+                                              "prefix_lens", "block_table", "lens",
+                                              "group_offsets") if getattr(c, n) is not None]
+        if not _one_device(*zip(*given)):
+            with torch.cuda.device(c.device):
+                return attention_decode_paged_prefix(**dict(given))
+        prefix_table, prefix_lens, block_table, lens, group_offsets = (
+            c.prefix_table, c.prefix_lens, c.block_table, c.lens, c.group_offsets)
+        B, Hq, Hkv, Nb, P, S, D, G, W = (c.B, c.Hq, c.Hkv, c.Nb, c.P, c.S, c.D, c.G, c.W)
+        dev = c.device.index
+    if group_offsets is None:
+        if G > 1:
+            raise ValueError("several groups need group_offsets")
+    elif group_offsets.shape[0] != G + 1:
+        raise ValueError("group_offsets must have an entry more than there are groups")
+    code = _CODE[q.dtype]
+    nbytes = _prefix_workspace(dev, code, B, Hq, Hkv, G, P, W, S, D)
+    out = torch.empty_like(q)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _fusedtok.attention_decode_paged_prefix_launch(
+        q.data_ptr(), code, k_pool.data_ptr(), v_pool.data_ptr(), prefix_table.data_ptr(),
+        None if prefix_lens is None else prefix_lens.data_ptr(),
+        None if group_offsets is None else group_offsets.data_ptr(), block_table.data_ptr(),
+        None if lens is None else lens.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes, B, Hq,
+        Hkv, G, Nb, P, W, S, D, _stream())
     return out
 
 

@@ -36,6 +36,7 @@ __all__ = [
     "block_table_extend",
     "kv_append_paged_int8",
     "attention_decode_paged_int8",
+    "attention_decode_paged_prefix",
     "qk_norm_rope",
     "qk_norm_rope_kv_append_paged",
     "rmsnorm_quant",
@@ -101,6 +102,12 @@ def attention_decode_paged_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: t
                                 k_scales: torch.Tensor, v_scales: torch.Tensor,
                                 block_table: IntArray, lens: Optional[IntArray] = ...
                                 ) -> torch.Tensor: ...
+
+# -- decode attention of sequences that share prefixes (GPU tensors only) ----------
+def attention_decode_paged_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                                  prefix_table: IntArray, prefix_lens: Optional[IntArray],
+                                  block_table: IntArray, lens: Optional[IntArray] = ...,
+                                  group_offsets: Optional[IntArray] = ...) -> torch.Tensor: ...
 
 # -- head norms with the rotation (GPU tensors only) -------------------------------
 def qk_norm_rope(qkv: torch.Tensor, q_heads: int, kv_heads: int,

@@ -43,6 +43,7 @@ HIP_SOURCES = [
     "sampling.hip",
     "cache8.hip",
     "qknorm.hip",
+    "prefix.hip",
 ]
 
 HIP_FLAGS = [

@@ -205,6 +205,37 @@ PYBIND11_MODULE(_fusedtok, m) {
           py::arg("q_heads"), py::arg("kv_heads"), py::arg("blocks"), py::arg("page"),
           py::arg("tbl_width"), py::arg("dim"), py::arg("stream") = 0);
 
+    // ---- decode attention of sequences that share prefixes ------------------
+    m.def("attention_decode_paged_prefix_workspace",
+          [](int dtype, int batch, int hq, int hkv, int groups, int page, int pwidth, int twidth,
+             int dim) {
+              long long bytes = 0;
+              check(ft_attention_decode_paged_prefix_workspace(dtype, batch, hq, hkv, groups, page,
+                                                               pwidth, twidth, dim, &bytes));
+              return bytes;
+          },
+          py::arg("dtype"), py::arg("batch"), py::arg("q_heads"), py::arg("kv_heads"),
+          py::arg("groups"), py::arg("page"), py::arg("prefix_width"), py::arg("tbl_width"),
+          py::arg("dim"));
+    m.def("attention_decode_paged_prefix_launch",
+          [](uintptr_t q, int dtype, uintptr_t kp, uintptr_t vp, uintptr_t ptable, py::object plens,
+             py::object offsets, uintptr_t table, py::object lens, uintptr_t out, uintptr_t ws,
+             long long ws_bytes, int batch, int hq, int hkv, int groups, int blocks, int page,
+             int pwidth, int twidth, int dim, uintptr_t stream) {
+              check(ft_attention_decode_paged_prefix_launch(
+                  P<const void>(q), dtype, P<const void>(kp), P<const void>(vp),
+                  P<const int>(ptable), P<const int>(opt_ptr(plens)),
+                  P<const int>(opt_ptr(offsets)), P<const int>(table),
+                  P<const int>(opt_ptr(lens)), P<void>(out), P<void>(ws), ws_bytes, batch, hq, hkv,
+                  groups, blocks, page, pwidth, twidth, dim, stream));
+          },
+          py::arg("q"), py::arg("dtype"), py::arg("k_pool"), py::arg("v_pool"),
+          py::arg("prefix_table"), py::arg("prefix_lens"), py::arg("group_offsets"),
+          py::arg("table"), py::arg("lens"), py::arg("out"), py::arg("workspace"),
+          py::arg("workspace_bytes"), py::arg("batch"), py::arg("q_heads"), py::arg("kv_heads"),
+          py::arg("groups"), py::arg("blocks"), py::arg("page"), py::arg("prefix_width"),
+          py::arg("tbl_width"), py::arg("dim"), py::arg("stream") = 0);
+
     // ---- head norms with the rotation --------------------------------------
     m.def("qk_norm_rope_launch",
           [](uintptr_t qkv, int dtype, long long ld, py::object qw, py::object kw, uintptr_t pos,

@@ -5,6 +5,7 @@
 // v_scales float32 [blocks, kv heads]; the value at row r of block n, head h is
 // code * scale[n, h]. A slot is block * page + row.
 #include "attn_common.hpp"
+#include "fast_div.hpp"
 #include "ft_common.hpp"
 
 #include <algorithm>
@@ -36,26 +37,6 @@ void check_aligned(const void* p, size_t bytes, const char* what) {
               std::to_string(bytes) + " bytes");
 }
 inline size_t size_of(int dtype) { return dtype == FT_DT_F32 ? 4 : 2; }
-
-// Division by a size known at launch, n / d for 0 <= n < 2^31: with l =
-// ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1, n / d = (mulhi(m, n) + n)
-// >> l (Granlund and Montgomery 1994). Three instructions for the ~25 of a
-// 32-bit division.
-struct FastDiv {
-    unsigned d, m, l;
-    FastDiv() = default;
-    explicit FastDiv(int by) : d((unsigned)by), m(0), l(0) {
-        while ((1ull << l) < d) ++l;
-        m = (unsigned)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
-    }
-    __device__ __forceinline__ int div(int n) const {
-        return (int)((__umulhi(m, (unsigned)n) + (unsigned)n) >> l);
-    }
-    __device__ __forceinline__ int up(int n) const {  // ceil(n / d), n <= 2^30
-        return div(n + (int)d - 1);
-    }
-    __device__ __forceinline__ int mod(int n) const { return n - div(n) * (int)d; }
-};
 
 // ---------------------------------------------------------------------------
 // Block tables and slot maps.

@@ -1,0 +1,978 @@
+// Decode attention of a batch whose sequences share long prefixes, for gfx950:
+//
+//   out[b, h] = softmax(q[b, h] . K / sqrt(D)) . V  over the tokens of the
+//   prefix of b's group, then b's own, both in one paged cache.
+//
+// q, out [B, Hq, D]; k_pool, v_pool [blocks, Hkv, P, D]; group g is the
+// sequences [off_g, off_g+1), its prefix lies in row g of prefix_table, a
+// sequence's own tokens in its row of table.
+//
+// Work split. An entry is a group's prefix or a sequence's own tokens: rows
+// (the q heads of its sequences that read one kv head) against n tokens. Its
+// units are (kv head, tile of rows), n tokens each; all units are laid end to
+// end and every workgroup takes one equal contiguous segment of that range,
+// whatever the mix of lengths. A segment is one or more pieces, one a unit it
+// touches; a piece leaves a float32 partial (m, l, acc[D]) a row, which
+// prefix_combine folds by the log-sum-exp rule: of each (b, h) the pieces of
+// the group's prefix and of its own tokens. A piece's partials start at row
+// 16 (8 segment + granules of the units before it), a granule being 16 rows of
+// a tile, 8 of them at most: pieces are ordered in both, so the places are
+// disjoint and both kernels work them out from the plan (the entries' sums),
+// which every workgroup scans by itself and the first leaves for the combine.
+// Nothing else passes between workgroups and the workspace is the caller's.
+#include "attn_common.hpp"
+#include "fast_div.hpp"
+#include "ft_common.hpp"
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+namespace ft {
+namespace {
+
+constexpr int kMaxDimP = 512;
+constexpr int kMaxEntries = 4096;  // groups and sequences of a call (their sums are in LDS)
+constexpr int kGranule = 16;       // rows
+constexpr int kTileGranules = 8;   // of a tile, at most
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// What the combine needs of an entry.
+struct Entry {
+    long long start;  // of its units in the range of all
+    int gran;         // granules before it
+    int n;            // tokens
+    int rows;         // rows a kv head
+    int first;        // its first sequence
+};
+
+struct PrefixArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    const int* ptable;
+    const int* plens;
+    const int* offsets;
+    const int* table;
+    const int* lens;
+    void* out;
+    float* ml;       // [rows][2]
+    float* acc;      // [rows][dim]
+    Entry* entries;  // [groups + batch + 1]; the last: start = the segments' length
+    int* group_of;   // [batch], -1: none
+    int batch, hq, hkv, gq, groups, blocks, pwidth, twidth, dim;
+    FastDiv page, gdiv;
+    float scale_log2;
+    int segs, min_seg;
+};
+
+// Rows of a tile. On the matrix cores (WIDE): up to 16 rows leave the keys of a
+// step to the four waves, more are shared out to them, 16 or 32 each.
+template <bool WIDE>
+__device__ __forceinline__ int tile_rows(int rows) {
+    if (!WIDE || rows <= 16) return 16;
+    return rows <= 64 ? 64 : 128;
+}
+__device__ __forceinline__ int up(int a, int b) { return (a + b - 1) / b; }
+
+// The plan, in LDS: sum of the tokens of all units before an entry, granules
+// before it, and the groups' first sequences.
+struct Plan {
+    long long* start;  // [E + 1]
+    int* gran;         // [E]
+    int* first;        // [G + 1]
+    int entries;
+    static size_t bytes(int entries, int groups) {
+        return 8 * (size_t)(entries + 1) + 4 * (size_t)entries + 4 * (size_t)(groups + 1);
+    }
+};
+
+// offsets in [0, batch] and not falling, whatever their values: the running
+// maximum of the clamped ones. So no sequence is in two groups.
+__device__ __forceinline__ int clamped_offset(const PrefixArgs& a, int g) {
+    if (!a.offsets) return g ? a.batch : 0;
+    return min(max(a.offsets[g], 0), a.batch);
+}
+
+__device__ __forceinline__ int entry_tokens(const PrefixArgs& a, int e) {
+    return e < a.groups ? clamp_len(a.plens, e, a.pwidth * (int)a.page.d)
+                        : clamp_len(a.lens, e - a.groups, a.twidth * (int)a.page.d);
+}
+__device__ __forceinline__ int entry_rows(const PrefixArgs& a, const Plan& p, int e) {
+    return e < a.groups ? (p.first[e + 1] - p.first[e]) * a.gq : a.gq;
+}
+
+template <bool WIDE>
+__device__ void make_plan(const PrefixArgs& a, const Plan& p, long long* s_sum, int* s_cnt) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // the groups' first sequences: thread t takes offsets [t per, ...)
+    {
+        const int n = a.groups + 1, per = up(n, 256);
+        const int lo = min(tid * per, n), hi = min(lo + per, n);
+        int most = 0;
+        for (int g = lo; g < hi; ++g) p.first[g] = most = max(most, clamped_offset(a, g));
+        int run = most;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(run, o, 64);
+            if (lane >= o) run = max(run, x);
+        }
+        if (lane == 63) s_cnt[wave] = run;
+        int before = __shfl_up(run, 1, 64);
+        if (lane == 0) before = 0;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) before = max(before, s_cnt[w]);
+        for (int g = lo; g < hi; ++g) p.first[g] = max(p.first[g], before);
+        __syncthreads();
+    }
+    const int E = p.entries, per = up(E, 256);
+    const int lo = min(tid * per, E), hi = min(lo + per, E);
+    long long sum = 0;
+    int gran = 0;
+    for (int e = lo; e < hi; ++e) {
+        const int rows = entry_rows(a, p, e);
+        p.start[e] = sum;
+        p.gran[e] = gran;
+        sum += (long long)entry_tokens(a, e) * a.hkv * up(rows, tile_rows<WIDE>(rows));
+        gran += a.hkv * up(rows, kGranule);
+    }
+    long long s = sum;
+    int c = gran;
+    for (int o = 1; o < 64; o <<= 1) {
+        const long long x = __shfl_up(s, o, 64);
+        const int y = __shfl_up(c, o, 64);
+        if (lane >= o) s += x, c += y;
+    }
+    if (lane == 63) s_sum[wave] = s, s_cnt[wave] = c;
+    __syncthreads();
+    s -= sum, c -= gran;
+    for (int w = 0; w < wave; ++w) s += s_sum[w], c += s_cnt[w];
+    for (int e = lo; e < hi; ++e) p.start[e] += s, p.gran[e] += c;
+    if (tid == 255) p.start[E] = s + sum;
+    __syncthreads();
+}
+
+// Tokens a segment: an equal share, in whole steps.
+__device__ __forceinline__ long long segment(const PrefixArgs& a, long long total) {
+    const long long s = (total + a.segs - 1) / a.segs;
+    return ((s < a.min_seg ? a.min_seg : s) + 63) & ~63LL;
+}
+
+// The combine's copy of the plan.
+__device__ void leave_plan(const PrefixArgs& a, const Plan& p, long long seg) {
+    for (int e = threadIdx.x; e <= p.entries; e += 256) {
+        Entry x{seg, 0, 0, 0, 0};
+        if (e < p.entries)
+            x = Entry{p.start[e], p.gran[e], entry_tokens(a, e), entry_rows(a, p, e),
+                      e < a.groups ? p.first[e] : e - a.groups};
+        a.entries[e] = x;
+    }
+    for (int b = threadIdx.x; b < a.batch; b += 256) {
+        int lo = 0, hi = a.groups;  // the last g with first[g] <= b
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            (p.first[mid] <= b ? lo : hi) = mid;
+        }
+        const bool in = a.groups > 0 && p.first[lo] <= b && b < p.first[lo + 1];
+        a.group_of[b] = in ? lo : -1;
+    }
+}
+
+// A segment's piece that starts at pos.
+struct Piece {
+    int entry, first, rows, kv, row0;  // row0: the tile's first row
+    int t0, n;
+    const int* table;
+    size_t slot;  // its partials' first row
+};
+template <bool WIDE>
+__device__ __forceinline__ Piece piece_at(const PrefixArgs& a, const Plan& p, long long pos,
+                                          long long end) {
+    int lo = 0, hi = p.entries;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        (p.start[mid] <= pos ? lo : hi) = mid;
+    }
+    Piece x;
+    x.entry = __builtin_amdgcn_readfirstlane(lo);
+    const int n = entry_tokens(a, x.entry);
+    x.rows = entry_rows(a, p, x.entry);
+    const bool own = x.entry >= a.groups;
+    x.first = own ? x.entry - a.groups : p.first[x.entry];
+    const int tr = tile_rows<WIDE>(x.rows), tiles = up(x.rows, tr);
+    const long long off = pos - p.start[x.entry];
+    const int unit = (int)(off / n);
+    x.t0 = (int)(off - (long long)unit * n);
+    x.n = (int)min((long long)(n - x.t0), end - pos);
+    x.kv = unit / tiles;
+    const int tile = unit - x.kv * tiles;
+    x.row0 = tile * tr;
+    x.table = own ? a.table + (size_t)x.first * a.twidth : a.ptable + (size_t)x.entry * a.pwidth;
+    const size_t gran = (size_t)kTileGranules * blockIdx.x + p.gran[x.entry] +
+                        (size_t)x.kv * up(x.rows, kGranule) + tile * (tr / kGranule);
+    x.slot = gran * kGranule;
+    // (the same in every lane)
+    x.first = __builtin_amdgcn_readfirstlane(x.first);
+    x.rows = __builtin_amdgcn_readfirstlane(x.rows);
+    x.kv = __builtin_amdgcn_readfirstlane(x.kv);
+    x.row0 = __builtin_amdgcn_readfirstlane(x.row0);
+    x.t0 = __builtin_amdgcn_readfirstlane(x.t0);
+    x.n = __builtin_amdgcn_readfirstlane(x.n);
+    x.slot = (size_t)uniform64((long long)x.slot);
+    return x;
+}
+
+// Row r of an entry: sequence first + r / gq, q head kv * gq + r % gq.
+__device__ __forceinline__ size_t q_row(const PrefixArgs& a, const Piece& p, int r) {
+    const int s = a.gdiv.div(r);
+    return (size_t)(p.first + s) * a.hq + (size_t)p.kv * a.gq + (r - s * a.gq);
+}
+
+// ---------------------------------------------------------------------------
+// bf16 / fp16 on the matrix cores, dim a multiple of 8 up to D (64 or 128; a
+// smaller dim's missing 16-byte chunks are zero), 16-byte aligned.
+//
+// A step is 64 tokens: K and V rows go through two LDS stages, the next one's
+// loads in flight while this one is computed. Everything is transposed, so an
+// accumulator's lane holds one row (r = lane % 16, g = lane / 16; operands of
+// v_mfma_f32_16x16x32: A[r][8g+j], B[8g+j][r], C[4g+i][r]):
+//
+//   scores  S^T[key][row] = K . Q^T, Q in registers for the whole piece;
+//   softmax online, a row's keys in 4 lanes; the maximum moves only when a
+//           step's exceeds it by 8 (log2), so weights are at most 2^8;
+//   PV      O^T[dim][row] += V^T . P^T, P straight from the scores: lane (r, g)
+//           holds keys 4g+i of each block of 16, so two blocks fill its 8
+//           slots, and V^T comes in the same order by ds_read_b64_tr_b16.
+//   weights in two parts of the storage type, the first truncated, the second
+//           rounded: 16 bits for bf16, 22 for fp16 (there times 2^7, so that
+//           weights down to 2^-31 of the maximum are held, finer than 2^-32).
+//           An error of 2^-17 of a weight is far below half a step of the
+//           output, 2^-9, and goes either way; sums are float32.
+//
+// Tiles of up to 16 rows (KEYS): wave w takes keys 16w .. of each step with a
+// softmax of its own, merged at the piece's end. Larger ones: 16 QB rows a
+// wave, all 64 keys.
+// ---------------------------------------------------------------------------
+template <typename T> struct PMma;
+template <> struct PMma<bf16> {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    static constexpr float kUp = 1.0f;
+    __device__ __forceinline__ static f32x4 mma(v8 a, v8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    // two weights as (first, second) parts, packed
+    __device__ __forceinline__ static int2 split(float a, float b) {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef bf16 t2 __attribute__((ext_vector_type(2)));
+        const unsigned u = __float_as_uint(a), w = __float_as_uint(b);
+        const f2 rest = {a - __uint_as_float(u & 0xffff0000u),
+                         b - __uint_as_float(w & 0xffff0000u)};
+        return make_int2((int)((u >> 16) | (w & 0xffff0000u)),
+                         __builtin_bit_cast(int, __builtin_convertvector(rest, t2)));
+    }
+};
+template <> struct PMma<f16> {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    static constexpr float kUp = 128.0f;
+    __device__ __forceinline__ static f32x4 mma(v8 a, v8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    __device__ __forceinline__ static int2 split(float a, float b) {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef f16 t2 __attribute__((ext_vector_type(2)));
+        const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+        const f2 rest = {a - (float)h[0], b - (float)h[1]};
+        return make_int2(__builtin_bit_cast(int, h),
+                         __builtin_bit_cast(int, __builtin_convertvector(rest, t2)));
+    }
+};
+
+template <int D>
+struct PCfg {
+    static constexpr int kPitch = 2 * D + 16;        // bytes of a staged row
+    static constexpr int kStage = 2 * 64 * kPitch;   // K rows, then V rows
+    static constexpr int kChunks = 64 * D / 8 / 256; // 16-byte chunks a thread, each of K and V
+    static constexpr int kS = D / 32;                // k-steps of the scores
+    static constexpr int kDB = D / 16;               // blocks of dims
+};
+
+template <typename T, int D, bool FULL, int QB, bool KEYS>
+__device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& pc, char* smem,
+                                             float (*s_ml)[2][16]) {
+    using M = PMma<T>;
+    using V8 = typename M::v8;
+    using C = PCfg<D>;
+    constexpr int KB = KEYS ? 1 : 4;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int dim = FULL ? D : a.dim;
+    const T* const kp = (const T*)a.k;
+    const T* const vp = (const T*)a.v;
+
+    // the wave's Q as B operands; rows past the entry's are zero
+    const int wrow = pc.row0 + (KEYS ? 0 : 16 * QB * wave);  // its first row
+    const bool active = wrow < pc.rows;
+    V8 qf[QB][C::kS];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const int r = wrow + 16 * qb + r16;
+        const bool on = r < pc.rows;
+        const T* const row = (const T*)a.q + q_row(a, pc, on ? r : pc.row0) * dim;
+#pragma unroll
+        for (int s = 0; s < C::kS; ++s) {
+            V8 x = {};
+            if (on && (FULL || 32 * s + 8 * g < dim))
+                x = *reinterpret_cast<const V8*>(row + 32 * s + 8 * g);
+            qf[qb][s] = x;
+        }
+    }
+
+    const int steps = (pc.n + 63) >> 6;
+    // lane l's key of step st: its table entry, -1 past the piece (and where
+    // the table has no block)
+    auto entry_of = [&](int st) {
+        const int t = 64 * st + lane;
+        if (t >= pc.n) return -1;
+        const int e = pc.table[a.page.div(pc.t0 + t)];
+        return (unsigned)e < (unsigned)a.blocks ? e : -1;
+    };
+    i32x4 kreg[C::kChunks], vreg[C::kChunks];
+    auto load = [&](int st, int ent) {
+#pragma unroll
+        for (int j = 0; j < C::kChunks; ++j) {
+            const int c = tid + 256 * j, row = c / (D / 8), ch = c % (D / 8);
+            const int e = __shfl(ent, row, 64);
+            const i32x4 z = {0, 0, 0, 0};
+            kreg[j] = vreg[j] = z;
+            if (e >= 0 && (FULL || 8 * ch < dim)) {
+                const size_t off =
+                    (((size_t)e * a.hkv + pc.kv) * a.page.d + a.page.mod(pc.t0 + 64 * st + row)) *
+                        dim + 8 * ch;
+                if constexpr (KEYS) {  // read once
+                    kreg[j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(kp + off));
+                    vreg[j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(vp + off));
+                } else {
+                    kreg[j] = *reinterpret_cast<const i32x4*>(kp + off);
+                    vreg[j] = *reinterpret_cast<const i32x4*>(vp + off);
+                }
+            }
+        }
+    };
+    auto stage = [&](int st) {
+        char* const ks = smem + (st & 1) * C::kStage;
+        char* const vs = ks + 64 * C::kPitch;
+#pragma unroll
+        for (int j = 0; j < C::kChunks; ++j) {
+            const int c = tid + 256 * j, at = (c / (D / 8)) * C::kPitch + 16 * (c % (D / 8));
+            *reinterpret_cast<i32x4*>(ks + at) = kreg[j];
+            *reinterpret_cast<i32x4*>(vs + at) = vreg[j];
+        }
+    };
+
+    f32x4 o[C::kDB][QB];
+#pragma unroll
+    for (int db = 0; db < C::kDB; ++db)
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_run[QB], l_run[QB];  // the maximum in log2 units, as it was subtracted
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) m_run[qb] = -INFINITY, l_run[qb] = 0.f;
+    const float c2 = a.scale_log2;
+
+    int ent = entry_of(0);
+    int next = steps > 1 ? entry_of(1) : -1;
+    load(0, ent);
+    unsigned long long held = __builtin_amdgcn_ballot_w64(ent >= 0);
+    stage(0);
+    __syncthreads();
+    for (int st = 0; st < steps; ++st) {
+        unsigned long long held_next = 0;
+        if (st + 1 < steps) {
+            load(st + 1, next);
+            held_next = __builtin_amdgcn_ballot_w64(next >= 0);
+            next = st + 2 < steps ? entry_of(st + 2) : -1;
+        }
+        if (active) {
+            const char* const ks = smem + (st & 1) * C::kStage;
+            const char* const vs = ks + 64 * C::kPitch;
+            const int k0 = KEYS ? 16 * wave : 0;  // the wave's first key
+            f32x4 sc[KB][QB];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) sc[kb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < C::kS; ++s)
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    const V8 kf = *reinterpret_cast<const V8*>(
+                        ks + (k0 + 16 * kb + r16) * C::kPitch + (32 * s + 8 * g) * 2);
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb)
+                        sc[kb][qb] = M::mma(kf, qf[qb][s], sc[kb][qb]);
+                }
+            if (held != ~0ull) {  // past the piece, or no block
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    const unsigned bits = (unsigned)(held >> (k0 + 16 * kb + 4 * g));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(bits >> i & 1)) {
+#pragma unroll
+                            for (int qb = 0; qb < QB; ++qb) sc[kb][qb][i] = -INFINITY;
+                        }
+                }
+            }
+            constexpr int KS = KEYS ? 1 : 2;  // k-steps of the PV product
+            i32x4 ph[QB][KS], pl[QB][KS];
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[kb][qb][i]);
+                top = max4_rows(top) * c2;
+                const bool moved = top > m_run[qb] + 8.0f;
+                const float m_new = moved ? top : m_run[qb];
+                const float m_use = m_new == -INFINITY ? 0.f : m_new;
+                const float alpha = __builtin_amdgcn_exp2f(m_run[qb] - m_use);
+                m_run[qb] = m_new;
+                float p[KB][4], sum = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        p[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][qb][i], c2, -m_use));
+                        sum += p[kb][i];
+                    }
+                l_run[qb] = l_run[qb] * alpha + sum;
+                if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+                    for (int db = 0; db < C::kDB; ++db) o[db][qb] *= alpha;
+                }
+#pragma unroll
+                for (int x = 0; x < KS; ++x)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        if (KEYS && w >= 2) {  // one block of keys: the other slots are empty
+                            ph[qb][x][w] = pl[qb][x][w] = 0;
+                            continue;
+                        }
+                        const float* const pp = p[KEYS ? 0 : 2 * x + (w >> 1)] + 2 * (w & 1);
+                        const int2 both = M::split(pp[0] * M::kUp, pp[1] * M::kUp);
+                        ph[qb][x][w] = both.x;
+                        pl[qb][x][w] = both.y;
+                    }
+            }
+            // V^T: dims 16 db + r, keys k0 + 32 x + 4g + (0..3) and 16 more
+#pragma unroll
+            for (int db = 0; db < C::kDB; ++db)
+#pragma unroll
+                for (int x = 0; x < KS; ++x) {
+                    typedef short v4s __attribute__((ext_vector_type(4)));
+                    typedef short v8s __attribute__((ext_vector_type(8)));
+                    const char* const p = vs + (k0 + 32 * x + 4 * g + (r16 >> 2)) * C::kPitch +
+                                          (16 * db + 4 * (r16 & 3)) * 2;
+                    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) v4s*)(p));
+                    v4s hi = {0, 0, 0, 0};
+                    if constexpr (!KEYS)
+                        hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) v4s*)(p + 16 * C::kPitch));
+                    const v8s vt = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    const V8 vf = __builtin_bit_cast(V8, vt);
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb) {
+                        o[db][qb] = M::mma(vf, __builtin_bit_cast(V8, ph[qb][x]), o[db][qb]);
+                        o[db][qb] = M::mma(vf, __builtin_bit_cast(V8, pl[qb][x]), o[db][qb]);
+                    }
+                }
+        }
+        if (st + 1 < steps) stage(st + 1);
+        held = held_next;
+        __syncthreads();
+    }
+
+    // partials: lane (r, g) holds dims 16 db + 4g + i of row r
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        l_run[qb] += __shfl_xor(l_run[qb], 16, 64);
+        l_run[qb] += __shfl_xor(l_run[qb], 32, 64);
+    }
+    if constexpr (!KEYS) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            const int r = wrow + 16 * qb + r16;
+            if (r >= pc.rows) continue;
+            const size_t row = pc.slot + (r - pc.row0);
+            if (g == 0) {
+                a.ml[2 * row] = m_run[qb];
+                a.ml[2 * row + 1] = l_run[qb];
+            }
+#pragma unroll
+            for (int db = 0; db < C::kDB; ++db)
+                if (FULL || 16 * db + 4 * g < dim)
+                    *reinterpret_cast<f32x4*>(a.acc + row * dim + 16 * db + 4 * g) =
+                        o[db][qb] * (1.0f / M::kUp);
+        }
+    } else {
+        // the waves' softmaxes are merged through the staging area
+        constexpr int kRow = D + 4;
+        float* const s_acc = reinterpret_cast<float*>(smem);
+        if (g == 0) {
+            s_ml[wave][0][r16] = m_run[0];
+            s_ml[wave][1][r16] = l_run[0];
+        }
+#pragma unroll
+        for (int db = 0; db < C::kDB; ++db)
+            *reinterpret_cast<f32x4*>(s_acc + (16 * wave + r16) * kRow + 16 * db + 4 * g) = o[db][0];
+        __syncthreads();
+        const int rr = tid >> 4, r = pc.row0 + rr;
+        if (r < pc.rows) {
+            float m = -INFINITY, l = 0.f, f[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) m = fmaxf(m, s_ml[w][0][rr]);
+            const float m_use = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                f[w] = __builtin_amdgcn_exp2f(s_ml[w][0][rr] - m_use);
+                l += f[w] * s_ml[w][1][rr];
+            }
+            const size_t row = pc.slot + rr;
+            if ((tid & 15) == 0) {
+                a.ml[2 * row] = m;
+                a.ml[2 * row + 1] = l;
+            }
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x) {
+                const int d = 64 * x + 4 * (tid & 15);
+                f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    y += f[w] * *reinterpret_cast<const f32x4*>(s_acc + (16 * w + rr) * kRow + d);
+                if (FULL || d < dim)
+                    *reinterpret_cast<f32x4*>(a.acc + row * dim + d) = y * (1.0f / M::kUp);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int D, bool FULL>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void prefix_attn(const PrefixArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ float s_ml[4][2][16];
+    __shared__ long long s_sum[4];
+    __shared__ int s_cnt[4];
+    Plan p;
+    p.entries = a.groups + a.batch;
+    p.start = reinterpret_cast<long long*>(smem + 2 * PCfg<D>::kStage);
+    p.gran = reinterpret_cast<int*>(p.start + p.entries + 1);
+    p.first = p.gran + p.entries;
+    make_plan<true>(a, p, s_sum, s_cnt);
+    const long long total = uniform64(p.start[p.entries]);
+    const long long seg = segment(a, total);
+    if (blockIdx.x == 0) leave_plan(a, p, seg);
+    long long pos = (long long)blockIdx.x * seg;
+    const long long end = min(pos + seg, total);
+    while (pos < end) {
+        const Piece pc = piece_at<true>(a, p, pos, end);
+        if (pc.rows <= 16) prefix_piece<T, D, FULL, 1, true>(a, pc, smem, s_ml);
+        else if (pc.rows <= 64) prefix_piece<T, D, FULL, 1, false>(a, pc, smem, s_ml);
+        else prefix_piece<T, D, FULL, 2, false>(a, pc, smem, s_ml);
+        pos += pc.n;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Every other type, head dim and alignment: 16 rows of a piece against 64
+// tokens a step on the vector ALU. Thread (row, x) scores tokens x, x + 16, ..
+// of the step; then threads own 4 dims of a few rows.
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void prefix_general(const PrefixArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ long long s_sum[4];
+    __shared__ int s_cnt[4];
+    __shared__ long long s_off[64];  // the step's rows in the pools, -1: none
+    __shared__ float s_p[16][64], s_alpha[16];
+    const int tid = threadIdx.x, dim = a.dim, dc = dim / 4;
+    float* const s_q = reinterpret_cast<float*>(smem);  // [16][dim]
+    Plan p;
+    p.entries = a.groups + a.batch;
+    p.start = reinterpret_cast<long long*>(smem + 64 * (size_t)dim);
+    p.gran = reinterpret_cast<int*>(p.start + p.entries + 1);
+    p.first = p.gran + p.entries;
+    make_plan<false>(a, p, s_sum, s_cnt);
+    const long long total = uniform64(p.start[p.entries]);
+    const long long seg = segment(a, total);
+    if (blockIdx.x == 0) leave_plan(a, p, seg);
+    const T* const kp = (const T*)a.k;
+    const T* const vp = (const T*)a.v;
+
+    const int row = tid >> 4, x16 = tid & 15;
+    // dims 4 d4 .. of rows y0, y0 + ys, ..
+    const int ys = 256 / dc < 16 ? 256 / dc : 16;
+    const int d4 = tid % dc, y0 = tid / dc;
+
+    long long pos = (long long)blockIdx.x * seg;
+    const long long end = min(pos + seg, total);
+    while (pos < end) {
+        const Piece pc = piece_at<false>(a, p, pos, end);
+        const int rows = min(16, pc.rows - pc.row0);
+        for (int i = tid; i < 16 * dim; i += 256) {
+            const int r = i / dim;
+            s_q[i] = r < rows ? St<T>::ld((const T*)a.q + q_row(a, pc, pc.row0 + r) * dim +
+                                          (i - r * dim)) : 0.f;
+        }
+        float4 acc[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) acc[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+        float m_run = -INFINITY, l_run = 0.f;
+        for (int st = 0; st < pc.n; st += 64) {
+            const int n = min(64, pc.n - st);
+            if (tid < 64) {
+                long long off = -1;
+                if (tid < n) {
+                    const int t = pc.t0 + st + tid, e = pc.table[a.page.div(t)];
+                    if ((unsigned)e < (unsigned)a.blocks)
+                        off = (((long long)e * a.hkv + pc.kv) * a.page.d + a.page.mod(t)) * dim;
+                }
+                s_off[tid] = off;
+            }
+            __syncthreads();
+            float s[4], top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const long long off = s_off[x16 + 16 * j];
+                s[j] = -INFINITY;
+                if (off < 0) continue;
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int c = 0; c < dc; ++c) {
+                    const float4 kv = St<T>::ld4(kp + off + 4 * c);
+                    const float4 qv = *reinterpret_cast<const float4*>(s_q + row * dim + 4 * c);
+                    part[0] = fmaf(kv.x, qv.x, part[0]);
+                    part[1] = fmaf(kv.y, qv.y, part[1]);
+                    part[2] = fmaf(kv.z, qv.z, part[2]);
+                    part[3] = fmaf(kv.w, qv.w, part[3]);
+                }
+                s[j] = ((part[0] + part[1]) + (part[2] + part[3])) * a.scale_log2;
+                top = fmaxf(top, s[j]);
+            }
+            for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            const float m_new = fmaxf(m_run, top);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = exp2f(m_run - m_use);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float w = exp2f(s[j] - m_use);
+                s_p[row][x16 + 16 * j] = w;
+                sum += w;
+            }
+            for (int o = 8; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            l_run = l_run * alpha + sum;
+            m_run = m_new;
+            if (x16 == 0) s_alpha[row] = alpha;
+            __syncthreads();
+            if (y0 < ys) {
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                    if (y0 + y * ys >= rows) break;
+                    const float al = s_alpha[y0 + y * ys];
+                    acc[y].x *= al; acc[y].y *= al; acc[y].z *= al; acc[y].w *= al;
+                }
+                for (int t = 0; t < n; ++t) {
+                    const long long off = s_off[t];
+                    if (off < 0) continue;
+                    const float4 vv = St<T>::ld4(vp + off + 4 * d4);
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        if (y0 + y * ys >= rows) break;
+                        const float w = s_p[y0 + y * ys][t];
+                        acc[y].x = fmaf(w, vv.x, acc[y].x);
+                        acc[y].y = fmaf(w, vv.y, acc[y].y);
+                        acc[y].z = fmaf(w, vv.z, acc[y].z);
+                        acc[y].w = fmaf(w, vv.w, acc[y].w);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (y0 < ys) {
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                if (y0 + y * ys >= rows) break;
+                *reinterpret_cast<float4*>(a.acc + (pc.slot + y0 + y * ys) * dim + 4 * d4) = acc[y];
+            }
+        }
+        if (row < rows && x16 == 0) {
+            a.ml[2 * (pc.slot + row)] = m_run;
+            a.ml[2 * (pc.slot + row) + 1] = l_run;
+        }
+        pos += pc.n;
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The fold: a workgroup a (b, h), its four waves taking the pieces in turn.
+// ---------------------------------------------------------------------------
+struct Pieces {
+    long long lo;  // first segment
+    int n;
+    size_t row;  // of the first piece's partial; the next is one segment's granules on
+};
+template <bool WIDE>
+__device__ __forceinline__ Pieces pieces_of(const PrefixArgs& a, int e, long long seg, int kv,
+                                            int b, int j) {
+    const Entry x = a.entries[e];
+    if (x.n == 0) return Pieces{0, 0, 0};
+    const int r = (b - x.first) * a.gq + j;
+    const int tr = tile_rows<WIDE>(x.rows), tiles = up(x.rows, tr), tile = r / tr;
+    const long long lo = x.start + ((long long)kv * tiles + tile) * x.n;
+    const long long s0 = lo / seg, s1 = (lo + x.n - 1) / seg;
+    const size_t gran = (size_t)kTileGranules * s0 + x.gran + (size_t)kv * up(x.rows, kGranule) +
+                        tile * (tr / kGranule);
+    return Pieces{s0, (int)(s1 - s0 + 1), gran * kGranule + (r - tile * tr)};
+}
+
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(256) void prefix_combine(const PrefixArgs a) {
+    __shared__ float s_m[4], s_l[4];
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float* const s_acc = reinterpret_cast<float*>(smem);  // [4][dim]
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int b = blockIdx.x / a.hq, h = blockIdx.x - b * a.hq;
+    const int kv = h / a.gq, j = h - kv * a.gq, dim = a.dim;
+    const long long seg = a.entries[a.groups + a.batch].start;
+    const int g = a.group_of[b];
+    Pieces p0{0, 0, 0};
+    if (g >= 0) p0 = pieces_of<WIDE>(a, g, seg, kv, b, j);
+    const Pieces p1 = pieces_of<WIDE>(a, a.groups + b, seg, kv, b, j);
+    const int n = p0.n + p1.n;
+    auto row = [&](int i) {
+        const bool own = i >= p0.n;
+        return (own ? p1.row : p0.row) +
+               (size_t)(kTileGranules * kGranule) * (own ? i - p0.n : i);
+    };
+    // the wave's pieces i = wave, wave + 4, ..: a lane each
+    float m = -INFINITY;
+    for (int i = wave + 4 * lane; i < n; i += 256) m = fmaxf(m, a.ml[2 * row(i)]);
+    m = wave_max(m);
+    const float m_use = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int i = wave + 4 * lane; i < n; i += 256) {
+        const size_t r = row(i);
+        l += exp2f(a.ml[2 * r] - m_use) * a.ml[2 * r + 1];
+    }
+    l = wave_sum(l);
+    // 4 dims a lane; dim > 256: again for the rest
+    for (int d0 = 0; d0 < dim; d0 += 256) {
+        const int d = d0 + 4 * lane;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (d < dim) {
+#pragma unroll 4
+            for (int i = wave; i < n; i += 4) {
+                const size_t r = row(i);
+                const float f = exp2f(a.ml[2 * r] - m_use);
+                const float4 x = *reinterpret_cast<const float4*>(a.acc + r * dim + d);
+                acc.x = fmaf(f, x.x, acc.x);
+                acc.y = fmaf(f, x.y, acc.y);
+                acc.z = fmaf(f, x.z, acc.z);
+                acc.w = fmaf(f, x.w, acc.w);
+            }
+            *reinterpret_cast<float4*>(s_acc + wave * dim + d) = acc;
+        }
+    }
+    if (lane == 0) s_m[wave] = m, s_l[wave] = l;
+    __syncthreads();
+    float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    top = top == -INFINITY ? 0.f : top;
+    float f[4], total = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = exp2f(s_m[w] - top);
+        total += f[w] * s_l[w];
+    }
+    const float inv = total > 0.f ? 1.0f / total : 0.f;
+    for (int d = tid; d < dim; d += 256) {
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) x = fmaf(f[w], s_acc[w * dim + d], x);
+        St<T>::st((T*)a.out + ((size_t)b * a.hq + h) * dim + d,
+                  total == 0.f ? 0.f : total > 0.f ? x * inv : total);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+struct PrefixShape {
+    int dtype, batch, hq, hkv, groups, page, pwidth, twidth, dim, segs;
+    bool wide;
+    size_t ml, acc, entries, group_of, bytes;  // offsets in the workspace
+};
+
+inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+PrefixShape prefix_shape(int dtype, int batch, int hq, int hkv, int groups, int page, int pwidth,
+                         int twidth, int dim) {
+    if (dtype != FT_DT_F32 && dtype != FT_DT_BF16 && dtype != FT_DT_F16)
+        inval("attention: unknown element type");
+    if (batch < 0 || groups < 0 || hq < 1 || hkv < 1 || pwidth < 0 || twidth < 0)
+        inval("attention shapes must satisfy batch, groups, widths >= 0, heads >= 1");
+    if (hq % hkv != 0) inval("q heads must be a multiple of kv heads (contiguous GQA groups)");
+    if (dim < 4 || dim % 4 != 0 || dim > kMaxDimP)
+        inval("dim must be a multiple of 4 and at most 512");
+    if (page < 1) inval("page must be >= 1");
+    if ((long long)page * pwidth > INT_MAX / 2 || (long long)page * twidth > INT_MAX / 2)
+        inval("attention: a table's capacity must be below 2^30 tokens");
+    if ((long long)batch + groups > kMaxEntries)
+        inval("attention: at most 4096 sequences and groups together");
+    if ((long long)batch * hq >= 1 << 24) inval("attention problem too large for one launch");
+    PrefixShape s{dtype, batch, hq, hkv, groups, page, pwidth, twidth, dim};
+    s.wide = dtype != FT_DT_F32 && dim % 8 == 0 && dim <= 128;
+    s.segs = 2 * dev_info().cu_count;
+    const size_t gq = hq / hkv;
+    // granules of every unit (a group's rows are rounded up once), and 8 a
+    // segment more
+    const size_t granules = (size_t)kTileGranules * s.segs +
+                            hkv * (batch * gq / kGranule + groups) +
+                            (size_t)batch * hkv * ((gq + kGranule - 1) / kGranule);
+    const size_t rows = granules * kGranule;
+    s.ml = 0;
+    s.acc = align256(rows * 8);
+    s.entries = s.acc + align256(rows * dim * 4);
+    s.group_of = s.entries + align256(sizeof(Entry) * (size_t)(batch + groups + 1));
+    s.bytes = s.group_of + align256(4 * (size_t)batch);
+    if (batch == 0) s.bytes = 0;
+    return s;
+}
+
+template <typename K>
+void allow_lds(K kernel, size_t bytes) {
+    if (bytes > 65536)
+        hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
+                  "hipFuncSetAttribute");
+}
+
+template <typename T, int D>
+void wide_run(const PrefixArgs& a, int segs, hipStream_t s) {
+    const size_t lds = 2 * PCfg<D>::kStage + Plan::bytes(a.groups + a.batch, a.groups);
+    if (a.dim == D) {
+        allow_lds(prefix_attn<T, D, true>, lds);
+        prefix_attn<T, D, true><<<segs, 256, lds, s>>>(a);
+    } else {
+        allow_lds(prefix_attn<T, D, false>, lds);
+        prefix_attn<T, D, false><<<segs, 256, lds, s>>>(a);
+    }
+}
+
+template <typename T>
+void prefix_run(const PrefixShape& sh, PrefixArgs a, hipStream_t s) {
+    const size_t lds = 16 * (size_t)sh.dim;
+    bool wide = false;
+    if constexpr (!std::is_same<T, float>::value) {
+        if (sh.wide) {
+            wide = true;
+            if (sh.dim <= 64) wide_run<T, 64>(a, sh.segs, s);
+            else wide_run<T, 128>(a, sh.segs, s);
+        }
+    }
+    if (!wide)  {
+        const size_t plan = 64 * (size_t)sh.dim + Plan::bytes(sh.groups + sh.batch, sh.groups);
+        allow_lds(prefix_general<T>, plan);
+        prefix_general<T><<<sh.segs, 256, plan, s>>>(a);
+    }
+    launch_check("shared-prefix attention kernel launch");
+    if (wide) prefix_combine<T, true><<<sh.batch * sh.hq, 256, lds, s>>>(a);
+    else prefix_combine<T, false><<<sh.batch * sh.hq, 256, lds, s>>>(a);
+    launch_check("shared-prefix combine kernel launch");
+}
+
+}  // namespace
+}  // namespace ft
+
+using namespace ft;
+
+extern "C" {
+
+int ft_attention_decode_paged_prefix_workspace(int dtype, int batch, int q_heads, int kv_heads,
+                                               int groups, int page, int prefix_width,
+                                               int tbl_width, int dim, long long* bytes) {
+    return guarded([&] {
+        if (!bytes) inval("attention: null operand");
+        *bytes = (long long)prefix_shape(dtype, batch, q_heads, kv_heads, groups, page,
+                                         prefix_width, tbl_width, dim).bytes;
+    });
+}
+
+int ft_attention_decode_paged_prefix_launch(
+    const void* q, int dtype, const void* k_pool, const void* v_pool, const int* prefix_table,
+    const int* prefix_lens, const int* group_offsets, const int* table, const int* lens, void* out,
+    void* workspace, long long workspace_bytes, int batch, int q_heads, int kv_heads, int groups,
+    int blocks, int page, int prefix_width, int tbl_width, int dim, uintptr_t stream) {
+    return guarded([&] {
+        PrefixShape sh = prefix_shape(dtype, batch, q_heads, kv_heads, groups, page, prefix_width,
+                                      tbl_width, dim);
+        if (blocks < 0) inval("attention: blocks must be >= 0");
+        if (groups > 1 && !group_offsets) inval("attention: several groups need group_offsets");
+        if (batch == 0) return;
+        if (!q || !out || (groups > 0 && prefix_width > 0 && !prefix_table) ||
+            (tbl_width > 0 && !table) || (blocks > 0 && (!k_pool || !v_pool)))
+            inval("attention: null operand");
+        const size_t by = dtype == FT_DT_F32 ? 16 : 8;   // 4 elements
+        auto off = [&](const void* p, size_t n) { return ((uintptr_t)p % n) != 0; };
+        if (off(q, by) || off(k_pool, by) || off(v_pool, by) || off(out, by))
+            inval("attention: operands must be aligned to 4 elements");
+        if (off(workspace, 16)) inval("attention: the workspace must be aligned to 16 bytes");
+        if (!workspace || workspace_bytes < (long long)sh.bytes)
+            inval("attention: this call needs " + std::to_string(sh.bytes) +
+                  " bytes of workspace");
+        // whole 16-byte chunks on the matrix-core path
+        if (off(q, 16) || off(k_pool, 16) || off(v_pool, 16)) sh.wide = false;
+        char* const ws = (char*)workspace;
+        PrefixArgs a{};
+        a.q = q;
+        a.k = k_pool;
+        a.v = v_pool;
+        a.ptable = prefix_table;
+        a.plens = prefix_lens;
+        a.offsets = group_offsets;
+        a.table = table;
+        a.lens = lens;
+        a.out = out;
+        a.ml = (float*)(ws + sh.ml);
+        a.acc = (float*)(ws + sh.acc);
+        a.entries = (Entry*)(ws + sh.entries);
+        a.group_of = (int*)(ws + sh.group_of);
+        a.batch = batch;
+        a.hq = q_heads;
+        a.hkv = kv_heads;
+        a.gq = q_heads / kv_heads;
+        a.groups = groups;
+        a.blocks = blocks;
+        a.pwidth = prefix_width;
+        a.twidth = tbl_width;
+        a.dim = dim;
+        a.page = FastDiv(page);
+        a.gdiv = FastDiv(a.gq);
+        a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)dim));
+        a.segs = sh.segs;
+        a.min_seg = 64;
+        const hipStream_t s = as_stream(stream);
+        if (dtype == FT_DT_F32) prefix_run<float>(sh, a, s);
+        else if (dtype == FT_DT_BF16) prefix_run<bf16>(sh, a, s);
+        else prefix_run<f16>(sh, a, s);
+    });
+}
+
+}  // extern "C"

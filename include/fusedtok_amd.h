@@ -293,6 +293,30 @@ int ft_attention_decode_paged_int8_launch(const void* q, int dtype, const signed
                                           int dim, uintptr_t stream);
 
 /* ------------------------------------------------------------------ */
+/* Decode attention of sequences that share prefixes (build addition).  */
+/* ------------------------------------------------------------------ */
+/* out [batch, q_heads, dim] (dtype FT_DT_*, q's and the pools') = softmax(q .
+ * k / sqrt(dim)) . v over the prefix of the sequence's group, then its own tokens.
+ * Group g: sequences [group_offsets[g], group_offsets[g + 1]) (NULL: one group
+ * of all), the first prefix_lens[g] tokens (NULL: prefix_width * page) of row g
+ * of prefix_table [groups, prefix_width]; own tokens: the first lens[b] (NULL:
+ * all) of row b of table [batch, tbl_width]; both in k_pool / v_pool [blocks,
+ * kv_heads, page, dim]. Any values in device memory are safe: lengths are
+ * clamped to the tables, offsets to [0, batch] and to those before them, tokens
+ * of an entry outside [0, blocks) weigh nothing. A row without a token gives
+ * zeros. batch + groups <= 4096, batch * q_heads < 2^24, a table's capacity
+ * below 2^30 tokens; dim a multiple of 4 up to 512; operands aligned to 4
+ * elements. The workspace (device memory, 16-byte aligned) is the caller's. */
+int ft_attention_decode_paged_prefix_workspace(int dtype, int batch, int q_heads, int kv_heads,
+                                               int groups, int page, int prefix_width,
+                                               int tbl_width, int dim, long long* bytes);
+int ft_attention_decode_paged_prefix_launch(
+    const void* q, int dtype, const void* k_pool, const void* v_pool, const int* prefix_table,
+    const int* prefix_lens, const int* group_offsets, const int* table, const int* lens, void* out,
+    void* workspace, long long workspace_bytes, int batch, int q_heads, int kv_heads, int groups,
+    int blocks, int page, int prefix_width, int tbl_width, int dim, uintptr_t stream);
+
+/* ------------------------------------------------------------------ */
 /* Norms of query and key heads with the rotation (build addition).     */
 /* ------------------------------------------------------------------ */
 /* qkv rows [tokens, (q_heads + 2 kv_heads) * dim] (dtype FT_DT_*, row stride

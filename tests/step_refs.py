@@ -31,3 +31,36 @@ def qk_norm_rope(qkv, hq, hkv, qw, kw, pos, rot, theta, eps, neox, sections=None
             part = part / np.sqrt((part ** 2).mean(-1, keepdims=True) + eps) * w
         parts.append(turn(part, pos, rot, theta, neox, sections))
     return parts[0], parts[1], x[:, hq + hkv:]
+
+
+def attend_prefix(q, k_pool, v_pool, ptable, plens, table, lens, offsets):
+    """The attention's rows, and for each row the sums that its bound needs:
+    the weighted magnitudes of V, and the largest magnitude of a score (in
+    nats, before the sum over dims cancels)."""
+    b, hq, d = q.shape
+    nb, hkv, page, _ = k_pool.shape
+    q, k_pool, v_pool = (x.astype(np.float64) for x in (q, k_pool, v_pool))
+    out, mass, size = np.zeros_like(q), np.zeros_like(q), np.zeros((b, hq, 1))
+
+    def rows(row, n):
+        t = np.arange(min(max(int(n), 0), len(row) * page))
+        e = np.asarray(row)[t // page]
+        ok = (e >= 0) & (e < nb)
+        return e[ok], t[ok] % page
+
+    for x in range(b):
+        e, o = rows(table[x], lens[x])
+        for g in range(len(plens)):
+            if offsets[g] <= x < offsets[g + 1]:
+                pe, po = rows(ptable[g], plens[g])
+                e, o = np.concatenate([pe, e]), np.concatenate([po, o])
+        if not len(e):
+            continue
+        for h in range(hq):
+            k, v = (p[e, h // (hq // hkv), o] for p in (k_pool, v_pool))
+            s = k @ q[x, h] / np.sqrt(d)
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            out[x, h], mass[x, h] = w @ v, w @ np.abs(v)
+            size[x, h] = (np.abs(k) @ np.abs(q[x, h])).max() / np.sqrt(d)
+    return out, mass, size

@@ -25,7 +25,9 @@ stubs __init__.pyi:99-107,208-236):
 - the post-logits step: ``argmax`` / ``argmax_batched`` (greedy),
   ``sample_topp`` / ``sample_topp_batched`` and ``decode_step`` /
   ``decode_step_batched`` (repetition penalty -> temperature -> nucleus
-  sampling, deterministic per seed).
+  sampling, deterministic per seed); ``sample_filtered_batched`` (build
+  addition: temperature, top-k, top-p and min-p of each row, given random
+  numbers).
 
 How a call runs: each op states its operands once, as a contract
 (``_contract.py``: symbolic shapes, element types, in-place operands, and
@@ -122,6 +124,7 @@ __all__ = [
     "sample_topp_batched",
     "decode_step",
     "decode_step_batched",
+    "sample_filtered_batched",
 ]
 
 # element-type codes of the C ABI (include/fusedtok_amd.h: FT_DT_*) and the
@@ -1671,6 +1674,88 @@ def decode_step_batched(logits, sampled_ids, penalty=1.0, *, p=0.9, temperature=
                 float(penalty), float(p), float(temperature), a[2], out.data_ptr(),
                 _stream()))
     return out if device_out else out.cpu()
+
+
+@functools.lru_cache(maxsize=1024)
+def _sample_workspace(rows, n):
+    """Workspace bytes of a sample_filtered_batched call of these sizes; the
+    checks of the sizes are made here."""
+    return _fusedtok.sample_filtered_batched_workspace(rows, n)
+
+
+def _row_values(v, name, dtype, rows, device):
+    """A parameter as (pointer or None, number): a GPU vector with an entry
+    for each row, or one number for all."""
+    if not torch.is_tensor(v):
+        if dtype is _TI and v != int(v):
+            raise TypeError(f"{name} must be an integer")
+        return None, int(v) if dtype is _TI else float(v)
+    if not v.is_cuda:
+        raise TypeError(f"{name} must be a number or a GPU tensor")
+    if v.dtype is not dtype:
+        raise TypeError(f"{name} must be {str(dtype)[6:]}")
+    if v.shape != (rows,) or not v.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector with an entry for each row")
+    if v.get_device() != device:
+        raise ValueError(f"operands are on different devices: logits on {device}, {name} on "
+                         f"{v.get_device()}")
+    return v.data_ptr(), 0
+
+
+def sample_filtered_batched(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """A token of every row of ``[rows, n]`` logits, from given random numbers.
+
+    logits: f32 / bf16 / fp16 (rows may be strided, as in a padded vocabulary);
+    uniforms: float32 [rows] in [0, 1). temperature (>= 0), top_k (0: none),
+    top_p in (0, 1] and min_p in [0, 1] are numbers for all rows or GPU vectors
+    with one for each (float32; top_k int32), so that a captured step takes a
+    batch of any requests. Returns int64 tokens [rows] on the GPU, without a
+    synchronisation.
+
+    A token weighs ``w = rint(2**40 * exp((x - max) / temperature))``, a whole
+    number. In the order of falling x, equals by index, the first top_k are
+    kept; of those the fewest whose weights come to top_p of their sum; of those
+    the ones with ``w >= min_p * 2**40``. The token is the first, in the order
+    of the indices, at which the sum of the kept weights passes ``floor(u *
+    their whole sum)``. Sums are exact, so a row's token depends on that row
+    alone. temperature 0 takes the largest logit, the first of equals. NaN
+    counts as -inf; a row with nothing else gives -1. Of vectors on the GPU any
+    values are safe: a temperature that is not > 0 counts as 0, a top_k below 1
+    as none, a top_p of 1 or more (or NaN) as none and one of 0 or less keeps
+    the first token, min_p counts as at most 1, a u below 0 (or NaN) as 0 and
+    one of 1 or more as the last kept token. n is at most 2**22. GPU tensors
+    only; each call has a workspace of its own from torch's allocator, so calls
+    on several streams are independent. Build addition: :func:`sample_topp_batched`
+    has one p and temperature for all rows, and draws from seeds."""
+    if not (torch.is_tensor(logits) and logits.is_cuda):
+        raise TypeError("logits must be a GPU tensor (this op has no host path)")
+    if logits.dtype not in _CODE:
+        raise TypeError("logits must be float32, bfloat16 or float16")
+    if logits.ndim != 2:
+        raise ValueError("logits must be 2-D [rows, vocab]")
+    rows, n = logits.shape
+    if n > 1 and logits.stride(1) != 1 and rows:
+        raise ValueError("logits rows must be contiguous")
+    if not torch.is_tensor(uniforms):
+        raise TypeError("uniforms must be a GPU tensor")
+    dev = logits.get_device()
+    u, _ = _row_values(uniforms, "uniforms", _TF, rows, dev)
+    t_ptr, t = _row_values(temperature, "temperature", _TF, rows, dev)
+    k_ptr, k = _row_values(top_k, "top_k", _TI, rows, dev)
+    p_ptr, p = _row_values(top_p, "top_p", _TF, rows, dev)
+    m_ptr, m = _row_values(min_p, "min_p", _TF, rows, dev)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return sample_filtered_batched(logits, uniforms, temperature=temperature,
+                                           top_k=top_k, top_p=top_p, min_p=min_p)
+    nbytes = _sample_workspace(rows, n)
+    out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+    _fusedtok.sample_filtered_batched_launch(
+        logits.data_ptr(), _CODE[logits.dtype], logits.stride(0) if rows > 1 else n, rows, n, u,
+        t_ptr, t, k_ptr, min(k, 2 ** 31 - 1), p_ptr, p, m_ptr, m, out.data_ptr(),
+        None if ws is None else ws.data_ptr(), nbytes, _stream())
+    return out
 
 
 from .layer import DecodeLayer, DecodeStack  # noqa: E402  (uses the loaded extension)

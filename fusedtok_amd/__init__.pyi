@@ -54,6 +54,7 @@ __all__ = [
     "sample_topp_batched",
     "decode_step",
     "decode_step_batched",
+    "sample_filtered_batched",
 ]
 
 def cuda_available() -> bool: ...
@@ -187,6 +188,11 @@ def decode_step_batched(logits: Array, sampled_ids: Histories, penalty: float = 
                         seeds: Optional[IntArray] = ...,
                         ids_offsets: Optional[IntArray] = ..., cuda: bool = ...,
                         device_out: bool = ...) -> Array: ...
+def sample_filtered_batched(logits: torch.Tensor, uniforms: torch.Tensor, *,
+                            temperature: Union[float, torch.Tensor] = ...,
+                            top_k: Union[int, torch.Tensor] = ...,
+                            top_p: Union[float, torch.Tensor] = ...,
+                            min_p: Union[float, torch.Tensor] = ...) -> torch.Tensor: ...
 
 class DecodeLayer:
     hidden: int

@@ -44,6 +44,7 @@ HIP_SOURCES = [
     "cache8.hip",
     "qknorm.hip",
     "prefix.hip",
+    "sample_filtered.hip",
 ]
 
 HIP_FLAGS = [

@@ -722,4 +722,28 @@ PYBIND11_MODULE(_fusedtok, m) {
           py::arg("batch"), py::arg("q_heads"), py::arg("kv_heads"), py::arg("dim"),
           py::arg("page"), py::arg("tbl_width"), py::arg("theta"),
           py::arg("pos_offset"), py::arg("neox"), py::arg("stream") = 0);
+
+    // ---- filtered sampling --------------------------------------------------
+    m.def("sample_filtered_batched_workspace",
+          [](int rows, int n) {
+              long long bytes = 0;
+              check(ft_sample_filtered_batched_workspace(rows, n, &bytes));
+              return bytes;
+          },
+          py::arg("rows"), py::arg("n"));
+    m.def("sample_filtered_batched_launch",
+          [](uintptr_t x, int dtype, long long ld, int rows, int n, uintptr_t u, py::object ts,
+             float t, py::object ks, int k, py::object ps, float p, py::object ms, float mp,
+             uintptr_t out, py::object ws, long long ws_bytes, uintptr_t stream) {
+              check(ft_sample_filtered_batched_launch(
+                  P<const void>(x), dtype, ld, rows, n, P<const float>(u),
+                  P<const float>(opt_ptr(ts)), t, P<const int>(opt_ptr(ks)), k,
+                  P<const float>(opt_ptr(ps)), p, P<const float>(opt_ptr(ms)), mp,
+                  P<long long>(out), P<void>(opt_ptr(ws)), ws_bytes, stream));
+          },
+          py::arg("logits"), py::arg("dtype"), py::arg("ld"), py::arg("rows"), py::arg("n"),
+          py::arg("uniforms"), py::arg("temperatures"), py::arg("temperature"),
+          py::arg("top_ks"), py::arg("top_k"), py::arg("top_ps"), py::arg("top_p"),
+          py::arg("min_ps"), py::arg("min_p"), py::arg("tokens"), py::arg("workspace"),
+          py::arg("workspace_bytes"), py::arg("stream") = 0);
 }

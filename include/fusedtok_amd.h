@@ -712,6 +712,27 @@ int ft_decode_step_batched_launch(const float* x, int rows, int n, const long lo
                                   const unsigned long long* seeds, long long* out,
                                   uintptr_t stream);
 
+/* ------------------------------------------------------------------ */
+/* Filtered sampling from given random numbers (build addition).        */
+/* ------------------------------------------------------------------ */
+/* A token of each row of logits [rows, n] (dtype FT_DT_*, row stride ld
+ * elements): w_i = rint(2^40 exp((x_i - max) / T)); in the order of falling x,
+ * equals by index, the first top_k are kept (< 1: all), of those the fewest
+ * whose weights come to top_p of their sum (>= 1: all), of those the ones
+ * with w >= min_p 2^40; the first token, by index, at which the sum of the
+ * kept weights passes floor(u * their sum). T <= 0: the largest logit, the
+ * first of equals. NaN counts as -inf, a row of nothing else gives -1.
+ * temperatures, top_ks, top_ps and min_ps [rows] in device memory, or NULL: the
+ * one number for all rows. n in [1, 2^22]. The workspace (device memory,
+ * 16-byte aligned; none for n <= 32768) is the caller's. */
+int ft_sample_filtered_batched_workspace(int rows, int n, long long* bytes);
+int ft_sample_filtered_batched_launch(const void* logits, int dtype, long long ld, int rows, int n,
+                                      const float* uniforms, const float* temperatures,
+                                      float temperature, const int* top_ks, int top_k,
+                                      const float* top_ps, float top_p, const float* min_ps,
+                                      float min_p, long long* tokens, void* workspace,
+                                      long long workspace_bytes, uintptr_t stream);
+
 #ifdef __cplusplus
 }
 #endif

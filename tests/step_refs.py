@@ -64,3 +64,32 @@ def attend_prefix(q, k_pool, v_pool, ptable, plens, table, lens, offsets):
             out[x, h], mass[x, h] = w @ v, w @ np.abs(v)
             size[x, h] = (np.abs(k) @ np.abs(q[x, h])).max() / np.sqrt(d)
     return out, mass, size
+
+
+def sample(x, u, temp, k, p, minp):
+    """One row's token (a Python int), from the definition: float64 weights as
+    whole numbers, a full sort, exact sums."""
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    top = x.max()
+    if top == -np.inf:
+        return -1
+    if not temp > 0:
+        return int(np.argmax(x))
+    with np.errstate(invalid="ignore"):
+        far = np.where(x == top, 0.0, (x - top) / np.float64(temp))
+    w = np.rint(np.exp(far) * 2.0 ** 40)
+    w = np.where(np.isnan(w), 0, w).astype(np.int64)
+    order = np.lexsort((np.arange(len(x)), -x))
+    if k > 0:
+        order = order[:k]
+    if p < 1:
+        sums = np.cumsum(w[order])
+        before = (sums - w[order]).astype(np.float64)
+        keep = before < np.float64(p) * np.float64(sums[-1])
+        keep[0] = True
+        order = order[keep]
+    kept = np.sort(order[w[order] >= min(float(minp), 1.0) * 2.0 ** 40])
+    sums = np.cumsum(w[kept])
+    aim = int(np.float64(u) * np.float64(sums[-1])) if u > 0 else 0
+    aim = min(aim, int(sums[-1]) - 1)
+    return int(kept[np.searchsorted(sums, aim, side="right")])

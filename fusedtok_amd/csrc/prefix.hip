@@ -66,7 +66,7 @@ struct PrefixArgs {
     int batch, hq, hkv, gq, groups, blocks, pwidth, twidth, dim;
     FastDiv page, gdiv;
     float scale_log2;
-    int segs, min_seg;
+    int segs, min_seg, start_cost, cost[3];
 };
 
 // Rows of a tile. On the matrix cores (WIDE): up to 16 rows leave the keys of a
@@ -77,6 +77,17 @@ __device__ __forceinline__ int tile_rows(int rows) {
     return rows <= 64 ? 64 : 128;
 }
 __device__ __forceinline__ int up(int a, int b) { return (a + b - 1) / b; }
+
+// The cost of a unit of n tokens: its start and its tokens, in the order of
+// the range that is cut into segments.
+template <bool WIDE>
+__device__ __forceinline__ int token_cost(const PrefixArgs& a, int rows) {
+    return a.cost[!WIDE || rows <= 16 ? 0 : rows <= 64 ? 1 : 2];
+}
+template <bool WIDE>
+__device__ __forceinline__ long long unit_cost(const PrefixArgs& a, int rows, int n) {
+    return n ? a.start_cost + (long long)n * token_cost<WIDE>(a, rows) : 0;
+}
 
 // The plan, in LDS: sum of the tokens of all units before an entry, granules
 // before it, and the groups' first sequences.
@@ -135,7 +146,8 @@ __device__ void make_plan(const PrefixArgs& a, const Plan& p, long long* s_sum, 
         const int rows = entry_rows(a, p, e);
         p.start[e] = sum;
         p.gran[e] = gran;
-        sum += (long long)entry_tokens(a, e) * a.hkv * up(rows, tile_rows<WIDE>(rows));
+        sum += unit_cost<WIDE>(a, rows, entry_tokens(a, e)) * a.hkv *
+               up(rows, tile_rows<WIDE>(rows));
         gran += a.hkv * up(rows, kGranule);
     }
     long long s = sum;
@@ -154,10 +166,10 @@ __device__ void make_plan(const PrefixArgs& a, const Plan& p, long long* s_sum, 
     __syncthreads();
 }
 
-// Tokens a segment: an equal share, in whole steps.
+// The cost of a segment: an equal share.
 __device__ __forceinline__ long long segment(const PrefixArgs& a, long long total) {
     const long long s = (total + a.segs - 1) / a.segs;
-    return ((s < a.min_seg ? a.min_seg : s) + 63) & ~63LL;
+    return s < a.min_seg ? a.min_seg : s;
 }
 
 // The combine's copy of the plan.
@@ -180,12 +192,14 @@ __device__ void leave_plan(const PrefixArgs& a, const Plan& p, long long seg) {
     }
 }
 
-// A segment's piece that starts at pos.
+// A segment's piece that starts at pos: the unit's tokens whose costs begin in
+// the segment; none where that is the unit's start alone.
 struct Piece {
     int entry, first, rows, kv, row0;  // row0: the tile's first row
     int t0, n;
     const int* table;
-    size_t slot;  // its partials' first row
+    size_t slot;     // its partials' first row
+    long long next;  // the position behind it
 };
 template <bool WIDE>
 __device__ __forceinline__ Piece piece_at(const PrefixArgs& a, const Plan& p, long long pos,
@@ -202,10 +216,17 @@ __device__ __forceinline__ Piece piece_at(const PrefixArgs& a, const Plan& p, lo
     const bool own = x.entry >= a.groups;
     x.first = own ? x.entry - a.groups : p.first[x.entry];
     const int tr = tile_rows<WIDE>(x.rows), tiles = up(x.rows, tr);
-    const long long off = pos - p.start[x.entry];
-    const int unit = (int)(off / n);
-    x.t0 = (int)(off - (long long)unit * n);
-    x.n = (int)min((long long)(n - x.t0), end - pos);
+    const int w = token_cost<WIDE>(a, x.rows);
+    const long long whole = unit_cost<WIDE>(a, x.rows, n), off = pos - p.start[x.entry];
+    const int unit = (int)(off / whole);
+    const long long in = off - unit * whole, base = pos - in;
+    const long long stop = min(whole, end - base);
+    auto token = [&](long long c) {
+        return c <= a.start_cost ? 0 : (int)((unsigned)(c - a.start_cost + w - 1) / (unsigned)w);
+    };
+    x.t0 = token(in);
+    x.n = token(stop) - x.t0;
+    x.next = base + stop;
     x.kv = unit / tiles;
     const int tile = unit - x.kv * tiles;
     x.row0 = tile * tr;
@@ -221,6 +242,7 @@ __device__ __forceinline__ Piece piece_at(const PrefixArgs& a, const Plan& p, lo
     x.t0 = __builtin_amdgcn_readfirstlane(x.t0);
     x.n = __builtin_amdgcn_readfirstlane(x.n);
     x.slot = (size_t)uniform64((long long)x.slot);
+    x.next = uniform64(x.next);
     return x;
 }
 
@@ -331,42 +353,52 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
     }
 
     const int steps = (pc.n + 63) >> 6;
-    // lane l's key of step st: its table entry, -1 past the piece (and where
-    // the table has no block)
+    // Nothing of a step's loads is waited for or branched on before its turn:
+    // lane l's table entry of step st (past the piece: its last token's) ..
     auto entry_of = [&](int st) {
-        const int t = 64 * st + lane;
-        if (t >= pc.n) return -1;
-        const int e = pc.table[a.page.div(pc.t0 + t)];
-        return (unsigned)e < (unsigned)a.blocks ? e : -1;
+        return pc.table[a.page.div(pc.t0 + min(64 * st + lane, pc.n - 1))];
     };
+    // .. which of them count: in the piece, and a block of the pools
+    auto held_of = [&](int st, int ent) {
+        return __builtin_amdgcn_ballot_w64(64 * st + lane < pc.n &&
+                                           (unsigned)ent < (unsigned)a.blocks);
+    };
+    // .. and the rows, 16 bytes a thread; block 0's where there is none
+    const int ch = tid % (D / 8);
+    const bool ch_on = FULL || 8 * ch < dim;
+    const size_t col = ch_on ? 8 * ch : 0;
     i32x4 kreg[C::kChunks], vreg[C::kChunks];
     auto load = [&](int st, int ent) {
+        ent = (unsigned)ent < (unsigned)a.blocks ? ent : 0;
 #pragma unroll
         for (int j = 0; j < C::kChunks; ++j) {
-            const int c = tid + 256 * j, row = c / (D / 8), ch = c % (D / 8);
+            const int row = (tid + 256 * j) / (D / 8);
             const int e = __shfl(ent, row, 64);
-            const i32x4 z = {0, 0, 0, 0};
-            kreg[j] = vreg[j] = z;
-            if (e >= 0 && (FULL || 8 * ch < dim)) {
-                const size_t off =
-                    (((size_t)e * a.hkv + pc.kv) * a.page.d + a.page.mod(pc.t0 + 64 * st + row)) *
-                        dim + 8 * ch;
-                if constexpr (KEYS) {  // read once
-                    kreg[j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(kp + off));
-                    vreg[j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(vp + off));
-                } else {
-                    kreg[j] = *reinterpret_cast<const i32x4*>(kp + off);
-                    vreg[j] = *reinterpret_cast<const i32x4*>(vp + off);
-                }
+            const int t = pc.t0 + min(64 * st + row, pc.n - 1);
+            const size_t off =
+                (((size_t)e * a.hkv + pc.kv) * a.page.d + a.page.mod(t)) * dim + col;
+            if constexpr (KEYS) {  // read once
+                kreg[j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(kp + off));
+                vreg[j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(vp + off));
+            } else {
+                kreg[j] = *reinterpret_cast<const i32x4*>(kp + off);
+                vreg[j] = *reinterpret_cast<const i32x4*>(vp + off);
             }
         }
     };
-    auto stage = [&](int st) {
+    // rows that do not count are zero, so that nothing in them is infinite
+    auto stage = [&](int st, unsigned long long held) {
         char* const ks = smem + (st & 1) * C::kStage;
         char* const vs = ks + 64 * C::kPitch;
+        if (held != ~0ull || !FULL) {
+#pragma unroll
+            for (int j = 0; j < C::kChunks; ++j)
+                if (!ch_on || !(held >> ((tid + 256 * j) / (D / 8)) & 1))
+                    kreg[j] = vreg[j] = i32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int j = 0; j < C::kChunks; ++j) {
-            const int c = tid + 256 * j, at = (c / (D / 8)) * C::kPitch + 16 * (c % (D / 8));
+            const int at = (tid + 256 * j) / (D / 8) * C::kPitch + 16 * ch;
             *reinterpret_cast<i32x4*>(ks + at) = kreg[j];
             *reinterpret_cast<i32x4*>(vs + at) = vreg[j];
         }
@@ -382,19 +414,20 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
     for (int qb = 0; qb < QB; ++qb) m_run[qb] = -INFINITY, l_run[qb] = 0.f;
     const float c2 = a.scale_log2;
 
-    int ent = entry_of(0);
-    int next = steps > 1 ? entry_of(1) : -1;
+    int ent = entry_of(0), next = entry_of(1);
     load(0, ent);
-    unsigned long long held = __builtin_amdgcn_ballot_w64(ent >= 0);
-    stage(0);
+    unsigned long long held = held_of(0, ent);
+    stage(0, held);
     __syncthreads();
     for (int st = 0; st < steps; ++st) {
         unsigned long long held_next = 0;
         if (st + 1 < steps) {
-            load(st + 1, next);
-            held_next = __builtin_amdgcn_ballot_w64(next >= 0);
-            next = st + 2 < steps ? entry_of(st + 2) : -1;
+            ent = next;
+            next = entry_of(st + 2);
+            load(st + 1, ent);
+            held_next = held_of(st + 1, ent);
         }
+        __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead
         if (active) {
             const char* const ks = smem + (st & 1) * C::kStage;
             const char* const vs = ks + 64 * C::kPitch;
@@ -492,7 +525,7 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
                     }
                 }
         }
-        if (st + 1 < steps) stage(st + 1);
+        if (st + 1 < steps) stage(st + 1, held_next);
         held = held_next;
         __syncthreads();
     }
@@ -582,10 +615,11 @@ void prefix_attn(const PrefixArgs a) {
     const long long end = min(pos + seg, total);
     while (pos < end) {
         const Piece pc = piece_at<true>(a, p, pos, end);
+        pos = pc.next;
+        if (pc.n == 0) continue;
         if (pc.rows <= 16) prefix_piece<T, D, FULL, 1, true>(a, pc, smem, s_ml);
         else if (pc.rows <= 64) prefix_piece<T, D, FULL, 1, false>(a, pc, smem, s_ml);
         else prefix_piece<T, D, FULL, 2, false>(a, pc, smem, s_ml);
-        pos += pc.n;
     }
 }
 
@@ -624,6 +658,8 @@ __global__ __launch_bounds__(256) void prefix_general(const PrefixArgs a) {
     const long long end = min(pos + seg, total);
     while (pos < end) {
         const Piece pc = piece_at<false>(a, p, pos, end);
+        pos = pc.next;
+        if (pc.n == 0) continue;
         const int rows = min(16, pc.rows - pc.row0);
         for (int i = tid; i < 16 * dim; i += 256) {
             const int r = i / dim;
@@ -715,7 +751,6 @@ __global__ __launch_bounds__(256) void prefix_general(const PrefixArgs a) {
             a.ml[2 * (pc.slot + row)] = m_run;
             a.ml[2 * (pc.slot + row) + 1] = l_run;
         }
-        pos += pc.n;
         __syncthreads();
     }
 }
@@ -735,8 +770,10 @@ __device__ __forceinline__ Pieces pieces_of(const PrefixArgs& a, int e, long lon
     if (x.n == 0) return Pieces{0, 0, 0};
     const int r = (b - x.first) * a.gq + j;
     const int tr = tile_rows<WIDE>(x.rows), tiles = up(x.rows, tr), tile = r / tr;
-    const long long lo = x.start + ((long long)kv * tiles + tile) * x.n;
-    const long long s0 = lo / seg, s1 = (lo + x.n - 1) / seg;
+    const int w = token_cost<WIDE>(a, x.rows);
+    const long long lo = x.start + a.start_cost +
+                         ((long long)kv * tiles + tile) * unit_cost<WIDE>(a, x.rows, x.n);
+    const long long s0 = lo / seg, s1 = (lo + (long long)w * (x.n - 1)) / seg;
     const size_t gran = (size_t)kTileGranules * s0 + x.gran + (size_t)kv * up(x.rows, kGranule) +
                         tile * (tr / kGranule);
     return Pieces{s0, (int)(s1 - s0 + 1), gran * kGranule + (r - tile * tr)};
@@ -937,8 +974,8 @@ int ft_attention_decode_paged_prefix_launch(
         if (!workspace || workspace_bytes < (long long)sh.bytes)
             inval("attention: this call needs " + std::to_string(sh.bytes) +
                   " bytes of workspace");
-        // whole 16-byte chunks on the matrix-core path
-        if (off(q, 16) || off(k_pool, 16) || off(v_pool, 16)) sh.wide = false;
+        // whole 16-byte chunks, and a block to read, on the matrix-core path
+        if (blocks == 0 || off(q, 16) || off(k_pool, 16) || off(v_pool, 16)) sh.wide = false;
         char* const ws = (char*)workspace;
         PrefixArgs a{};
         a.q = q;
@@ -967,7 +1004,10 @@ int ft_attention_decode_paged_prefix_launch(
         a.gdiv = FastDiv(a.gq);
         a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)dim));
         a.segs = sh.segs;
-        a.min_seg = 64;
+        auto env = [](const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; };
+        a.min_seg = env("PX_MIN", 512);
+        a.start_cost = env("PX_START", 256);
+        a.cost[0] = env("PX_C0", 1), a.cost[1] = env("PX_C1", 1), a.cost[2] = env("PX_C2", 1);
         const hipStream_t s = as_stream(stream);
         if (dtype == FT_DT_F32) prefix_run<float>(sh, a, s);
         else if (dtype == FT_DT_BF16) prefix_run<bf16>(sh, a, s);

@@ -40,13 +40,17 @@ constexpr int kTileGranules = 8;   // of a tile, at most
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// What the combine needs of an entry.
-struct Entry {
-    long long start;  // of its units in the range of all
+// What the combine needs of one of a sequence's two entries.
+struct Part {
+    long long start;  // of the first unit's tokens in the range of all
+    long long whole;  // from unit to unit
     int gran;         // granules before it
-    int n;            // tokens
+    int n;            // tokens (0: none)
     int rows;         // rows a kv head
     int first;        // its first sequence
+};
+struct Parts {
+    Part prefix, own;
 };
 
 struct PrefixArgs {
@@ -61,8 +65,8 @@ struct PrefixArgs {
     void* out;
     float* ml;       // [rows][2]
     float* acc;      // [rows][dim]
-    Entry* entries;  // [groups + batch + 1]; the last: start = the segments' length
-    int* group_of;   // [batch], -1: none
+    Parts* parts;    // [batch]
+    long long* seg;  // the segments' length
     int batch, hq, hkv, gq, groups, blocks, pwidth, twidth, dim;
     FastDiv page, gdiv;
     float scale_log2;
@@ -172,23 +176,25 @@ __device__ __forceinline__ long long segment(const PrefixArgs& a, long long tota
     return s < a.min_seg ? a.min_seg : s;
 }
 
-// The combine's copy of the plan.
+// The combine's copy of the plan, sequence by sequence.
+template <bool WIDE>
 __device__ void leave_plan(const PrefixArgs& a, const Plan& p, long long seg) {
-    for (int e = threadIdx.x; e <= p.entries; e += 256) {
-        Entry x{seg, 0, 0, 0, 0};
-        if (e < p.entries)
-            x = Entry{p.start[e], p.gran[e], entry_tokens(a, e), entry_rows(a, p, e),
-                      e < a.groups ? p.first[e] : e - a.groups};
-        a.entries[e] = x;
-    }
+    if (threadIdx.x == 0) *a.seg = seg;
+    auto part = [&](int e, int first) {
+        const int n = entry_tokens(a, e), rows = entry_rows(a, p, e);
+        return Part{p.start[e] + a.start_cost, unit_cost<WIDE>(a, rows, n), p.gran[e], n, rows,
+                    first};
+    };
     for (int b = threadIdx.x; b < a.batch; b += 256) {
         int lo = 0, hi = a.groups;  // the last g with first[g] <= b
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             (p.first[mid] <= b ? lo : hi) = mid;
         }
-        const bool in = a.groups > 0 && p.first[lo] <= b && b < p.first[lo + 1];
-        a.group_of[b] = in ? lo : -1;
+        Parts x{};
+        if (a.groups > 0 && p.first[lo] <= b && b < p.first[lo + 1]) x.prefix = part(lo, p.first[lo]);
+        x.own = part(a.groups + b, b);
+        a.parts[b] = x;
     }
 }
 
@@ -367,8 +373,10 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
     const int ch = tid % (D / 8);
     const bool ch_on = FULL || 8 * ch < dim;
     const size_t col = ch_on ? 8 * ch : 0;
-    i32x4 kreg[C::kChunks], vreg[C::kChunks];
-    auto load = [&](int st, int ent) {
+    struct Rows {
+        i32x4 k[C::kChunks], v[C::kChunks];
+    };
+    auto load = [&](int st, int ent, Rows& x) {
         ent = (unsigned)ent < (unsigned)a.blocks ? ent : 0;
 #pragma unroll
         for (int j = 0; j < C::kChunks; ++j) {
@@ -378,29 +386,29 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
             const size_t off =
                 (((size_t)e * a.hkv + pc.kv) * a.page.d + a.page.mod(t)) * dim + col;
             if constexpr (KEYS) {  // read once
-                kreg[j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(kp + off));
-                vreg[j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(vp + off));
+                x.k[j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(kp + off));
+                x.v[j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(vp + off));
             } else {
-                kreg[j] = *reinterpret_cast<const i32x4*>(kp + off);
-                vreg[j] = *reinterpret_cast<const i32x4*>(vp + off);
+                x.k[j] = *reinterpret_cast<const i32x4*>(kp + off);
+                x.v[j] = *reinterpret_cast<const i32x4*>(vp + off);
             }
         }
     };
     // rows that do not count are zero, so that nothing in them is infinite
-    auto stage = [&](int st, unsigned long long held) {
+    auto stage = [&](int st, unsigned long long held, Rows& x) {
         char* const ks = smem + (st & 1) * C::kStage;
         char* const vs = ks + 64 * C::kPitch;
         if (held != ~0ull || !FULL) {
 #pragma unroll
             for (int j = 0; j < C::kChunks; ++j)
                 if (!ch_on || !(held >> ((tid + 256 * j) / (D / 8)) & 1))
-                    kreg[j] = vreg[j] = i32x4{0, 0, 0, 0};
+                    x.k[j] = x.v[j] = i32x4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int j = 0; j < C::kChunks; ++j) {
             const int at = (tid + 256 * j) / (D / 8) * C::kPitch + 16 * ch;
-            *reinterpret_cast<i32x4*>(ks + at) = kreg[j];
-            *reinterpret_cast<i32x4*>(vs + at) = vreg[j];
+            *reinterpret_cast<i32x4*>(ks + at) = x.k[j];
+            *reinterpret_cast<i32x4*>(vs + at) = x.v[j];
         }
     };
 
@@ -414,29 +422,15 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
     for (int qb = 0; qb < QB; ++qb) m_run[qb] = -INFINITY, l_run[qb] = 0.f;
     const float c2 = a.scale_log2;
 
-    int ent = entry_of(0), next = entry_of(1);
-    load(0, ent);
-    unsigned long long held = held_of(0, ent);
-    stage(0, held);
-    __syncthreads();
-    for (int st = 0; st < steps; ++st) {
-        unsigned long long held_next = 0;
-        if (st + 1 < steps) {
-            ent = next;
-            next = entry_of(st + 2);
-            load(st + 1, ent);
-            held_next = held_of(st + 1, ent);
-        }
-        __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead
+    auto compute = [&](int st, unsigned long long held) {
         if (active) {
             const char* const ks = smem + (st & 1) * C::kStage;
             const char* const vs = ks + 64 * C::kPitch;
             const int k0 = KEYS ? 16 * wave : 0;  // the wave's first key
+            // the softmax and the staging go ahead of the SIMD's other wave's
+            // matrix instructions, which fill the gaps
+            __builtin_amdgcn_s_setprio(0);
             f32x4 sc[KB][QB];
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int qb = 0; qb < QB; ++qb) sc[kb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < C::kS; ++s)
 #pragma unroll
@@ -445,8 +439,10 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
                         ks + (k0 + 16 * kb + r16) * C::kPitch + (32 * s + 8 * g) * 2);
 #pragma unroll
                     for (int qb = 0; qb < QB; ++qb)
-                        sc[kb][qb] = M::mma(kf, qf[qb][s], sc[kb][qb]);
+                        sc[kb][qb] = M::mma(kf, qf[qb][s],
+                                            s ? sc[kb][qb] : f32x4{0.f, 0.f, 0.f, 0.f});
                 }
+            __builtin_amdgcn_s_setprio(1);
             if (held != ~0ull) {  // past the piece, or no block
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
@@ -501,6 +497,7 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
                         pl[qb][x][w] = both.y;
                     }
             }
+            __builtin_amdgcn_s_setprio(0);
             // V^T: dims 16 db + r, keys k0 + 32 x + 4g + (0..3) and 16 more
 #pragma unroll
             for (int db = 0; db < C::kDB; ++db)
@@ -525,7 +522,26 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
                     }
                 }
         }
-        if (st + 1 < steps) stage(st + 1, held_next);
+        __builtin_amdgcn_s_setprio(1);
+    };
+    // (Loads of two steps ahead, where 16 rows a wave leave the registers, were
+    // no faster: 64 sequences of 4000 tokens 174 for 169 us.)
+    int ent = entry_of(0), next = entry_of(1);
+    unsigned long long held = held_of(0, ent), held_next = 0;
+    Rows x;
+    load(0, ent, x);
+    stage(0, held, x);
+    __syncthreads();
+    for (int st = 0; st < steps; ++st) {
+        if (st + 1 < steps) {
+            ent = next;
+            next = entry_of(st + 2);
+            load(st + 1, ent, x);
+            held_next = held_of(st + 1, ent);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead
+        compute(st, held);
+        if (st + 1 < steps) stage(st + 1, held_next, x);
         held = held_next;
         __syncthreads();
     }
@@ -610,7 +626,7 @@ void prefix_attn(const PrefixArgs a) {
     make_plan<true>(a, p, s_sum, s_cnt);
     const long long total = uniform64(p.start[p.entries]);
     const long long seg = segment(a, total);
-    if (blockIdx.x == 0) leave_plan(a, p, seg);
+    if (blockIdx.x == 0) leave_plan<true>(a, p, seg);
     long long pos = (long long)blockIdx.x * seg;
     const long long end = min(pos + seg, total);
     while (pos < end) {
@@ -645,7 +661,7 @@ __global__ __launch_bounds__(256) void prefix_general(const PrefixArgs a) {
     make_plan<false>(a, p, s_sum, s_cnt);
     const long long total = uniform64(p.start[p.entries]);
     const long long seg = segment(a, total);
-    if (blockIdx.x == 0) leave_plan(a, p, seg);
+    if (blockIdx.x == 0) leave_plan<false>(a, p, seg);
     const T* const kp = (const T*)a.k;
     const T* const vp = (const T*)a.v;
 
@@ -756,105 +772,208 @@ __global__ __launch_bounds__(256) void prefix_general(const PrefixArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// The fold: a workgroup a (b, h), its four waves taking the pieces in turn.
+// The fold. A workgroup takes HEADS heads of a sequence: one, its pieces shared
+// out to the four waves; or, where there are heads enough for every CU, four:
+// a wave each, or all waves for one after another where one has many pieces.
+// A wave's lanes are
+// groups of dim / 4 that take pieces in turn; the first of them are on their
+// way before their maxima are known. What bounds it: the chain plan -> maxima
+// -> weights (4.5 us), the partials' bytes for long prefixes of many rows.
 // ---------------------------------------------------------------------------
+constexpr int kAlone = 32;  // pieces of a head that one wave folds
+constexpr int kAhead = 4;
+
+// A head's pieces: n0 of the prefix, then n1 of its own tokens.
 struct Pieces {
-    long long lo;  // first segment
-    int n;
-    size_t row;  // of the first piece's partial; the next is one segment's granules on
+    int n0, n1;
+    size_t row0, row1;  // first partials; the next is one segment's granules on
+    __device__ __forceinline__ size_t row(int i) const {
+        const bool own = i >= n0;
+        return (own ? row1 : row0) + (size_t)(kTileGranules * kGranule) * (own ? i - n0 : i);
+    }
 };
-template <bool WIDE>
-__device__ __forceinline__ Pieces pieces_of(const PrefixArgs& a, int e, long long seg, int kv,
-                                            int b, int j) {
-    const Entry x = a.entries[e];
-    if (x.n == 0) return Pieces{0, 0, 0};
-    const int r = (b - x.first) * a.gq + j;
-    const int tr = tile_rows<WIDE>(x.rows), tiles = up(x.rows, tr), tile = r / tr;
-    const int w = token_cost<WIDE>(a, x.rows);
-    const long long lo = x.start + a.start_cost +
-                         ((long long)kv * tiles + tile) * unit_cost<WIDE>(a, x.rows, x.n);
-    const long long s0 = lo / seg, s1 = (lo + (long long)w * (x.n - 1)) / seg;
-    const size_t gran = (size_t)kTileGranules * s0 + x.gran + (size_t)kv * up(x.rows, kGranule) +
-                        tile * (tr / kGranule);
-    return Pieces{s0, (int)(s1 - s0 + 1), gran * kGranule + (r - tile * tr)};
+
+// floor(x / d), below 2^20 (a segment's number): an estimate, one off at most
+__device__ __forceinline__ long long quotient(long long x, long long d, double inv) {
+    long long q = (long long)((double)x * inv);
+    if (q * d > x) --q;
+    return (q + 1) * d <= x ? q + 1 : q;
 }
 
-template <typename T, bool WIDE>
+template <bool WIDE>
+__device__ __forceinline__ void find_pieces(const PrefixArgs& a, const Part& x, long long seg,
+                                            double inv, int kv, int b, int j, int& n,
+                                            size_t& row) {
+    n = 0;
+    row = 0;
+    if (x.n == 0) return;
+    const int r = (b - x.first) * a.gq + j;
+    const int tr = tile_rows<WIDE>(x.rows);
+    const int log = tr == 16 ? 4 : tr == 64 ? 6 : 7, tile = r >> log;
+    const int tiles = (x.rows + tr - 1) >> log;
+    const long long lo = x.start + ((long long)kv * tiles + tile) * x.whole;
+    const long long s0 = quotient(lo, seg, inv);
+    const long long hi = lo + (long long)token_cost<WIDE>(a, x.rows) * (x.n - 1);
+    n = (int)(quotient(hi, seg, inv) - s0) + 1;
+    const size_t gran = (size_t)kTileGranules * s0 + x.gran +
+                        (size_t)kv * ((x.rows + kGranule - 1) / kGranule) +
+                        tile * (tr / kGranule);
+    row = gran * kGranule + (r - (tile << log));
+}
+
+template <typename T, bool WIDE, int HEADS>
 __global__ __launch_bounds__(256) void prefix_combine(const PrefixArgs a) {
+    __shared__ Pieces s_pieces[4];
     __shared__ float s_m[4], s_l[4];
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* const s_acc = reinterpret_cast<float*>(smem);  // [4][dim]
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int b = blockIdx.x / a.hq, h = blockIdx.x - b * a.hq;
-    const int kv = h / a.gq, j = h - kv * a.gq, dim = a.dim;
-    const long long seg = a.entries[a.groups + a.batch].start;
-    const int g = a.group_of[b];
-    Pieces p0{0, 0, 0};
-    if (g >= 0) p0 = pieces_of<WIDE>(a, g, seg, kv, b, j);
-    const Pieces p1 = pieces_of<WIDE>(a, a.groups + b, seg, kv, b, j);
-    const int n = p0.n + p1.n;
-    auto row = [&](int i) {
-        const bool own = i >= p0.n;
-        return (own ? p1.row : p0.row) +
-               (size_t)(kTileGranules * kGranule) * (own ? i - p0.n : i);
-    };
-    // the wave's pieces i = wave, wave + 4, ..: a lane each
-    float m = -INFINITY;
-    for (int i = wave + 4 * lane; i < n; i += 256) m = fmaxf(m, a.ml[2 * row(i)]);
-    m = wave_max(m);
-    const float m_use = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int i = wave + 4 * lane; i < n; i += 256) {
-        const size_t r = row(i);
-        l += exp2f(a.ml[2 * r] - m_use) * a.ml[2 * r + 1];
+    const int b = blockIdx.y, h = HEADS * blockIdx.x + wave % HEADS, dim = a.dim;
+    const long long seg = *a.seg;
+    const Parts parts = a.parts[b];
+    Pieces mine{0, 0, 0, 0};
+    if (h < a.hq) {
+        const int kv = a.gdiv.div(h), j = h - kv * a.gq;
+        const double inv = 1.0 / (double)seg;
+        find_pieces<WIDE>(a, parts.prefix, seg, inv, kv, b, j, mine.n0, mine.row0);
+        find_pieces<WIDE>(a, parts.own, seg, inv, kv, b, j, mine.n1, mine.row1);
     }
-    l = wave_sum(l);
-    // 4 dims a lane; dim > 256: again for the rest
-    for (int d0 = 0; d0 < dim; d0 += 256) {
-        const int d = d0 + 4 * lane;
+    if (lane == 0) s_pieces[wave] = mine;
+    __syncthreads();
+    int most = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) most = max(most, s_pieces[w].n0 + s_pieces[w].n1);
+
+    int size = 1;  // lanes a piece
+    while (size < 64 && 4 * size < dim) size *= 2;
+    const int groups = 64 / size, group = lane / size, d0 = 4 * (lane & (size - 1));
+    // pieces first, first + step, .. of `pc`: their maximum and sum, and 4 dims
+    // from d on in the lanes of group 0
+    auto fold = [&](const Pieces& pc, int first, int step, int d, float& m, float& l) {
+        const int n = pc.n0 + pc.n1;
+        float4 x[kAhead];
+        float xm[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = first + step * (group + groups * k);
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            xm[k] = -INFINITY;
+            if (i < n && d < dim) {
+                const size_t r = pc.row(i);
+                xm[k] = a.ml[2 * r];
+                x[k] = *reinterpret_cast<const float4*>(a.acc + r * dim + d);
+            }
+        }
+        m = -INFINITY;
+        l = 0.f;
+        float l_first = 0.f, m_first = -INFINITY;
+        {
+            const int i = first + step * lane;
+            if (i < n) {
+                const size_t r = pc.row(i);
+                m_first = a.ml[2 * r];
+                l_first = a.ml[2 * r + 1];
+            }
+            m = m_first;
+        }
+        for (int i = first + step * (lane + 64); i < n; i += 64 * step)
+            m = fmaxf(m, a.ml[2 * pc.row(i)]);
+        m = wave_max(m);
+        const float m_use = m == -INFINITY ? 0.f : m;
+        l = exp2f(m_first - m_use) * l_first;
+        for (int i = first + step * (lane + 64); i < n; i += 64 * step) {
+            const size_t r = pc.row(i);
+            l += exp2f(a.ml[2 * r] - m_use) * a.ml[2 * r + 1];
+        }
+        l = wave_sum(l);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float f, const float4& v) {
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
+        };
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) add(exp2f(xm[k] - m_use), x[k]);
         if (d < dim) {
 #pragma unroll 4
-            for (int i = wave; i < n; i += 4) {
-                const size_t r = row(i);
-                const float f = exp2f(a.ml[2 * r] - m_use);
-                const float4 x = *reinterpret_cast<const float4*>(a.acc + r * dim + d);
-                acc.x = fmaf(f, x.x, acc.x);
-                acc.y = fmaf(f, x.y, acc.y);
-                acc.z = fmaf(f, x.z, acc.z);
-                acc.w = fmaf(f, x.w, acc.w);
+            for (int i = first + step * (group + groups * kAhead); i < n; i += step * groups) {
+                const size_t r = pc.row(i);
+                add(exp2f(a.ml[2 * r] - m_use), *reinterpret_cast<const float4*>(a.acc + r * dim + d));
             }
-            *reinterpret_cast<float4*>(s_acc + wave * dim + d) = acc;
         }
+        for (int o = size; o < 64; o *= 2) {
+            acc.x += __shfl_xor(acc.x, o, 64);
+            acc.y += __shfl_xor(acc.y, o, 64);
+            acc.z += __shfl_xor(acc.z, o, 64);
+            acc.w += __shfl_xor(acc.w, o, 64);
+        }
+        return acc;
+    };
+    // a sum of 0 (no token) gives zeros, one that is not a number itself
+    auto scale = [](float l) { return l > 0.f ? 1.0f / l : l; };
+
+    if (HEADS > 1 && most <= kAlone) {
+        if (h >= a.hq) return;
+        for (int d = d0; d < ((dim + 255) & ~255); d += 256) {
+            float m, l;
+            const float4 x = fold(mine, 0, 1, d, m, l);
+            const float f = scale(l);
+            if (group == 0 && d < dim)
+                St<T>::st4((T*)a.out + ((size_t)b * a.hq + h) * dim + d,
+                           make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+            if (size < 64) break;
+        }
+        return;
     }
-    if (lane == 0) s_m[wave] = m, s_l[wave] = l;
-    __syncthreads();
-    float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    top = top == -INFINITY ? 0.f : top;
-    float f[4], total = 0.f;
+    for (int k = 0; k < HEADS && HEADS * (int)blockIdx.x + k < a.hq; ++k) {
+        const Pieces pc = s_pieces[k];
+        for (int d = d0; d < ((dim + 255) & ~255); d += 256) {
+            float m, l;
+            const float4 x = fold(pc, wave, 4, d, m, l);
+            if (group == 0 && d < dim) *reinterpret_cast<float4*>(s_acc + wave * dim + d) = x;
+            if (lane == 0) s_m[wave] = m, s_l[wave] = l;
+            if (size < 64) break;
+        }
+        __syncthreads();
+        float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+        top = top == -INFINITY ? 0.f : top;
+        float f[4], total = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        f[w] = exp2f(s_m[w] - top);
-        total += f[w] * s_l[w];
-    }
-    const float inv = total > 0.f ? 1.0f / total : 0.f;
-    for (int d = tid; d < dim; d += 256) {
-        float x = 0.f;
+        for (int w = 0; w < 4; ++w) {
+            f[w] = exp2f(s_m[w] - top);
+            total += f[w] * s_l[w];
+        }
+        const float inv = scale(total);
+        for (int d = tid; d < dim; d += 256) {
+            float x = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) x = fmaf(f[w], s_acc[w * dim + d], x);
-        St<T>::st((T*)a.out + ((size_t)b * a.hq + h) * dim + d,
-                  total == 0.f ? 0.f : total > 0.f ? x * inv : total);
+            for (int w = 0; w < 4; ++w) x = fmaf(f[w], s_acc[w * dim + d], x);
+            St<T>::st((T*)a.out + ((size_t)b * a.hq + HEADS * blockIdx.x + k) * dim + d, x * inv);
+        }
+        __syncthreads();
     }
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+// The cost of a unit's start (its table, Q and first rows arriving, its partials)
+// and of a token with up to 16, 64 and 128 rows. They balance the workgroups:
+// with starts free, 16 sequences of 1-500 tokens behind 131071 shared ones took
+// 215 us, a few workgroups being full of starts, for 120; 128 rows are bound by
+// the matrix cores (64 sequences behind 8192: 71 us at 6, 77 at 4 or 8).
+constexpr int kStartCost = 768;
+constexpr int kTokenCost[3] = {4, 4, 6};
+// The least cost of a segment (4 sequences behind 500 tokens, D = 64: 12.5 us, 14.3
+// at 1024, 17 at 2048).
+constexpr int kMinSegment = 256;
+
 struct PrefixShape {
     int dtype, batch, hq, hkv, groups, page, pwidth, twidth, dim, segs;
     bool wide;
-    size_t ml, acc, entries, group_of, bytes;  // offsets in the workspace
+    size_t ml, acc, parts, seg, bytes;  // offsets in the workspace
 };
 
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -878,17 +997,17 @@ PrefixShape prefix_shape(int dtype, int batch, int hq, int hkv, int groups, int 
     s.wide = dtype != FT_DT_F32 && dim % 8 == 0 && dim <= 128;
     s.segs = 2 * dev_info().cu_count;
     const size_t gq = hq / hkv;
-    // granules of every unit (a group's rows are rounded up once), and 8 a
-    // segment more
+    // granules of every unit (the rows of a group that is not empty are rounded
+    // up once), and 8 a segment more
     const size_t granules = (size_t)kTileGranules * s.segs +
-                            hkv * (batch * gq / kGranule + groups) +
+                            hkv * (batch * gq / kGranule + std::min(groups, batch)) +
                             (size_t)batch * hkv * ((gq + kGranule - 1) / kGranule);
     const size_t rows = granules * kGranule;
     s.ml = 0;
     s.acc = align256(rows * 8);
-    s.entries = s.acc + align256(rows * dim * 4);
-    s.group_of = s.entries + align256(sizeof(Entry) * (size_t)(batch + groups + 1));
-    s.bytes = s.group_of + align256(4 * (size_t)batch);
+    s.parts = s.acc + align256(rows * dim * 4);
+    s.seg = s.parts + align256(sizeof(Parts) * (size_t)batch);
+    s.bytes = s.seg + 256;
     if (batch == 0) s.bytes = 0;
     return s;
 }
@@ -920,18 +1039,22 @@ void prefix_run(const PrefixShape& sh, PrefixArgs a, hipStream_t s) {
     if constexpr (!std::is_same<T, float>::value) {
         if (sh.wide) {
             wide = true;
-            if (sh.dim <= 64) wide_run<T, 64>(a, sh.segs, s);
-            else wide_run<T, 128>(a, sh.segs, s);
+            if (sh.dim <= 64) wide_run<T, 64>(a, a.segs, s);
+            else wide_run<T, 128>(a, a.segs, s);
         }
     }
     if (!wide)  {
         const size_t plan = 64 * (size_t)sh.dim + Plan::bytes(sh.groups + sh.batch, sh.groups);
         allow_lds(prefix_general<T>, plan);
-        prefix_general<T><<<sh.segs, 256, plan, s>>>(a);
+        prefix_general<T><<<a.segs, 256, plan, s>>>(a);
     }
     launch_check("shared-prefix attention kernel launch");
-    if (wide) prefix_combine<T, true><<<sh.batch * sh.hq, 256, lds, s>>>(a);
-    else prefix_combine<T, false><<<sh.batch * sh.hq, 256, lds, s>>>(a);
+    const bool four = (long long)sh.batch * sh.hq > 4 * dev_info().cu_count;
+    const dim3 grid(four ? (sh.hq + 3) / 4 : sh.hq, sh.batch);
+    if (wide && four) prefix_combine<T, true, 4><<<grid, 256, lds, s>>>(a);
+    else if (wide) prefix_combine<T, true, 1><<<grid, 256, lds, s>>>(a);
+    else if (four) prefix_combine<T, false, 4><<<grid, 256, lds, s>>>(a);
+    else prefix_combine<T, false, 1><<<grid, 256, lds, s>>>(a);
     launch_check("shared-prefix combine kernel launch");
 }
 
@@ -989,8 +1112,8 @@ int ft_attention_decode_paged_prefix_launch(
         a.out = out;
         a.ml = (float*)(ws + sh.ml);
         a.acc = (float*)(ws + sh.acc);
-        a.entries = (Entry*)(ws + sh.entries);
-        a.group_of = (int*)(ws + sh.group_of);
+        a.parts = (Parts*)(ws + sh.parts);
+        a.seg = (long long*)(ws + sh.seg);
         a.batch = batch;
         a.hq = q_heads;
         a.hkv = kv_heads;
@@ -1004,10 +1127,17 @@ int ft_attention_decode_paged_prefix_launch(
         a.gdiv = FastDiv(a.gq);
         a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)dim));
         a.segs = sh.segs;
-        auto env = [](const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; };
-        a.min_seg = env("PX_MIN", 512);
-        a.start_cost = env("PX_START", 256);
-        a.cost[0] = env("PX_C0", 1), a.cost[1] = env("PX_C1", 1), a.cost[2] = env("PX_C2", 1);
+        a.min_seg = kMinSegment;
+        a.start_cost = kStartCost;
+        for (int i = 0; i < 3; ++i) a.cost[i] = kTokenCost[i];
+        // no more workgroups than the tables' capacity can fill
+        const long long gq = a.gq, c = kTokenCost[2];
+        const long long most =
+            kv_heads * ((batch * gq / kGranule + std::min(groups, batch)) *
+                            (kStartCost + c * page * prefix_width) +
+                        batch * ((gq + kGranule - 1) / kGranule) *
+                            (kStartCost + c * page * tbl_width));
+        a.segs = (int)std::min<long long>(sh.segs, most / a.min_seg + 1);
         const hipStream_t s = as_stream(stream);
         if (dtype == FT_DT_F32) prefix_run<float>(sh, a, s);
         else if (dtype == FT_DT_BF16) prefix_run<bf16>(sh, a, s);

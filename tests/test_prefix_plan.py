@@ -17,38 +17,52 @@ def tile_rows(rows, wide):
 
 
 class Plan:
-    def __init__(self, offsets, plens, lens, gq, hkv, segs, wide, min_seg=64):
-        b = len(lens)
+    START, MIN_SEGMENT = 768, 256
+
+    @staticmethod
+    def cost(rows, wide):
+        return 4 if not wide or rows <= 64 else 6
+
+    def unit(self, e):
+        return self.START + self.n[e] * self.cost(self.rows[e], self.wide) if self.n[e] else 0
+
+    def __init__(self, offsets, plens, lens, gq, hkv, segs, wide):
+        b, self.wide = len(lens), wide
         first = np.maximum.accumulate(np.clip(offsets, 0, b))
         self.first = [int(x) for x in first]
         self.groups = len(plens)
         self.rows = [(self.first[g + 1] - self.first[g]) * gq for g in range(self.groups)]
         self.rows += [gq] * b
         self.n = [int(x) for x in plens] + [int(x) for x in lens]
-        self.gq, self.hkv, self.wide = gq, hkv, wide
+        self.gq, self.hkv = gq, hkv
         self.start, self.gran = [0], [0]
-        for rows, n in zip(self.rows, self.n):
-            self.start.append(self.start[-1] + n * hkv * up(rows, tile_rows(rows, wide)))
+        for e, rows in enumerate(self.rows):
+            self.start.append(self.start[-1] +
+                              self.unit(e) * hkv * up(rows, tile_rows(rows, wide)))
             self.gran.append(self.gran[-1] + hkv * up(rows, 16))
         self.total = self.start[-1]
-        self.seg = (max(min_seg, up(self.total, segs)) + 63) // 64 * 64
+        self.seg = max(self.MIN_SEGMENT, up(self.total, segs))
         # as the host sizes the workspace
-        self.granules = 8 * segs + hkv * (b * gq // 16 + self.groups) + b * hkv * up(gq, 16)
+        self.granules = 8 * segs + hkv * (b * gq // 16 + min(self.groups, b)) + b * hkv * up(gq, 16)
 
     def pieces(self, s):
         """Segment s: (entry, kv, tile, t0, n, first partial row, rows)."""
         pos, end = s * self.seg, min((s + 1) * self.seg, self.total)
         while pos < end:
             e = int(np.searchsorted(self.start, pos, side="right")) - 1
-            off, n = pos - self.start[e], self.n[e]
-            tr = tile_rows(self.rows[e], self.wide)
+            off, whole = pos - self.start[e], self.unit(e)
+            tr, w = tile_rows(self.rows[e], self.wide), self.cost(self.rows[e], self.wide)
             tiles = up(self.rows[e], tr)
-            unit = off // n
-            kv, tile, t0 = unit // tiles, unit % tiles, off % n
-            m = min(n - t0, end - pos)
+            unit, inside = off // whole, off % whole
+            kv, tile = unit // tiles, unit % tiles
+            stop = min(whole, end - pos + inside)
+            t0, t1 = (up(max(c - self.START, 0), w) for c in (inside, stop))
+            m = t1 - t0
+            pos += stop - inside
+            if m == 0:
+                continue
             gran = 8 * s + self.gran[e] + kv * up(self.rows[e], 16) + tile * (tr // 16)
             yield e, kv, tile, t0, m, 16 * gran, min(tr, self.rows[e] - tile * tr)
-            pos += m
 
     def looked_for(self, e, b, kv, j):
         """The partial rows of (b, head kv * gq + j) in entry e."""
@@ -58,8 +72,9 @@ class Plan:
         r = (b - first) * self.gq + j
         tr = tile_rows(self.rows[e], self.wide)
         tiles, tile = up(self.rows[e], tr), r // tr
-        lo = self.start[e] + (kv * tiles + tile) * self.n[e]
-        s0, s1 = lo // self.seg, (lo + self.n[e] - 1) // self.seg
+        lo = self.start[e] + self.START + (kv * tiles + tile) * self.unit(e)
+        s0 = lo // self.seg
+        s1 = (lo + self.cost(self.rows[e], self.wide) * (self.n[e] - 1)) // self.seg
         gran = 8 * s0 + self.gran[e] + kv * up(self.rows[e], 16) + tile * (tr // 16)
         return [16 * gran + r - tile * tr + 128 * i for i in range(s1 - s0 + 1)]
 

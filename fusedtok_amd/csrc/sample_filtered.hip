@@ -19,7 +19,7 @@
 // and the first q in index order of those with x = xc (and w >= min_p 2^40). A
 // histogram of the weights over the distance log2(e) (max - x) / T, in bins of
 // 1/16, finds the bin in which a count (k) or a sum (p) is reached; inside it
-// histograms over the float's order bits, 1024 wide, narrow it down to the one
+// histograms over the float's order bits, 512 wide, narrow it down to the one
 // value. Nothing is sorted, and equal logits, thousands in 16 bits, cost
 // nothing extra.
 //
@@ -45,13 +45,14 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kBins = 656;           // bins of weights that are not 0: log2 distances below 41
+constexpr int kBins = 657;           // bins of weights that are not 0: log2 distances below 41
 constexpr int kSlice = 8192;         // tokens
 constexpr int kSliceNT = 256;
-constexpr int kRowNT = 1024;
+constexpr int kRowNT = 512;
 constexpr int kRowMost = 32768;      // tokens of a row that one workgroup holds
 constexpr int kMaxVocab = 1 << 22;   // 512 slices; sums of weights below 2^62
-constexpr int kLevel = 1024;         // bins of a histogram over order bits
+constexpr int kMinBins = 3;
+constexpr int kLevel = kRowNT;         // bins of a histogram over order bits
 
 struct SampleArgs {
     const void* x;
@@ -68,70 +69,119 @@ struct SampleArgs {
     // workspace of the sliced form
     float* top;        // [rows][slices]
     int* top_at;       // [rows][slices]
-    u64* sum;          // [rows][slices]: kept weights above the cut's bins
+    u64* sum;          // [rows][slices]: kept weights above the listed bins
+    u64* part;         // [rows][slices][kBins]: the slices' histograms
     unsigned* listed;  // [rows][slices]
     u64* mass;         // [rows][kBins]
     unsigned* count;   // [rows][kBins]
     unsigned* list;    // [rows][n]: order bits, slice s from kSlice s on
 };
 
-// 2^(j / 64), j < 64, in LDS. The caller synchronises.
+// 2^(j / 64), and a copy in LDS (the caller synchronises).
 constexpr int kPowers = 64;
+__device__ const double kPowerTable[kPowers] = {
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,
+};
 __device__ __forceinline__ void fill_powers(double* s) {
-    if (threadIdx.x < kPowers) s[threadIdx.x] = exp2((double)threadIdx.x / kPowers);
+    if (threadIdx.x < kPowers) s[threadIdx.x] = kPowerTable[threadIdx.x];
 }
 
-// rint(2^(40 + t)), t <= 0: with n = rint(64 t), 2^t = 2^(n / 64) 2^f, |f| <=
-// 1/128, the series of 2^f to f^4 (the next term is below 4e-14, 0.05 units of
-// the largest weight; the exponential by its series alone, to f^11, took twice
-// the registers and more time)
+// Distances t are in 1/64 of log2, 0 or less; from kFar on a weight is 0.
+constexpr double kFar = -41.0 * kPowers;
+// (the high words of numbers below 2624 in magnitude are below its own)
+__device__ __forceinline__ bool near(double t) {
+    return ((unsigned)(__double_as_longlong(t) >> 32) & 0x7fffffffu) < 0x40a48000u;
+}
+static_assert(kFar == -2624.0, "near's constant");
+// t to the nearest whole number, as an int and as a double: its last bits
+// after the addition (a conversion and a rounding take four times as long)
+constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
+__device__ __forceinline__ int nearest(double t) { return (int)__double_as_longlong(t + kRound); }
+
+// rint(2^(40 + t / 64)): with n the nearest to t, 2^(t / 64) = 2^(n / 64) 2^(f / 64),
+// |f| <= 1/2, the series of 2^(f / 64) to f^4 (the next term is below 4e-14, 0.05
+// units of the largest weight; the exponential by its series alone, to the
+// 11th power, took twice the registers and more time)
 __device__ __forceinline__ u64 weight(const double* powers, double t) {
-    if (!(t > -41.0)) return 0;
-    const double n = rint(t * 64.0), f = fma(n, -1.0 / 64.0, t);
-    double s = 9.61812910762847716e-3;   // ln(2)^4 / 24
-    s = fma(s, f, 5.55041086648215800e-2);
-    s = fma(s, f, 2.40226506959100712e-1);
-    s = fma(s, f, 6.93147180559945309e-1);
+    if (!near(t)) return 0;
+    const int k = nearest(t);
+    const double f = t - ((t + kRound) - kRound);
+    double s = 5.732851688640402e-10;  // (ln(2) / 64)^4 / 24
+    s = fma(s, f, 2.1173137155464774e-07);
+    s = fma(s, f, 5.864904955056169e-05);
+    s = fma(s, f, 1.0830424696249145e-02);
     s = fma(s, f, 1.0);
-    const int k = (int)n;
-    // (the last bits of 2^40 2^t + 2^52 are its nearest whole number)
-    const double v = ldexp(s * powers[k & 63], (k >> 6) + 40) + 4503599627370496.0;
+    // 2^(40 + n / 64): the power's exponent moved; then the last bits of its
+    // product + 2^52 are the nearest whole number
+    const long long p = __double_as_longlong(powers[k & 63]) +
+                        ((long long)((k >> 6) + 40) << 52);
+    const double v = fma(s, __longlong_as_double(p), 4503599627370496.0);
     return (u64)__double_as_longlong(v) & 0xfffffffffffffull;
 }
 
 // A row's parameters, the same in every thread.
 struct Row {
-    double top, c;  // maximum; log2(e) / T
-    double minw;    // least kept weight
-    float p;
+    double top, c;  // maximum; 64 log2(e) / T
+    u64 minw;       // least kept weight
+    float p, minp;
     int k;          // 0: none
-    bool greedy;
+    bool greedy, infinite;
     const double* powers;
     __device__ __forceinline__ Row(const SampleArgs& a, int r, float most, const double* s_powers)
         : powers(s_powers) {
         const float t = a.temp ? a.temp[r] : a.temp_all;
         greedy = !(t > 0.0f);
         top = (double)most;
-        c = greedy ? 0.0 : 1.4426950408889634074 / (double)t;
-        const float m = a.minp ? a.minp[r] : a.minp_all;
-        minw = (double)fminf(m, 1.0f) * 1099511627776.0;
+        infinite = most == INFINITY;
+        c = greedy ? 0.0 : 92.332482616893658 / (double)t;
+        minp = a.minp ? a.minp[r] : a.minp_all;
+        minp = minp < 1.0f ? fmaxf(minp, 0.0f) : 1.0f;  // (NaN: 1)
+        minw = (u64)ceil((double)minp * 1099511627776.0);
         p = a.p ? a.p[r] : a.p_all;
         k = a.k ? a.k[r] : a.k_all;
         if (k < 0 || k >= a.n) k = 0;
     }
     __device__ __forceinline__ bool cut() const { return k > 0 || p < 1.0f; }
-    // log2 of the weight over the largest
+    // 64 log2 of the weight over the largest (infinite ones share the mass)
     __device__ __forceinline__ double far(float x) const {
-        return (double)x == top ? 0.0 : ((double)x - top) * c;
+        if (infinite) return x == INFINITY ? 0.0 : 2.0 * kFar;
+        return ((double)x - top) * c;
+    }
+    // the first of the kMinBins bins that may hold weights on both sides of
+    // min-p: those before it are kept, those behind them not
+    __device__ __forceinline__ int least_bin() const {
+        return minp > 0.0f ? max((int)(-16.0f * log2f(minp)) - 1, 0) : kBins;
+    }
+    // floats that no logit of bin b lies outside of (a NaN: no bound)
+    __device__ __forceinline__ float2 around(int b) const {
+        const double lo = top - (4.0 * b + 3.75) / c, hi = top - (4.0 * b - 0.75) / c;
+        const double room = 1e-12 * (fabs(top) + fabs(lo));
+        const float f = (float)(lo - room), g = (float)(hi + room);
+        return make_float2(f - (fabsf(f) * 0x1p-22f + 0x1p-126f),
+                           g + (fabsf(g) * 0x1p-22f + 0x1p-126f));
     }
     __device__ __forceinline__ u64 weight_at(double t) const { return weight(powers, t); }
     __device__ __forceinline__ u64 weight_of(float x) const { return weight(powers, far(x)); }
-    __device__ __forceinline__ bool keeps(u64 w) const { return (double)w >= minw; }
+    __device__ __forceinline__ bool keeps(u64 w) const { return w >= minw; }
 };
 
-__device__ __forceinline__ int bin_of(double t) {
-    return t > -41.0 ? (int)(t * -16.0) : kBins;
-}
+// the bin, 1/16 of log2 wide
+__device__ __forceinline__ int bin_of(double t) { return near(t) ? -nearest(t) >> 2 : kBins; }
 
 // order bits: larger for larger x, equal for equal ones
 __device__ __forceinline__ unsigned order_bits(float x) {
@@ -142,29 +192,30 @@ __device__ __forceinline__ float from_bits(unsigned o) {
     return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
 
-__device__ __forceinline__ u64 shfl64(u64 v, int lane) {
-    const unsigned lo = __shfl((unsigned)v, lane, 64), hi = __shfl((unsigned)(v >> 32), lane, 64);
+// v of the lane that a DPP control names, 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved(u64 v) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
     return (u64)hi << 32 | lo;
 }
-__device__ __forceinline__ u64 wave_scan(u64 v) {  // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned lo = __shfl_up((unsigned)v, o, 64);
-        const unsigned hi = __shfl_up((unsigned)(v >> 32), o, 64);
-        if (lane >= o) v += (u64)hi << 32 | lo;
-    }
+__device__ __forceinline__ u64 lane64(u64 v, int lane) {  // the same in every lane
+    const unsigned lo = __builtin_amdgcn_readlane((int)v, lane);
+    const unsigned hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (u64)hi << 32 | lo;
+}
+// Inclusive prefix over a wave: shifts by 1, 2, 4 and 8 in rows of 16, then
+// the last lane of a row to the next, of a half to the other.
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    v += moved<0x143, 0xc>(v);
     return v;
 }
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const unsigned lo = __shfl_xor((unsigned)v, o, 64);
-        const unsigned hi = __shfl_xor((unsigned)(v >> 32), o, 64);
-        v += (u64)hi << 32 | lo;
-    }
-    return v;
-}
+__device__ __forceinline__ u64 wave_sum64(u64 v) { return lane64(wave_scan(v), 63); }
 // Exclusive prefix over the workgroup's threads and the total. s: LDS, 16
 // words; the caller synchronises before it is used again.
 template <int NT>
@@ -208,18 +259,6 @@ __device__ __forceinline__ void load_tokens(const T* row, int first, int end, fl
         if (!(x[j] >= -INFINITY)) x[j] = -INFINITY;
 }
 
-// Between two passes over the tokens: what the first worked out of them in
-// float64 is not kept in registers for the second (it would not fit).
-template <int TPT>
-__device__ __forceinline__ void next_pass(float (&x)[TPT]) {
-#pragma unroll
-    for (int j = 0; j < TPT; ++j) asm volatile("" : "+v"(x[j]));
-}
-// In a pass: two tokens' weights at a time, not all at once.
-__device__ __forceinline__ void next_pair(int j) {
-    if (j & 1) __builtin_amdgcn_sched_barrier(0);
-}
-
 // The largest of the workgroup's tokens and its first index. s: 2 words a wave.
 template <int NT, int TPT>
 __device__ __forceinline__ float block_top(const float (&x)[TPT], int first, float* s, int* s_at,
@@ -246,99 +285,196 @@ __device__ __forceinline__ float block_top(const float (&x)[TPT], int first, flo
     return top;
 }
 
-// A histogram in LDS, bins from the largest values on.
-struct Hist {
-    u64* mass;
-    unsigned* count;
-};
+// ---------------------------------------------------------------------------
+// What a row's workgroup holds in LDS.
+// ---------------------------------------------------------------------------
+constexpr int kFew = kRowNT / 8;  // logits that are ranked by comparing all with all
+constexpr int kWaves = kRowNT / 64;
+constexpr int kChunk = 4 * kRowNT;  // tokens of a pass of the workgroup
 
-// The last bin that is not empty and that a count or a sum of those before it
-// has not reached: before < k, or (double)before < want; bin 0 if there is
-// none.
-struct Crossing {
-    int bin;
-    u64 mass;        // before it
-    unsigned count;  // before it
-};
-struct CrossState {
-    u64 scan[16], scan2[16];
-    u64 mass;
-    unsigned count;
-    int bin;
-};
-__device__ __forceinline__ Crossing cross(const Hist& h, int bins, u64 mass0, u64 count0,
-                                          bool by_count, u64 k, double want, CrossState& s) {
-    const int b = threadIdx.x;  // a bin a thread
-    const u64 m = b < bins ? h.mass[b] : 0;
-    const unsigned c = b < bins ? h.count[b] : 0;
-    u64 total;
-    if (threadIdx.x == 0) s.bin = 0, s.mass = mass0, s.count = (unsigned)count0;
-    const u64 mb = mass0 + block_scan<kRowNT>(m, s.scan, total);
-    const u64 cb = count0 + block_scan<kRowNT>(c, s.scan2, total);
-    const bool on = c > 0 && (by_count ? cb < k : (double)mb < want);
-    if (on) atomicMax(&s.bin, b);
-    __syncthreads();
-    if (on && s.bin == b) s.mass = mb, s.count = (unsigned)cb;
-    __syncthreads();
-    const Crossing r{s.bin, s.mass, s.count};
-    __syncthreads();
-    return r;
-}
-
-// The one value at which the count or the sum is reached, among the order
-// bits that `each` visits (each(f) calls f(bits, is one) in every thread):
-// its bits, the mass and the count before it, and how many have it.
-struct Group {
+struct Group {  // the logits of one value: bits, how many, mass and count before
     unsigned bits, of;
     u64 mass, count;
 };
-template <typename Each>
-__device__ __forceinline__ Group resolve(const Row& row, const Hist& h, u64 mass0, u64 count0,
-                                         bool by_count, u64 k, double want, CrossState& s,
-                                         unsigned* s_range, Each&& each) {
-    // the range of the bits
-    unsigned lo = ~0u, hi = 0;
-    each([&](unsigned o, bool on) {
-        if (on) lo = min(lo, o), hi = max(hi, o);
-    });
+struct RowState {
+    double powers[kPowers];
+    // the histogram, bins from the largest values on; then (scan_bins) the sums
+    // before each bin
+    u64 mass[kBins];
+    unsigned count[kBins + 1];
+    u64 level_mass[kLevel];
+    unsigned level_count[kLevel];
+    u64 few_w[kFew];
+    unsigned few_key[kFew];
+    u64 scan[16], scan2[16];
+    u64 chunk_mass[kRowMost / kChunk * kWaves];
+    unsigned chunk_ties[kRowMost / kChunk * kWaves];
+    Group group;
+    u64 base, q, aim, before_mass;
+    unsigned few, best, before_count;
+    int bin, entry, slice;
+    float top[kWaves];
+    int top_at[kWaves];
+};
+
+// The tokens [first, end) of a row into s_x, up to a whole chunk (-inf behind
+// the end; NaN becomes -inf), at most MOST of them. Returns their largest and,
+// in `at`, its first index.
+template <typename T, int MOST>
+__device__ __forceinline__ float stage_tokens(const T* row, int first, int end, float* s_x,
+                                              RowState& s, int& at) {
+    float x[MOST / kRowNT];
+    load_tokens<T, kRowNT, MOST / kRowNT>(row, first, end, x);
+    float m = -INFINITY;
+    at = INT_MAX;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        lo = min(lo, (unsigned)__shfl_xor(lo, o, 64));
-        hi = max(hi, (unsigned)__shfl_xor(hi, o, 64));
+    for (int j = 0; j < MOST / kChunk; ++j) {
+        const int i = 4 * (j * kRowNT + (int)threadIdx.x);
+        if (first + j * kChunk < end)
+            *reinterpret_cast<float4*>(s_x + i) =
+                make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (x[4 * j + e] > m) m = x[4 * j + e], at = first + i + e;
     }
-    if (threadIdx.x == 0) s_range[0] = ~0u, s_range[1] = 0;
+    const float mine = m;
+    m = wave_max(m);
+    if (mine != m) at = INT_MAX;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
+    if ((threadIdx.x & 63) == 0) s.top[threadIdx.x >> 6] = m, s.top_at[threadIdx.x >> 6] = at;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
-        atomicMin(&s_range[0], lo);
-        atomicMax(&s_range[1], hi);
+    float top = s.top[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s.top[w]);
+    at = INT_MAX;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+        if (s.top[w] == top) at = min(at, s.top_at[w]);
+    return top;
+}
+
+// The histogram becomes the sums before each bin; returns the whole sum, the
+// tokens of it are count[kBins].
+__device__ __forceinline__ u64 scan_bins(RowState& s) {
+    constexpr int PER = (kBins + kRowNT - 1) / kRowNT;
+    u64 m[PER], c[PER], mass = 0, count = 0, total, tokens;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int b = threadIdx.x * PER + i;
+        m[i] = b < kBins ? s.mass[b] : 0;
+        c[i] = b < kBins ? s.count[b] : 0;
+        mass += m[i];
+        count += c[i];
     }
+    u64 mb = block_scan<kRowNT>(mass, s.scan, total);
+    u64 cb = block_scan<kRowNT>(count, s.scan2, tokens);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int b = threadIdx.x * PER + i;
+        if (b < kBins) s.mass[b] = mb, s.count[b] = (unsigned)cb;
+        mb += m[i];
+        cb += c[i];
+    }
+    if (threadIdx.x == 0) s.count[kBins] = (unsigned)tokens;
     __syncthreads();
-    lo = s_range[0], hi = s_range[1];
-    for (;;) {
-        const unsigned width = hi - lo;  // the last bit pattern that counts, from hi down
+    return total;
+}
+
+// A threshold in the order: a count or a sum (of weights before) to be reached.
+struct Limit {
+    bool by_count;
+    u64 k;
+    double want;
+    __device__ __forceinline__ bool open(u64 mass, u64 count) const {
+        return by_count ? count < k : (double)mass < want;
+    }
+};
+
+// The last bin that is not empty before which the limit is open; 0 if there is
+// none.
+__device__ __forceinline__ int limit_bin(const Limit& l, RowState& s) {
+    if (threadIdx.x == 0) s.bin = 0;
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += kRowNT)
+        if (s.count[b + 1] > s.count[b] && l.open(s.mass[b], s.count[b])) atomicMax(&s.bin, b);
+    __syncthreads();
+    return s.bin;
+}
+
+// The one value at which the limit is reached, among the n order bits that
+// `each` visits (each(f) calls f(bits, is one) in every thread), with mass0
+// and count0 before them, all in [lo, hi]. Few are compared all with all, 8
+// threads each; more are narrowed down by histograms, 512 wide, first.
+template <typename Each>
+__device__ __forceinline__ Group resolve(const Row& row, const Limit& l, unsigned n, u64 mass0,
+                                         u64 count0, unsigned lo, unsigned hi, RowState& s,
+                                         Each&& each) {
+    while (n > kFew) {
         int shift = 0;
-        while ((width >> shift) >= kLevel) ++shift;
-        h.mass[threadIdx.x] = 0;
-        h.count[threadIdx.x] = 0;
+        while (((hi - lo) >> shift) >= kLevel) ++shift;
+        s.level_mass[threadIdx.x] = 0;
+        s.level_count[threadIdx.x] = 0;
+        if (threadIdx.x == 0) s.bin = 0;
         __syncthreads();
         each([&](unsigned o, bool on) {
             if (!on || o > hi || o < lo) return;
             const unsigned b = (hi - o) >> shift;
-            atomicAdd(&h.mass[b], row.weight_of(from_bits(o)));
-            atomicAdd(&h.count[b], 1u);
+            atomicAdd(&s.level_mass[b], row.weight_of(from_bits(o)));
+            atomicAdd(&s.level_count[b], 1u);
         });
         __syncthreads();
-        const Crossing x = cross(h, kLevel, mass0, count0, by_count, k, want, s);
-        mass0 = x.mass, count0 = x.count;
-        hi -= (unsigned)x.bin << shift;
-        if (shift == 0) {
-            const Group g{hi, h.count[x.bin], mass0, count0};
-            __syncthreads();
-            return g;
-        }
-        const unsigned least = (1u << shift) - 1;
-        lo = hi - lo > least ? hi - least : lo;
+        const unsigned c = s.level_count[threadIdx.x];
+        u64 total;
+        const u64 mb = mass0 + block_scan<kRowNT>(s.level_mass[threadIdx.x], s.scan, total);
+        const u64 cb = count0 + block_scan<kRowNT>(c, s.scan2, total);
+        if (c && l.open(mb, cb)) atomicMax(&s.bin, threadIdx.x);
+        __syncthreads();
+        const int bin = s.bin;
+        if (threadIdx.x == bin) s.before_mass = mb, s.before_count = (unsigned)cb, s.few = c;
+        __syncthreads();
+        mass0 = s.before_mass, count0 = s.before_count, n = s.few;
+        hi -= (unsigned)bin << shift;
+        const unsigned span = (1u << shift) - 1;
+        lo = hi - lo > span ? hi - span : lo;
+        __syncthreads();
+        if (shift == 0) return Group{hi, n, mass0, count0};  // one value
     }
+    if (threadIdx.x == 0) s.few = 0, s.best = 0;
+    __syncthreads();
+    each([&](unsigned o, bool on) {
+        if (!on || o > hi || o < lo) return;
+        const unsigned i = atomicAdd(&s.few, 1u);
+        s.few_key[i] = o;
+        s.few_w[i] = row.weight_of(from_bits(o));
+    });
+    __syncthreads();
+    const unsigned mine = threadIdx.x >> 3;
+    const unsigned key = mine < n ? s.few_key[mine] : 0;
+    u64 m = 0;
+    unsigned c = 0, of = 0;
+    if (mine < n)
+        for (unsigned i = threadIdx.x & 7; i < n; i += 8) {
+            const unsigned o = s.few_key[i];
+            if (o > key) m += s.few_w[i], ++c;
+            of += o == key;
+        }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        const unsigned a = __shfl_xor((unsigned)m, o, 64), b = __shfl_xor((unsigned)(m >> 32), o, 64);
+        m += (u64)b << 32 | a;
+        c += __shfl_xor(c, o, 64);
+        of += __shfl_xor(of, o, 64);
+    }
+    const bool first = (threadIdx.x & 7) == 0 && mine < n;
+    if (first && l.open(mass0 + m, count0 + c)) atomicMax(&s.best, c + 1);
+    __syncthreads();
+    const unsigned best = s.best ? s.best - 1 : 0;
+    if (first && c == best) s.group = Group{key, of, mass0 + m, count0 + c};
+    __syncthreads();
+    const Group g = s.group;
+    __syncthreads();
+    return g;
 }
 
 // What is kept: x > xc, and the first q (by index) of those with x = xc (all
@@ -358,25 +494,25 @@ __device__ __forceinline__ u64 first_below(u64 mass, u64 w, u64 of, double want)
     return q;
 }
 
-// The cut from the histogram of the whole row's weights; each(f, bin) visits
-// the order bits of a bin. total: the sum of all.
+// The cut from the scanned histogram of the whole row's weights, `total` their
+// sum; each(f, bin) visits the order bits of a bin.
 template <typename Each>
-__device__ __forceinline__ Cut find_cut(const Row& row, const Hist& h, u64 total, unsigned tokens,
-                                        CrossState& s, const Hist& level, unsigned* s_range,
-                                        Each&& each) {
+__device__ __forceinline__ Cut find_cut(const Row& row, u64 total, RowState& s, Each&& each) {
     Cut cut{-INFINITY, 0, 0};
     u64 sum = total;
     // (a k that all weights but zeros come up to cuts nothing)
-    const bool by_k = row.k > 0 && (unsigned)row.k < tokens;
+    const bool by_k = row.k > 0 && (unsigned)row.k < s.count[kBins];
     for (int pass = by_k ? 0 : 1; pass < (row.p < 1.0f ? 2 : 1); ++pass) {
-        const bool by_count = pass == 0;
-        const double want = (double)row.p * (double)sum;
-        const Crossing x = cross(h, kBins, 0, 0, by_count, row.k, want, s);
-        const Group g = resolve(row, level, x.mass, x.count, by_count, row.k, want, s, s_range,
-                                [&](auto&& f) { each(f, x.bin); });
+        const Limit l{pass == 0, (u64)row.k, (double)row.p * (double)sum};
+        const int bin = limit_bin(l, s);
+        const float2 about = row.around(bin);
+        const Group g = resolve(row, l, s.count[bin + 1] - s.count[bin], s.mass[bin], s.count[bin],
+                                about.x >= -INFINITY ? order_bits(about.x) : 0,
+                                about.y <= INFINITY ? order_bits(about.y) : ~0u, s,
+                                [&](auto&& f) { each(f, bin); });
         cut.xc = from_bits(g.bits);
         cut.wc = row.weight_of(cut.xc);
-        cut.q = by_count ? (u64)row.k - g.count : first_below(g.mass, cut.wc, g.of, want);
+        cut.q = l.by_count ? (u64)row.k - g.count : first_below(g.mass, cut.wc, g.of, l.want);
         sum = g.mass + cut.q * cut.wc;
     }
     if (!row.keeps(cut.wc)) cut.wc = 0;
@@ -389,22 +525,14 @@ __device__ __forceinline__ u64 aim_at(float u, u64 total) {
     return d >= (double)total ? last : min((u64)d, last);
 }
 
-// The first token of the workgroup's whose running sum of kept weights passes
-// aim (~0: that of u of their whole sum). `q`: how many of the cut's equals
-// may still be kept here.
-struct PickState {
-    u64 mass[kRowMost / 4096 * 16];
-    unsigned ties[kRowMost / 4096 * 16];
-    u64 base, q, aim;
-    int entry;
-    long long token;
-};
-template <int TPT>
-__device__ __forceinline__ void pick(const Row& row, const Cut& cut, const float (&x)[TPT],
-                                     int first, u64 q, u64 aim, float u, PickState& s,
+// The first of the staged tokens (n of them, `first` the first one's index)
+// whose running sum of kept weights passes aim (~0: that of u of their whole
+// sum). q: how many of the cut's equals may still be kept here.
+__device__ __forceinline__ void pick(const Row& row, const Cut& cut, const float* s_x, int n,
+                                     int first, u64 q, u64 aim, float u, RowState& s,
                                      long long* out) {
-    constexpr int J = TPT / 4, kWaves = kRowNT / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int chunks = (n + kChunk - 1) / kChunk;
     auto kept = [&](float v) -> u64 {  // of those above the cut
         if (!(v > cut.xc)) return 0;
         const u64 w = row.weight_of(v);
@@ -412,43 +540,38 @@ __device__ __forceinline__ void pick(const Row& row, const Cut& cut, const float
     };
     auto tie = [&](float v) { return v == cut.xc; };
     // sums of every 256 tokens in a row: (chunk j, wave)
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-        u64 m = 0;
-        unsigned t = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            m += kept(x[4 * j + e]);
-            t += tie(x[4 * j + e]);
-            next_pair(e);
+    for (int j = 0; j < chunks; ++j) {
+        const float4 x = *reinterpret_cast<const float4*>(s_x + 4 * (j * kRowNT + threadIdx.x));
+        u64 m = kept(x.x) + kept(x.y) + kept(x.z) + kept(x.w);
+        unsigned t = tie(x.x) + tie(x.y) + tie(x.z) + tie(x.w);
+        if (__builtin_amdgcn_ballot_w64(m | t)) {
+            m = wave_sum64(m);
+            t = (unsigned)wave_sum64(t);
         }
-        m = wave_sum64(m);
-#pragma unroll
-        for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o, 64);
-        if (lane == 0) s.mass[j * kWaves + wave] = m, s.ties[j * kWaves + wave] = t;
+        if (lane == 0) s.chunk_mass[j * kWaves + wave] = m, s.chunk_ties[j * kWaves + wave] = t;
     }
     __syncthreads();
     if (wave == 0) {
-        constexpr int N = J * kWaves, PER = (N + 63) / 64;
-        u64 m[PER], t[PER], mine = 0;
+        constexpr int PER = kRowMost / kChunk * kWaves / 64;
+        const int entries = chunks * kWaves;
+        u64 m[PER], t[PER], had[PER], mine = 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int e = lane * PER + i;
-            t[i] = e < N ? s.ties[e] : 0;
+            t[i] = e < entries ? s.chunk_ties[e] : 0;
             mine += t[i];
         }
-        u64 before = wave_scan(mine) - mine;  // equals before the lane's entries
-        u64 sum = 0, had[PER];
+        u64 before = wave_scan(mine) - mine, sum = 0;  // equals before the lane's entries
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int e = lane * PER + i;
             had[i] = before;
             const u64 left = q > before ? q - before : 0;
-            m[i] = (e < N ? s.mass[e] : 0) + cut.wc * min(left, t[i]);
+            m[i] = (e < entries ? s.chunk_mass[e] : 0) + cut.wc * min(left, t[i]);
             before += t[i];
             sum += m[i];
         }
-        const u64 in = wave_scan(sum), total = shfl64(in, 63);
+        const u64 in = wave_scan(sum), total = lane64(in, 63);
         if (aim == ~0ull) aim = aim_at(u, total);
         u64 run = in - sum;
         const u64 hit = __builtin_amdgcn_ballot_w64(in > aim);
@@ -475,12 +598,9 @@ __device__ __forceinline__ void pick(const Row& row, const Cut& cut, const float
         return;
     }
     if (entry % kWaves != wave) return;
-    float v[4] = {};
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-        if (j == entry / kWaves)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = x[4 * j + e];
+    const int at = 4 * ((entry / kWaves) * kRowNT + (int)threadIdx.x);
+    const float4 x = *reinterpret_cast<const float4*>(s_x + at);
+    const float v[4] = {x.x, x.y, x.z, x.w};
     unsigned t = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) t += tie(v[e]);
@@ -497,82 +617,116 @@ __device__ __forceinline__ void pick(const Row& row, const Cut& cut, const float
     const u64 hit = __builtin_amdgcn_ballot_w64(in > s.aim);
     if (hit && lane == __ffsll(hit) - 1) {
         u64 run = in - sum;
-        int at = 3;
+        int e = 0;
 #pragma unroll
-        for (int e = 3; e >= 0; --e) {
-            u64 upto = run;
-#pragma unroll
-            for (int f = 0; f < 4; ++f)
-                if (f <= e) upto += w[f];
-            if (upto > s.aim) at = e;
+        for (int f = 0; f < 3; ++f) {
+            run += w[f];
+            if (run <= s.aim) e = f + 1;
         }
-        *out = (long long)first + 4 * ((entry / kWaves) * kRowNT + (int)threadIdx.x) + at;
+        *out = (long long)first + at + e;
     }
 }
 
 // ---------------------------------------------------------------------------
-// a workgroup a row
+// a workgroup a row, its logits in LDS
 // ---------------------------------------------------------------------------
-template <typename T, int TPT>
+template <typename T, int MOST>
 __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
-    __shared__ double s_powers[kPowers];
-    __shared__ float s_top[16];
-    __shared__ int s_at[16];
-    __shared__ u64 s_mass[kBins], s_level_mass[kLevel];
-    __shared__ unsigned s_count[kBins], s_level_count[kLevel], s_range[2];
-    __shared__ CrossState s_cross;
-    __shared__ PickState s_pick;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    RowState& s = *reinterpret_cast<RowState*>(smem);
+    float* const s_x = reinterpret_cast<float*>(smem + ((sizeof(RowState) + 15) & ~(size_t)15));
     const int r = blockIdx.x;
-    const T* const logits = (const T*)a.x + (long long)r * a.ld;
-    float x[TPT];
-    load_tokens<T, kRowNT, TPT>(logits, 0, a.n, x);
-    fill_powers(s_powers);
-    for (int b = threadIdx.x; b < kBins; b += kRowNT) s_mass[b] = 0, s_count[b] = 0;
+    for (int b = threadIdx.x; b < kBins; b += kRowNT) s.mass[b] = 0, s.count[b] = 0;
+    fill_powers(s.powers);
     int at;
-    const float top = block_top<kRowNT, TPT>(x, 0, s_top, s_at, at);
-    const Row row(a, r, top, s_powers);
+    const float top = stage_tokens<T, MOST>((const T*)a.x + (long long)r * a.ld, 0, a.n, s_x, s, at);
+    const Row row(a, r, top, s.powers);
     if (row.greedy || top == -INFINITY) {
         if (threadIdx.x == 0) a.out[r] = top == -INFINITY ? -1 : at;
         return;
     }
+    const int chunks = (a.n + kChunk - 1) / kChunk;
     Cut cut{-INFINITY, 0, 0};
     if (row.cut()) {
-        u64 mine = 0;
-        unsigned some = 0;
+        for (int j = 0; j < chunks; ++j) {
+            const float4 x = *reinterpret_cast<const float4*>(s_x + 4 * (j * kRowNT + threadIdx.x));
+            const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int j = 0; j < TPT; ++j) {
-            const double t = row.far(x[j]);
-            const int b = bin_of(t);
-            next_pair(j);
-            if (b >= kBins) continue;
-            const u64 w = row.weight_at(t);
-            mine += w;
-            ++some;
-            atomicAdd(&s_mass[b], w);
-            atomicAdd(&s_count[b], 1u);
+            for (int e = 0; e < 4; ++e) {
+                const double t = row.far(v[e]);
+                const int b = bin_of(t);
+                if (b >= kBins) continue;
+                atomicAdd(&s.mass[b], row.weight_at(t));
+                atomicAdd(&s.count[b], 1u);
+            }
         }
-        u64 total, tokens;
-        block_scan<kRowNT>(mine, s_cross.scan, total);
-        block_scan<kRowNT>(some, s_cross.scan2, tokens);
         __syncthreads();
-        cut = find_cut(row, Hist{s_mass, s_count}, total, (unsigned)tokens, s_cross,
-                       Hist{s_level_mass, s_level_count}, s_range, [&](auto&& f, int bin) {
-                           next_pass(x);
+        const u64 total = scan_bins(s);
+        cut = find_cut(row, total, s, [&](auto&& f, int bin) {
+            const float2 about = row.around(bin);
+            for (int j = 0; j < chunks; ++j) {
+                const float4 x =
+                    *reinterpret_cast<const float4*>(s_x + 4 * (j * kRowNT + threadIdx.x));
+                const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                           for (int j = 0; j < TPT; ++j) {
-                               f(order_bits(x[j]), bin_of(row.far(x[j])) == bin);
-                               next_pair(j);
-                           }
-                       });
+                for (int e = 0; e < 4; ++e)
+                    if (!(v[e] < about.x) && !(v[e] > about.y))
+                        f(order_bits(v[e]), bin_of(row.far(v[e])) == bin);
+            }
+        });
     }
-    next_pass(x);
-    pick<TPT>(row, cut, x, 0, cut.q, ~0ull, a.u[r], s_pick, a.out + r);
+    pick(row, cut, s_x, a.n, 0, cut.q, ~0ull, a.u[r], s, a.out + r);
 }
 
 // ---------------------------------------------------------------------------
 // slices
 // ---------------------------------------------------------------------------
 constexpr int kSliceTPT = kSlice / kSliceNT;
+
+// f(token, its place j) for a thread's tokens of a slice, with the loads of the next
+// ones under way (all loads first left every workgroup of a CU loading and
+// then computing at the same time).
+template <typename T>
+struct Tokens {
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    static constexpr int kSteps = kSliceTPT / 4, kAhead = 4;
+    const T* row;
+    int lo, hi;
+    bool vec;
+    float4 x[kAhead];
+    __device__ __forceinline__ float4 load(int j) const {
+        const int i = lo + 4 * (j * kSliceNT + (int)threadIdx.x);
+        if (vec && i + 4 <= hi) {
+            const v4 v = *reinterpret_cast<const v4*>(row + i);
+            return make_float4((float)v[0], (float)v[1], (float)v[2], (float)v[3]);
+        }
+        return make_float4(i < hi ? (float)row[i] : -INFINITY,
+                           i + 1 < hi ? (float)row[i + 1] : -INFINITY,
+                           i + 2 < hi ? (float)row[i + 2] : -INFINITY,
+                           i + 3 < hi ? (float)row[i + 3] : -INFINITY);
+    }
+    __device__ __forceinline__ Tokens(const SampleArgs& a, int r, int first, int end)
+        : row((const T*)a.x + (long long)r * a.ld), lo(first), hi(end),
+          vec(((uintptr_t)(row + first) & (4 * sizeof(T) - 1)) == 0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) x[j] = load(j);
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) {
+#pragma unroll 1
+        for (int j0 = 0; j0 < kSteps; j0 += kAhead)
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q) {
+                const float4 v = x[q];
+                if (j0 + kAhead < kSteps) x[q] = load(j0 + kAhead + q);
+                const int j = 4 * (j0 + q);
+                f(v.x, j);
+                f(v.y, j + 1);
+                f(v.z, j + 2);
+                f(v.w, j + 3);
+            }
+    }
+};
 
 template <typename T>
 __global__ __launch_bounds__(kSliceNT) void slice_max(const SampleArgs a) {
@@ -595,10 +749,14 @@ __global__ __launch_bounds__(kSliceNT) void slice_max(const SampleArgs a) {
     }
 }
 
-// The row's maximum from its slices', in every lane.
-__device__ __forceinline__ float row_top(const SampleArgs& a, int r) {
-    float m = -INFINITY;
-    for (int s = threadIdx.x & 63; s < a.slices; s += 64)
+// The row's maximum from its slices', in every lane: a lane's first one, then
+// the rest.
+__device__ __forceinline__ float slice_top(const SampleArgs& a, int r) {
+    const int s = threadIdx.x & 63;
+    return s < a.slices ? a.top[(size_t)r * a.slices + s] : -INFINITY;
+}
+__device__ __forceinline__ float row_top(const SampleArgs& a, int r, float m) {
+    for (int s = (threadIdx.x & 63) + 64; s < a.slices; s += 64)
         m = fmaxf(m, a.top[(size_t)r * a.slices + s]);
     return wave_max(m);
 }
@@ -611,63 +769,72 @@ __global__ __launch_bounds__(kSliceNT) void slice_hist(const SampleArgs a) {
     __shared__ u64 s_sum[4];
     const int r = blockIdx.x / a.slices, s = blockIdx.x - r * a.slices;
     const int lo = s * kSlice, hi = min(lo + kSlice, a.n);
-    float x[kSliceTPT];
-    load_tokens<T, kSliceNT, kSliceTPT>((const T*)a.x + (long long)r * a.ld, lo, hi, x);
+    const float some = slice_top(a, r);
+    Tokens<T> tokens(a, r, lo, hi);
     fill_powers(s_powers);
     for (int b = threadIdx.x; b < kBins; b += kSliceNT) s_mass[b] = 0, s_count[b] = 0;
     __syncthreads();
-    const float top = row_top(a, r);
+    const float top = row_top(a, r, some);
     const Row row(a, r, top, s_powers);
     if (row.greedy || top == -INFINITY) return;
     if (!row.cut()) {
         u64 sum = 0;
-#pragma unroll
-        for (int j = 0; j < kSliceTPT; ++j) {
-            const u64 w = row.weight_of(x[j]);
+        tokens.each([&](float x, int) {
+            const u64 w = row.weight_of(x);
             if (row.keeps(w)) sum += w;
-            next_pair(j);
-        }
+        });
         sum = wave_sum64(sum);
         if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
         __syncthreads();
         if (threadIdx.x == 0) a.sum[blockIdx.x] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
         return;
     }
-#pragma unroll
-    for (int j = 0; j < kSliceTPT; ++j) {
-        const double t = row.far(x[j]);
+    tokens.each([&](float x, int) {
+        const double t = row.far(x);
         const int b = bin_of(t);
-        next_pair(j);
-        if (b >= kBins) continue;
+        if (b >= kBins) return;
         atomicAdd(&s_mass[b], row.weight_at(t));
         atomicAdd(&s_count[b], 1u);
-    }
+    });
     __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += kSliceNT)
+    u64* const part = a.part + (size_t)blockIdx.x * kBins;
+    for (int b = threadIdx.x; b < kBins; b += kSliceNT) {
+        part[b] = s_mass[b];
         if (s_count[b]) {
             atomicAdd(&a.mass[(size_t)r * kBins + b], s_mass[b]);
             atomicAdd(&a.count[(size_t)r * kBins + b], s_count[b]);
         }
+    }
 }
+
+// A thread's bins of the row's histogram.
+struct BinRun {
+    static constexpr int PER = (kBins + kSliceNT - 1) / kSliceNT;
+    u64 m[PER];
+    unsigned c[PER];
+    __device__ __forceinline__ void load(const SampleArgs& a, int r) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int b = threadIdx.x * PER + i;
+            m[i] = b < kBins ? a.mass[(size_t)r * kBins + b] : 0;
+            c[i] = b < kBins ? a.count[(size_t)r * kBins + b] : 0;
+        }
+    }
+};
 
 // The bins that the cut can be in: [lo, hi], and k's own. Sums are exact but
 // for the part of bin `at_k` that k keeps, so p's want lies between two.
 struct Span {
     int lo, hi, at_k;  // at_k: -1 none
 };
-__device__ __forceinline__ Span cut_span(const Row& row, const Hist& h, u64* s_scan, u64* s_scan2,
-                                         int* s_bin) {
-    constexpr int PER = (kBins + kSliceNT - 1) / kSliceNT;
-    u64 m[PER], mine = 0, many = 0, total, tokens;
-    unsigned c[PER];
+__device__ __forceinline__ Span cut_span(const Row& row, const BinRun& h, u64* s_scan,
+                                         u64* s_scan2, int* s_bin) {
+    constexpr int PER = BinRun::PER;
+    const u64(&m)[PER] = h.m;
+    const unsigned(&c)[PER] = h.c;
+    u64 mine = 0, many = 0, total, tokens;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int b = threadIdx.x * PER + i;
-        m[i] = b < kBins ? h.mass[b] : 0;
-        c[i] = b < kBins ? h.count[b] : 0;
-        mine += m[i];
-        many += c[i];
-    }
+    for (int i = 0; i < PER; ++i) mine += m[i], many += c[i];
     if (threadIdx.x < 3) s_bin[threadIdx.x] = 0;
     u64 mb = block_scan<kSliceNT>(mine, s_scan, total);
     u64 cb = block_scan<kSliceNT>(many, s_scan2, tokens);
@@ -713,34 +880,54 @@ __device__ __forceinline__ Span cut_span(const Row& row, const Hist& h, u64* s_s
 
 template <typename T>
 __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
-    __shared__ double s_powers[kPowers];
     __shared__ u64 s_scan[4], s_scan2[4], s_sum[4];
     __shared__ int s_bin[3];
     __shared__ unsigned s_n;
     const int r = blockIdx.x / a.slices, s = blockIdx.x - r * a.slices;
     const int lo = s * kSlice, hi = min(lo + kSlice, a.n);
-    const float top = row_top(a, r);
-    const Row row(a, r, top, s_powers);
-    if (row.greedy || top == -INFINITY || !row.cut()) return;
-    float x[kSliceTPT];
-    load_tokens<T, kSliceNT, kSliceTPT>((const T*)a.x + (long long)r * a.ld, lo, hi, x);
-    if (threadIdx.x == 0) s_n = 0;
-    fill_powers(s_powers);
-    const Span span = cut_span(row, Hist{a.mass + (size_t)r * kBins, a.count + (size_t)r * kBins},
-                               s_scan, s_scan2, s_bin);
-    u64 sum = 0;
-    unsigned* const list = a.list + (size_t)r * a.n + lo;
+    __shared__ float s_near[kSlice];
+    const float some = slice_top(a, r);
+    Tokens<T> tokens(a, r, lo, hi);
+    BinRun bins;
+    bins.load(a, r);
+    u64 own[BinRun::PER];  // the slice's
 #pragma unroll
-    for (int j = 0; j < kSliceTPT; ++j) {
-        const double t = row.far(x[j]);
-        const int b = bin_of(t);
-        if (b >= kBins) continue;
-        if (b < span.lo) {
-            const u64 w = row.weight_at(t);
-            if (row.keeps(w)) sum += w;
+    for (int i = 0; i < BinRun::PER; ++i) {
+        const int b = threadIdx.x + i * kSliceNT;
+        own[i] = b < kBins ? a.part[(size_t)blockIdx.x * kBins + b] : 0;
+    }
+    const float top = row_top(a, r, some);
+    const Row row(a, r, top, nullptr);
+    if (row.greedy || top == -INFINITY || !row.cut()) return;
+    if (threadIdx.x == 0) s_n = 0;
+    const Span span = cut_span(row, bins, s_scan, s_scan2, s_bin);
+    // Above the bins that are listed all is kept: with min-p's own bin among
+    // them, and its own bins' sums at hand, a slice works out no weight here.
+    const int at_p = row.least_bin();
+    const int all = min(span.lo, at_p);
+    u64 sum = 0;
+#pragma unroll
+    for (int i = 0; i < BinRun::PER; ++i)
+        if ((int)threadIdx.x + i * kSliceNT < all) sum += own[i];
+    unsigned* const list = a.list + (size_t)r * a.n + lo;
+    // logits outside the listed bins are seen without their float64 distance
+    const float least = row.around(min(max(span.hi, span.at_k), kBins - 1)).x;
+    const float most = row.around(min(all, kBins - 1)).y;
+    unsigned some_of = 0;  // the thread's tokens that may be listed
+    tokens.each([&](float x, int j) {
+        if (!(x < least) && !(x > most)) {
+            some_of |= 1u << j;
+            s_near[j * kSliceNT + threadIdx.x] = x;
         }
-        if ((b >= span.lo && b <= span.hi) || b == span.at_k)
-            list[atomicAdd(&s_n, 1u)] = order_bits(x[j]);
+    });
+    while (some_of) {
+        const int j = __ffs(some_of) - 1;
+        some_of &= some_of - 1;
+        const float x = s_near[j * kSliceNT + threadIdx.x];
+        const int b = bin_of(row.far(x));
+        if (b < kBins && ((b >= span.lo && b <= span.hi) || b == span.at_k ||
+                          (b >= at_p && b < at_p + kMinBins && b < span.lo)))
+            list[atomicAdd(&s_n, 1u)] = order_bits(x);
     }
     sum = wave_sum64(sum);
     if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
@@ -751,99 +938,109 @@ __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
     }
 }
 
+constexpr int kListMost = 12288;  // listed logits of a row that are held in LDS
+
 template <typename T>
 __global__ __launch_bounds__(kRowNT) void sample_pick(const SampleArgs a) {
-    __shared__ double s_powers[kPowers];
-    __shared__ u64 s_mass[kBins], s_level_mass[kLevel];
-    __shared__ unsigned s_count[kBins], s_level_count[kLevel], s_range[2];
-    __shared__ CrossState s_cross;
-    __shared__ PickState s_pick;
-    __shared__ u64 s_base, s_q;
-    __shared__ int s_slice;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    RowState& s = *reinterpret_cast<RowState*>(smem);
+    // the list; then a slice's tokens
+    unsigned* const s_list =
+        reinterpret_cast<unsigned*>(smem + ((sizeof(RowState) + 15) & ~(size_t)15));
+    __shared__ unsigned s_off[kMaxVocab / kSlice + 1];
     const int r = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const float top = row_top(a, r);
-    const Row row(a, r, top, s_powers);
-    fill_powers(s_powers);
+    const int b = threadIdx.x;
+    const size_t row0 = (size_t)r * a.slices;
+    // (slice s in thread s)
+    const unsigned listed = b < a.slices ? a.listed[row0 + b] : 0;
+    for (int i = b; i < kBins; i += kRowNT) {
+        s.mass[i] = a.mass[(size_t)r * kBins + i];
+        s.count[i] = a.count[(size_t)r * kBins + i];
+    }
+    const float u = a.u[r];
+    const float top = row_top(a, r, slice_top(a, r));
+    const Row row(a, r, top, s.powers);
+    fill_powers(s.powers);
     if (row.greedy || top == -INFINITY) {
         if (wave == 0) {
             int at = INT_MAX;
-            for (int s = lane; s < a.slices; s += 64)
-                if (a.top[(size_t)r * a.slices + s] == top)
-                    at = min(at, a.top_at[(size_t)r * a.slices + s]);
+            for (int t = lane; t < a.slices; t += 64)
+                if (a.top[row0 + t] == top) at = min(at, a.top_at[row0 + t]);
 #pragma unroll
             for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
             if (lane == 0) a.out[r] = top == -INFINITY ? -1 : at;
         }
         return;
     }
-    const size_t row0 = (size_t)r * a.slices;
     Cut cut{-INFINITY, 0, 0};
-    // a slice a thread: kept weights above the cut, and the cut's equals
-    u64* const s_sum = s_level_mass;          // (after the cut is found)
-    unsigned* const s_ties = s_level_count;
+    // a slice's kept weights, and the cut's equals in it
+    u64* const s_sum = s.level_mass;  // (after the cut is found)
+    unsigned* const s_ties = s.level_count;
     if (row.cut()) {
-        u64 m = 0, c = 0, total, tokens;
-        const int b = threadIdx.x;
-        if (b < kBins) {
-            s_mass[b] = m = a.mass[(size_t)r * kBins + b];
-            s_count[b] = c = a.count[(size_t)r * kBins + b];
-        }
-        block_scan<kRowNT>(m, s_cross.scan, total);
-        block_scan<kRowNT>(c, s_cross.scan2, tokens);
+        u64 all;
+        const u64 off = block_scan<kRowNT>(listed, s.scan, all);
+        if (b < a.slices) s_off[b] = (unsigned)off;
+        if (b == 0) s_off[a.slices] = (unsigned)all;
         __syncthreads();
-        // slice s is wave s % 16's
-        cut = find_cut(row, Hist{s_mass, s_count}, total, (unsigned)tokens, s_cross,
-                       Hist{s_level_mass, s_level_count}, s_range, [&](auto&& f, int bin) {
-                           for (int s = wave; s < a.slices; s += kRowNT / 64) {
-                               const unsigned* const list = a.list + (size_t)r * a.n + s * kSlice;
-                               const int n = a.listed[row0 + s];
-                               for (int i = lane; i < n; i += 64) {
-                                   const unsigned o = list[i];
-                                   f(o, bin_of(row.far(from_bits(o))) == bin);
-                               }
-                           }
-                       });
-        for (int s = wave; s < a.slices; s += kRowNT / 64) {
+        const bool held = all <= kListMost;
+        // slice t is wave t % 16's
+        auto slices = [&](auto&& f) {
+            for (int t = wave; t < a.slices; t += kWaves) {
+                const unsigned n = s_off[t + 1] - s_off[t];
+                const unsigned* const list = a.list + (size_t)r * a.n + t * kSlice;
+                for (unsigned i = lane; i < n; i += 64) f(list[i]);
+            }
+        };
+        if (held)
+            for (int t = wave; t < a.slices; t += kWaves)
+                for (unsigned i = lane; i < s_off[t + 1] - s_off[t]; i += 64)
+                    s_list[s_off[t] + i] = a.list[(size_t)r * a.n + t * kSlice + i];
+        const u64 total = scan_bins(s);  // (synchronises)
+        cut = find_cut(row, total, s, [&](auto&& f, int bin) {
+            if (held)
+                for (unsigned i = b; i < (unsigned)all; i += kRowNT)
+                    f(s_list[i], bin_of(row.far(from_bits(s_list[i]))) == bin);
+            else
+                slices([&](unsigned o) { f(o, bin_of(row.far(from_bits(o))) == bin); });
+        });
+        for (int t = wave; t < a.slices; t += kWaves) {
             u64 sum = 0;
             unsigned ties = 0;
-            if (cut.xc > -INFINITY) {
-                const unsigned* const list = a.list + (size_t)r * a.n + s * kSlice;
-                const int n = a.listed[row0 + s];
-                for (int i = lane; i < n; i += 64) {
-                    const float v = from_bits(list[i]);
-                    if (v > cut.xc) {
-                        const u64 w = row.weight_of(v);
-                        if (row.keeps(w)) sum += w;
-                    }
-                    ties += v == cut.xc;
+            const unsigned n = cut.xc > -INFINITY ? s_off[t + 1] - s_off[t] : 0;
+            const unsigned* const list =
+                held ? s_list + s_off[t] : a.list + (size_t)r * a.n + t * kSlice;
+            for (unsigned i = lane; i < n; i += 64) {
+                const float v = from_bits(list[i]);
+                if (v > cut.xc) {
+                    const u64 w = row.weight_of(v);
+                    if (row.keeps(w)) sum += w;
                 }
-                sum = wave_sum64(sum);
-#pragma unroll
-                for (int o = 32; o; o >>= 1) ties += __shfl_xor(ties, o, 64);
+                ties += v == cut.xc;
             }
-            if (lane == 0) s_sum[s] = sum + a.sum[row0 + s], s_ties[s] = ties;
+            sum = wave_sum64(sum);
+            ties = (unsigned)wave_sum64(ties);
+            if (lane == 0) s_sum[t] = sum + a.sum[row0 + t], s_ties[t] = ties;
         }
-    } else {
-        for (int s = threadIdx.x; s < a.slices; s += kRowNT)
-            s_sum[s] = a.sum[row0 + s], s_ties[s] = 0;
+    } else if (b < a.slices) {
+        s_sum[b] = a.sum[row0 + b], s_ties[b] = 0;
     }
-    if (threadIdx.x == 0) s_slice = 0, s_base = 0, s_q = cut.q;
+    if (b == 0) s.slice = 0, s.base = 0, s.q = cut.q;
     __syncthreads();
-    const int s = threadIdx.x;
     u64 total;
-    const u64 ties = s < a.slices ? s_ties[s] : 0;
-    const u64 had = block_scan<kRowNT>(ties, s_cross.scan, total);
+    const u64 ties = b < a.slices ? s_ties[b] : 0;
+    const u64 had = block_scan<kRowNT>(ties, s.scan, total);
     const u64 left = cut.q > had ? cut.q - had : 0;
-    const u64 mine = s < a.slices ? s_sum[s] + cut.wc * min(left, ties) : 0;
-    const u64 before = block_scan<kRowNT>(mine, s_cross.scan2, total);
-    const u64 aim = aim_at(a.u[r], total);
-    if (before <= aim && aim < before + mine) s_slice = s, s_base = before, s_q = left;
+    const u64 mine = b < a.slices ? s_sum[b] + cut.wc * min(left, ties) : 0;
+    const u64 before = block_scan<kRowNT>(mine, s.scan2, total);
+    const u64 aim = aim_at(u, total);
+    if (before <= aim && aim < before + mine) s.slice = b, s.base = before, s.q = left;
     __syncthreads();
-    const int lo = s_slice * kSlice;
-    float x[kSlice / kRowNT];
-    load_tokens<T, kRowNT, kSlice / kRowNT>((const T*)a.x + (long long)r * a.ld, lo,
-                                            min(lo + kSlice, a.n), x);
-    pick<kSlice / kRowNT>(row, cut, x, lo, s_q, aim - s_base, 0.f, s_pick, a.out + r);
+    const int lo = s.slice * kSlice, hi = min(lo + kSlice, a.n);
+    const u64 base = s.base, q = s.q;
+    float* const s_x = reinterpret_cast<float*>(s_list);
+    int at;
+    stage_tokens<T, kSlice>((const T*)a.x + (long long)r * a.ld, lo, hi, s_x, s, at);
+    pick(row, cut, s_x, hi - lo, lo, q, aim - base, 0.f, s, a.out + r);
 }
 
 // ---------------------------------------------------------------------------
@@ -851,7 +1048,7 @@ __global__ __launch_bounds__(kRowNT) void sample_pick(const SampleArgs a) {
 // ---------------------------------------------------------------------------
 struct SampleShape {
     int slices;  // 0: a workgroup a row
-    size_t top, top_at, sum, listed, mass, count, list, bytes;
+    size_t top, top_at, sum, part, listed, mass, count, list, bytes;
 };
 
 SampleShape sample_shape(int rows, int n) {
@@ -872,6 +1069,7 @@ SampleShape sample_shape(int rows, int n) {
     s.top = take(4 * parts);
     s.top_at = take(4 * parts);
     s.sum = take(8 * parts);
+    s.part = take(8 * parts * kBins);
     s.listed = take(4 * parts);
     s.mass = take(8 * (size_t)rows * kBins);
     s.count = take(4 * (size_t)rows * kBins);
@@ -880,13 +1078,29 @@ SampleShape sample_shape(int rows, int n) {
     return s;
 }
 
+constexpr size_t kStateBytes = (sizeof(RowState) + 15) & ~(size_t)15;
+
+template <typename K>
+void allow_lds(K kernel, size_t bytes) {
+    if (bytes > 65536)
+        hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
+                  "hipFuncSetAttribute");
+}
+
+template <typename T, int MOST>
+void row_run(const SampleArgs& a, hipStream_t s) {
+    const size_t lds = kStateBytes + (size_t)(a.n + kChunk - 1) / kChunk * kChunk * 4;
+    allow_lds(sample_row<T, MOST>, lds);
+    sample_row<T, MOST><<<a.rows, kRowNT, lds, s>>>(a);
+}
+
 template <typename T>
 void sample_run(const SampleArgs& a, hipStream_t s) {
     if (!a.slices) {
-        if (a.n <= 4096) sample_row<T, 4><<<a.rows, kRowNT, 0, s>>>(a);
-        else if (a.n <= 8192) sample_row<T, 8><<<a.rows, kRowNT, 0, s>>>(a);
-        else if (a.n <= 16384) sample_row<T, 16><<<a.rows, kRowNT, 0, s>>>(a);
-        else sample_row<T, 32><<<a.rows, kRowNT, 0, s>>>(a);
+        if (a.n <= 4096) row_run<T, 4096>(a, s);
+        else if (a.n <= 16384) row_run<T, 16384>(a, s);
+        else row_run<T, 32768>(a, s);
         launch_check("sample_filtered_batched kernel launch");
         return;
     }
@@ -894,7 +1108,9 @@ void sample_run(const SampleArgs& a, hipStream_t s) {
     slice_max<T><<<grid, kSliceNT, 0, s>>>(a);
     slice_hist<T><<<grid, kSliceNT, 0, s>>>(a);
     slice_list<T><<<grid, kSliceNT, 0, s>>>(a);
-    sample_pick<T><<<a.rows, kRowNT, 0, s>>>(a);
+    const size_t lds = kStateBytes + 4 * (size_t)kListMost;
+    allow_lds(sample_pick<T>, lds);
+    sample_pick<T><<<a.rows, kRowNT, lds, s>>>(a);
     launch_check("sample_filtered_batched kernel launch");
 }
 
@@ -954,6 +1170,7 @@ int ft_sample_filtered_batched_launch(const void* logits, int dtype, long long l
         a.top = (float*)(ws + sh.top);
         a.top_at = (int*)(ws + sh.top_at);
         a.sum = (u64*)(ws + sh.sum);
+        a.part = (u64*)(ws + sh.part);
         a.listed = (unsigned*)(ws + sh.listed);
         a.mass = (u64*)(ws + sh.mass);
         a.count = (unsigned*)(ws + sh.count);

@@ -947,9 +947,10 @@ def _i32_operand(t, name, shape, what):
         raise ValueError(f"{name} must be contiguous")
 
 
-def _qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, pools, slots, sections,
-                  theta, rotary_dim, eps, neox):
-    q_heads, kv_heads = int(q_heads), int(kv_heads)
+def _qk_checked(qkv, q_heads, kv_heads, q_weight, k_weight, positions, pools, slots, sections,
+                rotary_dim):
+    """Every operand of the two ops; returns the weights as the kernel takes
+    them and whether all is on the current device."""
     if q_heads < 1 or kv_heads < 1:
         raise ValueError("q_heads and kv_heads must be >= 1")
     if not (torch.is_tensor(qkv) and qkv.is_cuda):
@@ -959,11 +960,9 @@ def _qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, pools, 
     heads = q_heads + 2 * kv_heads
     if qkv.ndim != 2 or qkv.shape[1] % heads or not qkv.shape[1]:
         raise ValueError("qkv must be [T, (q_heads + 2 * kv_heads) * D]")
-    T, width = qkv.shape
-    D = width // heads
+    T, D = qkv.shape[0], qkv.shape[1] // heads
     if qkv.stride(1) != 1:
         raise ValueError("qkv rows must be contiguous")
-    ld = qkv.stride(0) if T > 1 else width
     if (q_weight is None) != (k_weight is None):
         raise ValueError("q_weight and k_weight are given together or not at all")
     qw = _qk_weight(q_weight, "q_weight", D, qkv.device)
@@ -974,15 +973,16 @@ def _qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, pools, 
             raise ValueError("positions [axes, T] need sections with an entry for each axis")
         _i32_operand(positions, "positions", (axes, T), "positions must be [T] or [axes, T]")
     else:
-        axes = 1
         _i32_operand(positions, "positions", (T,), "positions must be [T] or [axes, T]")
         if sections is not None and len(sections) != 1:
             raise ValueError("sections need positions [axes, T] with a row for each")
+    if sections is not None and sum(int(n) for n in sections) != (
+            D if rotary_dim is None else int(rotary_dim)) // 2:
+        raise ValueError("sections must sum to rotary_dim / 2")
     names, operands = ["qkv", "positions"], [qkv, positions]
     if qw is not None:
         names += ["q_weight", "k_weight"]
         operands += [qw, kw]
-    Nb = P = 0
     if pools is not None:
         for name, t in zip(("k_pool", "v_pool"), pools):
             if not (torch.is_tensor(t) and t.is_cuda):
@@ -993,30 +993,60 @@ def _qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, pools, 
                 pools[0].shape[1] != kv_heads or pools[0].shape[3] != D or
                 not pools[0].is_contiguous() or not pools[1].is_contiguous()):
             raise ValueError(_QK_POOLS)
-        Nb, _, P, _ = pools[0].shape
         _i32_operand(slots, "slots", (T,), "slots must be 1-D with one entry per row")
         names += ["k_pool", "v_pool", "slots"]
         operands += [pools[0], pools[1], slots]
-    if not _one_device(names, operands):
-        with torch.cuda.device(qkv.device):
-            return _qk_norm_rope(qkv, q_heads, kv_heads, qw, kw, positions, pools, slots,
-                                 sections, theta, rotary_dim, eps, neox)
-    q = torch.empty((T, q_heads, D), dtype=qkv.dtype, device=qkv.device)
-    args = (qkv.data_ptr(), _CODE[qkv.dtype], ld, None if qw is None else qw.data_ptr(),
-            None if kw is None else kw.data_ptr(), positions.data_ptr(),
-            [D // 2 if rotary_dim is None else int(rotary_dim) // 2] if axes == 1
-            else [int(n) for n in sections],
-            D if rotary_dim is None else int(rotary_dim), float(theta), float(eps), bool(neox),
-            q.data_ptr())
+    return qw, kw, _one_device(names, operands)
+
+
+def _qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, pools, slots, sections,
+                  theta, rotary_dim, eps, neox):
+    q_heads, kv_heads = int(q_heads), int(kv_heads)
+    try:  # the usual case; every other goes through the checks
+        (T, width), dev = qkv.shape, qkv.get_device()
+        D, rest = divmod(width, q_heads + 2 * kv_heads)
+        ready = (rest == 0 and D > 0 and kv_heads > 0 and q_heads > 0 and qkv.is_cuda and
+                 dev == _current_device() and qkv.dtype in _CODE and qkv.stride(1) == 1 and
+                 q_weight.dtype is _TF and k_weight.dtype is _TF and q_weight.shape == (D,) and
+                 k_weight.shape == (D,) and q_weight.is_contiguous() and
+                 k_weight.is_contiguous() and
+                 q_weight.get_device() == k_weight.get_device() == dev and
+                 sections is None and positions.shape == (T,) and _i32_ready(dev, positions))
+        if ready and pools is not None:
+            k, v = pools
+            ready = (k.dtype is qkv.dtype and v.dtype is qkv.dtype and k.shape == v.shape and
+                     k.ndim == 4 and k.shape[1] == kv_heads and k.shape[3] == D and
+                     k.is_contiguous() and v.is_contiguous() and
+                     k.get_device() == v.get_device() == dev and slots.shape == (T,) and
+                     _i32_ready(dev, slots))
+    except (AttributeError, TypeError, ValueError, ZeroDivisionError):
+        ready = False
+    if not ready:
+        q_weight, k_weight, here = _qk_checked(qkv, q_heads, kv_heads, q_weight, k_weight,
+                                               positions, pools, slots, sections, rotary_dim)
+        if not here:
+            with torch.cuda.device(qkv.device):
+                return _qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions,
+                                     pools, slots, sections, theta, rotary_dim, eps, neox)
+        T, D = qkv.shape[0], qkv.shape[1] // (q_heads + 2 * kv_heads)
+    rot = D if rotary_dim is None else int(rotary_dim)
+    dtype, device = qkv.dtype, qkv.device
+    q = torch.empty((T, q_heads, D), dtype=dtype, device=device)
+    args = (qkv.data_ptr(), _CODE[dtype], qkv.stride(0) if T > 1 else qkv.shape[1],
+            None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), positions.data_ptr(),
+            [rot // 2] if positions.ndim == 1 else [int(n) for n in sections], rot,
+            float(theta), float(eps), bool(neox), q.data_ptr())
     if pools is not None:
         k, v = pools
+        Nb, P = k.shape[0], k.shape[2]
         if T and Nb and k.data_ptr() == v.data_ptr():
             raise ValueError("k and v must have pools of their own")
         _fusedtok.qk_norm_rope_kv_append_paged_launch(
             *args, k.data_ptr(), v.data_ptr(), slots.data_ptr(), T, q_heads, kv_heads, D, Nb, P,
             _stream())
         return q
-    k, v = torch.empty((2, T, kv_heads, D), dtype=qkv.dtype, device=qkv.device).unbind(0)
+    k, v = torch.empty((2, T, kv_heads, D), dtype=dtype, device=device).unbind(0)
     _fusedtok.qk_norm_rope_launch(*args, k.data_ptr(), v.data_ptr(), T, q_heads, kv_heads, D,
                                   _stream())
     return q, k, v

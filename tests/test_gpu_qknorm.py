@@ -213,17 +213,18 @@ def test_refusals():
             (lambda: f(qkv, 0, 1, *w, pos), ValueError, "heads"),
             (lambda: f(qkv.double(), 2, 1, *w, pos), TypeError, "float32"),
             (lambda: f(qkv.cpu(), 2, 1, *w, pos), TypeError, "GPU"),
-            (lambda: f(qkv.t(), 2, 1, *w, pos), ValueError, "qkv must be"),
+            (lambda: f(qkv.t(), 2, 1, *w, pos), ValueError, "contiguous"),
             (lambda: f(qkv, 2, 1, w[0], None, pos), ValueError, "together"),
             (lambda: f(qkv, 2, 1, w[0][:3], w[1], pos), ValueError, "D entries"),
             (lambda: f(qkv, 2, 1, *w, pos.long()), TypeError, "int32"),
             (lambda: f(qkv, 2, 1, *w, pos[:3]), ValueError, "positions"),
             (lambda: f(qkv, 2, 1, *w, pos.cpu()), TypeError, "positions"),
             (lambda: f(qkv, 2, 1, *w, pos, sections=[16, 16]), ValueError, "sections"),
+            (lambda: f(qkv, 2, 1, *w, pos, sections=[31]), ValueError, "sum"),
             (lambda: f(qkv, 2, 1, *w, pos.repeat(2, 1)), ValueError, "sections"),
             (lambda: f(qkv, 2, 1, *w, pos.repeat(2, 1), sections=[16, 17]), ValueError, "sum"),
             (lambda: f(qkv, 2, 1, *w, pos.repeat(2, 1), sections=[33, -1]), ValueError,
-             "sum"),
+             "sections must"),
             (lambda: f(qkv, 2, 1, *w, pos.repeat(5, 1), sections=[8, 8, 8, 4, 4]), ValueError,
              "axes"),
             (lambda: f(qkv, 2, 1, *w, pos, rotary_dim=66), ValueError, "rotary_dim"),

@@ -73,24 +73,27 @@ struct PrefixArgs {
     int segs, min_seg, start_cost, cost[3];
 };
 
-// Rows of a tile. On the matrix cores (WIDE): up to 16 rows leave the keys of a
-// step to the four waves, more are shared out to them, 16 or 32 each.
-template <bool WIDE>
+// Which kernel takes a call.
+enum Kind { kGeneral, kFloat, kHalf };
+
+// Rows of a tile. On the matrix cores up to 16 rows leave the keys of a step to
+// the four waves, more are shared out to them, 16 each or (kHalf) 32.
+template <Kind KIND>
 __device__ __forceinline__ int tile_rows(int rows) {
-    if (!WIDE || rows <= 16) return 16;
-    return rows <= 64 ? 64 : 128;
+    if (KIND == kGeneral || rows <= 16) return 16;
+    return KIND == kFloat || rows <= 64 ? 64 : 128;
 }
 __device__ __forceinline__ int up(int a, int b) { return (a + b - 1) / b; }
 
 // The cost of a unit of n tokens: its start and its tokens, in the order of
 // the range that is cut into segments.
-template <bool WIDE>
+template <Kind KIND>
 __device__ __forceinline__ int token_cost(const PrefixArgs& a, int rows) {
-    return a.cost[!WIDE || rows <= 16 ? 0 : rows <= 64 ? 1 : 2];
+    return a.cost[KIND == kGeneral || rows <= 16 ? 0 : KIND == kFloat || rows <= 64 ? 1 : 2];
 }
-template <bool WIDE>
+template <Kind KIND>
 __device__ __forceinline__ long long unit_cost(const PrefixArgs& a, int rows, int n) {
-    return n ? a.start_cost + (long long)n * token_cost<WIDE>(a, rows) : 0;
+    return n ? a.start_cost + (long long)n * token_cost<KIND>(a, rows) : 0;
 }
 
 // The plan, in LDS: sum of the tokens of all units before an entry, granules
@@ -120,7 +123,7 @@ __device__ __forceinline__ int entry_rows(const PrefixArgs& a, const Plan& p, in
     return e < a.groups ? (p.first[e + 1] - p.first[e]) * a.gq : a.gq;
 }
 
-template <bool WIDE>
+template <Kind KIND>
 __device__ void make_plan(const PrefixArgs& a, const Plan& p, long long* s_sum, int* s_cnt) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // the groups' first sequences: thread t takes offsets [t per, ...)
@@ -150,8 +153,8 @@ __device__ void make_plan(const PrefixArgs& a, const Plan& p, long long* s_sum, 
         const int rows = entry_rows(a, p, e);
         p.start[e] = sum;
         p.gran[e] = gran;
-        sum += unit_cost<WIDE>(a, rows, entry_tokens(a, e)) * a.hkv *
-               up(rows, tile_rows<WIDE>(rows));
+        sum += unit_cost<KIND>(a, rows, entry_tokens(a, e)) * a.hkv *
+               up(rows, tile_rows<KIND>(rows));
         gran += a.hkv * up(rows, kGranule);
     }
     long long s = sum;
@@ -177,12 +180,12 @@ __device__ __forceinline__ long long segment(const PrefixArgs& a, long long tota
 }
 
 // The combine's copy of the plan, sequence by sequence.
-template <bool WIDE>
+template <Kind KIND>
 __device__ void leave_plan(const PrefixArgs& a, const Plan& p, long long seg) {
     if (threadIdx.x == 0) *a.seg = seg;
     auto part = [&](int e, int first) {
         const int n = entry_tokens(a, e), rows = entry_rows(a, p, e);
-        return Part{p.start[e] + a.start_cost, unit_cost<WIDE>(a, rows, n), p.gran[e], n, rows,
+        return Part{p.start[e] + a.start_cost, unit_cost<KIND>(a, rows, n), p.gran[e], n, rows,
                     first};
     };
     for (int b = threadIdx.x; b < a.batch; b += 256) {
@@ -207,7 +210,7 @@ struct Piece {
     size_t slot;     // its partials' first row
     long long next;  // the position behind it
 };
-template <bool WIDE>
+template <Kind KIND>
 __device__ __forceinline__ Piece piece_at(const PrefixArgs& a, const Plan& p, long long pos,
                                           long long end) {
     int lo = 0, hi = p.entries;
@@ -221,9 +224,9 @@ __device__ __forceinline__ Piece piece_at(const PrefixArgs& a, const Plan& p, lo
     x.rows = entry_rows(a, p, x.entry);
     const bool own = x.entry >= a.groups;
     x.first = own ? x.entry - a.groups : p.first[x.entry];
-    const int tr = tile_rows<WIDE>(x.rows), tiles = up(x.rows, tr);
-    const int w = token_cost<WIDE>(a, x.rows);
-    const long long whole = unit_cost<WIDE>(a, x.rows, n), off = pos - p.start[x.entry];
+    const int tr = tile_rows<KIND>(x.rows), tiles = up(x.rows, tr);
+    const int w = token_cost<KIND>(a, x.rows);
+    const long long whole = unit_cost<KIND>(a, x.rows, n), off = pos - p.start[x.entry];
     const int unit = (int)(off / whole);
     const long long in = off - unit * whole, base = pos - in;
     const long long stop = min(whole, end - base);
@@ -325,6 +328,76 @@ struct PCfg {
     static constexpr int kS = D / 32;                // k-steps of the scores
     static constexpr int kDB = D / 16;               // blocks of dims
 };
+
+// A lane's share of its row's partials: D / 16 times 4 dims, piece(x, d) giving
+// the x-th and its first dim. KEYS: the waves' softmaxes over their keys are
+// merged through LDS first.
+template <int D, bool FULL, bool KEYS, typename F>
+__device__ __forceinline__ void leave_partials(const PrefixArgs& a, const Piece& pc, int r, float m,
+                                               float l, float scale, char* smem,
+                                               float (*s_ml)[2][16], F&& piece) {
+    const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int dim = FULL ? D : a.dim;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if constexpr (!KEYS) {
+        if (r >= pc.rows) return;
+        const size_t row = pc.slot + (r - pc.row0);
+        if (g == 0) {
+            a.ml[2 * row] = m;
+            a.ml[2 * row + 1] = l;
+        }
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {
+            int d;
+            const f32x4 v = piece(x, d);
+            if (FULL || d < dim) *reinterpret_cast<f32x4*>(a.acc + row * dim + d) = v * scale;
+        }
+    } else {
+        constexpr int kRow = D + 4;
+        float* const s_acc = reinterpret_cast<float*>(smem);
+        if (g == 0) {
+            s_ml[wave][0][r16] = m;
+            s_ml[wave][1][r16] = l;
+        }
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {
+            int d;
+            const f32x4 v = piece(x, d);
+            *reinterpret_cast<f32x4*>(s_acc + (16 * wave + r16) * kRow + d) = v;
+        }
+        __syncthreads();
+        const int rr = tid >> 4;
+        if (pc.row0 + rr < pc.rows) {
+            float top = -INFINITY, sum = 0.f, f[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ml[w][0][rr]);
+            const float top_use = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                f[w] = __builtin_amdgcn_exp2f(s_ml[w][0][rr] - top_use);
+                sum += f[w] * s_ml[w][1][rr];
+            }
+            const size_t row = pc.slot + rr;
+            if ((tid & 15) == 0) {
+                a.ml[2 * row] = top;
+                a.ml[2 * row + 1] = sum;
+            }
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x) {
+                const int d = 64 * x + 4 * (tid & 15);
+                f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    y += f[w] * *reinterpret_cast<const f32x4*>(s_acc + (16 * w + rr) * kRow + d);
+                if (FULL || d < dim)
+                    *reinterpret_cast<f32x4*>(a.acc + row * dim + d) = y * scale;
+            }
+        }
+        __syncthreads();
+    }
+}
 
 template <typename T, int D, bool FULL, int QB, bool KEYS>
 __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& pc, char* smem,
@@ -546,69 +619,14 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
         __syncthreads();
     }
 
-    // partials: lane (r, g) holds dims 16 db + 4g + i of row r
+    // lane (r, g) holds dims 16 db + 4g + i of row r
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-        l_run[qb] += __shfl_xor(l_run[qb], 16, 64);
-        l_run[qb] += __shfl_xor(l_run[qb], 32, 64);
-    }
-    if constexpr (!KEYS) {
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-            const int r = wrow + 16 * qb + r16;
-            if (r >= pc.rows) continue;
-            const size_t row = pc.slot + (r - pc.row0);
-            if (g == 0) {
-                a.ml[2 * row] = m_run[qb];
-                a.ml[2 * row + 1] = l_run[qb];
-            }
-#pragma unroll
-            for (int db = 0; db < C::kDB; ++db)
-                if (FULL || 16 * db + 4 * g < dim)
-                    *reinterpret_cast<f32x4*>(a.acc + row * dim + 16 * db + 4 * g) =
-                        o[db][qb] * (1.0f / M::kUp);
-        }
-    } else {
-        // the waves' softmaxes are merged through the staging area
-        constexpr int kRow = D + 4;
-        float* const s_acc = reinterpret_cast<float*>(smem);
-        if (g == 0) {
-            s_ml[wave][0][r16] = m_run[0];
-            s_ml[wave][1][r16] = l_run[0];
-        }
-#pragma unroll
-        for (int db = 0; db < C::kDB; ++db)
-            *reinterpret_cast<f32x4*>(s_acc + (16 * wave + r16) * kRow + 16 * db + 4 * g) = o[db][0];
-        __syncthreads();
-        const int rr = tid >> 4, r = pc.row0 + rr;
-        if (r < pc.rows) {
-            float m = -INFINITY, l = 0.f, f[4];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) m = fmaxf(m, s_ml[w][0][rr]);
-            const float m_use = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                f[w] = __builtin_amdgcn_exp2f(s_ml[w][0][rr] - m_use);
-                l += f[w] * s_ml[w][1][rr];
-            }
-            const size_t row = pc.slot + rr;
-            if ((tid & 15) == 0) {
-                a.ml[2 * row] = m;
-                a.ml[2 * row + 1] = l;
-            }
-#pragma unroll
-            for (int x = 0; x < D / 64; ++x) {
-                const int d = 64 * x + 4 * (tid & 15);
-                f32x4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < 4; ++w)
-                    y += f[w] * *reinterpret_cast<const f32x4*>(s_acc + (16 * w + rr) * kRow + d);
-                if (FULL || d < dim)
-                    *reinterpret_cast<f32x4*>(a.acc + row * dim + d) = y * (1.0f / M::kUp);
-            }
-        }
-        __syncthreads();
-    }
+    for (int qb = 0; qb < QB; ++qb)
+        leave_partials<D, FULL, KEYS>(a, pc, wrow + 16 * qb + r16, m_run[qb], l_run[qb],
+                                      1.0f / M::kUp, smem, s_ml, [&](int x, int& d) {
+                                          d = 16 * x + 4 * g;
+                                          return o[x][qb];
+                                      });
 }
 
 template <typename T, int D, bool FULL>
@@ -623,14 +641,14 @@ void prefix_attn(const PrefixArgs a) {
     p.start = reinterpret_cast<long long*>(smem + 2 * PCfg<D>::kStage);
     p.gran = reinterpret_cast<int*>(p.start + p.entries + 1);
     p.first = p.gran + p.entries;
-    make_plan<true>(a, p, s_sum, s_cnt);
+    make_plan<kHalf>(a, p, s_sum, s_cnt);
     const long long total = uniform64(p.start[p.entries]);
     const long long seg = segment(a, total);
-    if (blockIdx.x == 0) leave_plan<true>(a, p, seg);
+    if (blockIdx.x == 0) leave_plan<kHalf>(a, p, seg);
     long long pos = (long long)blockIdx.x * seg;
     const long long end = min(pos + seg, total);
     while (pos < end) {
-        const Piece pc = piece_at<true>(a, p, pos, end);
+        const Piece pc = piece_at<kHalf>(a, p, pos, end);
         pos = pc.next;
         if (pc.n == 0) continue;
         if (pc.rows <= 16) prefix_piece<T, D, FULL, 1, true>(a, pc, smem, s_ml);
@@ -640,7 +658,198 @@ void prefix_attn(const PrefixArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Every other type, head dim and alignment: 16 rows of a piece against 64
+// float32 on the float32 matrix instructions, dim a multiple of 4 up to D (64 or
+// 128), 16-byte aligned: the same steps of 64 tokens, tiles of 16 rows (KEYS) and
+// of 64, one LDS stage. With v_mfma_f32_16x16x4 (A[r][g], B[g][r], C[4g+i][r]) a
+// lane reads 4 dims at a time, 16 j + 4g .., and its four products take one of
+// them each: any order of dims serves the scores. V is read the same way, dims
+// 64 h + 4r .. of key 4g + i, so product c has dims 64 h + 4 m + c for m = 0..15 and a lane
+// ends with dims 64 h + 16g + 4i + c. Weights are float32, all 24 bits. What
+// bounds it: the matrix cores from 64 rows on (154 TFLOP/s at most), else memory.
+// ---------------------------------------------------------------------------
+template <int D, bool FULL, bool KEYS>
+__device__ __forceinline__ void prefix_piece_f32(const PrefixArgs& a, const Piece& pc, char* smem,
+                                                 float (*s_ml)[2][16]) {
+    constexpr int kPitch = 4 * D + 16, kChunks = D / 16, KB = KEYS ? 1 : 4;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int dim = FULL ? D : a.dim;
+    const float* const kp = (const float*)a.k;
+    const float* const vp = (const float*)a.v;
+    const int wrow = pc.row0 + (KEYS ? 0 : 16 * wave);
+    const bool active = wrow < pc.rows;
+
+    f32x4 qf[kChunks];
+    {
+        const bool on = wrow + r16 < pc.rows;
+        const float* const row = (const float*)a.q + q_row(a, pc, on ? wrow + r16 : pc.row0) * dim;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+            qf[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (on && (FULL || 16 * j + 4 * g < dim))
+                qf[j] = *reinterpret_cast<const f32x4*>(row + 16 * j + 4 * g);
+        }
+    }
+    const int steps = (pc.n + 63) >> 6;
+    // (as prefix_piece)
+    auto entry_of = [&](int st) {
+        return pc.table[a.page.div(pc.t0 + min(64 * st + lane, pc.n - 1))];
+    };
+    auto held_of = [&](int st, int ent) {
+        return __builtin_amdgcn_ballot_w64(64 * st + lane < pc.n &&
+                                           (unsigned)ent < (unsigned)a.blocks);
+    };
+    const int ch = tid % (D / 4);
+    const bool ch_on = FULL || 4 * ch < dim;
+    const size_t col = ch_on ? 4 * ch : 0;
+    f32x4 kx[kChunks], vx[kChunks];
+    auto load = [&](int st, int ent) {
+        ent = (unsigned)ent < (unsigned)a.blocks ? ent : 0;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+            const int row = (tid + 256 * j) / (D / 4);
+            const int e = __shfl(ent, row, 64);
+            const int t = pc.t0 + min(64 * st + row, pc.n - 1);
+            const size_t off =
+                (((size_t)e * a.hkv + pc.kv) * a.page.d + a.page.mod(t)) * dim + col;
+            kx[j] = *reinterpret_cast<const f32x4*>(kp + off);
+            vx[j] = *reinterpret_cast<const f32x4*>(vp + off);
+        }
+    };
+    char* const ks = smem;
+    char* const vs = smem + 64 * kPitch;
+    auto stage = [&](unsigned long long held) {
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+            const int row = (tid + 256 * j) / (D / 4);
+            if (!ch_on || !(held >> row & 1)) kx[j] = vx[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            *reinterpret_cast<f32x4*>(ks + row * kPitch + 16 * ch) = kx[j];
+            *reinterpret_cast<f32x4*>(vs + row * kPitch + 16 * ch) = vx[j];
+        }
+    };
+    f32x4 o[D / 64][4];
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[h][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.f;
+    const float c2 = a.scale_log2;
+    const int k0 = KEYS ? 16 * wave : 0;
+
+    int ent = entry_of(0), next = entry_of(1);
+    load(0, ent);
+    unsigned long long held = held_of(0, ent), held_next = 0;
+    stage(held);
+    __syncthreads();
+    for (int st = 0; st < steps; ++st) {
+        if (st + 1 < steps) {
+            ent = next;
+            next = entry_of(st + 2);
+            load(st + 1, ent);
+            held_next = held_of(st + 1, ent);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead
+        if (active) {
+            f32x4 sc[KB];
+            float top = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                f32x4 part[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) part[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j) {
+                    const f32x4 kf = *reinterpret_cast<const f32x4*>(
+                        ks + (k0 + 16 * kb + r16) * kPitch + (16 * j + 4 * g) * 4);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        part[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c], qf[j][c], part[c], 0,
+                                                                       0, 0);
+                }
+                sc[kb] = (part[0] + part[1]) + (part[2] + part[3]);
+                const unsigned bits = (unsigned)(held >> (k0 + 16 * kb + 4 * g));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!(bits >> i & 1)) sc[kb][i] = -INFINITY;
+                    top = fmaxf(top, sc[kb][i]);
+                }
+            }
+            const float m_new = fmaxf(m_run, max4_rows(top) * c2);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+            m_run = m_new;
+            float sum = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], c2, -m_use));
+                    sum += sc[kb][i];
+                }
+            l_run = l_run * alpha + sum;
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+                for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[h][c] *= alpha;
+            }
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 vf = *reinterpret_cast<const f32x4*>(
+                            vs + (k0 + 16 * kb + 4 * g + i) * kPitch + (64 * h + 4 * r16) * 4);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            o[h][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[c], sc[kb][i],
+                                                                           o[h][c], 0, 0, 0);
+                    }
+        }
+        __syncthreads();
+        if (st + 1 < steps) stage(held_next);
+        held = held_next;
+        __syncthreads();
+    }
+    leave_partials<D, FULL, KEYS>(a, pc, wrow + r16, m_run, l_run, 1.0f, smem, s_ml,
+                                  [&](int x, int& d) {
+                                      d = 64 * (x / 4) + 16 * g + 4 * (x % 4);
+                                      return f32x4{o[x / 4][0][x % 4], o[x / 4][1][x % 4],
+                                                   o[x / 4][2][x % 4], o[x / 4][3][x % 4]};
+                                  });
+}
+
+template <int D, bool FULL>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void prefix_attn_f32(const PrefixArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ float s_ml[4][2][16];
+    __shared__ long long s_sum[4];
+    __shared__ int s_cnt[4];
+    Plan p;
+    p.entries = a.groups + a.batch;
+    p.start = reinterpret_cast<long long*>(smem + 2 * 64 * (4 * D + 16));
+    p.gran = reinterpret_cast<int*>(p.start + p.entries + 1);
+    p.first = p.gran + p.entries;
+    make_plan<kFloat>(a, p, s_sum, s_cnt);
+    const long long total = uniform64(p.start[p.entries]);
+    const long long seg = segment(a, total);
+    if (blockIdx.x == 0) leave_plan<kFloat>(a, p, seg);
+    long long pos = (long long)blockIdx.x * seg;
+    const long long end = min(pos + seg, total);
+    while (pos < end) {
+        const Piece pc = piece_at<kFloat>(a, p, pos, end);
+        pos = pc.next;
+        if (pc.n == 0) continue;
+        if (pc.rows <= 16) prefix_piece_f32<D, FULL, true>(a, pc, smem, s_ml);
+        else prefix_piece_f32<D, FULL, false>(a, pc, smem, s_ml);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Every other head dim and alignment: 16 rows of a piece against 64
 // tokens a step on the vector ALU. Thread (row, x) scores tokens x, x + 16, ..
 // of the step; then threads own 4 dims of a few rows.
 // ---------------------------------------------------------------------------
@@ -658,10 +867,10 @@ __global__ __launch_bounds__(256) void prefix_general(const PrefixArgs a) {
     p.start = reinterpret_cast<long long*>(smem + 64 * (size_t)dim);
     p.gran = reinterpret_cast<int*>(p.start + p.entries + 1);
     p.first = p.gran + p.entries;
-    make_plan<false>(a, p, s_sum, s_cnt);
+    make_plan<kGeneral>(a, p, s_sum, s_cnt);
     const long long total = uniform64(p.start[p.entries]);
     const long long seg = segment(a, total);
-    if (blockIdx.x == 0) leave_plan<false>(a, p, seg);
+    if (blockIdx.x == 0) leave_plan<kGeneral>(a, p, seg);
     const T* const kp = (const T*)a.k;
     const T* const vp = (const T*)a.v;
 
@@ -673,7 +882,7 @@ __global__ __launch_bounds__(256) void prefix_general(const PrefixArgs a) {
     long long pos = (long long)blockIdx.x * seg;
     const long long end = min(pos + seg, total);
     while (pos < end) {
-        const Piece pc = piece_at<false>(a, p, pos, end);
+        const Piece pc = piece_at<kGeneral>(a, p, pos, end);
         pos = pc.next;
         if (pc.n == 0) continue;
         const int rows = min(16, pc.rows - pc.row0);
@@ -800,7 +1009,7 @@ __device__ __forceinline__ long long quotient(long long x, long long d, double i
     return (q + 1) * d <= x ? q + 1 : q;
 }
 
-template <bool WIDE>
+template <Kind KIND>
 __device__ __forceinline__ void find_pieces(const PrefixArgs& a, const Part& x, long long seg,
                                             double inv, int kv, int b, int j, int& n,
                                             size_t& row) {
@@ -808,12 +1017,12 @@ __device__ __forceinline__ void find_pieces(const PrefixArgs& a, const Part& x, 
     row = 0;
     if (x.n == 0) return;
     const int r = (b - x.first) * a.gq + j;
-    const int tr = tile_rows<WIDE>(x.rows);
+    const int tr = tile_rows<KIND>(x.rows);
     const int log = tr == 16 ? 4 : tr == 64 ? 6 : 7, tile = r >> log;
     const int tiles = (x.rows + tr - 1) >> log;
     const long long lo = x.start + ((long long)kv * tiles + tile) * x.whole;
     const long long s0 = quotient(lo, seg, inv);
-    const long long hi = lo + (long long)token_cost<WIDE>(a, x.rows) * (x.n - 1);
+    const long long hi = lo + (long long)token_cost<KIND>(a, x.rows) * (x.n - 1);
     n = (int)(quotient(hi, seg, inv) - s0) + 1;
     const size_t gran = (size_t)kTileGranules * s0 + x.gran +
                         (size_t)kv * ((x.rows + kGranule - 1) / kGranule) +
@@ -821,7 +1030,7 @@ __device__ __forceinline__ void find_pieces(const PrefixArgs& a, const Part& x, 
     row = gran * kGranule + (r - (tile << log));
 }
 
-template <typename T, bool WIDE, int HEADS>
+template <typename T, Kind KIND, int HEADS>
 __global__ __launch_bounds__(256) void prefix_combine(const PrefixArgs a) {
     __shared__ Pieces s_pieces[4];
     __shared__ float s_m[4], s_l[4];
@@ -836,8 +1045,8 @@ __global__ __launch_bounds__(256) void prefix_combine(const PrefixArgs a) {
     if (h < a.hq) {
         const int kv = a.gdiv.div(h), j = h - kv * a.gq;
         const double inv = 1.0 / (double)seg;
-        find_pieces<WIDE>(a, parts.prefix, seg, inv, kv, b, j, mine.n0, mine.row0);
-        find_pieces<WIDE>(a, parts.own, seg, inv, kv, b, j, mine.n1, mine.row1);
+        find_pieces<KIND>(a, parts.prefix, seg, inv, kv, b, j, mine.n0, mine.row0);
+        find_pieces<KIND>(a, parts.own, seg, inv, kv, b, j, mine.n1, mine.row1);
     }
     if (lane == 0) s_pieces[wave] = mine;
     __syncthreads();
@@ -960,19 +1169,20 @@ __global__ __launch_bounds__(256) void prefix_combine(const PrefixArgs a) {
 // host
 // ---------------------------------------------------------------------------
 // The cost of a unit's start (its table, Q and first rows arriving, its partials)
-// and of a token with up to 16, 64 and 128 rows. They balance the workgroups:
+// and of a token with up to 16, 64 and 128 rows (float32: up to 16 and 64, where the
+// matrix cores bound it). They balance the workgroups:
 // with starts free, 16 sequences of 1-500 tokens behind 131071 shared ones took
 // 215 us, a few workgroups being full of starts, for 120; 128 rows are bound by
 // the matrix cores (64 sequences behind 8192: 71 us at 6, 77 at 4 or 8).
 constexpr int kStartCost = 768;
-constexpr int kTokenCost[3] = {4, 4, 6};
+constexpr int kTokenCost[3] = {4, 4, 6}, kTokenCostFloat[3] = {4, 10, 10};
 // The least cost of a segment (4 sequences behind 500 tokens, D = 64: 12.5 us, 14.3
 // at 1024, 17 at 2048).
 constexpr int kMinSegment = 256;
 
 struct PrefixShape {
     int dtype, batch, hq, hkv, groups, page, pwidth, twidth, dim, segs;
-    bool wide;
+    Kind kind;
     size_t ml, acc, parts, seg, bytes;  // offsets in the workspace
 };
 
@@ -994,7 +1204,7 @@ PrefixShape prefix_shape(int dtype, int batch, int hq, int hkv, int groups, int 
         inval("attention: at most 4096 sequences and groups together");
     if ((long long)batch * hq >= 1 << 24) inval("attention problem too large for one launch");
     PrefixShape s{dtype, batch, hq, hkv, groups, page, pwidth, twidth, dim};
-    s.wide = dtype != FT_DT_F32 && dim % 8 == 0 && dim <= 128;
+    s.kind = dim > 128 ? kGeneral : dtype == FT_DT_F32 ? kFloat : dim % 8 == 0 ? kHalf : kGeneral;
     s.segs = 2 * dev_info().cu_count;
     const size_t gq = hq / hkv;
     // granules of every unit (the rows of a group that is not empty are rounded
@@ -1032,30 +1242,48 @@ void wide_run(const PrefixArgs& a, int segs, hipStream_t s) {
     }
 }
 
-template <typename T>
-void prefix_run(const PrefixShape& sh, PrefixArgs a, hipStream_t s) {
-    const size_t lds = 16 * (size_t)sh.dim;
-    bool wide = false;
-    if constexpr (!std::is_same<T, float>::value) {
-        if (sh.wide) {
-            wide = true;
-            if (sh.dim <= 64) wide_run<T, 64>(a, a.segs, s);
-            else wide_run<T, 128>(a, a.segs, s);
-        }
+template <int D>
+void float_run(const PrefixArgs& a, int segs, hipStream_t s) {
+    const size_t lds = 2 * 64 * (4 * D + 16) + Plan::bytes(a.groups + a.batch, a.groups);
+    if (a.dim == D) {
+        allow_lds(prefix_attn_f32<D, true>, lds);
+        prefix_attn_f32<D, true><<<segs, 256, lds, s>>>(a);
+    } else {
+        allow_lds(prefix_attn_f32<D, false>, lds);
+        prefix_attn_f32<D, false><<<segs, 256, lds, s>>>(a);
     }
-    if (!wide)  {
-        const size_t plan = 64 * (size_t)sh.dim + Plan::bytes(sh.groups + sh.batch, sh.groups);
-        allow_lds(prefix_general<T>, plan);
-        prefix_general<T><<<a.segs, 256, plan, s>>>(a);
+}
+
+template <typename T, Kind KIND>
+void combine_run(const PrefixArgs& a, hipStream_t s) {
+    const size_t lds = 16 * (size_t)a.dim;
+    if ((long long)a.batch * a.hq > 4 * dev_info().cu_count)
+        prefix_combine<T, KIND, 4><<<dim3((a.hq + 3) / 4, a.batch), 256, lds, s>>>(a);
+    else
+        prefix_combine<T, KIND, 1><<<dim3(a.hq, a.batch), 256, lds, s>>>(a);
+    launch_check("shared-prefix combine kernel launch");
+}
+
+template <typename T>
+void prefix_run(const PrefixShape& sh, const PrefixArgs& a, hipStream_t s) {
+    constexpr Kind kFast = std::is_same<T, float>::value ? kFloat : kHalf;
+    if (sh.kind == kGeneral) {
+        const size_t lds = 64 * (size_t)sh.dim + Plan::bytes(sh.groups + sh.batch, sh.groups);
+        allow_lds(prefix_general<T>, lds);
+        prefix_general<T><<<a.segs, 256, lds, s>>>(a);
+        launch_check("shared-prefix attention kernel launch");
+        combine_run<T, kGeneral>(a, s);
+        return;
+    }
+    if constexpr (kFast == kFloat) {
+        if (sh.dim <= 64) float_run<64>(a, a.segs, s);
+        else float_run<128>(a, a.segs, s);
+    } else {
+        if (sh.dim <= 64) wide_run<T, 64>(a, a.segs, s);
+        else wide_run<T, 128>(a, a.segs, s);
     }
     launch_check("shared-prefix attention kernel launch");
-    const bool four = (long long)sh.batch * sh.hq > 4 * dev_info().cu_count;
-    const dim3 grid(four ? (sh.hq + 3) / 4 : sh.hq, sh.batch);
-    if (wide && four) prefix_combine<T, true, 4><<<grid, 256, lds, s>>>(a);
-    else if (wide) prefix_combine<T, true, 1><<<grid, 256, lds, s>>>(a);
-    else if (four) prefix_combine<T, false, 4><<<grid, 256, lds, s>>>(a);
-    else prefix_combine<T, false, 1><<<grid, 256, lds, s>>>(a);
-    launch_check("shared-prefix combine kernel launch");
+    combine_run<T, kFast>(a, s);
 }
 
 }  // namespace
@@ -1098,7 +1326,7 @@ int ft_attention_decode_paged_prefix_launch(
             inval("attention: this call needs " + std::to_string(sh.bytes) +
                   " bytes of workspace");
         // whole 16-byte chunks, and a block to read, on the matrix-core path
-        if (blocks == 0 || off(q, 16) || off(k_pool, 16) || off(v_pool, 16)) sh.wide = false;
+        if (blocks == 0 || off(q, 16) || off(k_pool, 16) || off(v_pool, 16)) sh.kind = kGeneral;
         char* const ws = (char*)workspace;
         PrefixArgs a{};
         a.q = q;
@@ -1129,9 +1357,10 @@ int ft_attention_decode_paged_prefix_launch(
         a.segs = sh.segs;
         a.min_seg = kMinSegment;
         a.start_cost = kStartCost;
-        for (int i = 0; i < 3; ++i) a.cost[i] = kTokenCost[i];
+        for (int i = 0; i < 3; ++i)
+            a.cost[i] = sh.kind == kFloat ? kTokenCostFloat[i] : kTokenCost[i];
         // no more workgroups than the tables' capacity can fill
-        const long long gq = a.gq, c = kTokenCost[2];
+        const long long gq = a.gq, c = a.cost[2];
         const long long most =
             kv_heads * ((batch * gq / kGranule + std::min(groups, batch)) *
                             (kStartCost + c * page * prefix_width) +

@@ -104,7 +104,8 @@ def test_pages(page, dtype):
 @pytest.mark.parametrize("b", [1, 2, 4, 5, 16, 17, 32, 33, 40, 70])
 def test_rows_of_a_prefix(b, d):
     """1 to 280 rows a kv head: every kind of tile, whole and not."""
-    Case(b, 8, 2, d, 16, [700], [b], [(7 * i) % 30 for i in range(b)], torch.bfloat16).check()
+    for dtype in (torch.bfloat16, torch.float32):
+        Case(b, 8, 2, d, 16, [700], [b], [(7 * i) % 30 for i in range(b)], dtype).check()
 
 
 @pytest.mark.parametrize("dtype", TYPES)

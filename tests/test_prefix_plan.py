@@ -12,22 +12,24 @@ def up(a, b):
     return -(-a // b)
 
 
-def tile_rows(rows, wide):
-    return 16 if not wide or rows <= 16 else 64 if rows <= 64 else 128
+def tile_rows(rows, kind):
+    return 16 if kind == "general" or rows <= 16 else 64 if kind == "float" or rows <= 64 else 128
 
 
 class Plan:
     START, MIN_SEGMENT = 768, 256
 
     @staticmethod
-    def cost(rows, wide):
-        return 4 if not wide or rows <= 64 else 6
+    def cost(rows, kind):
+        if kind == "general" or rows <= 16:
+            return 4
+        return 10 if kind == "float" else 4 if rows <= 64 else 6
 
     def unit(self, e):
-        return self.START + self.n[e] * self.cost(self.rows[e], self.wide) if self.n[e] else 0
+        return self.START + self.n[e] * self.cost(self.rows[e], self.kind) if self.n[e] else 0
 
-    def __init__(self, offsets, plens, lens, gq, hkv, segs, wide):
-        b, self.wide = len(lens), wide
+    def __init__(self, offsets, plens, lens, gq, hkv, segs, kind):
+        b, self.kind = len(lens), kind
         first = np.maximum.accumulate(np.clip(offsets, 0, b))
         self.first = [int(x) for x in first]
         self.groups = len(plens)
@@ -38,7 +40,7 @@ class Plan:
         self.start, self.gran = [0], [0]
         for e, rows in enumerate(self.rows):
             self.start.append(self.start[-1] +
-                              self.unit(e) * hkv * up(rows, tile_rows(rows, wide)))
+                              self.unit(e) * hkv * up(rows, tile_rows(rows, kind)))
             self.gran.append(self.gran[-1] + hkv * up(rows, 16))
         self.total = self.start[-1]
         self.seg = max(self.MIN_SEGMENT, up(self.total, segs))
@@ -51,7 +53,7 @@ class Plan:
         while pos < end:
             e = int(np.searchsorted(self.start, pos, side="right")) - 1
             off, whole = pos - self.start[e], self.unit(e)
-            tr, w = tile_rows(self.rows[e], self.wide), self.cost(self.rows[e], self.wide)
+            tr, w = tile_rows(self.rows[e], self.kind), self.cost(self.rows[e], self.kind)
             tiles = up(self.rows[e], tr)
             unit, inside = off // whole, off % whole
             kv, tile = unit // tiles, unit % tiles
@@ -70,18 +72,18 @@ class Plan:
             return []
         first = self.first[e] if e < self.groups else e - self.groups
         r = (b - first) * self.gq + j
-        tr = tile_rows(self.rows[e], self.wide)
+        tr = tile_rows(self.rows[e], self.kind)
         tiles, tile = up(self.rows[e], tr), r // tr
         lo = self.start[e] + self.START + (kv * tiles + tile) * self.unit(e)
         s0 = lo // self.seg
-        s1 = (lo + self.cost(self.rows[e], self.wide) * (self.n[e] - 1)) // self.seg
+        s1 = (lo + self.cost(self.rows[e], self.kind) * (self.n[e] - 1)) // self.seg
         gran = 8 * s0 + self.gran[e] + kv * up(self.rows[e], 16) + tile * (tr // 16)
         return [16 * gran + r - tile * tr + 128 * i for i in range(s1 - s0 + 1)]
 
 
-@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("kind", ["half", "float", "general"])
 @pytest.mark.parametrize("seed", range(40))
-def test_pieces_and_partials(seed, wide):
+def test_pieces_and_partials(seed, kind):
     r = random.Random(seed)
     b, groups = r.randint(1, 40), r.choice([0, 1, 2, 7])
     gq, hkv, segs = r.choice([1, 3, 4, 8, 16, 33, 64]), r.choice([1, 2, 8]), r.choice([1, 16, 512])
@@ -91,7 +93,7 @@ def test_pieces_and_partials(seed, wide):
         offsets = sorted(r.randint(0, b) for _ in range(groups + 1))
     plens = [r.choice([0, 1, 63, 64, 1000, 5000]) for _ in range(groups)]
     lens = [r.choice([0, 0, 1, 64, 129, 700]) for _ in range(b)]
-    p = Plan(offsets if groups else [0], plens, lens, gq, hkv, segs, wide)
+    p = Plan(offsets if groups else [0], plens, lens, gq, hkv, segs, kind)
     assert p.seg * segs >= p.total
 
     seen, left = {}, {}
@@ -103,10 +105,10 @@ def test_pieces_and_partials(seed, wide):
             assert not taken[row:row + rows].any()
             taken[row:row + rows] = True
             for i in range(rows):
-                left.setdefault((e, kv, tile * tile_rows(p.rows[e], wide) + i), []).append(row + i)
+                left.setdefault((e, kv, tile * tile_rows(p.rows[e], kind) + i), []).append(row + i)
     for e, (rows, n) in enumerate(zip(p.rows, p.n)):
         for kv in range(hkv):
-            for tile in range(up(rows, tile_rows(rows, wide))):
+            for tile in range(up(rows, tile_rows(rows, kind))):
                 at = 0
                 for t0, m in seen.get((e, kv, tile), []):   # in order, without a gap
                     assert t0 == at

@@ -1188,8 +1188,8 @@ struct PrefixShape {
 
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-PrefixShape prefix_shape(int dtype, int batch, int hq, int hkv, int groups, int page, int pwidth,
-                         int twidth, int dim) {
+void check_shape(int dtype, int batch, int hq, int hkv, int groups, int page, int pwidth,
+                 int twidth, int dim) {
     if (dtype != FT_DT_F32 && dtype != FT_DT_BF16 && dtype != FT_DT_F16)
         inval("attention: unknown element type");
     if (batch < 0 || groups < 0 || hq < 1 || hkv < 1 || pwidth < 0 || twidth < 0)
@@ -1203,6 +1203,10 @@ PrefixShape prefix_shape(int dtype, int batch, int hq, int hkv, int groups, int 
     if ((long long)batch + groups > kMaxEntries)
         inval("attention: at most 4096 sequences and groups together");
     if ((long long)batch * hq >= 1 << 24) inval("attention problem too large for one launch");
+}
+
+PrefixShape prefix_shape(int dtype, int batch, int hq, int hkv, int groups, int page, int pwidth,
+                         int twidth, int dim) {
     PrefixShape s{dtype, batch, hq, hkv, groups, page, pwidth, twidth, dim};
     s.kind = dim > 128 ? kGeneral : dtype == FT_DT_F32 ? kFloat : dim % 8 == 0 ? kHalf : kGeneral;
     s.segs = 2 * dev_info().cu_count;
@@ -1298,6 +1302,7 @@ int ft_attention_decode_paged_prefix_workspace(int dtype, int batch, int q_heads
                                                int tbl_width, int dim, long long* bytes) {
     return guarded([&] {
         if (!bytes) inval("attention: null operand");
+        check_shape(dtype, batch, q_heads, kv_heads, groups, page, prefix_width, tbl_width, dim);
         *bytes = (long long)prefix_shape(dtype, batch, q_heads, kv_heads, groups, page,
                                          prefix_width, tbl_width, dim).bytes;
     });
@@ -1309,8 +1314,7 @@ int ft_attention_decode_paged_prefix_launch(
     void* workspace, long long workspace_bytes, int batch, int q_heads, int kv_heads, int groups,
     int blocks, int page, int prefix_width, int tbl_width, int dim, uintptr_t stream) {
     return guarded([&] {
-        PrefixShape sh = prefix_shape(dtype, batch, q_heads, kv_heads, groups, page, prefix_width,
-                                      tbl_width, dim);
+        check_shape(dtype, batch, q_heads, kv_heads, groups, page, prefix_width, tbl_width, dim);
         if (blocks < 0) inval("attention: blocks must be >= 0");
         if (groups > 1 && !group_offsets) inval("attention: several groups need group_offsets");
         if (batch == 0) return;
@@ -1322,6 +1326,8 @@ int ft_attention_decode_paged_prefix_launch(
         if (off(q, by) || off(k_pool, by) || off(v_pool, by) || off(out, by))
             inval("attention: operands must be aligned to 4 elements");
         if (off(workspace, 16)) inval("attention: the workspace must be aligned to 16 bytes");
+        PrefixShape sh = prefix_shape(dtype, batch, q_heads, kv_heads, groups, page, prefix_width,
+                                      tbl_width, dim);
         if (!workspace || workspace_bytes < (long long)sh.bytes)
             inval("attention: this call needs " + std::to_string(sh.bytes) +
                   " bytes of workspace");

@@ -1717,7 +1717,7 @@ def _row_values(v, name, dtype, rows, device):
     """A parameter as (pointer or None, number): a GPU vector with an entry
     for each row, or one number for all."""
     if not torch.is_tensor(v):
-        if dtype is _TI and v != int(v):
+        if dtype is _TI and not float(v).is_integer():
             raise TypeError(f"{name} must be an integer")
         return None, int(v) if dtype is _TI else float(v)
     if not v.is_cuda:

@@ -91,6 +91,10 @@ const DevInfo& dev_info();
 // True if `s` is being captured into a HIP graph.
 bool stream_capturing(hipStream_t s);
 
+// Lets a kernel be launched with that many bytes of dynamic LDS on the current
+// device (more than 64 KiB has to be asked for, once).
+void allow_lds(const void* kernel, size_t bytes);
+
 // Tuning and test switches. Each is read once per process, on first use,
 // from the environment variable of the same name, and can be overridden at
 // run time through ft_set_tuning() / ft_clear_tuning() (tests, sweeps). The

@@ -231,7 +231,8 @@ __device__ __forceinline__ Piece piece_at(const PrefixArgs& a, const Plan& p, lo
     const long long in = off - unit * whole, base = pos - in;
     const long long stop = min(whole, end - base);
     auto token = [&](long long c) {
-        return c <= a.start_cost ? 0 : (int)((unsigned)(c - a.start_cost + w - 1) / (unsigned)w);
+        // (below 2^34: the float64 quotient's floor is exact)
+        return c <= a.start_cost ? 0 : (int)((double)(c - a.start_cost + w - 1) / (double)w);
     };
     x.t0 = token(in);
     x.n = token(stop) - x.t0;
@@ -1226,22 +1227,14 @@ PrefixShape prefix_shape(int dtype, int batch, int hq, int hkv, int groups, int 
     return s;
 }
 
-template <typename K>
-void allow_lds(K kernel, size_t bytes) {
-    if (bytes > 65536)
-        hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
-                  "hipFuncSetAttribute");
-}
-
 template <typename T, int D>
 void wide_run(const PrefixArgs& a, int segs, hipStream_t s) {
     const size_t lds = 2 * PCfg<D>::kStage + Plan::bytes(a.groups + a.batch, a.groups);
     if (a.dim == D) {
-        allow_lds(prefix_attn<T, D, true>, lds);
+        allow_lds((const void*)prefix_attn<T, D, true>, lds);
         prefix_attn<T, D, true><<<segs, 256, lds, s>>>(a);
     } else {
-        allow_lds(prefix_attn<T, D, false>, lds);
+        allow_lds((const void*)prefix_attn<T, D, false>, lds);
         prefix_attn<T, D, false><<<segs, 256, lds, s>>>(a);
     }
 }
@@ -1250,10 +1243,10 @@ template <int D>
 void float_run(const PrefixArgs& a, int segs, hipStream_t s) {
     const size_t lds = 2 * 64 * (4 * D + 16) + Plan::bytes(a.groups + a.batch, a.groups);
     if (a.dim == D) {
-        allow_lds(prefix_attn_f32<D, true>, lds);
+        allow_lds((const void*)prefix_attn_f32<D, true>, lds);
         prefix_attn_f32<D, true><<<segs, 256, lds, s>>>(a);
     } else {
-        allow_lds(prefix_attn_f32<D, false>, lds);
+        allow_lds((const void*)prefix_attn_f32<D, false>, lds);
         prefix_attn_f32<D, false><<<segs, 256, lds, s>>>(a);
     }
 }
@@ -1273,7 +1266,7 @@ void prefix_run(const PrefixShape& sh, const PrefixArgs& a, hipStream_t s) {
     constexpr Kind kFast = std::is_same<T, float>::value ? kFloat : kHalf;
     if (sh.kind == kGeneral) {
         const size_t lds = 64 * (size_t)sh.dim + Plan::bytes(sh.groups + sh.batch, sh.groups);
-        allow_lds(prefix_general<T>, lds);
+        allow_lds((const void*)prefix_general<T>, lds);
         prefix_general<T><<<a.segs, 256, lds, s>>>(a);
         launch_check("shared-prefix attention kernel launch");
         combine_run<T, kGeneral>(a, s);

@@ -267,6 +267,8 @@ void qk_run(QkArgs<T> a, bool neox, hipStream_t s) {
     if (a.tokens < 4 * cus) a.heads = std::min(all, step);
     const dim3 grid((a.tokens + a.tt - 1) / a.tt, (all + a.heads - 1) / a.heads);
     if (grid.y > 65535) inval("qk_norm_rope: too many heads");
+    // (a launch has fewer than 2^32 threads)
+    if ((long long)grid.x * 256 >= 1LL << 32) inval("qk_norm_rope: too many tokens for one call");
     const size_t lds = 8 * kMaxTok + (size_t)a.tt * rp * sizeof(float2);
     if (neox && vec) qk_norm_rope_kernel<T, true, true><<<grid, 256, lds, s>>>(a);
     else if (neox) qk_norm_rope_kernel<T, true, false><<<grid, 256, lds, s>>>(a);

@@ -118,6 +118,18 @@ int tune(Tune which, int dflt) {
                                                      : dflt;
 }
 
+void allow_lds(const void* kernel, size_t bytes) {
+    if (bytes <= 65536) return;
+    static std::mutex mutex;
+    static std::map<std::pair<const void*, int>, size_t> allowed;
+    const std::lock_guard<std::mutex> lock(mutex);
+    size_t& most = allowed[{kernel, current_device()}];
+    if (bytes <= most) return;
+    hip_check(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
+              "hipFuncSetAttribute");
+    most = bytes;
+}
+
 bool stream_capturing(hipStream_t s) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     hip_check(hipStreamIsCapturing(s, &status), "hipStreamIsCapturing");

@@ -1056,10 +1056,14 @@ SampleShape sample_shape(int rows, int n) {
     if (n < 1) inval("sample of empty logits");
     if (n > kMaxVocab) inval("sample_filtered_batched: at most 2^22 logits a row");
     SampleShape s{};
+    // (a launch has fewer than 2^32 threads)
+    if ((long long)rows * kRowNT >= 1LL << 32)
+        inval("sample_filtered_batched: too many rows for one call");
     if (n <= kRowMost || rows == 0) return s;
     s.slices = (n + kSlice - 1) / kSlice;
     const size_t parts = (size_t)rows * s.slices;
-    if (parts > INT_MAX) inval("sample_filtered_batched: too many rows for one call");
+    if (parts * kSliceNT >= 1ULL << 32)
+        inval("sample_filtered_batched: too many rows for one call");
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t p = at;
@@ -1080,18 +1084,10 @@ SampleShape sample_shape(int rows, int n) {
 
 constexpr size_t kStateBytes = (sizeof(RowState) + 15) & ~(size_t)15;
 
-template <typename K>
-void allow_lds(K kernel, size_t bytes) {
-    if (bytes > 65536)
-        hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
-                  "hipFuncSetAttribute");
-}
-
 template <typename T, int MOST>
 void row_run(const SampleArgs& a, hipStream_t s) {
     const size_t lds = kStateBytes + (size_t)(a.n + kChunk - 1) / kChunk * kChunk * 4;
-    allow_lds(sample_row<T, MOST>, lds);
+    allow_lds((const void*)sample_row<T, MOST>, lds);
     sample_row<T, MOST><<<a.rows, kRowNT, lds, s>>>(a);
 }
 
@@ -1109,7 +1105,7 @@ void sample_run(const SampleArgs& a, hipStream_t s) {
     slice_hist<T><<<grid, kSliceNT, 0, s>>>(a);
     slice_list<T><<<grid, kSliceNT, 0, s>>>(a);
     const size_t lds = kStateBytes + 4 * (size_t)kListMost;
-    allow_lds(sample_pick<T>, lds);
+    allow_lds((const void*)sample_pick<T>, lds);
     sample_pick<T><<<a.rows, kRowNT, lds, s>>>(a);
     launch_check("sample_filtered_batched kernel launch");
 }

@@ -52,6 +52,8 @@ constexpr int kRowNT = 512;
 constexpr int kRowMost = 32768;      // tokens of a row that one workgroup holds
 constexpr int kMaxVocab = 1 << 22;   // 512 slices; sums of weights below 2^62
 constexpr int kMinBins = 3;
+constexpr int kGroups = 16;          // parts of a slice
+constexpr int kFloorOf = 256;        // parts of a row whose largest logits give its floor
 constexpr int kLevel = kRowNT;         // bins of a histogram over order bits
 
 struct SampleArgs {
@@ -69,6 +71,8 @@ struct SampleArgs {
     // workspace of the sliced form
     float* top;        // [rows][slices]
     int* top_at;       // [rows][slices]
+    float* groups;     // [rows][slices][kGroups]: the largest of each part of a slice
+    float* floors;     // [rows]: below it none of the first k
     u64* sum;          // [rows][slices]: kept weights above the listed bins
     u64* part;         // [rows][slices][kBins]: the slices' histograms
     unsigned* listed;  // [rows][slices]
@@ -234,6 +238,25 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* s, u64& total) {
     return before;
 }
 
+// A bound that the k-th largest logit is not below: of kFloorOf parts' largest
+// ones, 4 a lane (`parts` of them: the rest is -inf), the k-th, to 16 bits of
+// its order bits. -inf where there are fewer than k. What lies below is none
+// of the first k: neither the histogram nor the list needs it.
+__device__ __forceinline__ float floor_of(float4 g, int k, int parts) {
+    if (k <= 0 || k > parts) return -INFINITY;
+    const unsigned o[4] = {order_bits(g.x), order_bits(g.y), order_bits(g.z), order_bits(g.w)};
+    unsigned at = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+        const unsigned next = at | 1u << bit;
+        int many = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) many += __popcll(__builtin_amdgcn_ballot_w64(o[i] >= next));
+        if (many >= k) at = next;
+    }
+    return at > order_bits(-INFINITY) ? from_bits(at) : -INFINITY;
+}
+
 // A thread's tokens: 4 in a row of every 4 NT, from `first` on, x = -inf
 // where there is none. NaN becomes -inf.
 template <typename T, int NT, int TPT>
@@ -259,14 +282,20 @@ __device__ __forceinline__ void load_tokens(const T* row, int first, int end, fl
         if (!(x[j] >= -INFINITY)) x[j] = -INFINITY;
 }
 
-// The largest of the workgroup's tokens and its first index. s: 2 words a wave.
+// The largest of the workgroup's tokens and its first index, and of each 16
+// threads. s: 2 words a wave.
 template <int NT, int TPT>
 __device__ __forceinline__ float block_top(const float (&x)[TPT], int first, float* s, int* s_at,
-                                           int& at) {
+                                           float* groups, int& at) {
+    static_assert(NT == 16 * kGroups, "parts of 16 threads");
     float m = x[0];
 #pragma unroll
     for (int j = 1; j < TPT; ++j) m = fmaxf(m, x[j]);
-    m = wave_max(m);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 15) == 0) groups[threadIdx.x >> 4] = m;
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     int i = INT_MAX;
 #pragma unroll
     for (int j = TPT - 1; j >= 0; --j)
@@ -300,7 +329,7 @@ struct RowState {
     double powers[kPowers];
     // the histogram, bins from the largest values on; then (scan_bins) the sums
     // before each bin
-    u64 mass[kBins];
+    u64 mass[kBins + 1];
     unsigned count[kBins + 1];
     u64 level_mass[kLevel];
     unsigned level_count[kLevel];
@@ -315,12 +344,13 @@ struct RowState {
     int bin, entry, slice;
     float top[kWaves];
     int top_at[kWaves];
+    __attribute__((aligned(16))) float parts[kFloorOf];
 };
 
 // The tokens [first, end) of a row into s_x, up to a whole chunk (-inf behind
 // the end; NaN becomes -inf), at most MOST of them. Returns their largest and,
-// in `at`, its first index.
-template <typename T, int MOST>
+// in `at`, its first index; PARTS: and leaves the parts' largest.
+template <typename T, int MOST, bool PARTS>
 __device__ __forceinline__ float stage_tokens(const T* row, int first, int end, float* s_x,
                                               RowState& s, int& at) {
     float x[MOST / kRowNT];
@@ -338,6 +368,13 @@ __device__ __forceinline__ float stage_tokens(const T* row, int first, int end, 
             if (x[4 * j + e] > m) m = x[4 * j + e], at = first + i + e;
     }
     const float mine = m;
+    if (PARTS) {
+        constexpr int LANES = kRowNT / kFloorOf;
+        float part = m;
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) part = fmaxf(part, __shfl_xor(part, o, 64));
+        if (threadIdx.x % LANES == 0) s.parts[threadIdx.x / LANES] = part;
+    }
     m = wave_max(m);
     if (mine != m) at = INT_MAX;
 #pragma unroll
@@ -376,7 +413,7 @@ __device__ __forceinline__ u64 scan_bins(RowState& s) {
         mb += m[i];
         cb += c[i];
     }
-    if (threadIdx.x == 0) s.count[kBins] = (unsigned)tokens;
+    if (threadIdx.x == 0) s.mass[kBins] = total, s.count[kBins] = (unsigned)tokens;
     __syncthreads();
     return total;
 }
@@ -389,22 +426,25 @@ struct Limit {
     __device__ __forceinline__ bool open(u64 mass, u64 count) const {
         return by_count ? count < k : (double)mass < want;
     }
+    // open before a bin and not behind it: one bin, as both sums rise
+    __device__ __forceinline__ bool closes(u64 mass, u64 count, u64 mass1, u64 count1) const {
+        return open(mass, count) && !open(mass1, count1);
+    }
 };
 
-// The last bin that is not empty before which the limit is open; 0 if there is
-// none.
+// The bin in which the limit is reached; 0 for one that asks for nothing.
 __device__ __forceinline__ int limit_bin(const Limit& l, RowState& s) {
     if (threadIdx.x == 0) s.bin = 0;
     __syncthreads();
     for (int b = threadIdx.x; b < kBins; b += kRowNT)
-        if (s.count[b + 1] > s.count[b] && l.open(s.mass[b], s.count[b])) atomicMax(&s.bin, b);
+        if (l.closes(s.mass[b], s.count[b], s.mass[b + 1], s.count[b + 1])) s.bin = b;
     __syncthreads();
     return s.bin;
 }
 
 // The one value at which the limit is reached, among the n order bits that
-// `each` visits (each(f) calls f(bits, is one) in every thread), with mass0
-// and count0 before them, all in [lo, hi]. Few are compared all with all, 8
+// `each` visits (each(f) calls f(bits, one) in every thread, one() telling
+// whether they are of them), with mass0 and count0 before them, all in [lo, hi]. Few are compared all with all, 8
 // threads each; more are narrowed down by histograms, 512 wide, first.
 template <typename Each>
 __device__ __forceinline__ Group resolve(const Row& row, const Limit& l, unsigned n, u64 mass0,
@@ -417,8 +457,8 @@ __device__ __forceinline__ Group resolve(const Row& row, const Limit& l, unsigne
         s.level_count[threadIdx.x] = 0;
         if (threadIdx.x == 0) s.bin = 0;
         __syncthreads();
-        each([&](unsigned o, bool on) {
-            if (!on || o > hi || o < lo) return;
+        each([&](unsigned o, auto&& one) {
+            if (o > hi || o < lo || !one()) return;
             const unsigned b = (hi - o) >> shift;
             atomicAdd(&s.level_mass[b], row.weight_of(from_bits(o)));
             atomicAdd(&s.level_count[b], 1u);
@@ -426,9 +466,10 @@ __device__ __forceinline__ Group resolve(const Row& row, const Limit& l, unsigne
         __syncthreads();
         const unsigned c = s.level_count[threadIdx.x];
         u64 total;
-        const u64 mb = mass0 + block_scan<kRowNT>(s.level_mass[threadIdx.x], s.scan, total);
+        const u64 m = s.level_mass[threadIdx.x];
+        const u64 mb = mass0 + block_scan<kRowNT>(m, s.scan, total);
         const u64 cb = count0 + block_scan<kRowNT>(c, s.scan2, total);
-        if (c && l.open(mb, cb)) atomicMax(&s.bin, threadIdx.x);
+        if (l.closes(mb, cb, mb + m, cb + c)) s.bin = threadIdx.x;
         __syncthreads();
         const int bin = s.bin;
         if (threadIdx.x == bin) s.before_mass = mb, s.before_count = (unsigned)cb, s.few = c;
@@ -442,12 +483,13 @@ __device__ __forceinline__ Group resolve(const Row& row, const Limit& l, unsigne
     }
     if (threadIdx.x == 0) s.few = 0, s.best = 0;
     __syncthreads();
-    each([&](unsigned o, bool on) {
-        if (!on || o > hi || o < lo) return;
-        const unsigned i = atomicAdd(&s.few, 1u);
-        s.few_key[i] = o;
-        s.few_w[i] = row.weight_of(from_bits(o));
+    each([&](unsigned o, auto&& one) {
+        if (o > hi || o < lo || !one()) return;
+        s.few_key[atomicAdd(&s.few, 1u)] = o;
     });
+    __syncthreads();
+    // (weights after: a wave goes through a loop's body for each lane's find)
+    if (threadIdx.x < n) s.few_w[threadIdx.x] = row.weight_of(from_bits(s.few_key[threadIdx.x]));
     __syncthreads();
     const unsigned mine = threadIdx.x >> 3;
     const unsigned key = mine < n ? s.few_key[mine] : 0;
@@ -500,8 +542,8 @@ template <typename Each>
 __device__ __forceinline__ Cut find_cut(const Row& row, u64 total, RowState& s, Each&& each) {
     Cut cut{-INFINITY, 0, 0};
     u64 sum = total;
-    // (a k that all weights but zeros come up to cuts nothing)
-    const bool by_k = row.k > 0 && (unsigned)row.k < s.count[kBins];
+    // (a k beyond all weights that are not 0 cuts nothing)
+    const bool by_k = row.k > 0 && (unsigned)row.k <= s.count[kBins];
     for (int pass = by_k ? 0 : 1; pass < (row.p < 1.0f ? 2 : 1); ++pass) {
         const Limit l{pass == 0, (u64)row.k, (double)row.p * (double)sum};
         const int bin = limit_bin(l, s);
@@ -542,6 +584,11 @@ __device__ __forceinline__ void pick(const Row& row, const Cut& cut, const float
     // sums of every 256 tokens in a row: (chunk j, wave)
     for (int j = 0; j < chunks; ++j) {
         const float4 x = *reinterpret_cast<const float4*>(s_x + 4 * (j * kRowNT + threadIdx.x));
+        const float most = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
+        if (!__builtin_amdgcn_ballot_w64(most >= cut.xc)) {  // nothing is kept here
+            if (lane == 0) s.chunk_mass[j * kWaves + wave] = 0, s.chunk_ties[j * kWaves + wave] = 0;
+            continue;
+        }
         u64 m = kept(x.x) + kept(x.y) + kept(x.z) + kept(x.w);
         unsigned t = tie(x.x) + tie(x.y) + tie(x.z) + tie(x.w);
         if (__builtin_amdgcn_ballot_w64(m | t)) {
@@ -639,7 +686,7 @@ __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
     for (int b = threadIdx.x; b < kBins; b += kRowNT) s.mass[b] = 0, s.count[b] = 0;
     fill_powers(s.powers);
     int at;
-    const float top = stage_tokens<T, MOST>((const T*)a.x + (long long)r * a.ld, 0, a.n, s_x, s, at);
+    const float top = stage_tokens<T, MOST, true>((const T*)a.x + (long long)r * a.ld, 0, a.n, s_x, s, at);
     const Row row(a, r, top, s.powers);
     if (row.greedy || top == -INFINITY) {
         if (threadIdx.x == 0) a.out[r] = top == -INFINITY ? -1 : at;
@@ -648,11 +695,15 @@ __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
     const int chunks = (a.n + kChunk - 1) / kChunk;
     Cut cut{-INFINITY, 0, 0};
     if (row.cut()) {
+        const float floor =
+            floor_of(*reinterpret_cast<const float4*>(s.parts + 4 * (threadIdx.x & 63)), row.k,
+                     kFloorOf);
         for (int j = 0; j < chunks; ++j) {
             const float4 x = *reinterpret_cast<const float4*>(s_x + 4 * (j * kRowNT + threadIdx.x));
             const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
+                if (v[e] < floor) continue;
                 const double t = row.far(v[e]);
                 const int b = bin_of(t);
                 if (b >= kBins) continue;
@@ -664,14 +715,23 @@ __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
         const u64 total = scan_bins(s);
         cut = find_cut(row, total, s, [&](auto&& f, int bin) {
             const float2 about = row.around(bin);
+            const float least = fmaxf(about.x, floor);  // (of a NaN: the other)
+            const float* const x0 = s_x + 4 * threadIdx.x;
+            u64 some = 0;  // the thread's tokens about the bin
+#pragma unroll 4
             for (int j = 0; j < chunks; ++j) {
-                const float4 x =
-                    *reinterpret_cast<const float4*>(s_x + 4 * (j * kRowNT + threadIdx.x));
+                const float4 x = *reinterpret_cast<const float4*>(x0 + j * kChunk);
                 const float v[4] = {x.x, x.y, x.z, x.w};
+                unsigned in = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (!(v[e] < about.x) && !(v[e] > about.y))
-                        f(order_bits(v[e]), bin_of(row.far(v[e])) == bin);
+                    in |= !(v[e] < least) && !(v[e] > about.y) ? 1u << e : 0;
+                some |= (u64)in << (4 * j);
+            }
+            for (; some; some &= some - 1) {
+                const int j = __ffsll(some) - 1;
+                const float v = x0[(j >> 2) * kChunk + (j & 3)];
+                f(order_bits(v), [&] { return bin_of(row.far(v)) == bin; });
             }
         });
     }
@@ -686,10 +746,10 @@ constexpr int kSliceTPT = kSlice / kSliceNT;
 // f(token, its place j) for a thread's tokens of a slice, with the loads of the next
 // ones under way (all loads first left every workgroup of a CU loading and
 // then computing at the same time).
-template <typename T>
+template <typename T, int AHEAD = 4>
 struct Tokens {
     typedef T v4 __attribute__((ext_vector_type(4)));
-    static constexpr int kSteps = kSliceTPT / 4, kAhead = 4;
+    static constexpr int kSteps = kSliceTPT / 4, kAhead = AHEAD;
     const T* row;
     int lo, hi;
     bool vec;
@@ -742,7 +802,8 @@ __global__ __launch_bounds__(kSliceNT) void slice_max(const SampleArgs a) {
         a.count[(size_t)r * kBins + b] = 0;
     }
     int at;
-    const float top = block_top<kSliceNT, kSliceTPT>(x, lo, s_top, s_at, at);
+    const float top = block_top<kSliceNT, kSliceTPT>(
+        x, lo, s_top, s_at, a.groups + (size_t)blockIdx.x * kGroups, at);
     if (threadIdx.x == 0) {
         a.top[blockIdx.x] = top;
         a.top_at[blockIdx.x] = at;
@@ -770,6 +831,11 @@ __global__ __launch_bounds__(kSliceNT) void slice_hist(const SampleArgs a) {
     const int r = blockIdx.x / a.slices, s = blockIdx.x - r * a.slices;
     const int lo = s * kSlice, hi = min(lo + kSlice, a.n);
     const float some = slice_top(a, r);
+    const int parts = min(a.slices * kGroups, kFloorOf);
+    float4 of_parts = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (4 * (int)(threadIdx.x & 63) < parts)
+        of_parts = *reinterpret_cast<const float4*>(a.groups + (size_t)r * a.slices * kGroups +
+                                                    4 * (threadIdx.x & 63));
     Tokens<T> tokens(a, r, lo, hi);
     fill_powers(s_powers);
     for (int b = threadIdx.x; b < kBins; b += kSliceNT) s_mass[b] = 0, s_count[b] = 0;
@@ -789,7 +855,10 @@ __global__ __launch_bounds__(kSliceNT) void slice_hist(const SampleArgs a) {
         if (threadIdx.x == 0) a.sum[blockIdx.x] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
         return;
     }
+    const float floor = floor_of(of_parts, row.k, parts);
+    if (s == 0 && threadIdx.x == 0) a.floors[r] = floor;
     tokens.each([&](float x, int) {
+        if (x < floor) return;
         const double t = row.far(x);
         const int b = bin_of(t);
         if (b >= kBins) return;
@@ -840,12 +909,12 @@ __device__ __forceinline__ Span cut_span(const Row& row, const BinRun& h, u64* s
     u64 cb = block_scan<kSliceNT>(many, s_scan2, tokens);
     __shared__ u64 s_w[2];
     if (threadIdx.x == 0) s_w[0] = s_w[1] = total;
-    const bool by_k = row.k > 0 && (u64)row.k < tokens;
+    const bool by_k = row.k > 0 && (u64)row.k <= tokens;
     if (by_k) {
         u64 q = cb;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            if (c[i] && q < (u64)row.k) atomicMax(&s_bin[2], threadIdx.x * PER + i);
+            if (q < (u64)row.k && q + c[i] >= (u64)row.k) s_bin[2] = threadIdx.x * PER + i;
             q += c[i];
         }
     }
@@ -863,9 +932,10 @@ __device__ __forceinline__ Span cut_span(const Row& row, const BinRun& h, u64* s
         const double w0 = (double)row.p * (double)s_w[0], w1 = (double)row.p * (double)s_w[1];
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            if (c[i] && (double)mb < w0) atomicMax(&s_bin[0], threadIdx.x * PER + i);
-            if (c[i] && (double)mb < w1) atomicMax(&s_bin[1], threadIdx.x * PER + i);
-            mb += m[i];
+            const u64 next = mb + m[i];
+            if ((double)mb < w0 && !((double)next < w0)) s_bin[0] = threadIdx.x * PER + i;
+            if ((double)mb < w1 && !((double)next < w1)) s_bin[1] = threadIdx.x * PER + i;
+            mb = next;
         }
     }
     __syncthreads();
@@ -886,8 +956,7 @@ __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
     const int r = blockIdx.x / a.slices, s = blockIdx.x - r * a.slices;
     const int lo = s * kSlice, hi = min(lo + kSlice, a.n);
     __shared__ float s_near[kSlice];
-    const float some = slice_top(a, r);
-    Tokens<T> tokens(a, r, lo, hi);
+    const float some = slice_top(a, r), floor = a.floors[r];
     BinRun bins;
     bins.load(a, r);
     u64 own[BinRun::PER];  // the slice's
@@ -896,6 +965,8 @@ __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
         const int b = threadIdx.x + i * kSliceNT;
         own[i] = b < kBins ? a.part[(size_t)blockIdx.x * kBins + b] : 0;
     }
+    // (on their way while the bins are searched)
+    Tokens<T, kSliceTPT / 4> tokens(a, r, lo, hi);
     const float top = row_top(a, r, some);
     const Row row(a, r, top, nullptr);
     if (row.greedy || top == -INFINITY || !row.cut()) return;
@@ -911,7 +982,7 @@ __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
         if ((int)threadIdx.x + i * kSliceNT < all) sum += own[i];
     unsigned* const list = a.list + (size_t)r * a.n + lo;
     // logits outside the listed bins are seen without their float64 distance
-    const float least = row.around(min(max(span.hi, span.at_k), kBins - 1)).x;
+    const float least = fmaxf(row.around(min(max(span.hi, span.at_k), kBins - 1)).x, floor);
     const float most = row.around(min(all, kBins - 1)).y;
     unsigned some_of = 0;  // the thread's tokens that may be listed
     tokens.each([&](float x, int j) {
@@ -998,10 +1069,14 @@ __global__ __launch_bounds__(kRowNT) void sample_pick(const SampleArgs a) {
         const u64 total = scan_bins(s);  // (synchronises)
         cut = find_cut(row, total, s, [&](auto&& f, int bin) {
             if (held)
-                for (unsigned i = b; i < (unsigned)all; i += kRowNT)
-                    f(s_list[i], bin_of(row.far(from_bits(s_list[i]))) == bin);
+                for (unsigned i = b; i < (unsigned)all; i += kRowNT) {
+                    const unsigned o = s_list[i];
+                    f(o, [&] { return bin_of(row.far(from_bits(o))) == bin; });
+                }
             else
-                slices([&](unsigned o) { f(o, bin_of(row.far(from_bits(o))) == bin); });
+                slices([&](unsigned o) {
+                    f(o, [&] { return bin_of(row.far(from_bits(o))) == bin; });
+                });
         });
         for (int t = wave; t < a.slices; t += kWaves) {
             u64 sum = 0;
@@ -1039,7 +1114,7 @@ __global__ __launch_bounds__(kRowNT) void sample_pick(const SampleArgs a) {
     const u64 base = s.base, q = s.q;
     float* const s_x = reinterpret_cast<float*>(s_list);
     int at;
-    stage_tokens<T, kSlice>((const T*)a.x + (long long)r * a.ld, lo, hi, s_x, s, at);
+    stage_tokens<T, kSlice, false>((const T*)a.x + (long long)r * a.ld, lo, hi, s_x, s, at);
     pick(row, cut, s_x, hi - lo, lo, q, aim - base, 0.f, s, a.out + r);
 }
 
@@ -1048,7 +1123,7 @@ __global__ __launch_bounds__(kRowNT) void sample_pick(const SampleArgs a) {
 // ---------------------------------------------------------------------------
 struct SampleShape {
     int slices;  // 0: a workgroup a row
-    size_t top, top_at, sum, part, listed, mass, count, list, bytes;
+    size_t top, top_at, groups, floors, sum, part, listed, mass, count, list, bytes;
 };
 
 SampleShape sample_shape(int rows, int n) {
@@ -1072,6 +1147,8 @@ SampleShape sample_shape(int rows, int n) {
     };
     s.top = take(4 * parts);
     s.top_at = take(4 * parts);
+    s.groups = take(4 * parts * kGroups);
+    s.floors = take(4 * (size_t)rows);
     s.sum = take(8 * parts);
     s.part = take(8 * parts * kBins);
     s.listed = take(4 * parts);
@@ -1165,6 +1242,8 @@ int ft_sample_filtered_batched_launch(const void* logits, int dtype, long long l
         a.slices = sh.slices;
         a.top = (float*)(ws + sh.top);
         a.top_at = (int*)(ws + sh.top_at);
+        a.groups = (float*)(ws + sh.groups);
+        a.floors = (float*)(ws + sh.floors);
         a.sum = (u64*)(ws + sh.sum);
         a.part = (u64*)(ws + sh.part);
         a.listed = (unsigned*)(ws + sh.listed);

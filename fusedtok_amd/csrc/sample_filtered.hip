@@ -746,7 +746,7 @@ constexpr int kSliceTPT = kSlice / kSliceNT;
 // f(token, its place j) for a thread's tokens of a slice, with the loads of the next
 // ones under way (all loads first left every workgroup of a CU loading and
 // then computing at the same time).
-template <typename T, int AHEAD = 4>
+template <typename T, int AHEAD>
 struct Tokens {
     typedef T v4 __attribute__((ext_vector_type(4)));
     static constexpr int kSteps = kSliceTPT / 4, kAhead = AHEAD;
@@ -836,7 +836,7 @@ __global__ __launch_bounds__(kSliceNT) void slice_hist(const SampleArgs a) {
     if (4 * (int)(threadIdx.x & 63) < parts)
         of_parts = *reinterpret_cast<const float4*>(a.groups + (size_t)r * a.slices * kGroups +
                                                     4 * (threadIdx.x & 63));
-    Tokens<T> tokens(a, r, lo, hi);
+    Tokens<T, 2> tokens(a, r, lo, hi);
     fill_powers(s_powers);
     for (int b = threadIdx.x; b < kBins; b += kSliceNT) s_mass[b] = 0, s_count[b] = 0;
     __syncthreads();
@@ -955,7 +955,7 @@ __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
     __shared__ unsigned s_n;
     const int r = blockIdx.x / a.slices, s = blockIdx.x - r * a.slices;
     const int lo = s * kSlice, hi = min(lo + kSlice, a.n);
-    __shared__ float s_near[kSlice];
+    __shared__ T s_near[kSlice];
     const float some = slice_top(a, r), floor = a.floors[r];
     BinRun bins;
     bins.load(a, r);
@@ -966,7 +966,7 @@ __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
         own[i] = b < kBins ? a.part[(size_t)blockIdx.x * kBins + b] : 0;
     }
     // (on their way while the bins are searched)
-    Tokens<T, kSliceTPT / 4> tokens(a, r, lo, hi);
+    Tokens<T, 4> tokens(a, r, lo, hi);
     const float top = row_top(a, r, some);
     const Row row(a, r, top, nullptr);
     if (row.greedy || top == -INFINITY || !row.cut()) return;
@@ -988,13 +988,13 @@ __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
     tokens.each([&](float x, int j) {
         if (!(x < least) && !(x > most)) {
             some_of |= 1u << j;
-            s_near[j * kSliceNT + threadIdx.x] = x;
+            s_near[j * kSliceNT + threadIdx.x] = (T)x;
         }
     });
     while (some_of) {
         const int j = __ffs(some_of) - 1;
         some_of &= some_of - 1;
-        const float x = s_near[j * kSliceNT + threadIdx.x];
+        const float x = (float)s_near[j * kSliceNT + threadIdx.x];
         const int b = bin_of(row.far(x));
         if (b < kBins && ((b >= span.lo && b <= span.hi) || b == span.at_k ||
                           (b >= at_p && b < at_p + kMinBins && b < span.lo)))

@@ -23,21 +23,37 @@
 // value. Nothing is sorted, and equal logits, thousands in 16 bits, cost
 // nothing extra.
 //
-// n <= 32768: a workgroup a row, its logits in registers, one launch
-// (sample_row). Else slices of 8192 tokens, a workgroup each, in four:
-//   slice_max   maximum and its index, clears the row's histogram;
-//   slice_hist  weights into the row's histogram (or, without a cut, the sum
-//               of the slice's kept weights);
-//   slice_list  every workgroup finds the bin of the cut from the histogram
-//               (the bins, where k and p leave more than one), sums its
-//               weights above and lists its logits inside;
+// The floor. With k, the k-th largest of the largest logits of 256 parts of the
+// row is a bound that the first k are not below, whatever lies in the parts.
+// Below it neither histogram nor list need a logit, and the weights of few are
+// worked out (2 rows of 32000, k = 40: 4.4 us for the histogram, 11.7 without).
+//
+// n <= 32768: a workgroup a row, its logits in LDS, one launch (sample_row).
+// Above that they do not fit beside the rest; slices of 8192 tokens, a workgroup
+// each, in four launches:
+//   slice_max   maximum and its index, the parts' maxima, clears the row's
+//               histogram;
+//   slice_hist  weights into the slice's histogram and the row's (or, without
+//               a cut, the sum of the slice's kept weights);
+//   slice_list  every workgroup finds the bin of the cut from the row's
+//               histogram (the bins, where k and p leave more than one, and
+//               those of min-p), sums its own bins above and lists its logits
+//               inside;
 //   sample_pick a workgroup a row: the cut, each slice's kept sum, the slice
 //               that holds the token, and the token in it.
-// What bounds it: one read of the logits from HBM and up to two from the
-// caches, and the float64 arithmetic of the weights (12 operations a token).
+//
+// What bounds it. One read of the logits from HBM and two from the caches: 64
+// rows of 128256 float32 (32.8 MB, a quarter of them without k) 6 + 13.7 + 11.6
+// + 21 us, 54-56 a call, the reads at 5.1 TB/s 6.4; 301 of 50257 bf16, p alone,
+// 11 + 24 + 16.5 + 27, 75 a call. slice_hist without a floor waits for the LDS
+// (a table's word and an atomic a token) and float64 (10 operations a token),
+// slice_list for the row's bins, sample_pick and sample_row (2 x 32000: 23.7 us)
+// for their 30 steps, one behind the other, with a barrier between each: 1024
+// threads instead of 512 took 25 and 46 us for sample_pick's 21 and 27.
 #include "ft_common.hpp"
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 
 namespace ft {
@@ -49,7 +65,7 @@ constexpr int kBins = 657;           // bins of weights that are not 0: log2 dis
 constexpr int kSlice = 8192;         // tokens
 constexpr int kSliceNT = 256;
 constexpr int kRowNT = 512;
-constexpr int kRowMost = 32768;      // tokens of a row that one workgroup holds
+constexpr int kRowMost = 32768;      // tokens of a row that one workgroup holds in LDS
 constexpr int kMaxVocab = 1 << 22;   // 512 slices; sums of weights below 2^62
 constexpr int kMinBins = 3;
 constexpr int kGroups = 16;          // parts of a slice
@@ -81,7 +97,7 @@ struct SampleArgs {
     unsigned* list;    // [rows][n]: order bits, slice s from kSlice s on
 };
 
-// 2^(j / 64), and a copy in LDS (the caller synchronises).
+// 2^(j / 64), and 2^40 times it in LDS (the caller synchronises).
 constexpr int kPowers = 64;
 __device__ const double kPowerTable[kPowers] = {
     1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
@@ -102,7 +118,7 @@ __device__ const double kPowerTable[kPowers] = {
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,
 };
 __device__ __forceinline__ void fill_powers(double* s) {
-    if (threadIdx.x < kPowers) s[threadIdx.x] = kPowerTable[threadIdx.x];
+    if (threadIdx.x < kPowers) s[threadIdx.x] = 1099511627776.0 * kPowerTable[threadIdx.x];
 }
 
 // Distances t are in 1/64 of log2, 0 or less; from kFar on a weight is 0.
@@ -121,8 +137,8 @@ __device__ __forceinline__ int nearest(double t) { return (int)__double_as_longl
 // |f| <= 1/2, the series of 2^(f / 64) to f^4 (the next term is below 4e-14, 0.05
 // units of the largest weight; the exponential by its series alone, to the
 // 11th power, took twice the registers and more time)
-__device__ __forceinline__ u64 weight(const double* powers, double t) {
-    if (!near(t)) return 0;
+// (weight_near: of a t that is not much below kFar, where it is 0)
+__device__ __forceinline__ u64 weight_near(const double* powers, double t) {
     const int k = nearest(t);
     const double f = t - ((t + kRound) - kRound);
     double s = 5.732851688640402e-10;  // (ln(2) / 64)^4 / 24
@@ -130,12 +146,16 @@ __device__ __forceinline__ u64 weight(const double* powers, double t) {
     s = fma(s, f, 5.864904955056169e-05);
     s = fma(s, f, 1.0830424696249145e-02);
     s = fma(s, f, 1.0);
-    // 2^(40 + n / 64): the power's exponent moved; then the last bits of its
-    // product + 2^52 are the nearest whole number
-    const long long p = __double_as_longlong(powers[k & 63]) +
-                        ((long long)((k >> 6) + 40) << 52);
-    const double v = fma(s, __longlong_as_double(p), 4503599627370496.0);
+    // 2^(40 + n / 64): the power's exponent moved, in its high word; then the
+    // last bits of its product + 2^52 are the nearest whole number
+    const double power = powers[k & 63];
+    const double p = __hiloint2double(__double2hiint(power) + ((k << 14) & (int)0xfff00000),
+                                      __double2loint(power));
+    const double v = fma(s, p, 4503599627370496.0);
     return (u64)__double_as_longlong(v) & 0xfffffffffffffull;
+}
+__device__ __forceinline__ u64 weight(const double* powers, double t) {
+    return near(t) ? weight_near(powers, t) : 0;
 }
 
 // A row's parameters, the same in every thread.
@@ -150,8 +170,10 @@ struct Row {
         : powers(s_powers) {
         const float t = a.temp ? a.temp[r] : a.temp_all;
         greedy = !(t > 0.0f);
-        top = (double)most;
-        infinite = most == INFINITY;
+        // (the same in every lane: a branch on it costs a token nothing)
+        const int bits = __builtin_amdgcn_readfirstlane(__float_as_int(most));
+        top = (double)__int_as_float(bits);
+        infinite = bits == 0x7f800000;
         c = greedy ? 0.0 : 92.332482616893658 / (double)t;
         minp = a.minp ? a.minp[r] : a.minp_all;
         minp = minp < 1.0f ? fmaxf(minp, 0.0f) : 1.0f;  // (NaN: 1)
@@ -164,8 +186,9 @@ struct Row {
     // 64 log2 of the weight over the largest (infinite ones share the mass)
     __device__ __forceinline__ double far(float x) const {
         if (infinite) return x == INFINITY ? 0.0 : 2.0 * kFar;
-        return ((double)x - top) * c;
+        return finite_far(x);
     }
+    __device__ __forceinline__ double finite_far(float x) const { return ((double)x - top) * c; }
     // the first of the kMinBins bins that may hold weights on both sides of
     // min-p: those before it are kept, those behind them not
     __device__ __forceinline__ int least_bin() const {
@@ -179,13 +202,19 @@ struct Row {
         return make_float2(f - (fabsf(f) * 0x1p-22f + 0x1p-126f),
                            g + (fabsf(g) * 0x1p-22f + 0x1p-126f));
     }
-    __device__ __forceinline__ u64 weight_at(double t) const { return weight(powers, t); }
+    // no logit of bin b or one before it lies below it, nor below floor
+    __device__ __forceinline__ float least_of(int b, float floor) const {
+        return fmaxf(around(b).x, floor);  // (of a NaN: the other)
+    }
     __device__ __forceinline__ u64 weight_of(float x) const { return weight(powers, far(x)); }
     __device__ __forceinline__ bool keeps(u64 w) const { return w >= minw; }
 };
 
-// the bin, 1/16 of log2 wide
-__device__ __forceinline__ int bin_of(double t) { return near(t) ? -nearest(t) >> 2 : kBins; }
+// the bin, 1/16 of log2 wide; kBins and more: none (with weights of 0 the last
+// bin ends a little behind kFar)
+constexpr double kFarthest = -65536.0;
+__device__ __forceinline__ int bin_near(double t) { return -nearest(t) >> 2; }  // t > kFarthest
+__device__ __forceinline__ int bin_of(double t) { return t > kFarthest ? bin_near(t) : kBins; }
 
 // order bits: larger for larger x, equal for equal ones
 __device__ __forceinline__ unsigned order_bits(float x) {
@@ -240,10 +269,11 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* s, u64& total) {
 
 // A bound that the k-th largest logit is not below: of kFloorOf parts' largest
 // ones, 4 a lane (`parts` of them: the rest is -inf), the k-th, to 16 bits of
-// its order bits. -inf where there are fewer than k. What lies below is none
-// of the first k: neither the histogram nor the list needs it.
+// its order bits. Where there are fewer than k, the least finite value. What
+// lies below is none of the first k, or has no weight: neither the histogram
+// nor the list needs it.
 __device__ __forceinline__ float floor_of(float4 g, int k, int parts) {
-    if (k <= 0 || k > parts) return -INFINITY;
+    if (k <= 0 || k > parts) return -FLT_MAX;
     const unsigned o[4] = {order_bits(g.x), order_bits(g.y), order_bits(g.z), order_bits(g.w)};
     unsigned at = 0;
 #pragma unroll
@@ -254,7 +284,7 @@ __device__ __forceinline__ float floor_of(float4 g, int k, int parts) {
         for (int i = 0; i < 4; ++i) many += __popcll(__builtin_amdgcn_ballot_w64(o[i] >= next));
         if (many >= k) at = next;
     }
-    return at > order_bits(-INFINITY) ? from_bits(at) : -INFINITY;
+    return at > order_bits(-FLT_MAX) ? from_bits(at) : -FLT_MAX;
 }
 
 // A thread's tokens: 4 in a row of every 4 NT, from `first` on, x = -inf
@@ -698,16 +728,16 @@ __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
         const float floor =
             floor_of(*reinterpret_cast<const float4*>(s.parts + 4 * (threadIdx.x & 63)), row.k,
                      kFloorOf);
+        const float near_floor = row.least_of(kBins - 1, floor);
         for (int j = 0; j < chunks; ++j) {
             const float4 x = *reinterpret_cast<const float4*>(s_x + 4 * (j * kRowNT + threadIdx.x));
             const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (v[e] < floor) continue;
+                if (!(v[e] >= near_floor)) continue;
                 const double t = row.far(v[e]);
-                const int b = bin_of(t);
-                if (b >= kBins) continue;
-                atomicAdd(&s.mass[b], row.weight_at(t));
+                const int b = min(bin_of(t), kBins);  // (kBins: nobody's)
+                atomicAdd(&s.mass[b], weight(s.powers, t));
                 atomicAdd(&s.count[b], 1u);
             }
         }
@@ -715,7 +745,7 @@ __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
         const u64 total = scan_bins(s);
         cut = find_cut(row, total, s, [&](auto&& f, int bin) {
             const float2 about = row.around(bin);
-            const float least = fmaxf(about.x, floor);  // (of a NaN: the other)
+            const float least = row.least_of(bin, floor);
             const float* const x0 = s_x + 4 * threadIdx.x;
             u64 some = 0;  // the thread's tokens about the bin
 #pragma unroll 4
@@ -725,7 +755,7 @@ __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
                 unsigned in = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    in |= !(v[e] < least) && !(v[e] > about.y) ? 1u << e : 0;
+                    in |= v[e] >= least && !(v[e] > about.y) ? 1u << e : 0;
                 some |= (u64)in << (4 * j);
             }
             for (; some; some &= some - 1) {
@@ -743,48 +773,57 @@ __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int kSliceTPT = kSlice / kSliceNT;
 
-// f(token, its place j) for a thread's tokens of a slice, with the loads of the next
-// ones under way (all loads first left every workgroup of a CU loading and
-// then computing at the same time).
+// f(token, its place j) for a thread's tokens of a slice (-inf behind its end),
+// AHEAD loads under way: all loads first left every workgroup of a CU loading
+// and then computing at the same time. A load is unconditional and its values
+// are touched only when their turn comes, so nothing waits for it before: whole
+// slices of aligned rows 4 tokens at once, others one by one, the last one again
+// behind the end.
 template <typename T, int AHEAD>
 struct Tokens {
     typedef T v4 __attribute__((ext_vector_type(4)));
-    static constexpr int kSteps = kSliceTPT / 4, kAhead = AHEAD;
+    static constexpr int kSteps = kSliceTPT / 4;
     const T* row;
     int lo, hi;
-    bool vec;
-    float4 x[kAhead];
-    __device__ __forceinline__ float4 load(int j) const {
+    bool whole;
+    v4 x[AHEAD];
+    template <bool WHOLE>
+    __device__ __forceinline__ v4 load(int j) const {
         const int i = lo + 4 * (j * kSliceNT + (int)threadIdx.x);
-        if (vec && i + 4 <= hi) {
-            const v4 v = *reinterpret_cast<const v4*>(row + i);
-            return make_float4((float)v[0], (float)v[1], (float)v[2], (float)v[3]);
-        }
-        return make_float4(i < hi ? (float)row[i] : -INFINITY,
-                           i + 1 < hi ? (float)row[i + 1] : -INFINITY,
-                           i + 2 < hi ? (float)row[i + 2] : -INFINITY,
-                           i + 3 < hi ? (float)row[i + 3] : -INFINITY);
+        if (WHOLE) return *reinterpret_cast<const v4*>(row + i);
+        v4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = row[min(i + e, hi - 1)];
+        return v;
     }
     __device__ __forceinline__ Tokens(const SampleArgs& a, int r, int first, int end)
         : row((const T*)a.x + (long long)r * a.ld), lo(first), hi(end),
-          vec(((uintptr_t)(row + first) & (4 * sizeof(T) - 1)) == 0) {
+          whole(first + kSlice <= end && ((uintptr_t)(row + first) & (4 * sizeof(T) - 1)) == 0) {
+        if (whole) start<true>();
+        else start<false>();
+    }
+    template <bool WHOLE>
+    __device__ __forceinline__ void start() {
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) x[j] = load(j);
+        for (int j = 0; j < AHEAD; ++j) x[j] = load<WHOLE>(j);
+    }
+    template <bool WHOLE, typename F>
+    __device__ __forceinline__ void run(F&& f) {
+#pragma unroll 1
+        for (int j0 = 0; j0 < kSteps; j0 += AHEAD)
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int j = 4 * (j0 + q), i = lo + j * kSliceNT + 4 * (int)threadIdx.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    f(WHOLE || i + e < hi ? (float)x[q][e] : -INFINITY, j + e);
+                if (j0 + AHEAD < kSteps) x[q] = load<WHOLE>(j0 + AHEAD + q);
+            }
     }
     template <typename F>
     __device__ __forceinline__ void each(F&& f) {
-#pragma unroll 1
-        for (int j0 = 0; j0 < kSteps; j0 += kAhead)
-#pragma unroll
-            for (int q = 0; q < kAhead; ++q) {
-                const float4 v = x[q];
-                if (j0 + kAhead < kSteps) x[q] = load(j0 + kAhead + q);
-                const int j = 4 * (j0 + q);
-                f(v.x, j);
-                f(v.y, j + 1);
-                f(v.z, j + 2);
-                f(v.w, j + 3);
-            }
+        if (whole) run<true>(f);
+        else run<false>(f);
     }
 };
 
@@ -825,8 +864,12 @@ __device__ __forceinline__ float row_top(const SampleArgs& a, int r, float m) {
 template <typename T>
 __global__ __launch_bounds__(kSliceNT) void slice_hist(const SampleArgs a) {
     __shared__ double s_powers[kPowers];
-    __shared__ u64 s_mass[kBins];
-    __shared__ unsigned s_count[kBins];
+    // A histogram a wave, mass and count in one word: 2048 tokens, so at most
+    // 2^51 and 2^11. (One of both for the workgroup: two atomics a token, and
+    // LDS is what the loop waits for.) The last bin: weights that are 0.
+    constexpr int kCountAt = 52;
+    static_assert(kSliceTPT * 64 <= 1 << 11, "a wave's tokens");
+    __shared__ u64 s_hist[kSliceNT / 64][kBins + 1];
     __shared__ u64 s_sum[4];
     const int r = blockIdx.x / a.slices, s = blockIdx.x - r * a.slices;
     const int lo = s * kSlice, hi = min(lo + kSlice, a.n);
@@ -838,7 +881,7 @@ __global__ __launch_bounds__(kSliceNT) void slice_hist(const SampleArgs a) {
                                                     4 * (threadIdx.x & 63));
     Tokens<T, 2> tokens(a, r, lo, hi);
     fill_powers(s_powers);
-    for (int b = threadIdx.x; b < kBins; b += kSliceNT) s_mass[b] = 0, s_count[b] = 0;
+    for (int b = threadIdx.x; b < kSliceNT / 64 * (kBins + 1); b += kSliceNT) s_hist[0][b] = 0;
     __syncthreads();
     const float top = row_top(a, r, some);
     const Row row(a, r, top, s_powers);
@@ -857,21 +900,37 @@ __global__ __launch_bounds__(kSliceNT) void slice_hist(const SampleArgs a) {
     }
     const float floor = floor_of(of_parts, row.k, parts);
     if (s == 0 && threadIdx.x == 0) a.floors[r] = floor;
-    tokens.each([&](float x, int) {
-        if (x < floor) return;
-        const double t = row.far(x);
-        const int b = bin_of(t);
-        if (b >= kBins) return;
-        atomicAdd(&s_mass[b], row.weight_at(t));
-        atomicAdd(&s_count[b], 1u);
-    });
+    const float least = row.least_of(kBins - 1, floor);
+    u64* const hist = s_hist[threadIdx.x >> 6];
+    auto add = [&](int b, u64 w) { atomicAdd(&hist[b], w | 1ull << kCountAt); };
+    // (where T is so small that the bound's own rounding is far: all checks)
+    if (row.infinite || !(row.far(least) > kFarthest))
+        tokens.each([&](float x, int) {
+            const double t = row.far(x);
+            const int b = bin_of(t);
+            if (x >= floor && b < kBins) add(b, weight(s_powers, t));
+        });
+    else
+        tokens.each([&](float x, int) {
+            if (!(x >= least)) return;
+            const double t = row.finite_far(x);
+            add(min(bin_near(t), kBins), weight_near(s_powers, t));
+        });
     __syncthreads();
     u64* const part = a.part + (size_t)blockIdx.x * kBins;
     for (int b = threadIdx.x; b < kBins; b += kSliceNT) {
-        part[b] = s_mass[b];
-        if (s_count[b]) {
-            atomicAdd(&a.mass[(size_t)r * kBins + b], s_mass[b]);
-            atomicAdd(&a.count[(size_t)r * kBins + b], s_count[b]);
+        u64 mass = 0;
+        unsigned count = 0;
+#pragma unroll
+        for (int w = 0; w < kSliceNT / 64; ++w) {
+            const u64 v = s_hist[w][b];
+            mass += v & ((1ull << kCountAt) - 1);
+            count += (unsigned)(v >> kCountAt);
+        }
+        part[b] = mass;
+        if (count) {
+            atomicAdd(&a.mass[(size_t)r * kBins + b], mass);
+            atomicAdd(&a.count[(size_t)r * kBins + b], count);
         }
     }
 }
@@ -982,11 +1041,11 @@ __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
         if ((int)threadIdx.x + i * kSliceNT < all) sum += own[i];
     unsigned* const list = a.list + (size_t)r * a.n + lo;
     // logits outside the listed bins are seen without their float64 distance
-    const float least = fmaxf(row.around(min(max(span.hi, span.at_k), kBins - 1)).x, floor);
+    const float least = row.least_of(min(max(span.hi, span.at_k), kBins - 1), floor);
     const float most = row.around(min(all, kBins - 1)).y;
     unsigned some_of = 0;  // the thread's tokens that may be listed
     tokens.each([&](float x, int j) {
-        if (!(x < least) && !(x > most)) {
+        if (x >= least && !(x > most)) {
             some_of |= 1u << j;
             s_near[j * kSliceNT + threadIdx.x] = (T)x;
         }

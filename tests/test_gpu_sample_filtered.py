@@ -142,6 +142,42 @@ def test_temperatures(temp, n):
     check(x, u, temp, 20)
 
 
+@pytest.mark.parametrize("n", [900, 20000, 50257, 140000])
+@pytest.mark.parametrize("k", [1, 30, 112, 113, 256, 257, 700])
+def test_where_the_first_k_lie(k, n):
+    """k on both sides of the parts whose largest logits bound the first k;
+    the largest logits all in one part, a part each, equal, or too few."""
+    rng = np.random.default_rng(k)
+    x = rng.standard_normal((8, n)).astype(np.float32)
+    x[1] = np.sort(x[1])[::-1]                   # the first k side by side
+    x[2] = np.sort(x[2])
+    x[3] = np.round(4 * x[3])                    # many equal at any bound
+    x[4] = -3.0
+    x[5, k // 2 + 1:] = -np.inf                  # fewer than k have weight
+    x[6, rng.permutation(n)[:k + 5]] = np.inf    # more than k share it all
+    x[7] = -np.finfo(np.float32).max
+    x[7, n // 2] = 1.0
+    u = rng.random(8).astype(np.float32)
+    check(dev(x), u, 0.9, k)
+    check(dev(x), u, 1.1, k, 0.8, 0.02)
+
+
+@pytest.mark.parametrize("n", [2000, 36000])
+@pytest.mark.parametrize("temp", [1e-44, 1e-30, 1e-9, 1e-5])
+def test_cold_neighbours(temp, n):
+    """Logits a rounding apart and far, under temperatures that make either
+    far: no distance runs over into the bins."""
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((4, n)).astype(np.float32) * 1e-3 + 20.0
+    x[1] = np.nextafter(np.float32(7.0), np.float32(np.inf)) - np.float32(2 ** -22) * (
+        np.arange(n) % 9)
+    x[2] *= np.float32(1e36)
+    x[3, ::2] = -np.finfo(np.float32).max
+    u = rng.random(4).astype(np.float32)
+    for k, p in ((0, 0.9), (3, 1.0), (50, 0.7), (0, 1.0)):
+        check(dev(x), u, temp, k, p)
+
+
 @pytest.mark.parametrize("n", [2000, 36000])
 def test_values_of_vectors_are_safe(n):
     x, u = logits(8, 8, n, torch.float32)

@@ -287,29 +287,67 @@ __device__ __forceinline__ float floor_of(float4 g, int k, int parts) {
     return at > order_bits(-FLT_MAX) ? from_bits(at) : -FLT_MAX;
 }
 
+// Two at once. s: 32 words.
+template <int NT>
+__device__ __forceinline__ void block_scan2(u64& v, u64& w, u64* s, u64& all_v, u64& all_w) {
+    const u64 in_v = wave_scan(v), in_w = wave_scan(w);
+    if ((threadIdx.x & 63) == 63) {
+        s[threadIdx.x >> 6] = in_v;
+        s[16 + (threadIdx.x >> 6)] = in_w;
+    }
+    __syncthreads();
+    v = in_v - v, w = in_w - w;
+    all_v = all_w = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+        const u64 x = s[i], y = s[16 + i];
+        if (i < (int)(threadIdx.x >> 6)) v += x, w += y;
+        all_v += x, all_w += y;
+    }
+}
+
 // A thread's tokens: 4 in a row of every 4 NT, from `first` on, x = -inf
-// where there is none. NaN becomes -inf.
+// where there is none; NaN stays, every comparison with it is false. All loads
+// are unconditional and converted behind the last one: a conversion in a branch
+// waits there for its load (301 rows of 50257 bf16: slice_max 11 us so).
 template <typename T, int NT, int TPT>
 __device__ __forceinline__ void load_tokens(const T* row, int first, int end, float (&x)[TPT]) {
     typedef T v4 __attribute__((ext_vector_type(4)));
-    const bool vec = ((uintptr_t)(row + first) & (4 * sizeof(T) - 1)) == 0;
+    const T* const p = row + first;
+    const int len = end - first, mine = 4 * (int)threadIdx.x;
+    v4 v[TPT / 4];
+    if (len >= 4 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0) {
+        const int whole = len & ~3;
 #pragma unroll
-    for (int j = 0; j < TPT / 4; ++j) {
-        const int i = first + 4 * (j * NT + (int)threadIdx.x);
-        v4 v;
-        if (vec && i + 4 <= end) {
-            v = *reinterpret_cast<const v4*>(row + i);
+        for (int j = 0; j < TPT / 4; ++j)
+            v[j] = *reinterpret_cast<const v4*>(p + min(4 * j * NT + mine, whole - 4));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * j + e] = (float)v[e];
-        } else {
+        for (int j = 0; j < TPT / 4; ++j) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                x[4 * j + e] = i + e < end ? (float)row[i + e] : -INFINITY;
+                x[4 * j + e] = 4 * j * NT + mine < whole ? (float)v[j][e] : -INFINITY;
         }
-    }
+        if (whole < len) {  // the last one to three
+            float rest[3];
 #pragma unroll
-    for (int j = 0; j < TPT; ++j)
-        if (!(x[j] >= -INFINITY)) x[j] = -INFINITY;
+            for (int e = 0; e < 3; ++e) rest[e] = whole + e < len ? (float)p[whole + e] : -INFINITY;
+#pragma unroll
+            for (int j = 0; j < TPT / 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (4 * j * NT + mine == whole) x[4 * j + e] = rest[e];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < TPT / 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j][e] = p[min(4 * j * NT + mine + e, len - 1)];
+#pragma unroll
+        for (int j = 0; j < TPT / 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[4 * j + e] = 4 * j * NT + mine + e < len ? (float)v[j][e] : -INFINITY;
+    }
 }
 
 // The largest of the workgroup's tokens and its first index, and of each 16
@@ -318,9 +356,9 @@ template <int NT, int TPT>
 __device__ __forceinline__ float block_top(const float (&x)[TPT], int first, float* s, int* s_at,
                                            float* groups, int& at) {
     static_assert(NT == 16 * kGroups, "parts of 16 threads");
-    float m = x[0];
+    float m = -INFINITY;
 #pragma unroll
-    for (int j = 1; j < TPT; ++j) m = fmaxf(m, x[j]);
+    for (int j = 0; j < TPT; ++j) m = fmaxf(m, x[j]);
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     if ((threadIdx.x & 15) == 0) groups[threadIdx.x >> 4] = m;
@@ -348,6 +386,7 @@ __device__ __forceinline__ float block_top(const float (&x)[TPT], int first, flo
 // What a row's workgroup holds in LDS.
 // ---------------------------------------------------------------------------
 constexpr int kFew = kRowNT / 8;  // logits that are ranked by comparing all with all
+constexpr int kFirst = 512;       // logits above a floor that are listed
 constexpr int kWaves = kRowNT / 64;
 constexpr int kChunk = 4 * kRowNT;  // tokens of a pass of the workgroup
 
@@ -363,9 +402,10 @@ struct RowState {
     unsigned count[kBins + 1];
     u64 level_mass[kLevel];
     unsigned level_count[kLevel];
+    unsigned first[kFirst], firsts;  // sample_row's logits above a floor
     u64 few_w[kFew];
     unsigned few_key[kFew];
-    u64 scan[16], scan2[16];
+    u64 scan[32];
     u64 chunk_mass[kRowMost / kChunk * kWaves];
     unsigned chunk_ties[kRowMost / kChunk * kWaves];
     Group group;
@@ -378,7 +418,7 @@ struct RowState {
 };
 
 // The tokens [first, end) of a row into s_x, up to a whole chunk (-inf behind
-// the end; NaN becomes -inf), at most MOST of them. Returns their largest and,
+// the end), at most MOST of them. Returns their largest and,
 // in `at`, its first index; PARTS: and leaves the parts' largest.
 template <typename T, int MOST, bool PARTS>
 __device__ __forceinline__ float stage_tokens(const T* row, int first, int end, float* s_x,
@@ -434,8 +474,8 @@ __device__ __forceinline__ u64 scan_bins(RowState& s) {
         mass += m[i];
         count += c[i];
     }
-    u64 mb = block_scan<kRowNT>(mass, s.scan, total);
-    u64 cb = block_scan<kRowNT>(count, s.scan2, tokens);
+    block_scan2<kRowNT>(mass, count, s.scan, total, tokens);
+    u64 mb = mass, cb = count;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int b = threadIdx.x * PER + i;
@@ -495,10 +535,10 @@ __device__ __forceinline__ Group resolve(const Row& row, const Limit& l, unsigne
         });
         __syncthreads();
         const unsigned c = s.level_count[threadIdx.x];
-        u64 total;
         const u64 m = s.level_mass[threadIdx.x];
-        const u64 mb = mass0 + block_scan<kRowNT>(m, s.scan, total);
-        const u64 cb = count0 + block_scan<kRowNT>(c, s.scan2, total);
+        u64 mb = m, cb = c, total, tokens;
+        block_scan2<kRowNT>(mb, cb, s.scan, total, tokens);
+        mb += mass0, cb += count0;
         if (l.closes(mb, cb, mb + m, cb + c)) s.bin = threadIdx.x;
         __syncthreads();
         const int bin = s.bin;
@@ -622,8 +662,10 @@ __device__ __forceinline__ void pick(const Row& row, const Cut& cut, const float
         u64 m = kept(x.x) + kept(x.y) + kept(x.z) + kept(x.w);
         unsigned t = tie(x.x) + tie(x.y) + tie(x.z) + tie(x.w);
         if (__builtin_amdgcn_ballot_w64(m | t)) {
-            m = wave_sum64(m);
-            t = (unsigned)wave_sum64(t);
+            // (in one word: 256 weights are at most 2^48)
+            const u64 both = wave_sum64(m | (u64)t << 52);
+            m = both & ((1ull << 52) - 1);
+            t = (unsigned)(both >> 52);
         }
         if (lane == 0) s.chunk_mass[j * kWaves + wave] = m, s.chunk_ties[j * kWaves + wave] = t;
     }
@@ -715,6 +757,7 @@ __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
     const int r = blockIdx.x;
     for (int b = threadIdx.x; b < kBins; b += kRowNT) s.mass[b] = 0, s.count[b] = 0;
     fill_powers(s.powers);
+    if (threadIdx.x == 0) s.firsts = 0;
     int at;
     const float top = stage_tokens<T, MOST, true>((const T*)a.x + (long long)r * a.ld, 0, a.n, s_x, s, at);
     const Row row(a, r, top, s.powers);
@@ -729,6 +772,7 @@ __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
             floor_of(*reinterpret_cast<const float4*>(s.parts + 4 * (threadIdx.x & 63)), row.k,
                      kFloorOf);
         const float near_floor = row.least_of(kBins - 1, floor);
+        const bool few = floor > -FLT_MAX;
         for (int j = 0; j < chunks; ++j) {
             const float4 x = *reinterpret_cast<const float4*>(s_x + 4 * (j * kRowNT + threadIdx.x));
             const float v[4] = {x.x, x.y, x.z, x.w};
@@ -739,11 +783,24 @@ __global__ __launch_bounds__(kRowNT) void sample_row(const SampleArgs a) {
                 const int b = min(bin_of(t), kBins);  // (kBins: nobody's)
                 atomicAdd(&s.mass[b], weight(s.powers, t));
                 atomicAdd(&s.count[b], 1u);
+                if (few) {
+                    const unsigned i = atomicAdd(&s.firsts, 1u);
+                    if (i < kFirst) s.first[i] = order_bits(v[e]);
+                }
             }
         }
         __syncthreads();
+        // (a floor's finds are looked through again, not the row)
+        const unsigned firsts = few ? s.firsts : kFirst + 1;
         const u64 total = scan_bins(s);
         cut = find_cut(row, total, s, [&](auto&& f, int bin) {
+            if (firsts <= kFirst) {
+                for (unsigned i = threadIdx.x; i < firsts; i += kRowNT) {
+                    const unsigned o = s.first[i];
+                    f(o, [&] { return bin_of(row.far(from_bits(o))) == bin; });
+                }
+                return;
+            }
             const float2 about = row.around(bin);
             const float least = row.least_of(bin, floor);
             const float* const x0 = s_x + 4 * threadIdx.x;
@@ -828,7 +885,7 @@ struct Tokens {
 };
 
 template <typename T>
-__global__ __launch_bounds__(kSliceNT) void slice_max(const SampleArgs a) {
+__global__ __launch_bounds__(kSliceNT, 8) void slice_max(const SampleArgs a) {
     __shared__ float s_top[4];
     __shared__ int s_at[4];
     const int r = blockIdx.x / a.slices, s = blockIdx.x - r * a.slices;
@@ -956,7 +1013,7 @@ struct Span {
     int lo, hi, at_k;  // at_k: -1 none
 };
 __device__ __forceinline__ Span cut_span(const Row& row, const BinRun& h, u64* s_scan,
-                                         u64* s_scan2, int* s_bin) {
+                                         int* s_bin) {
     constexpr int PER = BinRun::PER;
     const u64(&m)[PER] = h.m;
     const unsigned(&c)[PER] = h.c;
@@ -964,8 +1021,9 @@ __device__ __forceinline__ Span cut_span(const Row& row, const BinRun& h, u64* s
 #pragma unroll
     for (int i = 0; i < PER; ++i) mine += m[i], many += c[i];
     if (threadIdx.x < 3) s_bin[threadIdx.x] = 0;
-    u64 mb = block_scan<kSliceNT>(mine, s_scan, total);
-    u64 cb = block_scan<kSliceNT>(many, s_scan2, tokens);
+    block_scan2<kSliceNT>(mine, many, s_scan, total, tokens);
+    u64 mb = mine;
+    const u64 cb = many;
     __shared__ u64 s_w[2];
     if (threadIdx.x == 0) s_w[0] = s_w[1] = total;
     const bool by_k = row.k > 0 && (u64)row.k <= tokens;
@@ -1009,7 +1067,7 @@ __device__ __forceinline__ Span cut_span(const Row& row, const BinRun& h, u64* s
 
 template <typename T>
 __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
-    __shared__ u64 s_scan[4], s_scan2[4], s_sum[4];
+    __shared__ u64 s_scan[32], s_sum[4];
     __shared__ int s_bin[3];
     __shared__ unsigned s_n;
     const int r = blockIdx.x / a.slices, s = blockIdx.x - r * a.slices;
@@ -1030,7 +1088,7 @@ __global__ __launch_bounds__(kSliceNT) void slice_list(const SampleArgs a) {
     const Row row(a, r, top, nullptr);
     if (row.greedy || top == -INFINITY || !row.cut()) return;
     if (threadIdx.x == 0) s_n = 0;
-    const Span span = cut_span(row, bins, s_scan, s_scan2, s_bin);
+    const Span span = cut_span(row, bins, s_scan, s_bin);
     // Above the bins that are listed all is kept: with min-p's own bin among
     // them, and its own bins' sums at hand, a slice works out no weight here.
     const int at_p = row.least_bin();
@@ -1165,7 +1223,7 @@ __global__ __launch_bounds__(kRowNT) void sample_pick(const SampleArgs a) {
     const u64 had = block_scan<kRowNT>(ties, s.scan, total);
     const u64 left = cut.q > had ? cut.q - had : 0;
     const u64 mine = b < a.slices ? s_sum[b] + cut.wc * min(left, ties) : 0;
-    const u64 before = block_scan<kRowNT>(mine, s.scan2, total);
+    const u64 before = block_scan<kRowNT>(mine, s.scan + 16, total);
     const u64 aim = aim_at(u, total);
     if (before <= aim && aim < before + mine) s.slice = b, s.base = before, s.q = left;
     __syncthreads();

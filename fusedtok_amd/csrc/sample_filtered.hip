@@ -43,11 +43,11 @@
 //               that holds the token, and the token in it.
 //
 // What bounds it. One read of the logits from HBM and two from the caches: 64
-// rows of 128256 float32 (32.8 MB, a quarter of them without k) 6 + 13.7 + 11.6
-// + 21 us, 54-56 a call, the reads at 5.1 TB/s 6.4; 301 of 50257 bf16, p alone,
-// 11 + 24 + 16.5 + 27, 75 a call. slice_hist without a floor waits for the LDS
+// rows of 128256 float32 (32.8 MB, a quarter of them without k) 5.5 + 13.7 +
+// 11.8 + 20 us, 52-54 a call, the reads at 5.1 TB/s 6.4; 301 of 50257 bf16, p
+// alone, 8 + 24 + 16.5 + 26, 70 a call. slice_hist without a floor waits for the LDS
 // (a table's word and an atomic a token) and float64 (10 operations a token),
-// slice_list for the row's bins, sample_pick and sample_row (2 x 32000: 23.7 us)
+// slice_list for the row's bins, sample_pick and sample_row (2 x 32000: 21.9 us)
 // for their 30 steps, one behind the other, with a barrier between each: 1024
 // threads instead of 512 took 25 and 46 us for sample_pick's 21 and 27.
 #include "ft_common.hpp"
@@ -155,7 +155,8 @@ __device__ __forceinline__ u64 weight_near(const double* powers, double t) {
     return (u64)__double_as_longlong(v) & 0xfffffffffffffull;
 }
 __device__ __forceinline__ u64 weight(const double* powers, double t) {
-    return near(t) ? weight_near(powers, t) : 0;
+    const u64 w = weight_near(powers, t);
+    return near(t) ? w : 0;
 }
 
 // A row's parameters, the same in every thread.
@@ -645,10 +646,9 @@ __device__ __forceinline__ void pick(const Row& row, const Cut& cut, const float
                                      long long* out) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int chunks = (n + kChunk - 1) / kChunk;
-    auto kept = [&](float v) -> u64 {  // of those above the cut
-        if (!(v > cut.xc)) return 0;
+    auto kept = [&](float v) -> u64 {  // of those above the cut (no branch: four at once)
         const u64 w = row.weight_of(v);
-        return row.keeps(w) ? w : 0;
+        return v > cut.xc && row.keeps(w) ? w : 0;
     };
     auto tie = [&](float v) { return v == cut.xc; };
     // sums of every 256 tokens in a row: (chunk j, wave)
@@ -884,6 +884,7 @@ struct Tokens {
     }
 };
 
+// (8 waves a SIMD: 301 x 50257 bf16 in 8.1 us, with the registers of 5 in 9.7)
 template <typename T>
 __global__ __launch_bounds__(kSliceNT, 8) void slice_max(const SampleArgs a) {
     __shared__ float s_top[4];

@@ -11,9 +11,9 @@
 // the angle (float64), rounded once at the end.
 //
 // What bounds it: HBM, each value read and written once (16384 tokens of 32 + 2 *
-// 8 heads, D = 128, bf16: 403 MB in 75.7 us, 5.3 TB/s; stores that bypass the
+// 8 heads, D = 128, bf16: 403 MB in 74.3 us, 5.4 TB/s; stores that bypass the
 // caches: 87-91 us without, or with loads that do too), and for few tokens
-// latency (64 tokens 5.7 us).
+// latency (64 tokens 5.6 us).
 //
 // Work split. A head is a group of lanes, 16 bytes of each half of its pairs
 // a lane (D = 128, 2-byte types: 8 lanes, 8 heads a wave); a workgroup takes
@@ -100,29 +100,35 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkArgs<T> a) {
     // the lane's 16-byte pieces: both halves of its pairs, or its pairs in a row
     const int c0 = NEOX ? at0(p0) : 2 * p0, c1 = NEOX ? at1(p0) : 2 * p0 + NP;
 
-    auto load = [&](const T* row, float (&x)[NP], float (&y)[NP]) {
+    // A head's values as they come, and as pairs. Loads are unconditional (a lane
+    // past the head reads its start) and nothing touches their values before
+    // their turn: a conversion or a branch around them waits for them at once.
+    const int l0 = lane_on ? c0 : 0, l1 = lane_on ? c1 : 0;
+    vec raw0, raw1;
+    auto load = [&](const T* row) {
         if constexpr (VEC) {
-            if (lane_on) {
-                const vec u = *reinterpret_cast<const vec*>(row + c0);
-                const vec w = *reinterpret_cast<const vec*>(row + c1);
+            raw0 = *reinterpret_cast<const vec*>(row + l0);
+            raw1 = *reinterpret_cast<const vec*>(row + l1);
+        } else {
 #pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    if constexpr (NEOX) {
-                        x[i] = (float)u[i];
-                        y[i] = (float)w[i];
-                    } else {
-                        x[i] = (float)(2 * i < NP ? u[(2 * i) % NP] : w[(2 * i) % NP]);
-                        y[i] = (float)(2 * i < NP ? u[(2 * i + 1) % NP] : w[(2 * i + 1) % NP]);
-                    }
-                }
-                return;
+            for (int i = 0; i < NP; ++i) {
+                const bool on = p0 + i < half;
+                raw0[i] = row[on ? at0(p0 + i) : 0];
+                raw1[i] = row[on ? at1(p0 + i) : 0];
             }
         }
+    };
+    auto unpack = [&](float (&x)[NP], float (&y)[NP]) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const bool on = !VEC && p0 + i < half;
-            x[i] = on ? (float)row[at0(p0 + i)] : 0.0f;
-            y[i] = on ? (float)row[at1(p0 + i)] : 0.0f;
+            T u = raw0[i], w = raw1[i];
+            if constexpr (VEC && !NEOX) {
+                u = 2 * i < NP ? raw0[(2 * i) % NP] : raw1[(2 * i) % NP];
+                w = 2 * i < NP ? raw0[(2 * i + 1) % NP] : raw1[(2 * i + 1) % NP];
+            }
+            const bool on = VEC ? lane_on : p0 + i < half;
+            x[i] = on ? (float)u : 0.0f;
+            y[i] = on ? (float)w : 0.0f;
         }
     };
     auto store = [&](T* row, const float (&x)[NP], const float (&y)[NP]) {
@@ -157,20 +163,19 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkArgs<T> a) {
     // the first head's values are on their way while the angles are computed
     int tok = 0, head = tid >> a.lanes_log2;
     while (head >= nh && tok < nt) head -= nh, ++tok;
-    float x[NP], y[NP];
     const T* const rows = a.qkv + (long long)t0 * a.ld + (long long)h0 * a.dim;
-    if (tok < nt) load(rows + tok * a.ld + (long long)head * a.dim, x, y);
+    if (tok < nt) load(rows + tok * a.ld + (long long)head * a.dim);
 
     // weights of the lane's pairs
     float wq0[NP], wq1[NP], wk0[NP], wk1[NP];
     const bool norm = a.qw != nullptr;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        const bool on = norm && p0 + i < half;
-        wq0[i] = on ? a.qw[at0(p0 + i)] : 1.0f;
-        wq1[i] = on ? a.qw[at1(p0 + i)] : 1.0f;
-        wk0[i] = on ? a.kw[at0(p0 + i)] : 1.0f;
-        wk1[i] = on ? a.kw[at1(p0 + i)] : 1.0f;
+        const int p = min(p0 + i, half - 1);
+        wq0[i] = norm ? a.qw[at0(p)] : 1.0f;
+        wq1[i] = norm ? a.qw[at1(p)] : 1.0f;
+        wk0[i] = norm ? a.kw[at0(p)] : 1.0f;
+        wk1[i] = norm ? a.kw[at1(p)] : 1.0f;
     }
 
     for (int e = tid; e < nt * rp; e += 256) {
@@ -202,11 +207,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkArgs<T> a) {
     while (tok < nt) {
         const int h = h0 + head, t = tok;
         float u[NP], w[NP];
-#pragma unroll
-        for (int i = 0; i < NP; ++i) u[i] = x[i], w[i] = y[i];
+        unpack(u, w);
         head += step;
         while (head >= nh && tok < nt) head -= nh, ++tok;
-        if (tok < nt) load(rows + tok * a.ld + (long long)head * a.dim, x, y);
+        if (tok < nt) load(rows + tok * a.ld + (long long)head * a.dim);
 
         if (h < a.hq + a.hkv) {
             const bool is_q = h < a.hq;

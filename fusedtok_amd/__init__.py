@@ -851,9 +851,10 @@ def attention_decode_paged_prefix(q, k_pool, v_pool, prefix_table, prefix_lens, 
     Any group size Hq / Hkv, D a multiple of 4 up to 512 (on the matrix cores: bf16
     and fp16 with D % 8 == 0 up to 128, tensors aligned to 16 bytes), at most
     4096 sequences and groups together, B * Hq below 2**24. Softmax and sums are
-    float32; bf16 / fp16 weights go into the product with V as two parts of the
-    type, off by at most 2**-17 of a weight, and fp16 weights below 2**-32 of a
-    row's largest count as 0. K and V of the tokens that count are finite;
+    float32; bf16 weights go into the product with V as three parts of the
+    type, which hold all of a float32's bits, fp16 weights as two, off by at most
+    2**-22 of a weight or 2**-32 of a row's largest. K and V of the tokens that
+    count are finite;
     whatever lies in the blocks behind them does not matter. Host-origin tables
     and lengths are range-checked; of GPU-resident ones any values are safe:
     lengths are clamped to the tables, tokens of a table entry outside [0, Nb)

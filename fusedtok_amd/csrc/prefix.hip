@@ -23,17 +23,20 @@
 //
 // A unit's cost is its tokens times a cost a token, by the rows of its tile,
 // and its start: equal shares of tokens alone left 131071 tokens of 64 rows at
-// 200 us, the workgroups with many short units behind; with costs 117.
+// 200 us, the workgroups with many short units behind; with costs 117 (both with
+// two parts of a weight, below; 122 with three).
 //
 // What bounds it: HBM, each K / V row read once a tile of rows of a kv head (up
 // to 128 rows on the matrix cores, so once for a group of 128 rows and fewer). A
 // prefix of 8192 tokens and 64 sequences of 16-2000, 32 / 8 heads, D = 128, bf16:
-// 296 MB in 64 + 5.7 us (attention and combine; 4.6 TB/s); 5 prefixes of
-// 1000-16000 and 48 of 0-3001, 64 / 8 heads, fp16: 469 MB in 93 + 6.8 (5.0); 131071 tokens
-// of 16 sequences: 553 MB in 107 + 8.1 (5.2). Own tokens alone (64 x 4000) reach
-// 6.2 TB/s. What the prefixes lose is the matrix cores' chain from scores to
-// products (128 rows: 35% of their time, the products with V twice, weights in
-// two parts) and the ~6 us of a segment's start, as long as two steps of 64 tokens
+// 296 MB in 70 + 6.1 us (attention and combine; 4.2 TB/s); 5 prefixes of
+// 1000-16000 and 48 of 0-3001, 64 / 8 heads, fp16: 469 MB in 90 + 6.9 (5.2); 131071 tokens
+// of 16 sequences: 553 MB in 110 + 8.1 (5.0). Own tokens alone (64 x 4000) reach
+// 6.1 TB/s. What the prefixes lose is the matrix cores' chain from scores to
+// products (128 rows of bf16 behind 131071 tokens: 174 us, the matrix cores busy
+// for 43% of them, the products with V three times; 152 and 64 us for the first
+// case with two parts of a weight, whose error showed in the output's last bits)
+// and the ~6 us of a segment's start, as long as two steps of 64 tokens
 // for each piece. Loads two steps ahead gained nothing.
 #include "attn_common.hpp"
 #include "fast_div.hpp"
@@ -292,47 +295,51 @@ __device__ __forceinline__ size_t q_row(const PrefixArgs& a, const Piece& p, int
 //   PV      O^T[dim][row] += V^T . P^T, P straight from the scores: lane (r, g)
 //           holds keys 4g+i of each block of 16, so two blocks fill its 8
 //           slots, and V^T comes in the same order by ds_read_b64_tr_b16.
-//   weights in two parts of the storage type, the first truncated, the second
-//           rounded: 16 bits for bf16, 22 for fp16 (there times 2^7, so that
-//           weights down to 2^-31 of the maximum are held, finer than 2^-32).
-//           An error of 2^-17 of a weight is far below half a step of the
-//           output, 2^-9, and goes either way; sums are float32.
+//   weights in parts of the storage type, what one leaves in the next: three
+//           for bf16, 8 bits each, all 24 of a float32; two for fp16, 22 bits
+//           (2^-22 of a weight, as the exponential's own error; there times 2^7,
+//           so that parts down to 2^-32 of the maximum are held). Sums are
+//           float32.
 //
 // Tiles of up to 16 rows (KEYS): wave w takes keys 16w .. of each step with a
-// softmax of its own, merged at the piece's end. Larger ones: 16 QB rows a
-// wave, all 64 keys.
+// softmax of its own, merged at the piece's end. One block of 16 keys leaves
+// half of the slots empty: they hold the second parts, against the same V.
+// Larger ones: 16 QB rows a wave, all 64 keys, a product for each part.
 // ---------------------------------------------------------------------------
 template <typename T> struct PMma;
 template <> struct PMma<bf16> {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     static constexpr float kUp = 1.0f;
+    static constexpr int kParts = 3;
     __device__ __forceinline__ static f32x4 mma(v8 a, v8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
-    // two weights as (first, second) parts, packed
-    __device__ __forceinline__ static int2 split(float a, float b) {
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        typedef bf16 t2 __attribute__((ext_vector_type(2)));
-        const unsigned u = __float_as_uint(a), w = __float_as_uint(b);
-        const f2 rest = {a - __uint_as_float(u & 0xffff0000u),
-                         b - __uint_as_float(w & 0xffff0000u)};
-        return make_int2((int)((u >> 16) | (w & 0xffff0000u)),
-                         __builtin_bit_cast(int, __builtin_convertvector(rest, t2)));
+    // two weights' parts, packed, each the upper half of what is left
+    __device__ __forceinline__ static void split(float a, float b, int (&part)[kParts]) {
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+            const unsigned u = __float_as_uint(a), w = __float_as_uint(b);
+            part[i] = (int)((u >> 16) | (w & 0xffff0000u));
+            a -= __uint_as_float(u & 0xffff0000u);
+            b -= __uint_as_float(w & 0xffff0000u);
+        }
     }
 };
 template <> struct PMma<f16> {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     static constexpr float kUp = 128.0f;
+    static constexpr int kParts = 2;
     __device__ __forceinline__ static f32x4 mma(v8 a, v8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
-    __device__ __forceinline__ static int2 split(float a, float b) {
+    // (the first truncated, the second rounded)
+    __device__ __forceinline__ static void split(float a, float b, int (&part)[kParts]) {
         typedef float f2 __attribute__((ext_vector_type(2)));
         typedef f16 t2 __attribute__((ext_vector_type(2)));
         const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
         const f2 rest = {a - (float)h[0], b - (float)h[1]};
-        return make_int2(__builtin_bit_cast(int, h),
-                         __builtin_bit_cast(int, __builtin_convertvector(rest, t2)));
+        part[0] = __builtin_bit_cast(int, h);
+        part[1] = __builtin_bit_cast(int, __builtin_convertvector(rest, t2));
     }
 };
 
@@ -545,7 +552,6 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
                 }
             }
             constexpr int KS = KEYS ? 1 : 2;  // k-steps of the PV product
-            i32x4 ph[QB][KS], pl[QB][KS];
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
                 float top = -INFINITY;
@@ -559,57 +565,60 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const Piece& p
                 const float m_use = m_new == -INFINITY ? 0.f : m_new;
                 const float alpha = __builtin_amdgcn_exp2f(m_run[qb] - m_use);
                 m_run[qb] = m_new;
-                float p[KB][4], sum = 0.f;
+                float sum = 0.f;
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        p[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][qb][i], c2, -m_use));
-                        sum += p[kb][i];
+                        sc[kb][qb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][qb][i], c2, -m_use));
+                        sum += sc[kb][qb][i];
                     }
                 l_run[qb] = l_run[qb] * alpha + sum;
                 if (__builtin_amdgcn_ballot_w64(moved)) {
 #pragma unroll
                     for (int db = 0; db < C::kDB; ++db) o[db][qb] *= alpha;
                 }
-#pragma unroll
-                for (int x = 0; x < KS; ++x)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        if (KEYS && w >= 2) {  // one block of keys: the other slots are empty
-                            ph[qb][x][w] = pl[qb][x][w] = 0;
-                            continue;
-                        }
-                        const float* const pp = p[KEYS ? 0 : 2 * x + (w >> 1)] + 2 * (w & 1);
-                        const int2 both = M::split(pp[0] * M::kUp, pp[1] * M::kUp);
-                        ph[qb][x][w] = both.x;
-                        pl[qb][x][w] = both.y;
-                    }
             }
-            __builtin_amdgcn_s_setprio(0);
-            // V^T: dims 16 db + r, keys k0 + 32 x + 4g + (0..3) and 16 more
 #pragma unroll
-            for (int db = 0; db < C::kDB; ++db)
+            for (int x = 0; x < KS; ++x) {
+                // the weights' operands: a part each, or (KEYS) two of them in one
+                constexpr int OPS = KEYS ? (M::kParts + 1) / 2 : M::kParts;
+                i32x4 pw[QB][OPS];
 #pragma unroll
-                for (int x = 0; x < KS; ++x) {
+                for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                    for (int w = 0; w < (KEYS ? 2 : 4); ++w) {
+                        const f32x4 p = sc[KEYS ? 0 : 2 * x + (w >> 1)][qb];
+                        int part[M::kParts];
+                        M::split(p[2 * (w & 1)] * M::kUp, p[2 * (w & 1) + 1] * M::kUp, part);
+#pragma unroll
+                        for (int i = 0; i < (KEYS ? 2 * OPS : OPS); ++i)
+                            pw[qb][KEYS ? i / 2 : i][KEYS ? w + 2 * (i & 1) : w] =
+                                i < M::kParts ? part[i] : 0;
+                    }
+                __builtin_amdgcn_s_setprio(0);
+                // V^T: dims 16 db + r, keys k0 + 32 x + 4g + (0..3) and 16 more
+#pragma unroll
+                for (int db = 0; db < C::kDB; ++db) {
                     typedef short v4s __attribute__((ext_vector_type(4)));
                     typedef short v8s __attribute__((ext_vector_type(8)));
                     const char* const p = vs + (k0 + 32 * x + 4 * g + (r16 >> 2)) * C::kPitch +
                                           (16 * db + 4 * (r16 & 3)) * 2;
                     const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                         (__attribute__((address_space(3))) v4s*)(p));
-                    v4s hi = {0, 0, 0, 0};
+                    v4s hi = lo;
                     if constexpr (!KEYS)
                         hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                             (__attribute__((address_space(3))) v4s*)(p + 16 * C::kPitch));
                     const v8s vt = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
                     const V8 vf = __builtin_bit_cast(V8, vt);
 #pragma unroll
-                    for (int qb = 0; qb < QB; ++qb) {
-                        o[db][qb] = M::mma(vf, __builtin_bit_cast(V8, ph[qb][x]), o[db][qb]);
-                        o[db][qb] = M::mma(vf, __builtin_bit_cast(V8, pl[qb][x]), o[db][qb]);
-                    }
+                    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                        for (int i = 0; i < OPS; ++i)
+                            o[db][qb] = M::mma(vf, __builtin_bit_cast(V8, pw[qb][i]), o[db][qb]);
                 }
+            }
         }
         __builtin_amdgcn_s_setprio(1);
     };
@@ -1189,7 +1198,7 @@ __global__ __launch_bounds__(256) void prefix_combine(const PrefixArgs a) {
 // matrix cores bound it). They balance the workgroups:
 // with starts free, 16 sequences of 1-500 tokens behind 131071 shared ones took
 // 215 us, a few workgroups being full of starts, for 120; 128 rows are bound by
-// the matrix cores (64 sequences behind 8192: 71 us at 6, 77 at 4 or 8).
+// the matrix cores (64 sequences behind 8192, by graph replays: 78 us at 6, 88 at 4, 80 at 8).
 constexpr int kStartCost = 768;
 constexpr int kTokenCost[3] = {4, 4, 6}, kTokenCostFloat[3] = {4, 10, 10};
 // The least cost of a segment (4 sequences behind 500 tokens, D = 64: 12.5 us, 14.3

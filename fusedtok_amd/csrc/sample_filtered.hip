@@ -412,7 +412,7 @@ struct RowState {
     Group group;
     u64 base, q, aim, before_mass;
     unsigned few, best, before_count;
-    int bin, entry, slice;
+    int bin, level_bin, entry, slice;
     float top[kWaves];
     int top_at[kWaves];
     __attribute__((aligned(16))) float parts[kFloorOf];
@@ -526,7 +526,8 @@ __device__ __forceinline__ Group resolve(const Row& row, const Limit& l, unsigne
         while (((hi - lo) >> shift) >= kLevel) ++shift;
         s.level_mass[threadIdx.x] = 0;
         s.level_count[threadIdx.x] = 0;
-        if (threadIdx.x == 0) s.bin = 0;
+        // (a word of its own: s.bin may still be read by the waves behind)
+        if (threadIdx.x == 0) s.level_bin = 0;
         __syncthreads();
         each([&](unsigned o, auto&& one) {
             if (o > hi || o < lo || !one()) return;
@@ -540,9 +541,9 @@ __device__ __forceinline__ Group resolve(const Row& row, const Limit& l, unsigne
         u64 mb = m, cb = c, total, tokens;
         block_scan2<kRowNT>(mb, cb, s.scan, total, tokens);
         mb += mass0, cb += count0;
-        if (l.closes(mb, cb, mb + m, cb + c)) s.bin = threadIdx.x;
+        if (l.closes(mb, cb, mb + m, cb + c)) s.level_bin = threadIdx.x;
         __syncthreads();
-        const int bin = s.bin;
+        const int bin = s.level_bin;
         if (threadIdx.x == bin) s.before_mass = mb, s.before_count = (unsigned)cb, s.few = c;
         __syncthreads();
         mass0 = s.before_mass, count0 = s.before_count, n = s.few;

@@ -181,6 +181,8 @@ struct Row {
         minw = (u64)ceil((double)minp * 1099511627776.0);
         p = a.p ? a.p[r] : a.p_all;
         k = a.k ? a.k[r] : a.k_all;
+        // (the first token alone: a limit of 0 would never be open)
+        if (p <= 0.0f) k = 1, p = 1.0f;
         if (k < 0 || k >= a.n) k = 0;
     }
     __device__ __forceinline__ bool cut() const { return k > 0 || p < 1.0f; }
@@ -503,7 +505,9 @@ struct Limit {
     }
 };
 
-// The bin in which the limit is reached; 0 for one that asks for nothing.
+// The bin in which the limit is reached. Every limit is open at 0 (k >= 1; p > 0, so
+// want > 0) and not behind all weights (k is at most their count; p < 1), so it
+// is one bin, here and in the narrower histograms of that bin.
 __device__ __forceinline__ int limit_bin(const Limit& l, RowState& s) {
     if (threadIdx.x == 0) s.bin = 0;
     __syncthreads();

@@ -26,3 +26,25 @@ def test_both_limits_in_full_bins(n, dtype):
     for k, p in ((n // 2, 0.6), (n // 3, 0.97), (n - 2, 0.2), (0, 0.8), (n // 5, 1.0)):
         check(x, u, 1.0, k, p)
     check(x, u, 1.0, rng.integers(1, n, 96).astype(np.int32), rng.uniform(0.05, 0.99, 96), 0.2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 65, 2000, 32768, 40000])
+@pytest.mark.parametrize("values", [1, 3, 1000])
+def test_a_top_p_of_nothing_keeps_the_first_token(values, n, dtype):
+    """p of 0 and less, in rows of which many logits share the first bin:
+    equal ones (zeros too), a few values, a dense line."""
+    rng = np.random.default_rng(n + values)
+    x = rng.integers(0, values, (12, n)) * (0.3 / values)
+    x = np.concatenate([x, x + 3.0, -3.0 - x, np.zeros((4, n))])
+    x[-1, n // 2 + 1:] = -np.inf
+    x, u = dev(x, dtype), rng.random(len(x)).astype(np.float32)
+    first = np.argmax(x.float().cpu().numpy(), 1).tolist()
+    rows = np.arange(len(x))
+    p = np.array([0.0, -2.0, -0.0, -np.inf, 2.0 ** -149])[rows % 5]
+    for temp, k, minp in ((1.0, 0, 0.0), (1.0, 40, 0.0), (0.3, 0, 0.7), (5.0, 700, 1.0)):
+        got = check(x, u, temp, k, p, minp)
+        assert got.tolist() == first
+    # among rows with limits of their own
+    p = np.where(rows % 3, p, 0.6)
+    check(x, u, 1.0, np.where(rows % 2, 0, 100), p)

@@ -1201,10 +1201,11 @@ __global__ __launch_bounds__(kRowNT) void sample_pick(const SampleArgs a) {
                     f(o, [&] { return bin_of(row.far(from_bits(o))) == bin; });
                 });
         });
+        // (also where nothing is cut off: min-p's bins are listed, not summed)
         for (int t = wave; t < a.slices; t += kWaves) {
             u64 sum = 0;
             unsigned ties = 0;
-            const unsigned n = cut.xc > -INFINITY ? s_off[t + 1] - s_off[t] : 0;
+            const unsigned n = s_off[t + 1] - s_off[t];
             const unsigned* const list =
                 held ? s_list + s_off[t] : a.list + (size_t)r * a.n + t * kSlice;
             for (unsigned i = lane; i < n; i += 64) {

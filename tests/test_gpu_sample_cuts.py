@@ -48,3 +48,38 @@ def test_a_top_p_of_nothing_keeps_the_first_token(values, n, dtype):
     # among rows with limits of their own
     p = np.where(rows % 3, p, 0.6)
     check(x, u, 1.0, np.where(rows % 2, 0, 100), p)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("minp", [0.02, 0.05, 0.5, 1.0])
+@pytest.mark.parametrize("n", [20000, 33000, 50257])
+def test_a_mask_that_leaves_fewer_than_k(n, minp, dtype):
+    """k beyond the tokens that have weight cuts nothing and min-p does: masked
+    rows (-inf, the type's lowest value, far logits), weights all over and next
+    to min-p's border, in one slice and in all of them."""
+    rng = np.random.default_rng(n)
+    rows, left = 24, 30
+    low = [-np.inf, torch.finfo(dtype).min, -200.0]
+    x = np.empty((rows, n))
+    for r in range(rows):
+        x[r] = low[r % 3]
+        at = rng.choice(n if r % 4 else 5000, left, False)
+        x[r, at] = rng.standard_normal(left) if r % 2 else np.log(minp) + rng.normal(0, 0.06, left)
+        x[r, at[0]] = x[r, at].max() if r % 2 else 0.0
+        x[r, at[1]] = x[r, at[0]]
+    x, u = dev(x, dtype), rng.random(rows).astype(np.float32)
+    for v in (u, u / 8, 1 - u / 16):
+        check(x, v, 1.0, 50, 1.0, minp)
+        check(x, v, 1.0, 50, 0.9, minp)
+    # left and left + 1: the last k that cuts nothing and the first that may
+    for k in (left - 1, left, left + 1, 10000):
+        check(x, u, 0.8, k, 1.0, minp)
+
+
+def test_a_token_behind_k_that_min_p_keeps():
+    """Two tokens with weight, far apart: the second has its share."""
+    x = torch.full((1000, 40000), -100.0, device="cuda")
+    x[:, 0], x[:, 20000] = 0.0, float(np.log(0.052))
+    u = (np.arange(1000) + 0.5).astype(np.float32) / 1000
+    got = check(x, u, 1.0, 10, 1.0, 0.05)
+    assert abs(got.eq(20000).sum().item() - 1000 * 0.052 / 1.052) <= 1

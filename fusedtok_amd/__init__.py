@@ -1066,8 +1066,8 @@ def qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, *, secti
     to 4 axes (time, height, width), with ``sections`` the number of pairs
     that turn by each axis, in order. The first ``rotary_dim`` values of a head
     (None: D) turn as :func:`rope` does, pair j by ``position *
-    theta^(-2j/rotary_dim)``; ``neox=True`` pairs (j, j + rotary_dim/2), else (2j,
-    2j+1). Returns ``(q [T, q_heads, D], k [T, kv_heads, D], v [T, kv_heads,
+    theta^(-2j/rotary_dim)``, theta at least 2**-10; ``neox=True`` pairs (j, j +
+    rotary_dim/2), else (2j, 2j+1). Returns ``(q [T, q_heads, D], k [T, kv_heads, D], v [T, kv_heads,
     D])``, contiguous, as the appends and the attention take them; v is a copy.
     All in float32 (angles in float64), rounded once. Build addition."""
     return _qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, None, None,

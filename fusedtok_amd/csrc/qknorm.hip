@@ -60,7 +60,8 @@ struct QkArgs {
     int tt, heads;            // tokens and heads of a workgroup
 };
 
-// cosine and sine of a (float64 radians)
+// cosine and sine of a (float64 radians, below 2^41: what is left of it after
+// quarter turns is within pi / 4 and right to 6e-17; from 2^48 on it is not)
 __device__ __forceinline__ float2 cos_sin(double a) {
     const double n = rint(a * 0.63661977236758134308);  // 2 / pi
     double r = fma(n, -1.57079632679489655800, a);      // pi / 2 in two parts
@@ -295,7 +296,9 @@ int qk_norm_rope(const void* qkv, int dtype, long long ld, const float* q_weight
             inval("dim must be even and at most 512");
         if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > dim)
             inval("rotary_dim must be even, at least 2 and at most dim");
-        if (!(theta > 0.0) || !std::isfinite(theta)) inval("theta must be > 0 and finite");
+        // (an angle is below 2^31 / theta: cos_sin's range)
+        if (!(theta >= 0x1p-10) || !std::isfinite(theta))
+            inval("theta must be at least 2^-10 and finite");
         if (!(eps >= 0.0f)) inval("eps must be >= 0");
         if (axes < 1 || axes > kMaxAxes) inval("positions must have 1 to 4 axes");
         if ((long long)q_heads + 2LL * kv_heads > (1 << 20)) inval("qk_norm_rope: too many heads");

@@ -326,8 +326,8 @@ int ft_attention_decode_paged_prefix_launch(
  * theta^(-2j / rotary_dim); v heads are copied. positions [axes, tokens],
  * axes 1..4; sections (host memory, axes entries that sum to rotary_dim / 2;
  * ignored for one axis): the pairs of each axis in order. q_out [tokens,
- * q_heads, dim], k_out / v_out [tokens, kv_heads, dim]. dim even, up to 512. The
- * outputs overlap no input. */
+ * q_heads, dim], k_out / v_out [tokens, kv_heads, dim]. dim even, up to 512;
+ * theta at least 2^-10. The outputs overlap no input. */
 int ft_qk_norm_rope_launch(const void* qkv, int dtype, long long ld, const float* q_weight,
                            const float* k_weight, const int* positions, int axes,
                            const int* sections, int rotary_dim, double theta, float eps, int neox,

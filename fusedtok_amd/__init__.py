@@ -845,12 +845,14 @@ def attention_decode_paged_prefix(q, k_pool, v_pool, prefix_table, prefix_lens, 
     b of ``block_table`` [B, S] as :func:`attention_decode_paged` has it,
     counted from 0: a sequence's own tokens start in a block of their own. A
     sequence in no group has no prefix. A prefix' keys and values are read once
-    for all heads of its group that share them, up to 128 rows at a time, so
-    this pays from two sequences on.
+    for all q heads of its group that share them (sequences times Hq / Hkv), up
+    to 128 of them at a time for bf16 and fp16, 64 for float32, so this pays from
+    two sequences on.
 
-    Any group size Hq / Hkv, D a multiple of 4 up to 512 (on the matrix cores: bf16
-    and fp16 with D % 8 == 0 up to 128, tensors aligned to 16 bytes), at most
-    4096 sequences and groups together, B * Hq below 2**24. Softmax and sums are
+    Any group size Hq / Hkv, D a multiple of 4 up to 512, at most 4096 sequences and
+    groups together, B * Hq below 2**24. The matrix cores take D up to 128, tensors
+    aligned to 16 bytes and, for bf16 and fp16, D % 8 == 0; every other call goes 16
+    q heads at a time through the vector ALU, many times slower (D = 256). Softmax and sums are
     float32; bf16 weights go into the product with V as three parts of the
     type, which hold all of a float32's bits, fp16 weights as two, off by at most
     2**-22 of a weight or 2**-32 of a row's largest. K and V of the tokens that
@@ -1060,8 +1062,8 @@ def qk_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, *, secti
 
     qkv: [T, (q_heads + 2 * kv_heads) * D] (f32 / bf16 / fp16; rows may be
     strided), each row a token's q heads, k heads and v heads; D even, up to 512.
-    q_weight / k_weight: [D] norm weights (float32; others are upcast), ``n = x
-    * rsqrt(mean(x^2) + eps) * weight`` over a head's D values, or None both: no
+    q_weight / k_weight: [D] norm weights (float32; others are converted, at each
+    call), ``n = x * rsqrt(mean(x^2) + eps) * weight`` over a head's D values, or None both: no
     norm. positions: int32 [T] (any values), or [axes, T] for positions of up
     to 4 axes (time, height, width), with ``sections`` the number of pairs
     that turn by each axis, in order. The first ``rotary_dim`` values of a head
@@ -1748,8 +1750,8 @@ def sample_filtered_batched(logits, uniforms, *, temperature=1.0, top_k=0, top_p
     kept; of those the fewest whose weights come to top_p of their sum; of those
     the ones with ``w >= min_p * 2**40``. The token is the first, in the order
     of the indices, at which the sum of the kept weights passes ``floor(u *
-    their whole sum)``. Sums are exact, so a row's token depends on that row
-    alone. temperature 0 takes the largest logit, the first of equals. NaN
+    their whole sum)``. Sums are exact (the two products are float64), so a row's
+    token depends on that row alone. temperature 0 takes the largest logit, the first of equals. NaN
     counts as -inf; a row with nothing else gives -1. Of vectors on the GPU any
     values are safe: a temperature that is not > 0 counts as 0, a top_k below 1
     as none, a top_p of 1 or more (or NaN) as none and one of 0 or less keeps

@@ -11,9 +11,13 @@
 // the angle (float64), rounded once at the end.
 //
 // What bounds it: HBM, each value read and written once (16384 tokens of 32 + 2 *
-// 8 heads, D = 128, bf16: 403 MB in 74.3 us, 5.4 TB/s; stores that bypass the
-// caches: 87-91 us without, or with loads that do too), and for few tokens
-// latency (64 tokens 5.6 us).
+// 8 heads, D = 128, bf16: 403 MB in 70-74 us, 5.4-5.8 TB/s, with the same inputs
+// again and again, 88 with others from call to call; stores that bypass the
+// caches: 87-91 us without, or with loads that do too, same inputs), and for few
+// tokens latency (64 tokens 5.6 us). Where the pieces are not whole 16 bytes
+// (VEC false: rows or halves of the rotated part) loads and stores are single
+// elements: the same tokens 241 us in unaligned rows, 231 with D = 80, R = 40 (D = 80
+// whole: 81).
 //
 // Work split. A head is a group of lanes, 16 bytes of each half of its pairs
 // a lane (D = 128, 2-byte types: 8 lanes, 8 heads a wave); a workgroup takes
@@ -26,7 +30,7 @@
 // float64 parts, so it is right to a float64 step, as far positions need it
 // (a position of 2^31 scales its error to 5e-7); pos * freq is reduced to
 // +-pi/4 in float64, the sine and cosine of what is left are their Taylor
-// series in float32 (next terms 2e-9 and 2e-9).
+// series in float32 (next terms 2e-9 and 1e-10).
 #include "ft_common.hpp"
 
 #include <algorithm>

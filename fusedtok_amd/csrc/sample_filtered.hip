@@ -13,7 +13,9 @@
 //
 // Weights come from float64, so that they are the same to a unit in 2^40
 // whoever computes them, and every sum of them is exact and the same in any
-// order: results depend neither on how a row is cut nor on atomics' order.
+// order: results depend neither on how a row is cut nor on atomics' order. The
+// products p * sum and u * sum are float64, as are the sums that p * sum is
+// compared with.
 //
 // The cut. All filters keep a prefix of the order, so what is kept is x > xc,
 // and the first q in index order of those with x = xc (and w >= min_p 2^40). A
@@ -49,7 +51,9 @@
 // (a table's word and an atomic a token) and float64 (10 operations a token),
 // slice_list for the row's bins, sample_pick and sample_row (2 x 32000: 21.9 us)
 // for their 30 steps, one behind the other, with a barrier between each: 1024
-// threads instead of 512 took 25 and 46 us for sample_pick's 21 and 27.
+// threads instead of 512 took 25 and 46 us for sample_pick's 21 and 27. Without k
+// sample_row has every token's two atomics in one histogram besides (64 x 32000,
+// p alone: 43 us a call, 24.5 with k = 50).
 #include "ft_common.hpp"
 
 #include <algorithm>
@@ -1177,7 +1181,7 @@ __global__ __launch_bounds__(kRowNT) void sample_pick(const SampleArgs a) {
         if (b == 0) s_off[a.slices] = (unsigned)all;
         __syncthreads();
         const bool held = all <= kListMost;
-        // slice t is wave t % 16's
+        // slice t is wave t % kWaves'
         auto slices = [&](auto&& f) {
             for (int t = wave; t < a.slices; t += kWaves) {
                 const unsigned n = s_off[t + 1] - s_off[t];
